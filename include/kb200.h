@@ -223,6 +223,71 @@ int kb200_residual_ln_mod(void* x, const void* r, int64_t rows, int64_t dim, int
                           float eps, void* y, void* stream);
 
 /* ---------------------------------------------------------------------
+ * Causal attention over packed prompts with grouped heads (forward).
+ * Sequence s has the queries cu_q[s] .. cu_q[s+1] and the keys cu_k[s] .. cu_k[s+1] of
+ * the packed tokens; with n queries and m keys, query i sees keys j <= i + m - n (the
+ * queries are the last n of the m tokens), or all m when `causal` is 0.  Query head h
+ * reads kv head h / (Hq / Hkv).  A query that sees no key gets o = 0 and lse = -inf;
+ * rows at and behind cu_q[N] are left as they were.  A masked key's values reach no
+ * output, whatever they are.  D = 64 or 128; dtype 0 bf16, 1 fp16.  Strides in
+ * elements, multiples of 8; channels contiguous.  cu_q, cu_k are device arrays, not
+ * read by the host; offsets are clamped to the tokens there are.
+ * --------------------------------------------------------------------- */
+typedef struct KB200PromptArgs {
+  const void* q;              /* [Tq, Hq, D]                                      */
+  const void* k; const void* v; /* [Tk, Hkv, D]                                   */
+  void* o;                    /* out [Tq, Hq, D]                                  */
+  float* lse;                 /* out [Tq, Hq] log of the softmax sum, or NULL     */
+  const int32_t* cu_q;        /* device [N+1]                                     */
+  const int32_t* cu_k;        /* device [N+1]                                     */
+  int64_t Tq, Tk, N, Hq, Hkv, D;
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride;
+  int64_t v_token_stride, v_head_stride, o_token_stride, o_head_stride;
+  float softmax_scale;
+  int causal;
+  int dtype;
+} KB200PromptArgs;
+int kb200_attn_prompt_fwd(const KB200PromptArgs* a, void* stream);
+
+/* ---------------------------------------------------------------------
+ * 8-bit paged key/value cache: a pool of pages of `page` tokens (16, 32, 64 or 128)
+ * with e4m3 codes [num_pages, H, page, D] for k and v and one fp32 scale per
+ * (page, head) [num_pages, H], a power of two; a value is code * scale.  D = 64 or 128.
+ * A page table [B, max_pages] int32 (device) lists the pages of each sequence in
+ * order.  Entries outside [0, num_pages) are pages that are not there: nothing is
+ * written to them, attention skips their tokens, a gather reads them as 0.
+ * --------------------------------------------------------------------- */
+typedef struct KB200KvCache {
+  void* k_pages; void* v_pages;
+  float* k_scale; float* v_scale;
+  int64_t num_pages, H, page, D;
+} KB200KvCache;
+/* Quantises new tokens k, v [T, H, D] (dtype 0 bf16, 1 fp16; strides in elements,
+ * multiples of 8) into the pages.  Sequence b's new tokens are the packed rows
+ * cu_new[b] .. cu_new[b+1], and the LAST of its lengths[b] tokens (lengths count them
+ * already).  A page's scale is the smallest power of two that holds the largest finite
+ * magnitude of its tokens within 448; when it grows, the codes already in the page
+ * are re-encoded.  NaN and infinities become NaN codes and set no scale.  Pages that
+ * the call writes must belong to one sequence only. */
+int kb200_kv_append(const KB200KvCache* c, const void* k, const void* v, int64_t k_token_stride, int64_t k_head_stride,
+                    int64_t v_token_stride, int64_t v_head_stride, const int32_t* page_table, int64_t max_pages,
+                    const int32_t* lengths, const int32_t* cu_new, int64_t B, int64_t T, int dtype, void* stream);
+/* Dequantises tokens starts[b] .. starts[b] + cu[b+1] - cu[b] of each sequence into the
+ * packed rows cu[b] .. of k, v [T, H, D]; rows at and behind cu[B] are left as they were. */
+int kb200_kv_gather(const KB200KvCache* c, const int32_t* page_table, int64_t max_pages, const int32_t* starts,
+                    const int32_t* cu, int64_t B, int64_t T, void* k, void* v, int dtype, void* stream);
+/* Attention of the last Sq tokens of each sequence over the cache: q [B, Sq, Hq, D]
+ * (strides in elements, multiples of 8), o [B, Sq, Hq, D] contiguous, lse [B, Sq, Hq] or
+ * NULL.  Query i sees the sequence's keys j < lengths[b] - Sq + 1 + i; none: o = 0,
+ * lse = -inf.  Lengths are clamped to max_pages * page. */
+size_t kb200_attn_cached_workspace_size(int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv, int64_t D, int64_t page,
+                                        int64_t max_pages);
+int kb200_attn_cached_fwd(const void* q, int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride,
+                          const KB200KvCache* c, const int32_t* page_table, int64_t max_pages, const int32_t* lengths,
+                          void* o, float* lse, int64_t B, int64_t Sq, int64_t Hq, float softmax_scale, int dtype,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------
  * Failure-path test hooks (no counterpart in the reference).
  * kb200_wait_probe: one CTA waits on an mbarrier nothing arrives on, with the
  * bounded wait every kernel here uses and a budget of `budget_cycles` SM

@@ -52,6 +52,30 @@ class GdnPrologueArgs(ctypes.Structure):
     ]
 
 
+class PromptArgs(ctypes.Structure):
+    """Mirror of ``KB200PromptArgs`` (include/kb200.h)."""
+    _fields_ = [
+        ('q', ctypes.c_void_p), ('k', ctypes.c_void_p), ('v', ctypes.c_void_p), ('o', ctypes.c_void_p),
+        ('lse', ctypes.c_void_p), ('cu_q', ctypes.c_void_p), ('cu_k', ctypes.c_void_p),
+        ('Tq', ctypes.c_int64), ('Tk', ctypes.c_int64), ('N', ctypes.c_int64),
+        ('Hq', ctypes.c_int64), ('Hkv', ctypes.c_int64), ('D', ctypes.c_int64),
+        ('q_token_stride', ctypes.c_int64), ('q_head_stride', ctypes.c_int64),
+        ('k_token_stride', ctypes.c_int64), ('k_head_stride', ctypes.c_int64),
+        ('v_token_stride', ctypes.c_int64), ('v_head_stride', ctypes.c_int64),
+        ('o_token_stride', ctypes.c_int64), ('o_head_stride', ctypes.c_int64),
+        ('softmax_scale', ctypes.c_float), ('causal', ctypes.c_int), ('dtype', ctypes.c_int),
+    ]
+
+
+class KvCacheArgs(ctypes.Structure):
+    """Mirror of ``KB200KvCache`` (include/kb200.h)."""
+    _fields_ = [
+        ('k_pages', ctypes.c_void_p), ('v_pages', ctypes.c_void_p),
+        ('k_scale', ctypes.c_void_p), ('v_scale', ctypes.c_void_p),
+        ('num_pages', ctypes.c_int64), ('H', ctypes.c_int64), ('page', ctypes.c_int64), ('D', ctypes.c_int64),
+    ]
+
+
 _ATTN_SIG = (ctypes.c_int, [ctypes.c_void_p] * 4 + [ctypes.c_int64] * 5 +
              [ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p])
 
@@ -82,6 +106,17 @@ SIGNATURES = {
                             [ctypes.c_float, ctypes.c_void_p]),
     'kb200_residual_ln_mod': (ctypes.c_int, [ctypes.c_void_p] * 2 + [ctypes.c_int64] * 3 +
                               [ctypes.c_void_p] * 3 + [ctypes.c_int, ctypes.c_float] + [ctypes.c_void_p] * 2),
+    'kb200_attn_prompt_fwd': (ctypes.c_int, [ctypes.POINTER(PromptArgs), ctypes.c_void_p]),
+    'kb200_kv_append': (ctypes.c_int, [ctypes.POINTER(KvCacheArgs)] + [ctypes.c_void_p] * 2 + [ctypes.c_int64] * 4 +
+                        [ctypes.c_void_p, ctypes.c_int64] + [ctypes.c_void_p] * 2 + [ctypes.c_int64] * 2 +
+                        [ctypes.c_int, ctypes.c_void_p]),
+    'kb200_kv_gather': (ctypes.c_int, [ctypes.POINTER(KvCacheArgs), ctypes.c_void_p, ctypes.c_int64] +
+                        [ctypes.c_void_p] * 2 + [ctypes.c_int64] * 2 + [ctypes.c_void_p] * 2 +
+                        [ctypes.c_int, ctypes.c_void_p]),
+    'kb200_attn_cached_workspace_size': (ctypes.c_size_t, [ctypes.c_int64] * 7),
+    'kb200_attn_cached_fwd': (ctypes.c_int, [ctypes.c_void_p] + [ctypes.c_int64] * 3 + [ctypes.POINTER(KvCacheArgs),
+                              ctypes.c_void_p, ctypes.c_int64] + [ctypes.c_void_p] * 3 + [ctypes.c_int64] * 3 +
+                              [ctypes.c_float, ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
 }
 
 

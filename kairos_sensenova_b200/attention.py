@@ -17,10 +17,14 @@ dilation is a rearrangement before this call); key tiles outside every window of
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 import torch.nn as nn
 
 from . import _lib
+from .kv_cache import _DTYPES, _forward_only, _index
+from .kv_cache import _rows as _kv_rows
 
 
 def attention_fp8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, num_heads: int,
@@ -96,3 +100,59 @@ class AttentionModule(nn.Module):
 
 
 FP8AttentionModule = AttentionModule
+
+
+def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens_q: torch.Tensor,
+                     cu_seqlens_k: torch.Tensor | None = None, softmax_scale: float | None = None,
+                     causal: bool = True, out: torch.Tensor | None = None, return_lse: bool = False, check: bool = False):
+    """Causal attention over packed prompts with grouped heads, bf16 or fp16, forward.
+
+    ``q``: ``[Tq, Hq, D]``, ``k``, ``v``: ``[Tk, Hkv, D]`` of one type, D 64 or 128, Hq a multiple
+    of Hkv (query head h reads kv head ``h // (Hq / Hkv)``); views of a fused projection are
+    read in place.  Sequence s has query rows ``cu_seqlens_q[s] .. [s+1]`` and key rows
+    ``cu_seqlens_k[s] .. [s+1]`` (int32 on the device; default: the same).  With n queries and m
+    keys the queries are the last n of the m tokens: query i sees the first ``i + 1 + m - n``
+    keys (``causal=False``: all m).  A query that sees none gets 0; the values of keys that a
+    query does not see never reach it, NaN and infinities included.  Returns ``[Tq, Hq, D]``
+    (``out``: to write into; rows behind the last sequence are left as they were); with
+    ``return_lse`` also the fp32 log of the softmax sum ``[Tq, Hq]``.  ``check=True`` looks at
+    the offsets on the host first (it synchronises) and raises ``ValueError``."""
+    what = 'attention_prompt'
+    dev = q.device
+    if dev.type != 'cuda':
+        raise RuntimeError(f'{what}: inputs must be CUDA tensors (no CPU path)')
+    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or k.shape[2] != q.shape[2] or k.shape[1] < 1 \
+            or q.shape[1] < 1 or q.shape[1] % k.shape[1]:
+        raise ValueError(f'{what}: q must be [Tq, Hq, D] and k, v [Tk, Hkv, D] with Hq a multiple of Hkv, got '
+                         f'{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}')
+    if q.dtype not in _DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f'{what}: q, k and v must all be bfloat16 or all float16, got {q.dtype}, {k.dtype}, {v.dtype}')
+    if k.device != dev or v.device != dev:
+        raise ValueError(f'{what}: q, k and v must be on one device')
+    _forward_only(what, q, k, v)
+    N = cu_seqlens_q.shape[0] - 1 if cu_seqlens_q.dim() == 1 else -1
+    if N < 0:
+        raise ValueError(f'{what}: cu_seqlens_q must be [N + 1], got {tuple(cu_seqlens_q.shape)}')
+    cu_q = _index(cu_seqlens_q, (N + 1,), what, 'cu_seqlens_q', dev)
+    cu_k = cu_q if cu_seqlens_k is None else _index(cu_seqlens_k, (N + 1,), what, 'cu_seqlens_k', dev)
+    if check:
+        for name, cu, T in (('cu_seqlens_q', cu_q, q.shape[0]), ('cu_seqlens_k', cu_k, k.shape[0])):
+            at = cu.tolist()
+            if at[0] != 0 or at[-1] > T or any(b < a for a, b in zip(at, at[1:])):
+                raise ValueError(f'{what}: {name} must rise from 0 to at most {T}')
+    Tq, Hq, D = q.shape
+    if softmax_scale is None:
+        softmax_scale = D ** -0.5
+    q, k, v = _kv_rows(q), _kv_rows(k), _kv_rows(v)
+    with torch.cuda.device(dev):
+        if out is None:
+            out = torch.empty(Tq, Hq, D, device=dev, dtype=q.dtype)
+        elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or _kv_rows(out) is not out:
+            raise ValueError(f'{what}: out must be {q.dtype} {list(q.shape)} on {dev}, its rows 16-byte aligned')
+        lse = torch.empty(Tq, Hq, device=dev, dtype=torch.float32) if return_lse else None
+        a = _lib.PromptArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(),
+                            cu_q.data_ptr(), cu_k.data_ptr(), Tq, k.shape[0], N, Hq, k.shape[1], D,
+                            q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+                            out.stride(0), out.stride(1), float(softmax_scale), int(bool(causal)), _DTYPES[q.dtype])
+        _lib.check(_lib.lib().kb200_attn_prompt_fwd(ctypes.byref(a), torch.cuda.current_stream(dev).cuda_stream), what)
+    return (out, lse) if return_lse else out

@@ -1,0 +1,263 @@
+"""The 8-bit paged key/value cache and the attention that reads it.
+
+``layers.Cache`` carries the GatedDeltaNet layers' state from piece to piece; this is its
+counterpart for softmax attention.  A :class:`KVCache` is a pool of pages of 16 to 128
+tokens, e4m3 codes with one fp32 scale per (page, head) that is always a power of two;
+the caller keeps the page table ``[B, max_pages]`` and the lengths ``[B]`` (int32, on the
+device), so none of the calls waits for the host:
+
+* :func:`kv_cache_append` quantises new tokens (whole prompts, pieces, single tokens,
+  packed) into the pages;
+* :func:`kv_cache_gather` gives a token range of each sequence back as packed K and V
+  (the context of a prompt's next piece, for ``attention.attention_prompt``);
+* :func:`attention_cached` attends the last token, or the last few, of each sequence to
+  the cache.
+
+A page table entry outside the pool is a page that is not there: nothing is written to
+it, attention skips its tokens and a gather reads 0.  ``check=True`` looks at the lengths
+and the table on the host first (it synchronises) and raises ``ValueError``.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+PAGE_SIZES = (16, 32, 64, 128)
+HEAD_DIMS = (64, 128)
+
+
+class KVCache:
+    """Pages of one attention layer: ``k_pages``, ``v_pages`` ``[num_pages, heads, page, D]``
+    (``torch.float8_e4m3fn`` or ``uint8`` codes), ``k_scale``, ``v_scale`` ``[num_pages, heads]``
+    fp32 powers of two, all contiguous.  A value is ``code * scale``."""
+
+    __slots__ = ('k_pages', 'v_pages', 'k_scale', 'v_scale', '_args')
+
+    def __init__(self, k_pages, v_pages, k_scale, v_scale):
+        if k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
+            raise ValueError(f'KVCache: k_pages and v_pages must share shape [pages, heads, page, D], got '
+                             f'{tuple(k_pages.shape)}, {tuple(v_pages.shape)}')
+        P, H, page, D = k_pages.shape
+        if page not in PAGE_SIZES or D not in HEAD_DIMS:
+            raise ValueError(f'KVCache: pages of {page} tokens and head dim {D}; supported are {PAGE_SIZES} and {HEAD_DIMS}')
+        if P < 1 or H < 1:
+            raise ValueError(f'KVCache: {P} pages of {H} heads')
+        if k_scale.shape != (P, H) or v_scale.shape != (P, H):
+            raise ValueError(f'KVCache: scales must be [{P}, {H}], got {tuple(k_scale.shape)}, {tuple(v_scale.shape)}')
+        for t in (k_pages, v_pages):
+            if t.dtype not in (torch.float8_e4m3fn, torch.uint8):
+                raise ValueError(f'KVCache: pages must be float8_e4m3fn or uint8, got {t.dtype}')
+        for t in (k_scale, v_scale):
+            if t.dtype != torch.float32:
+                raise ValueError(f'KVCache: scales must be float32, got {t.dtype}')
+        for t in (k_pages, v_pages, k_scale, v_scale):
+            if t.device != k_pages.device:
+                raise ValueError('KVCache: pages and scales must be on one device')
+            if not t.is_contiguous():
+                raise ValueError('KVCache: pages and scales must be contiguous')
+        self.k_pages, self.v_pages, self.k_scale, self.v_scale = k_pages, v_pages, k_scale, v_scale
+        self._args = _lib.KvCacheArgs(k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                                      P, H, page, D)
+
+    @classmethod
+    def empty(cls, num_pages: int, num_heads: int, head_dim: int, page_size: int = 64, device='cuda'):
+        """A pool without tokens (codes 0, scales 1)."""
+        codes = [torch.zeros(num_pages, num_heads, page_size, head_dim, device=device, dtype=torch.uint8)
+                 .view(torch.float8_e4m3fn) for _ in range(2)]
+        return cls(*codes, *(torch.ones(num_pages, num_heads, device=device) for _ in range(2)))
+
+    @property
+    def num_pages(self):
+        return self._args.num_pages
+
+    @property
+    def num_heads(self):
+        return self._args.H
+
+    @property
+    def page_size(self):
+        return self._args.page
+
+    @property
+    def head_dim(self):
+        return self._args.D
+
+    @property
+    def device(self):
+        return self.k_pages.device
+
+
+def _index(t, shape, what, name, dev):
+    """An int32 contiguous tensor of that shape on `dev` (None: any extent)."""
+    if t.device != dev:
+        raise ValueError(f'{what}: {name} must be on {dev}, got {t.device}')
+    if t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)):
+        raise ValueError(f'{what}: {name} must be {list(shape)}, got {tuple(t.shape)}')
+    if t.dtype != torch.int32:
+        if t.dtype != torch.int64:
+            raise ValueError(f'{what}: {name} must be int32, got {t.dtype}')
+        t = t.to(torch.int32)
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _rows(t):
+    """`t` itself if its rows can be read in 16-byte steps in place, else a contiguous copy."""
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in t.stride()[:-1]):
+        return t
+    return t.contiguous()
+
+
+def _forward_only(what, *tensors):
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise NotImplementedError(f'kairos_sensenova_b200.{what} is forward-only')
+
+
+def _cuda(what, cache):
+    if cache.device.type != 'cuda':
+        raise RuntimeError(f'{what}: the cache must be on a CUDA device (no CPU path)')
+    return cache.device
+
+
+def check_tables(cache: KVCache, page_table, last, what='kv_cache', first=None, unique=False):
+    """Raises ``ValueError`` if tokens ``first[b] .. last[b]`` (default from 0) of a sequence lie
+    outside its table row or on a page outside the pool; with ``unique`` also if two of
+    those pages are the same.  Reads the tensors on the host."""
+    table, last = page_table.tolist(), last.tolist()
+    first = [0] * len(last) if first is None else first.tolist()
+    seen = set()
+    for b, (lo, hi) in enumerate(zip(first, last)):
+        if lo < 0 or hi < lo or hi > len(table[b]) * cache.page_size:
+            raise ValueError(f'{what}: sequence {b} has tokens {lo} .. {hi}, its table row holds '
+                             f'{len(table[b]) * cache.page_size}')
+        for pg in table[b][lo // cache.page_size:-(-hi // cache.page_size)] if hi > lo else ():
+            if not 0 <= pg < cache.num_pages:
+                raise ValueError(f'{what}: sequence {b} names page {pg} of a pool of {cache.num_pages}')
+            if unique and pg in seen:
+                raise ValueError(f'{what}: page {pg} would be written twice')
+            seen.add(pg)
+
+
+def kv_cache_append(cache: KVCache, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor,
+                    lengths: torch.Tensor, cu_seqlens: torch.Tensor, check: bool = False) -> None:
+    """Quantise new tokens into their pages, in place.
+
+    ``k``, ``v``: ``[T, heads, D]`` bf16 or fp16, the new tokens of all sequences packed
+    (views of a fused projection are read in place); those of sequence b are rows
+    ``cu_seqlens[b] .. cu_seqlens[b+1]`` and are the LAST tokens of its ``lengths[b]``
+    (the lengths count them already).  A sequence whose tokens do not fit its table row
+    is left out.  The scale of a page and head is the smallest power of two that holds the
+    largest finite magnitude within e4m3's 448; when a later token needs a larger one, the
+    codes already there are re-encoded (exact but for subnormals).  NaN and infinities
+    are stored as NaN and set no scale.  The pages a call writes must each belong to one
+    sequence (``check=True`` raises otherwise)."""
+    what = 'kv_cache_append'
+    dev = _cuda(what, cache)
+    H, D = cache.num_heads, cache.head_dim
+    if k.dim() != 3 or k.shape[1:] != (H, D) or v.shape != k.shape:
+        raise ValueError(f'{what}: k and v must be [T, {H}, {D}], got {tuple(k.shape)}, {tuple(v.shape)}')
+    if k.dtype not in _DTYPES or v.dtype != k.dtype:
+        raise ValueError(f'{what}: k and v must both be bfloat16 or float16, got {k.dtype}, {v.dtype}')
+    if k.device != dev or v.device != dev:
+        raise ValueError(f'{what}: k and v must be on {dev}')
+    _forward_only(what, k, v)
+    page_table = _index(page_table, (None, None), what, 'page_table', dev)
+    B, max_pages = page_table.shape
+    lengths = _index(lengths, (B,), what, 'lengths', dev)
+    cu = _index(cu_seqlens, (B + 1,), what, 'cu_seqlens', dev)
+    if check:
+        check_tables(cache, page_table, lengths, what, lengths - (cu[1:] - cu[:-1]), unique=True)
+        if int(cu[0]) != 0 or int(cu[-1]) > k.shape[0]:
+            raise ValueError(f'{what}: cu_seqlens runs from {int(cu[0])} to {int(cu[-1])}, there are {k.shape[0]} tokens')
+    k, v = _rows(k), _rows(v)
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().kb200_kv_append(
+            ctypes.byref(cache._args), k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+            page_table.data_ptr(), max_pages, lengths.data_ptr(), cu.data_ptr(), B, k.shape[0], _DTYPES[k.dtype],
+            torch.cuda.current_stream(dev).cuda_stream), what)
+
+
+def kv_cache_gather(cache: KVCache, page_table: torch.Tensor, starts: torch.Tensor, cu_seqlens: torch.Tensor, total: int,
+                    dtype: torch.dtype = torch.bfloat16, out=None, check: bool = False):
+    """Tokens ``starts[b] ..`` of each sequence, ``cu_seqlens[b+1] - cu_seqlens[b]`` of them, as
+    packed ``(k, v)`` ``[total, heads, D]`` in ``dtype`` (bf16: exact).  ``total`` is known to
+    the host (``cu_seqlens[-1]``, or more: rows behind it are left as they were).  ``out``:
+    ``(k, v)`` to write into, contiguous."""
+    what = 'kv_cache_gather'
+    dev = _cuda(what, cache)
+    if dtype not in _DTYPES:
+        raise ValueError(f'{what}: dtype must be bfloat16 or float16, got {dtype}')
+    page_table = _index(page_table, (None, None), what, 'page_table', dev)
+    B, max_pages = page_table.shape
+    starts = _index(starts, (B,), what, 'starts', dev)
+    cu = _index(cu_seqlens, (B + 1,), what, 'cu_seqlens', dev)
+    shape = (int(total), cache.num_heads, cache.head_dim)
+    if shape[0] < 0:
+        raise ValueError(f'{what}: total {total}')
+    if check:
+        check_tables(cache, page_table, starts + cu[1:] - cu[:-1], what, starts)
+        if int(cu[0]) != 0 or int(cu[-1]) > shape[0]:
+            raise ValueError(f'{what}: cu_seqlens runs from {int(cu[0])} to {int(cu[-1])}, total is {shape[0]}')
+    with torch.cuda.device(dev):
+        if out is None:
+            k, v = torch.empty(shape, device=dev, dtype=dtype), torch.empty(shape, device=dev, dtype=dtype)
+        else:
+            k, v = out
+            for t in (k, v):
+                if t.shape != shape or t.dtype != dtype or t.device != dev or not t.is_contiguous() or t.data_ptr() % 16:
+                    raise ValueError(f'{what}: out must be contiguous 16-byte aligned {dtype} {list(shape)} on {dev}')
+        _lib.check(_lib.lib().kb200_kv_gather(
+            ctypes.byref(cache._args), page_table.data_ptr(), max_pages, starts.data_ptr(), cu.data_ptr(), B, shape[0],
+            k.data_ptr(), v.data_ptr(), _DTYPES[dtype], torch.cuda.current_stream(dev).cuda_stream), what)
+    return k, v
+
+
+def attention_cached(q: torch.Tensor, cache: KVCache, page_table: torch.Tensor, lengths: torch.Tensor,
+                     softmax_scale: float | None = None, out: torch.Tensor | None = None, return_lse: bool = False,
+                     check: bool = False):
+    """Attention of the last Sq tokens of each sequence over its cached tokens.
+
+    ``q``: ``[B, Sq, Hq, D]`` bf16 or fp16 (Hq a multiple of the cache's heads; query head h
+    reads kv head ``h // (Hq / heads)``); ``lengths[b]`` counts the cached tokens, the Sq
+    themselves included, and query i sees the first ``lengths[b] - Sq + 1 + i`` of them.  A
+    query that sees none (an idle slot of length 0) gets 0.  Returns ``[B, Sq, Hq, D]`` in
+    q's type (``out``: contiguous, to write into); with ``return_lse`` also the fp32 log of
+    the softmax sum ``[B, Sq, Hq]`` (-inf where nothing is seen)."""
+    what = 'attention_cached'
+    dev = _cuda(what, cache)
+    H, D = cache.num_heads, cache.head_dim
+    if q.dim() != 4 or q.shape[3] != D or q.shape[2] < 1 or q.shape[2] % H:
+        raise ValueError(f'{what}: q must be [B, Sq, Hq, {D}] with Hq a multiple of {H}, got {tuple(q.shape)}')
+    if q.dtype not in _DTYPES:
+        raise ValueError(f'{what}: q must be bfloat16 or float16, got {q.dtype}')
+    if q.device != dev:
+        raise ValueError(f'{what}: q must be on {dev}, got {q.device}')
+    _forward_only(what, q)
+    B, Sq, Hq, _ = q.shape
+    page_table = _index(page_table, (B, None), what, 'page_table', dev)
+    lengths = _index(lengths, (B,), what, 'lengths', dev)
+    max_pages = page_table.shape[1]
+    if check:
+        check_tables(cache, page_table, lengths, what)
+    if softmax_scale is None:
+        softmax_scale = D ** -0.5
+    q = _rows(q)
+    L = _lib.lib()
+    with torch.cuda.device(dev):
+        if out is None:
+            out = torch.empty(q.shape, device=dev, dtype=q.dtype)
+        elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous() or out.data_ptr() % 16:
+            raise ValueError(f'{what}: out must be contiguous 16-byte aligned {q.dtype} {list(q.shape)} on {dev}')
+        lse = torch.empty(q.shape[:3], device=dev, dtype=torch.float32) if return_lse else None
+        nbytes = L.kb200_attn_cached_workspace_size(B, Sq, Hq, H, D, cache.page_size, max_pages)
+        if nbytes == 0:
+            _lib.check(1, what)
+        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+        _lib.check(L.kb200_attn_cached_fwd(
+            q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), ctypes.byref(cache._args), page_table.data_ptr(), max_pages,
+            lengths.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(), B, Sq, Hq, float(softmax_scale),
+            _DTYPES[q.dtype], ws.data_ptr(), nbytes, torch.cuda.current_stream(dev).cuda_stream), what)
+    return (out, lse) if return_lse else out

@@ -1,0 +1,413 @@
+"""attention_prompt, the 8-bit paged cache and attention_cached against ``oracle.serving`` (64 bits).
+
+Bounds.  With u the half step of the output type (bf16 2^-8, fp16 2^-11) and u_p that of the
+probabilities (attention_prompt rounds them to the input type, attention_cached to fp16),
+|o - ref| <= u_p A + u |ref| + c A, A = sum_j softmax_j |v_j|.  c covers the fp32 chain: a score's error
+is at most D 2^-24 sum_d |q_d k_d| scale <= 128 * 2^-24 * |q| |k| scale, and |q| |k| scale < 32 for the data
+here, so 2 * 128 * 32 * 2^-24 = 2^-11 relative in a probability at the very most; the sums add n 2^-24."""
+import math
+
+import pytest
+import torch
+
+from kairos_sensenova_b200 import KVCache, attention_cached, attention_prompt, kv_cache_append, kv_cache_gather
+from oracle import serving as ref
+
+pytestmark = pytest.mark.gpu
+
+HALF_STEP = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+CHAIN = 2.0 ** -11
+
+
+def close(o, want, A, dtype, u_p=None):
+    u = HALF_STEP[dtype]
+    bound = (HALF_STEP[dtype] if u_p is None else u_p) * A + u * want.abs() + CHAIN * A + 1e-7
+    nan = torch.isnan(want)
+    assert torch.equal(torch.isnan(o), nan), 'NaN in other places'
+    inf = torch.isinf(want)
+    assert torch.equal(o[inf].double(), want[inf])
+    off = torch.where(nan | inf, 0.0, (o.double() - want).abs() - bound)
+    assert (off <= 0).all(), f'{off.max().item():.3e} over the bound at {(off > 0).nonzero()[:4].tolist()}'
+
+
+def close_lse(lse, want):
+    fin = torch.isfinite(want)
+    assert torch.equal(lse[~fin].double(), want[~fin])
+    assert ((lse.double() - want)[fin].abs() <= 2.0 ** -11 + want[fin].abs() * 2.0 ** -22).all()
+
+
+def cu(lens):
+    at = [0]
+    for n in lens:
+        at.append(at[-1] + n)
+    return at
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device='cuda')
+
+
+def gen(seed):
+    return torch.Generator(device='cuda').manual_seed(seed)
+
+
+def randn(g, *shape, dtype=torch.bfloat16):
+    return torch.randn(*shape, generator=g, device='cuda').to(dtype)
+
+
+# ------------------------------------------------------------------ prompts
+LENS = [
+    ([1], [1]), ([0], [0]), ([5, 0, 3], [5, 0, 3]), ([128], [128]), ([129, 1, 127], [129, 1, 127]),
+    ([255, 256, 257], [255, 256, 257]), ([640, 33], [640, 33]),
+    ([1, 7, 64], [300, 129, 64]),            # queries at the end of more keys
+    ([0, 4], [50, 0]),                       # no queries; no keys at all
+    ([300, 20], [40, 20]),                   # more queries than keys: the first see nothing
+    ([3] * 70, [5] * 70),
+]
+
+
+@pytest.mark.parametrize('nq,nk', LENS)
+@pytest.mark.parametrize('heads,kv,dim,dtype', [(4, 4, 128, torch.bfloat16), (6, 2, 64, torch.float16),
+                                                (7, 1, 128, torch.float16), (5, 5, 64, torch.bfloat16)])
+def test_prompt(nq, nk, heads, kv, dim, dtype):
+    g = gen(len(nq) * 1000 + sum(nq) + heads)
+    q, k, v = randn(g, sum(nq), heads, dim, dtype=dtype), randn(g, sum(nk), kv, dim, dtype=dtype), \
+        randn(g, sum(nk), kv, dim, dtype=dtype)
+    for causal in (True, False):
+        o, lse = attention_prompt(q, k, v, i32(cu(nq)), i32(cu(nk)), causal=causal, return_lse=True, check=True)
+        want, wlse, A = ref.prompt(q, k, v, cu(nq), cu(nk), dim ** -0.5, causal)
+        close(o, want, A, dtype)
+        close_lse(lse, wlse)
+
+
+@pytest.mark.parametrize('heads,kv,dim,dtype,n', [(24, 8, 128, torch.bfloat16, 3001), (32, 1, 64, torch.float16, 1500),
+                                                  (2, 2, 128, torch.float16, 5000), (96, 1, 128, torch.bfloat16, 700),
+                                                  (300, 1, 64, torch.bfloat16, 65)])
+def test_prompt_long(heads, kv, dim, dtype, n):
+    g = gen(n)
+    x = randn(g, n, heads + 2 * kv, dim, dtype=dtype)         # views of a fused projection
+    q, k, v = x[:, :heads], x[:, heads:heads + kv], x[:, heads + kv:]
+    o = attention_prompt(q, k, v, i32([0, n]))
+    want, _, A = ref.prompt(q, k, v, [0, n], [0, n], dim ** -0.5)
+    close(o, want, A, dtype)
+    assert torch.equal(o, attention_prompt(q, k, v, i32([0, n])))
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('value', [math.nan, math.inf])
+def test_prompt_masked_values_do_not_leak(dtype, value):
+    """K and V of one token not finite: rows that do not see it, in its sequence and in the neighbours, are as without."""
+    g = gen(3)
+    nq = [200, 150, 90]
+    q, k, v = (randn(g, sum(nq), 3, 128, dtype=dtype) for _ in range(3))
+    clean = attention_prompt(q, k, v, i32(cu(nq)))
+    at = 200 + 100                                            # token 100 of the second sequence
+    kb, vb = k.clone(), v.clone()
+    vb[at, 1, 5] = value
+    kb[at, 2] = value
+    o = attention_prompt(q, kb, vb, i32(cu(nq)))
+    hit = torch.zeros_like(o, dtype=torch.bool)
+    hit[at:350, 1, 5] = True
+    hit[at:350, 2] = True
+    assert torch.equal(o[~hit], clean[~hit])
+    assert not torch.isfinite(o[at:350, 1, 5]).any()
+    assert torch.isnan(o[at:350, 2]).all() or value == math.inf
+    # the first token of the next sequence: the sequence before ends in the same key tile
+    vb = v.clone()
+    vb[350] = value
+    o = attention_prompt(q, k, vb, i32(cu(nq)))
+    assert torch.equal(o[:350], clean[:350])
+
+
+def test_prompt_extremes():
+    """Scores up to the largest finite ones, equal scores, and a row maximum that keeps rising along the keys."""
+    n, dt = 700, torch.bfloat16
+    g = gen(5)
+    q, k, v = (randn(g, n, 2, 64, dtype=dt) for _ in range(3))
+    k[:, 0] = (k[:, 0].float() * torch.linspace(0.1, 30, n, device='cuda')[:, None]).to(dt)
+    k[:, 1] = 1.0
+    o, lse = attention_prompt(q, k, v, i32([0, n]), return_lse=True)
+    want, wlse, A = ref.prompt(q, k, v, [0, n], [0, n], 64 ** -0.5)
+    # scores here reach 30 times the usual: so does the fp32 chain's bound
+    close(o, want, A * 30 * CHAIN / (HALF_STEP[dt] + CHAIN) + A, dt)
+    assert ((lse.double() - wlse).abs() <= 30 * 2.0 ** -11 + wlse.abs() * 2.0 ** -22).all()
+    q[:] = 3e38
+    k[:] = -1.0
+    o = attention_prompt(q, k, v, i32([0, n]))               # every score is -inf: no key counts
+    assert (o == 0).all()
+
+
+def test_prompt_rows_behind_the_last_sequence_and_out():
+    g = gen(7)
+    q, k, v = (randn(g, 300, 2, 128) for _ in range(3))
+    out = torch.full((300, 4, 128), 7.0, device='cuda', dtype=torch.bfloat16)[:, 1:3]
+    r = attention_prompt(q, k, v, i32([0, 100, 211]), out=out)
+    assert r is out and (out[211:] == 7).all() and (out._base[:, 0] == 7).all() and (out._base[:, 3] == 7).all()
+    want, _, A = ref.prompt(q, k, v, [0, 100, 211], [0, 100, 211], 128 ** -0.5)
+    close(out[:211], want[:211], A[:211], torch.bfloat16)
+    # offsets past the tokens are clamped to them
+    out2 = attention_prompt(q, k, v, i32([0, 100, 5000]))
+    want, _, A = ref.prompt(q, k, v, [0, 100, 300], [0, 100, 300], 128 ** -0.5)
+    close(out2, want, A, torch.bfloat16)
+
+
+def test_prompt_far_offsets():
+    """Element offsets over 2^31 in k and v."""
+    n, ld = 66000, 33000
+    base = torch.empty(n, ld, device='cuda', dtype=torch.bfloat16)
+    g = gen(9)
+    k, v = base[:, 32872 - 128:32872].view(n, 1, 128), base[:, 32872:33000].view(n, 1, 128)
+    k.copy_(randn(g, n, 1, 128))
+    v.copy_(randn(g, n, 1, 128))
+    q = randn(g, 40, 1, 128)
+    o = attention_prompt(q, k, v, i32([0, 40]), i32([0, n]))
+    want, _, A = ref.prompt(q, k, v, [0, 40], [0, n], 128 ** -0.5)
+    close(o, want, A, torch.bfloat16)
+
+
+# ------------------------------------------------------------------ the cache
+def make_cache(lens, H, D, page, seed, extra=2):
+    """A filled pool, shuffled pages, random codes (NaN codes on pages and slots that nobody owns)."""
+    g = gen(seed)
+    need = [-(-n // page) for n in lens]
+    P = sum(need) + extra
+    order = torch.randperm(P, generator=torch.Generator().manual_seed(seed)).tolist()
+    table, at = [], 0
+    width = max(max(need), 1)
+    for n in need:
+        table.append(order[at:at + n] + [-1] * (width - n))
+        at += n
+    used = torch.zeros(P, page, dtype=torch.bool, device='cuda')
+    for b, n in enumerate(lens):
+        for j, pg in enumerate(table[b][:need[b]]):
+            used[pg, :min(page, n - j * page)] = True
+    pools, scales = [], []
+    for _ in range(2):
+        x = (torch.randn(P, H, page, D, generator=g, device='cuda') * 60).clamp(-448, 448)
+        c = x.to(torch.float8_e4m3fn)
+        c.view(torch.uint8).masked_fill_(~used[:, None, :, None], 0x7f)
+        pools.append(c)
+        scales.append(torch.exp2(torch.randint(-8, -4, (P, H), generator=g, device='cuda').float()))
+    return KVCache(*pools, *scales), table, used
+
+
+def values(codes):
+    return codes.float().double()
+
+
+@pytest.mark.parametrize('new,old', [([1], [0]), ([1, 1, 1], [0, 15, 16]), ([16, 17, 1], [0, 0, 130]), ([200, 0, 3], [5, 40, 127]),
+                                     ([1] * 40, list(range(40))), ([700], [0]), ([0], [9])])
+@pytest.mark.parametrize('H,D,page,dtype', [(1, 128, 64, torch.bfloat16), (3, 64, 16, torch.float16),
+                                            (2, 128, 128, torch.float16), (8, 64, 32, torch.bfloat16), (5, 128, 16, torch.bfloat16),
+                                            (2, 64, 128, torch.bfloat16), (2, 64, 64, torch.float16), (3, 128, 32, torch.bfloat16)])
+def test_append_and_gather(new, old, H, D, page, dtype):
+    lens = [a + b for a, b in zip(new, old)]
+    cache, table, used = make_cache(lens, H, D, page, seed=sum(lens) + H)
+    g = gen(D + page)
+    k, v = randn(g, sum(new), H, D, dtype=dtype) * 3, randn(g, sum(new), H, D, dtype=dtype)
+    want = []
+    for codes, scale, x in ((cache.k_pages, cache.k_scale, k), (cache.v_pages, cache.v_scale, v)):
+        w, s = values(codes), scale.clone()
+        ref.append(w, s, x, table, lens, cu(new))
+        want.append((w, s))
+    kv_cache_append(cache, k, v, i32(table), i32(lens), i32(cu(new)), check=True)
+    for codes, scale, (w, s) in ((cache.k_pages, cache.k_scale, want[0]), (cache.v_pages, cache.v_scale, want[1])):
+        assert torch.equal(scale, s)
+        got = values(codes)
+        assert torch.equal(torch.isnan(got), torch.isnan(w)) and torch.equal(got.nan_to_num(), w.nan_to_num())
+    # all of it back, and a range from the middle
+    for starts in ([0] * len(lens), [n // 2 for n in lens]):
+        counts = [n - s for n, s in zip(lens, starts)]
+        for dt in (torch.bfloat16, torch.float16):
+            kg, vg = kv_cache_gather(cache, i32(table), i32(starts), i32(cu(counts)), sum(counts), dtype=dt, check=True)
+            for got, (w, s) in ((kg, want[0]), (vg, want[1])):
+                assert torch.equal(got, ref.gather(w, s, table, starts, counts).to(dt))
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
+def test_append_extremes(dtype):
+    """Zeros, subnormals, the borders of a scale, the largest values, NaN and infinities, token by token into one page."""
+    H, D, page = 2, 64, 16
+    cache = KVCache.empty(3, H, D, page)
+    rows = torch.zeros(14, H, D, device='cuda', dtype=dtype)
+    big = torch.finfo(dtype).max / 4
+    for i, x in enumerate([0.0, 2.0 ** -20, 448.0, 449.0 if dtype == torch.float16 else 450.0, 0.4375, 3.0, math.nan, math.inf, -math.inf, 7.5,
+                           big, -big, 1.0, 2.0 ** -24]):
+        rows[i] = torch.linspace(-1, 1, D, device='cuda').to(dtype) * 0.01
+        rows[i, 0, 3] = x
+        rows[i, 1] = x
+    w, s = values(cache.k_pages), cache.k_scale.clone()
+    table = [[1]]
+    for i in range(14):
+        ref.append(w, s, rows[i:i + 1], table, [i + 1], [0, 1])
+        kv_cache_append(cache, rows[i:i + 1], rows[i:i + 1], i32(table), i32([i + 1]), i32([0, 1]))
+        assert torch.equal(cache.k_scale, s) and torch.equal(cache.v_scale, s), i
+        got = values(cache.k_pages)
+        assert torch.equal(torch.isnan(got), torch.isnan(w)) and torch.equal(got.nan_to_num(), w.nan_to_num()), i
+
+
+def test_append_leaves_out_what_does_not_fit():
+    """Pages outside the pool, lengths over the table row and new tokens over the length: nothing of them is written."""
+    cache = KVCache.empty(4, 1, 64, 16)
+    before = cache.k_pages.clone().view(torch.uint8)
+    x = torch.ones(40, 1, 64, device='cuda', dtype=torch.bfloat16)
+    table, lens, new = [[0, 9], [-1, -5], [1, 2], [3, 3]], [32, 16, 100, 2], [20, 10, 5, 5]
+    kv_cache_append(cache, x, x, i32(table), i32(lens), i32(cu(new)))
+    got = cache.k_pages.view(torch.uint8)
+    assert torch.equal(got[1:], before[1:])                   # sequences 1, 2, 3 wrote nothing
+    assert (got[0, 0, 12:] != 0).all() and (got[0, 0, :12] == 0).all()   # sequence 0: its page 9 is left out
+    kg, _ = kv_cache_gather(cache, i32(table), i32([0, 0, 90, 0]), i32([0, 32, 48, 58, 60]), 64)
+    assert (kg[12:16] == 1).all() and (kg[16:60] == 0).all()
+
+
+def test_gather_leaves_other_rows():
+    cache, table, _ = make_cache([30], 2, 128, 16, 1)
+    out = [torch.full((50, 2, 128), 5.0, device='cuda', dtype=torch.bfloat16) for _ in range(2)]
+    kv_cache_gather(cache, i32(table), i32([3]), i32([0, 27]), 50, out=out)
+    assert all((t[27:] == 5).all() and (t[:27] != 5).any() for t in out)
+
+
+# ------------------------------------------------------------------ attention over the cache
+@pytest.mark.parametrize('lens,sq', [([1], 1), ([0, 5, 0], 1), ([127, 128, 129], 1), ([16, 17, 1000], 1), ([2, 300, 0], 4),
+                                     ([64] * 33, 1), ([513], 9), ([3000, 1], 2)])
+@pytest.mark.parametrize('heads,H,D,page,dtype', [(8, 2, 128, 64, torch.bfloat16), (3, 3, 64, 16, torch.float16),
+                                                  (16, 1, 64, 32, torch.bfloat16), (14, 2, 128, 128, torch.float16),
+                                                  (40, 1, 128, 16, torch.bfloat16), (5, 1, 64, 128, torch.bfloat16)])
+def test_cached(lens, sq, heads, H, D, page, dtype):
+    cache, table, _ = make_cache(lens, H, D, page, seed=len(lens) + sum(lens))
+    q = randn(gen(heads), len(lens), sq, heads, D, dtype=dtype)
+    o, lse = attention_cached(q, cache, i32(table), i32(lens), return_lse=True, check=True)
+    want, wlse, A = ref.cached(q, values(cache.k_pages), values(cache.v_pages), cache.k_scale, cache.v_scale, table, lens,
+                               D ** -0.5)
+    close(o, want, A, dtype, u_p=2.0 ** -11)
+    close_lse(lse, wlse)
+    assert torch.equal(o, attention_cached(q, cache, i32(table), i32(lens)))
+
+
+def test_cached_many_rows_and_long():
+    for lens, sq, heads, H, D, page in (([700, 20], 40, 8, 2, 128, 64), ([40000, 3], 1, 4, 4, 64, 16), ([9000], 3, 200, 1, 128, 32)):
+        cache, table, _ = make_cache(lens, H, D, page, seed=sq)
+        q = randn(gen(sq), len(lens), sq, heads, D)
+        o, lse = attention_cached(q, cache, i32(table), i32(lens), return_lse=True)
+        want, wlse, A = ref.cached(q, values(cache.k_pages), values(cache.v_pages), cache.k_scale, cache.v_scale, table,
+                                   lens, D ** -0.5)
+        close(o, want, A, torch.bfloat16, u_p=2.0 ** -11)
+        close_lse(lse, wlse)
+
+
+def test_cached_scales_far_apart():
+    """V scales 2^40 apart, the largest on a page whose keys get no weight; queries of any size; a strided q."""
+    lens, H, D, page = [64], 1, 128, 16
+    cache, table, _ = make_cache(lens, H, D, page, seed=2)
+    cache.v_scale[table[0][1]] = 2.0 ** 30
+    cache.v_scale[table[0][2]] = 2.0 ** -30
+    k = values(cache.k_pages)
+    cache.k_pages[table[0][1]] = torch.tensor(-448.0, device='cuda').to(torch.float8_e4m3fn)
+    k = values(cache.k_pages)
+    q = torch.full((1, 2, 6, D), 1.0, device='cuda', dtype=torch.bfloat16)
+    q[:, :, 1] = 2.0 ** -100
+    q[:, :, 2] = torch.randn(D, generator=gen(1), device='cuda').bfloat16() * 1e-3
+    q = q[:, :, ::2]                                          # heads 0, 2, 4
+    o = attention_cached(q, cache, i32(table), i32(lens), softmax_scale=0.02)
+    want, _, A = ref.cached(q, k, values(cache.v_pages), cache.k_scale, cache.v_scale, table, lens, 0.02)
+    close(o, want, A, torch.bfloat16, u_p=2.0 ** -11)
+
+
+def test_cached_hidden_nan_and_missing_pages():
+    """A NaN code of the newest token reaches only the queries that see it; a missing page is skipped."""
+    lens, H, D, page = [100], 2, 128, 32
+    cache, table, _ = make_cache(lens, H, D, page, seed=4)
+    q = randn(gen(4), 1, 3, 4, D)
+    clean = attention_cached(q, cache, i32(table), i32(lens))
+    pg = table[0][99 // page]
+    cache.v_pages.view(torch.uint8)[pg, 0, 99 % page, 7] = 0x7f     # the last token: query 2 alone sees it
+    cache.k_pages.view(torch.uint8)[pg, 1, 98 % page] = 0xff        # the one before: queries 1 and 2
+    o = attention_cached(q, cache, i32(table), i32(lens))
+    hit = torch.zeros_like(o, dtype=torch.bool)
+    hit[0, 2, :2, 7] = True
+    hit[0, 1:, 2:] = True
+    assert torch.equal(o[~hit], clean[~hit]) and torch.isnan(o[hit]).all()
+    # all keys NaN: NaN, not 0
+    cache.k_pages.view(torch.uint8)[:] = 0x7f
+    assert torch.isnan(attention_cached(q, cache, i32(table), i32(lens))).all()
+    # a table entry outside the pool: its tokens are not there
+    cache, table, _ = make_cache([96], H, D, page, seed=5)
+    holed = [[table[0][0], 10 ** 9, table[0][2]]]
+    o, lse = attention_cached(q, cache, i32(holed), i32([96]), return_lse=True)
+    short = [[table[0][0], table[0][2]]]
+    w, wl = attention_cached(q, cache, i32(short), i32([64]), return_lse=True)
+    assert (o.float() - w.float()).abs().max() <= 2.0 ** -7 * w.float().abs().max() and (lse - wl).abs().max() < 1e-3
+    # lengths over the table row are cut to it
+    assert torch.equal(attention_cached(q, cache, i32(table), i32([5000])), attention_cached(q, cache, i32(table), i32([96])))
+
+
+def test_cached_far_pages():
+    """Code offsets over 2^31 bytes."""
+    H, D, page, P = 4, 128, 128, 40000                       # 2.6 GB each for k and v
+    k = torch.zeros(P, H, page, D, device='cuda', dtype=torch.uint8).view(torch.float8_e4m3fn)
+    v = torch.zeros_like(k)
+    cache = KVCache(k, v, torch.ones(P, H, device='cuda'), torch.ones(P, H, device='cuda'))
+    table, lens = [[39999, 39998, 7]], [300]
+    g = gen(11)
+    x, y = randn(g, 300, H, D), randn(g, 300, H, D)
+    kv_cache_append(cache, x, y, i32(table), i32(lens), i32([0, 300]))
+    xg, yg = kv_cache_gather(cache, i32(table), i32([0]), i32([0, 300]), 300)
+    assert ((xg.float() - x.float()).abs() <= 2.0 ** -4 * x.float().abs() + 2.0 ** -10 * 4).all()
+    q = randn(g, 1, 1, 8, D)
+    o = attention_cached(q, cache, i32(table), i32(lens))
+    want, _, A = ref.prompt(q[0], xg, yg, [0, 1], [0, 300], D ** -0.5)
+    close(o[0], want, A, torch.bfloat16, u_p=2.0 ** -11)
+
+
+# ------------------------------------------------------------------ together, as they are used
+def test_serving_run_in_pieces_streams_and_graph():
+    """Prompts, their next pieces over the gathered context, then decode steps replayed as a graph, on a side stream;
+    every step against attention over the tokens that the cache holds."""
+    H, heads, D, page, B = 2, 6, 128, 16, 3
+    g = gen(21)
+    lens = [37, 5, 130]
+    cache = KVCache.empty(64, H, D, page)
+    perm = torch.randperm(64, generator=torch.Generator().manual_seed(1)).tolist()
+    table_l = [perm[i * 20:(i + 1) * 20] for i in range(B)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        table = i32(table_l)
+        done = [0] * B
+        for piece in (lens, [16, 0, 3]):
+            q, k, v = randn(g, sum(piece), heads, D), randn(g, sum(piece), H, D), randn(g, sum(piece), H, D)
+            done = [a + b for a, b in zip(done, piece)]
+            kv_cache_append(cache, k, v, table, i32(done), i32(cu(piece)))
+            kc, vc = kv_cache_gather(cache, table, i32([0] * B), i32(cu(done)), sum(done))
+            o = attention_prompt(q, kc, vc, i32(cu(piece)), i32(cu(done)))
+            want, _, A = ref.prompt(q, kc, vc, cu(piece), cu(done), D ** -0.5)
+            close(o, want, A, torch.bfloat16)
+        # a decode step as a graph: lengths grow inside it
+        length = i32(done)
+        q, k, v = randn(g, B, 1, heads, D), randn(g, B, H, D), randn(g, B, H, D)
+        steps = i32(list(range(B + 1)))
+
+        def step():
+            length.add_(1)
+            kv_cache_append(cache, k, v, table, length, steps)
+            return attention_cached(q, cache, table, length)
+        step()
+        done = [n + 1 for n in done]
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        o = step()
+    other = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(other, stream=side):
+        o2 = attention_cached(q, cache, table, length)
+    for i in range(20):
+        q.copy_(randn(g, B, 1, heads, D))
+        k.copy_(randn(g, B, H, D))
+        v.copy_(randn(g, B, H, D))
+        graph.replay()
+        other.replay()
+        done = [n + 1 for n in done]
+        assert length.tolist() == done and torch.equal(o, o2)
+        want, _, A = ref.cached(q, values(cache.k_pages), values(cache.v_pages), cache.k_scale, cache.v_scale, table_l, done,
+                                D ** -0.5)
+        close(o, want, A, torch.bfloat16, u_p=2.0 ** -11)

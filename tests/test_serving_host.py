@@ -1,0 +1,107 @@
+"""Refusals of the serving operators (no GPU: the checks run before anything is launched) and the oracle itself."""
+import ctypes
+
+import pytest
+import torch
+
+from kairos_sensenova_b200 import KVCache, _lib, attention_cached, attention_prompt, kv_cache_append, kv_cache_gather
+from kairos_sensenova_b200.kv_cache import _index, _rows, check_tables
+from oracle import serving as ref
+
+i32 = lambda x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+
+
+def test_cache_refuses_other_layouts():
+    k, s = torch.zeros(4, 2, 16, 64, dtype=torch.uint8), torch.ones(4, 2)
+    c = KVCache(k, k.clone(), s, s.clone())
+    assert (c.num_pages, c.num_heads, c.page_size, c.head_dim) == (4, 2, 16, 64)
+    assert KVCache.empty(3, 2, 128, 32, device='cpu').k_pages.dtype == torch.float8_e4m3fn
+    for bad in ((k[0], k[0], s, s), (k, k[:3], s, s), (k, k, s[:3], s), (k, k, s.double(), s), (k.float(), k, s, s),
+                (k[:, :, :8], k[:, :, :8], s, s), (k[..., :32], k[..., :32], s, s), (k.transpose(0, 1), k.transpose(0, 1), s.T, s.T),
+                (k[:0], k[:0], s[:0], s[:0]), (torch.zeros(4, 2, 64, 16, dtype=torch.uint8).transpose(2, 3),) * 2 + (s, s)):
+        with pytest.raises(ValueError, match='KVCache'):
+            KVCache(*bad)
+
+
+def test_operators_refuse_cpu_tensors():
+    c = KVCache.empty(3, 2, 64, 16, device='cpu')
+    x = torch.zeros(4, 2, 64, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match='CUDA'):
+        attention_prompt(x, x, x, i32([0, 4]))
+    with pytest.raises(RuntimeError, match='CUDA'):
+        kv_cache_append(c, x, x, i32([[0]]), i32([4]), i32([0, 4]))
+    with pytest.raises(RuntimeError, match='CUDA'):
+        kv_cache_gather(c, i32([[0]]), i32([0]), i32([0, 4]), 4)
+    with pytest.raises(RuntimeError, match='CUDA'):
+        attention_cached(x[None], c, i32([[0]]), i32([4]))
+
+
+def test_index_and_rows():
+    cpu = torch.device('cpu')
+    assert _index(torch.tensor([1, 2]), (2,), 'x', 'y', cpu).dtype == torch.int32
+    for bad in (torch.zeros(3), torch.zeros(2, 2, dtype=torch.int32), torch.zeros(3, dtype=torch.int16)):
+        with pytest.raises(ValueError, match='x: y'):
+            _index(bad, (3,), 'x', 'y', cpu)
+    x = torch.zeros(10, 6, 64, dtype=torch.bfloat16)
+    assert _rows(x[:, 2:4]) .data_ptr() == x[:, 2:4].data_ptr()
+    assert _rows(x[..., 1:]).is_contiguous() and _rows(x.transpose(1, 2)).is_contiguous()
+
+
+def test_check_tables():
+    c = KVCache.empty(4, 1, 64, 16, device='cpu')
+    check_tables(c, i32([[0, 1], [2, -1]]), i32([32, 16]))
+    check_tables(c, i32([[0, -1]]), i32([0]))
+    check_tables(c, i32([[-1, 1]]), i32([20]), first=i32([16]))
+    for table, last, first in (([[0, 1]], [33], None), ([[0, 4]], [17], None), ([[0, -1]], [17], None), ([[0, 1]], [-1], None),
+                               ([[0, 1]], [3], i32([-1]))):
+        with pytest.raises(ValueError):
+            check_tables(c, i32(table), i32(last), first=first)
+    with pytest.raises(ValueError, match='twice'):
+        check_tables(c, i32([[0, 1], [1, 0]]), i32([17, 17]), first=i32([16, 16]) - 1, unique=True)
+
+
+def test_c_entries_refuse():
+    L = _lib.lib()
+    cache = lambda **kw: ctypes.byref(_lib.KvCacheArgs(**{**dict(k_pages=16, v_pages=16, k_scale=16, v_scale=16, num_pages=4, H=2,  # noqa: E731
+                                                                page=16, D=64), **kw}))
+    app = lambda c, k=16, B=1, T=1, dt=0, ts=64: L.kb200_kv_append(c, k, 16, ts, 64, ts, 64, 16, 4, 16, 16, B, T, dt, None)  # noqa: E731
+    assert app(cache(), T=0) == 0 and app(cache(), B=0) == 0
+    for bad in (dict(D=96), dict(page=8), dict(page=48), dict(H=0), dict(num_pages=0), dict(k_pages=0), dict(num_pages=1 << 40)):
+        assert app(cache(**bad)) == 1, bad
+    assert app(cache(k_pages=8)) == 2 and app(cache(), k=24) == 2 and app(cache(), ts=65) == 2
+    assert app(cache(), dt=2) == 1 and app(cache(), T=-1) == 1 and app(cache(), k=None) == 1
+    assert L.kb200_kv_gather(cache(), 16, 4, 16, 16, 1, 0, None, None, 0, None) == 0
+    assert L.kb200_kv_gather(cache(), 16, 4, 16, 16, 1, 5, None, None, 0, None) == 1
+    assert L.kb200_kv_gather(cache(), 16, 4, 16, 16, 1, 5, 24, 16, 0, None) == 2
+    size = lambda *a: L.kb200_attn_cached_workspace_size(*a)  # noqa: E731
+    assert size(1, 1, 8, 2, 64, 16, 4) > 0 and size(1, 1, 7, 2, 64, 16, 4) == 0 and size(-1, 1, 8, 2, 64, 16, 4) == 0
+    att = lambda q=16, B=1, Hq=4, dt=0, ws=None, n=0, qs=64: L.kb200_attn_cached_fwd(  # noqa: E731
+        q, qs, qs, qs, cache(), 16, 4, 16, 16, None, B, 1, Hq, 1.0, dt, ws, n, None)
+    assert att(B=0) == 0 and att(Hq=3) == 1 and att(dt=5) == 1 and att(q=None) == 1 and att(q=8) == 2 and att(qs=4) == 2
+    assert att() == 3 and b'workspace' in L.kb200_last_error()
+    base = dict(q=16, k=16, v=16, o=16, cu_q=16, cu_k=16, Tq=4, Tk=4, N=1, Hq=4, Hkv=2, D=64, q_token_stride=64, softmax_scale=1.0)
+    pr = lambda **kw: L.kb200_attn_prompt_fwd(ctypes.byref(_lib.PromptArgs(**{**base, **kw})), None)  # noqa: E731
+    assert pr(N=0) == 0 and pr(Tq=0) == 0
+    for bad in (dict(D=96), dict(Hq=3), dict(Hkv=0), dict(Tq=-1), dict(dtype=2), dict(q=None), dict(k=None), dict(cu_k=None)):
+        assert pr(**bad) == 1, bad
+    assert pr(v=8) == 2 and pr(o_head_stride=4) == 2
+
+
+def test_oracle_rounds_as_torch_does():
+    x = torch.cat([torch.linspace(-448, 448, 20001), torch.linspace(-0.05, 0.05, 4001), 2.0 ** torch.linspace(-12, 8, 999)])
+    assert torch.equal(ref.round_e4m3(x).float(), x.to(torch.float8_e4m3fn).float())
+    a = torch.tensor([0.0, 448.0, 448.5, 3.5, 3.51, 1e-30, 1.0])
+    assert torch.equal(ref.scale_exponent(a), torch.tensor([-117, 0, 1, -7, -6, -108, -8], dtype=torch.int32))
+
+
+def test_oracle_attention_is_the_formula():
+    torch.manual_seed(0)
+    q, k, v = torch.randn(3, 8), torch.randn(5, 8), torch.randn(5, 8)
+    o, lse, A = ref.attend(q, k, v, torch.tensor([0, 2, 5]), 0.5)
+    assert (o[0] == 0).all() and lse[0] == -float('inf')
+    for i, n in ((1, 2), (2, 5)):
+        w = torch.softmax(q[i].double() @ k[:n].double().T * 0.5, 0)
+        assert torch.allclose(o[i], w @ v[:n].double()) and torch.allclose(A[i], w @ v[:n].double().abs())
+    v[4] = float('nan')
+    o2 = ref.attend(q, k, v, torch.tensor([0, 2, 5]), 0.5)[0]
+    assert torch.equal(o2[:2], o[:2]) and torch.isnan(o2[2]).all()
