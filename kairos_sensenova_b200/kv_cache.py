@@ -106,7 +106,7 @@ def _index(t, shape, what, name, dev):
 
 def _rows(t):
     """`t` itself if its rows can be read in 16-byte steps in place, else a contiguous copy."""
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in t.stride()[:-1]):
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 and s > 0 for s in t.stride()[:-1]):
         return t
     return t.contiguous()
 

@@ -96,11 +96,13 @@ def test_prompt_long(heads, kv, dim, dtype, n):
 @pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize('value', [math.nan, math.inf])
 def test_prompt_masked_values_do_not_leak(dtype, value):
-    """K and V of one token not finite: rows that do not see it, in its sequence and in the neighbours, are as without."""
+    """K and V of one token not finite: rows that do not see it, in its sequence and in the neighbours, keep within
+    the bound of the formula without it.  (Not the same bits: a tile that meets a NaN is summed in another order, so the
+    two results differ by up to the bound each has of the formula.)"""
     g = gen(3)
     nq = [200, 150, 90]
     q, k, v = (randn(g, sum(nq), 3, 128, dtype=dtype) for _ in range(3))
-    clean = attention_prompt(q, k, v, i32(cu(nq)))
+    want, _, A = ref.prompt(q, k, v, cu(nq), cu(nq), 128 ** -0.5)
     at = 200 + 100                                            # token 100 of the second sequence
     kb, vb = k.clone(), v.clone()
     vb[at, 1, 5] = value
@@ -109,14 +111,14 @@ def test_prompt_masked_values_do_not_leak(dtype, value):
     hit = torch.zeros_like(o, dtype=torch.bool)
     hit[at:350, 1, 5] = True
     hit[at:350, 2] = True
-    assert torch.equal(o[~hit], clean[~hit])
+    close(o[~hit], want[~hit], A[~hit], dtype)
     assert not torch.isfinite(o[at:350, 1, 5]).any()
     assert torch.isnan(o[at:350, 2]).all() or value == math.inf
     # the first token of the next sequence: the sequence before ends in the same key tile
     vb = v.clone()
     vb[350] = value
     o = attention_prompt(q, k, vb, i32(cu(nq)))
-    assert torch.equal(o[:350], clean[:350])
+    close(o[:350], want[:350], A[:350], dtype)
 
 
 def test_prompt_extremes():
