@@ -6,6 +6,7 @@ to load, :func:`lib` raises -- there is no CPU or eager fallback.
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from pathlib import Path
 
@@ -67,6 +68,11 @@ class PromptArgs(ctypes.Structure):
     ]
 
 
+# the same bytes packed directly (a ctypes structure of this many fields costs several times as much to fill)
+PROMPT_ARGS = struct.Struct('@7P14qfii4x')
+assert PROMPT_ARGS.size == ctypes.sizeof(PromptArgs)
+
+
 class KvCacheArgs(ctypes.Structure):
     """Mirror of ``KB200KvCache`` (include/kb200.h)."""
     _fields_ = [
@@ -106,7 +112,7 @@ SIGNATURES = {
                             [ctypes.c_float, ctypes.c_void_p]),
     'kb200_residual_ln_mod': (ctypes.c_int, [ctypes.c_void_p] * 2 + [ctypes.c_int64] * 3 +
                               [ctypes.c_void_p] * 3 + [ctypes.c_int, ctypes.c_float] + [ctypes.c_void_p] * 2),
-    'kb200_attn_prompt_fwd': (ctypes.c_int, [ctypes.POINTER(PromptArgs), ctypes.c_void_p]),
+    'kb200_attn_prompt_fwd': (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),   # PromptArgs or its packed bytes
     'kb200_kv_append': (ctypes.c_int, [ctypes.POINTER(KvCacheArgs)] + [ctypes.c_void_p] * 2 + [ctypes.c_int64] * 4 +
                         [ctypes.c_void_p, ctypes.c_int64] + [ctypes.c_void_p] * 2 + [ctypes.c_int64] * 2 +
                         [ctypes.c_int, ctypes.c_void_p]),

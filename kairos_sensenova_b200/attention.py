@@ -17,14 +17,11 @@ dilation is a rearrangement before this call); key tiles outside every window of
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 import torch.nn as nn
 
 from . import _lib
-from .kv_cache import _DTYPES, _forward_only, _index
-from .kv_cache import _rows as _kv_rows
+from .kv_cache import _DTYPES, _forward_only, _index, _launch, _rows
 
 
 def attention_fp8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, num_heads: int,
@@ -121,11 +118,13 @@ def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     dev = q.device
     if dev.type != 'cuda':
         raise RuntimeError(f'{what}: inputs must be CUDA tensors (no CPU path)')
-    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or k.shape[2] != q.shape[2] or k.shape[1] < 1 \
-            or q.shape[1] < 1 or q.shape[1] % k.shape[1]:
+    shape, kshape = q.shape, k.shape
+    if len(shape) != 3 or len(kshape) != 3 or v.shape != kshape or kshape[2] != shape[2] or kshape[1] < 1 \
+            or shape[1] < 1 or shape[1] % kshape[1]:
         raise ValueError(f'{what}: q must be [Tq, Hq, D] and k, v [Tk, Hkv, D] with Hq a multiple of Hkv, got '
-                         f'{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}')
-    if q.dtype not in _DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+                         f'{tuple(shape)}, {tuple(kshape)}, {tuple(v.shape)}')
+    dtype = _DTYPES.get(q.dtype)
+    if dtype is None or k.dtype is not q.dtype or v.dtype is not q.dtype:
         raise ValueError(f'{what}: q, k and v must all be bfloat16 or all float16, got {q.dtype}, {k.dtype}, {v.dtype}')
     if k.device != dev or v.device != dev:
         raise ValueError(f'{what}: q, k and v must be on one device')
@@ -135,24 +134,29 @@ def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         raise ValueError(f'{what}: cu_seqlens_q must be [N + 1], got {tuple(cu_seqlens_q.shape)}')
     cu_q = _index(cu_seqlens_q, (N + 1,), what, 'cu_seqlens_q', dev)
     cu_k = cu_q if cu_seqlens_k is None else _index(cu_seqlens_k, (N + 1,), what, 'cu_seqlens_k', dev)
+    Tq, Hq, D = shape
+    Tk, Hkv, _ = kshape
     if check:
-        for name, cu, T in (('cu_seqlens_q', cu_q, q.shape[0]), ('cu_seqlens_k', cu_k, k.shape[0])):
+        for name, cu, T in (('cu_seqlens_q', cu_q, Tq), ('cu_seqlens_k', cu_k, Tk)):
             at = cu.tolist()
             if at[0] != 0 or at[-1] > T or any(b < a for a, b in zip(at, at[1:])):
                 raise ValueError(f'{what}: {name} must rise from 0 to at most {T}')
-    Tq, Hq, D = q.shape
     if softmax_scale is None:
         softmax_scale = D ** -0.5
-    q, k, v = _kv_rows(q), _kv_rows(k), _kv_rows(v)
-    with torch.cuda.device(dev):
-        if out is None:
-            out = torch.empty(Tq, Hq, D, device=dev, dtype=q.dtype)
-        elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or _kv_rows(out) is not out:
-            raise ValueError(f'{what}: out must be {q.dtype} {list(q.shape)} on {dev}, its rows 16-byte aligned')
-        lse = torch.empty(Tq, Hq, device=dev, dtype=torch.float32) if return_lse else None
-        a = _lib.PromptArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(),
-                            cu_q.data_ptr(), cu_k.data_ptr(), Tq, k.shape[0], N, Hq, k.shape[1], D,
-                            q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-                            out.stride(0), out.stride(1), float(softmax_scale), int(bool(causal)), _DTYPES[q.dtype])
-        _lib.check(_lib.lib().kb200_attn_prompt_fwd(ctypes.byref(a), torch.cuda.current_stream(dev).cuda_stream), what)
+    q, qp, qs = _rows(q)
+    k, kp, ks = _rows(k)
+    v, vp, vs = _rows(v)
+    if out is None:
+        out = q.new_empty(shape)
+        op, os = out.data_ptr(), (Hq * D, D)
+    else:
+        same, op, os = _rows(out)
+        if out.shape != shape or out.dtype != q.dtype or out.device != dev or same is not out:
+            raise ValueError(f'{what}: out must be {q.dtype} {list(shape)} on {dev}, its rows 16-byte aligned')
+    lse = torch.empty((Tq, Hq), device=dev, dtype=torch.float32) if return_lse else None
+    args = _lib.PROMPT_ARGS.pack(
+        qp, kp, vp, op, lse.data_ptr() if return_lse else 0, cu_q.data_ptr(),
+        cu_k.data_ptr(), Tq, Tk, N, Hq, Hkv, D, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1], float(softmax_scale),
+        1 if causal else 0, dtype)
+    _launch(dev, what, _lib.lib().kb200_attn_prompt_fwd, args)
     return (out, lse) if return_lse else out

@@ -6,15 +6,16 @@
 // Bound: HBM, 2 D bytes per cached token and kv head.  Rows are the R = Sq * (Hq / Hkv)
 // queries that share a kv head, so the cache is read once for all of them.
 //
-// Split of the work: the tiles of 128 cached tokens of all (sequence, kv head, row
+// Split of the work: the groups of 16 (or 32) cached tokens of all (sequence, kv head, row
 // block) units are laid end to end and every CTA takes an equal, contiguous share; the
 // shares are computed on the device from the lengths, so ragged batches balance without
 // the host knowing them.  A unit inside one share is finished there; one that crosses
 // shares leaves a partial (m, l, O) per CTA, joined in share order (no atomics: the
-// result does not depend on timing) by a second kernel.
+// result does not depend on timing) by a second, dependent kernel.
 //
-// A CTA: one producer warp streams K and V pages by TMA (128-byte swizzle) into a ring
-// of 128-token stages; 8 consumer warps = key groups x row groups.  Per 16 tokens:
+// A CTA: one producer warp streams K and V by TMA; every consumer warp has a ring of its
+// own and takes every WK-th group, so a warp never waits for another one inside a unit.
+// Per 16 tokens:
 //   S^T = K Q^T  mma.m16n8k16 f16 (16 tokens x 8 rows), codes widened to f16 in
 //                registers (exact); the contraction index is permuted so that a lane's
 //                operands are 16 consecutive bytes of the page
@@ -30,9 +31,6 @@
 namespace kb {
 namespace cached {
 
-constexpr int TK = 128;            // tokens per stage
-constexpr int NW = 8;              // consumer warps
-constexpr int THREADS = (NW + 1) * 32;
 constexpr float SHIFT = 8.f;       // P = 2^(s - m + SHIFT), s <= m + TAU: below 2^12, inside f16
 constexpr float TAU = 4.f;         // O and l are rescaled when the maximum grows by more than this (log2 units)
 
@@ -45,8 +43,10 @@ struct Params {
   float* part;                     // [2 G][rows][D] partial O, then [2 G][rows][2] (m, l)
   int64_t q_bs, q_ts, q_hs;        // batch, token, head strides of q, elements
   int B, Sq, Hq, H, G, R;          // G = Hq / H query heads per kv head, R = Sq * G
-  int rblocks, rows;               // row blocks per (sequence, kv head), rows of a block
+  int rblocks;                     // row blocks per (sequence, kv head)
   int num_pages, max_pages, page;
+  int page_log2;
+  int box;                         // tokens of one TMA box: min(page, tokens of a group)
   float scale_log2;
 };
 
@@ -76,22 +76,25 @@ KB_DEVI int seq_len(const Params& p, int b) {
   const int64_t cap = (int64_t)p.max_pages * p.page;
   return (int)min(max((int64_t)p.lengths[b], (int64_t)0), min(cap, (int64_t)0x7fffff00));
 }
-KB_DEVI int seq_tiles(const Params& p, int b) { return (seq_len(p, b) + TK - 1) / TK; }
-
-// Sum of the tiles of all sequences, by one warp.
-KB_DEVI int64_t warp_total_tiles(const Params& p, int lane) {
-  int64_t s = 0;
-  for (int b = lane; b < p.B; b += 32) s += seq_tiles(p, b);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  return s;
+// Groups of GT tokens of sequence b, and the length that each of its units takes in the flat
+// order: PAD more, positions without work that stand for what a segment costs apart from
+// its groups (Q, the join, the stores), so that shares of many short units balance too.
+constexpr int PAD = 8;
+template <int GT>
+KB_DEVI int seq_groups(const Params& p, int b) { return (seq_len(p, b) + GT - 1) / GT; }
+template <int GT>
+KB_DEVI int seq_span(const Params& p, int b) {
+  const int n = seq_groups<GT>(p, b);
+  return n ? n + PAD : 0;
 }
-// Sequence that holds the flat tile position `at` (tiles of one sequence: units * seq_tiles),
-// and the position where it begins; by one warp.  at < total.
+
+// Flat position (a sequence takes units * seq_span) -> the sequence that holds
+// it and the position where that begins; by one warp.  at < total.
+template <int GT>
 KB_DEVI void warp_find(const Params& p, int64_t units, int64_t at, int lane, int& b_out, int64_t& begin_out) {
   int64_t base = 0;
   for (int b0 = 0; b0 < p.B; b0 += 32) {
-    const int64_t mine = b0 + lane < p.B ? units * seq_tiles(p, b0 + lane) : 0;
+    const int64_t mine = b0 + lane < p.B ? units * seq_span<GT>(p, b0 + lane) : 0;
     int64_t inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -111,28 +114,82 @@ KB_DEVI void warp_find(const Params& p, int64_t units, int64_t at, int lane, int
   begin_out = base;
 }
 
-// What a CTA works on: shares of `per` flat tiles, CTA c has [c * per, (c + 1) * per).
+// CTA c works on the flat positions [c * per, (c + 1) * per): a multiple of the consumer warps.
 struct Share {
   int64_t total, per;
 };
-KB_DEVI Share share_of(const Params& p, int64_t units, int64_t sum_tiles, int ctas) {
+KB_DEVI Share share_of(int64_t units, int64_t sum_spans, int ctas, int wk) {
   Share s;
-  s.total = sum_tiles * units;
-  s.per = (s.total + ctas - 1) / ctas;
+  s.total = sum_spans * units;
+  s.per = (s.total + (int64_t)ctas * wk - 1) / ((int64_t)ctas * wk) * wk;
   return s;
 }
 
-template <int D, int NT, int WR, int STAGES>
+// The launch shapes.  NT: 8-row tiles of a CTA (rows up to 8: 1, else 2); a group is NT * 16
+// tokens.  WK consumer warps and their producer, OCC CTAs per SM: as many warps as the
+// registers allow (8 rows need under 128 at D = 128, 16 rows under 168).
+template <int D, int NT>
+struct Shape {
+  static constexpr int GT = NT * 16, ROWS = NT * 8;
+  static constexpr int WK = D == 128 && NT == 2 ? 11 : 7;
+  static constexpr int OCC = D == 128 ? (NT == 1 ? 2 : 1) : (NT == 1 ? 3 : 2);
+  static constexpr int STAGES = D == 128 ? (NT == 1 ? 3 : 2) : (NT == 1 ? 4 : 3);
+  static constexpr int THREADS = (WK + 1) * 32;
+  static constexpr int MAXBOX = NT;          // boxes of a group: GT / box, box at least 16
+};
+
+// A CTA's segments, in order: the groups [g0, g0 + count) of unit (b, h, rb); `ng` are all of
+// the unit's.  (Parts of a share that are padding alone are passed over.)
+template <int GT>
+struct Walk {
+  int64_t left;                        // flat positions still to come
+  int b, u, x;                         // the next one: sequence, unit, position in the unit
+  int h, rb, len, ng, g0, count;
+  KB_DEVI Walk(const Params& p, int64_t at, int64_t end, int b_, int64_t begin) : left(end - at), b(b_) {
+    const int span = seq_span<GT>(p, b);
+    u = (int)((at - begin) / span);
+    x = (int)((at - begin) - (int64_t)u * span);
+  }
+  KB_DEVI bool next(const Params& p, int units) {
+    while (left > 0) {
+      len = seq_len(p, b);
+      ng = (len + GT - 1) / GT;
+      if (ng == 0 || u == units) {
+        ++b;
+        u = x = 0;
+        continue;
+      }
+      const int take = (int)min((int64_t)(ng + PAD - x), left);
+      left -= take;
+      g0 = x;
+      count = min(x + take, ng) - x;
+      h = u / p.rblocks;
+      rb = u - h * p.rblocks;
+      x += take;
+      if (x == ng + PAD) {
+        x = 0;
+        ++u;
+      }
+      if (count > 0) return true;
+    }
+    return false;
+  }
+};
+
+template <int D, int NT>
 struct Smem {
-  static constexpr int ROWS = NT * 8 * WR;
-  uint8_t k[STAGES][TK * D];       // swizzled page rows
-  uint8_t v[STAGES][TK * D];
-  float o[NW / WR][ROWS][D];       // the warps' O, joined at the end of a unit
-  float ml[NW / WR][ROWS][2];
-  float sk[STAGES][TK / 16], sv[STAGES][TK / 16];   // page scales of 16-token groups; sk < 0: no such page
-  uint64_t full[STAGES], empty[STAGES];
+  using S = Shape<D, NT>;
+  struct Slot {
+    uint8_t k[S::GT * D], v[S::GT * D];      // swizzled page rows
+  };
+  static_assert(sizeof(Slot) == S::ROWS * D * sizeof(float), "a slot also holds a warp's O");
+  Slot slot[S::WK][S::STAGES];
+  float ml[S::WK][S::ROWS][2];
+  float2 scale[S::WK][S::STAGES][S::MAXBOX]; // page scales (k, v) of each box; k < 0: no such page
+  uint64_t full[S::WK][S::STAGES], empty[S::WK][S::STAGES];
   int64_t total, begin;
   int first_b;
+  int held[S::WK];                           // the slot that holds the warp's O, -1: none
   int abort_flag;
 };
 
@@ -143,30 +200,39 @@ KB_DEVI uint32_t swz(int r, int c) {
   else return (uint32_t)(r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
 }
 
-template <int D, bool F16, int NT, int WR, int STAGES, int OCC>
-__global__ void __launch_bounds__(THREADS, OCC) attn_cached_kernel(const __grid_constant__ Maps maps, Params p) {
-  using SM = Smem<D, NT, WR, STAGES>;
-  constexpr int WK = NW / WR, ROWS = SM::ROWS;
+template <int D, bool F16, int NT>
+__global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
+    attn_cached_kernel(const __grid_constant__ Maps maps, Params p) {
+  using S = Shape<D, NT>;
+  using SM = Smem<D, NT>;
+  constexpr int WK = S::WK, STAGES = S::STAGES, GT = S::GT, ROWS = S::ROWS;
   constexpr int MT = D / 16;               // 16-wide tiles of D
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   SM& sm = *reinterpret_cast<SM*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t units = (int64_t)p.H * p.rblocks;
+  const int boxes = GT / p.box;
 
-  if (tid == 0) {
-    for (int s = 0; s < STAGES; ++s) {
-      tc::mbar_init(&sm.full[s], 32);
-      tc::mbar_init(&sm.empty[s], NW);
+  if (warp == WK) {
+    for (int i = lane; i < WK * STAGES; i += 32) {
+      tc::mbar_init(&sm.full[0][0] + i, boxes);
+      tc::mbar_init(&sm.empty[0][0] + i, 1);
     }
-    sm.abort_flag = 0;
+    if (lane == 0) {
+      sm.abort_flag = 0;
+      tc::prefetch_tmap(&maps.k);
+      tc::prefetch_tmap(&maps.v);
+    }
     tc::fence_barrier_init();
-  }
-  if (warp == 0) {
-    const int64_t sum = warp_total_tiles(p, lane);
-    const Share sh = share_of(p, units, sum, gridDim.x);
+  } else if (warp == 0) {
+    int64_t sum = 0;
+    for (int b = lane; b < p.B; b += 32) sum += seq_span<GT>(p, b);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const Share sh = share_of(units, sum, gridDim.x, WK);
     int b = 0;
     int64_t begin = 0;
-    if ((int64_t)blockIdx.x * sh.per < sh.total) warp_find(p, units, blockIdx.x * sh.per, lane, b, begin);
+    if ((int64_t)blockIdx.x * sh.per < sh.total) warp_find<GT>(p, units, blockIdx.x * sh.per, lane, b, begin);
     if (lane == 0) {
       sm.total = sum;
       sm.first_b = b;
@@ -174,116 +240,144 @@ __global__ void __launch_bounds__(THREADS, OCC) attn_cached_kernel(const __grid_
     }
   }
   __syncthreads();
-  const Share sh = share_of(p, units, sm.total, gridDim.x);
+  const Share sh = share_of(units, sm.total, gridDim.x, WK);
   const int64_t at0 = (int64_t)blockIdx.x * sh.per, at1 = min(at0 + sh.per, sh.total);
+  // the join may be scheduled as soon as CTAs leave; it waits for all of them before it reads
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   if (at0 >= at1) return;
   auto aborted = [&]() { return *((volatile int*)&sm.abort_flag) != 0; };
 
-  // Every warp walks the CTA's segments (unit, tile range) in the same order.
-  int b = sm.first_b;
-  int64_t begin = sm.begin, at = at0;
-  int st = 0;                              // stage counter
-  int seg = 0;
-  if (warp == NW) {
+  // Every warp walks the CTA's segments in the same order.  Group i of a segment goes to
+  // consumer warp (i + rot) % WK, so that short segments use all of them in turn.
+  Walk<GT> seg(p, at0, at1, sm.first_b, sm.begin);
+  int rot = 0;
+  if (warp == WK) {
     // ---------------------------------------------------------------- producer
-    if (lane == 0) {
-      tc::prefetch_tmap(&maps.k);
-      tc::prefetch_tmap(&maps.v);
-    }
+    // Lane w * boxes + i loads box i of consumer warp w's groups.  A round gives every warp
+    // one group.  Page ids are read AHEAD rounds before their use and scales half of that,
+    // across segments: with one round ahead the producer took a loaded memory latency per
+    // round and the CTA no more than 4 KB * WK in that time.
+    constexpr int AHEAD = 6, HALF = 3;
+    struct Round {
+      int state;                           // 0: the work is over, 1: no group for this lane, 2: a group
+      int pg, h, off;                      // its page in the pool (-1: none), head, first row in the page
+    };
+    const int w = lane / boxes, bi = lane % boxes;
+    int i0 = 0, base = 0;                  // rounds of the current segment begin at group i0; rot at its start
+    bool live = seg.next(p, (int)units);
+    auto next_round = [&]() {
+      Round r{0, -1, 0, 0};
+      if (live && i0 >= seg.count) {
+        base = (base + seg.count) % WK;
+        i0 = 0;
+        live = seg.next(p, (int)units);
+      }
+      if (!live) return r;
+      r.state = 1;
+      const int i = i0 + (w >= base ? w - base : w + WK - base);
+      i0 += WK;
+      if (w < WK && i < seg.count) {
+        r.state = 2;
+        const int tok = (seg.g0 + i) * GT + bi * p.box, pi = tok >> p.page_log2;
+        r.off = tok & (p.page - 1);
+        r.h = seg.h;
+        if (tok < seg.len) r.pg = __ldg(p.table + (int64_t)seg.b * p.max_pages + pi);
+      }
+      return r;
+    };
+    auto scale_of = [&](const Round& r) {
+      float2 s = make_float2(-1.f, 0.f);
+      if (r.pg >= 0 && r.pg < p.num_pages) {
+        s.x = __ldg(p.k_scale + (int64_t)r.pg * p.H + r.h);
+        s.y = __ldg(p.v_scale + (int64_t)r.pg * p.H + r.h);
+      }
+      return s;
+    };
+    int it = 0;                            // groups of this lane's ring
     bool ok = true;
-    const int per_stage = TK / p.page, gpp = p.page / 16;
-    while (at < at1 && ok) {
-      int nt = seq_tiles(p, b);
-      while (nt == 0 || at >= begin + units * nt) {
-        begin += units * nt;
-        nt = seq_tiles(p, ++b);
-      }
-      const int len = seq_len(p, b), npages = (len + p.page - 1) / p.page;
-      const int u = (int)((at - begin) / nt), t0 = (int)((at - begin) % nt);
-      const int t1 = (int)min((int64_t)nt, t0 + (at1 - at));
-      const int h = u / p.rblocks;
-      const int32_t* row = p.table + (int64_t)b * p.max_pages;
-      // lane i < per_stage holds page i of the stage
-      const int pi0 = t0 * per_stage + lane;
-      int next = lane < per_stage && pi0 < npages ? __ldg(row + pi0) : -1;
-      for (int t = t0; t < t1; ++t, ++st) {
-        const int pg = next;
-        const int pn = (t + 1) * per_stage + lane;
-        next = t + 1 < t1 && lane < per_stage && pn < npages ? __ldg(row + pn) : -1;
-        const bool have = pg >= 0 && pg < p.num_pages;
-        float ks = -1.f, vs = 0.f;
-        if (have) {
-          ks = __ldg(p.k_scale + (int64_t)pg * p.H + h);
-          vs = __ldg(p.v_scale + (int64_t)pg * p.H + h);
-        }
-        const int s = st % STAGES;
-        if (st >= STAGES && !tc::mbar_wait(&sm.empty[s], (st / STAGES - 1) & 1)) { sm.abort_flag = 1; ok = false; }
-        ok = __all_sync(0xffffffffu, ok) && !aborted();
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        if (lane < per_stage)
-          for (int g = 0; g < gpp; ++g) {
-            sm.sk[s][lane * gpp + g] = ks;
-            sm.sv[s][lane * gpp + g] = vs;
+    Round r[AHEAD];
+    float2 sc[HALF];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) r[i] = next_round();
+#pragma unroll
+    for (int i = 0; i < HALF; ++i) sc[i] = scale_of(r[i]);
+    while (r[0].state) {
+      if (r[0].state == 2 && ok) {
+        const int s = it % STAGES;
+        if (it >= STAGES && !tc::mbar_wait(&sm.empty[w][s], (it / STAGES - 1) & 1)) { sm.abort_flag = 1; ok = false; }
+        if (aborted()) ok = false;
+        if (ok) {
+          typename SM::Slot& sl = sm.slot[w][s];
+          if (r[0].pg >= 0 && r[0].pg < p.num_pages) {
+            const int y = (r[0].pg * p.H + r[0].h) * p.page + r[0].off;
+            tc::mbar_expect_tx_only(&sm.full[w][s], (uint32_t)(2 * p.box * D));
+            tc::tma_load_2d(sl.k + bi * p.box * D, &maps.k, &sm.full[w][s], 0, y);
+            tc::tma_load_2d(sl.v + bi * p.box * D, &maps.v, &sm.full[w][s], 0, y);
           }
-        const int loads = __popc(__ballot_sync(0xffffffffu, have));
-        if (lane == 0) tc::mbar_expect_tx(&sm.full[s], (uint32_t)(loads * 2 * p.page * D));
-        __syncwarp();
-        if (have) {
-          const int y = (pg * p.H + h) * p.page;
-          tc::tma_load_2d(sm.k[s] + lane * p.page * D, &maps.k, &sm.full[s], 0, y);
-          tc::tma_load_2d(sm.v[s] + lane * p.page * D, &maps.v, &sm.full[s], 0, y);
+          sm.scale[w][s][bi] = sc[0];
+          tc::mbar_arrive(&sm.full[w][s]);
+          ++it;
         }
-        if (lane != 0) tc::mbar_arrive(&sm.full[s]);
       }
-      at += t1 - t0;
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+#pragma unroll
+      for (int i = 0; i + 1 < HALF; ++i) sc[i] = sc[i + 1];
+      sc[HALF - 1] = scale_of(r[HALF]);
+#pragma unroll
+      for (int i = 0; i + 1 < AHEAD; ++i) r[i] = r[i + 1];
+      r[AHEAD - 1] = next_round();
     }
+    const bool mine = w < WK;
     // every load lands before the CTA may exit
-    for (int i = st > STAGES ? st - STAGES : 0; i < st; ++i) tc::mbar_wait(&sm.full[i % STAGES], (i / STAGES) & 1);
+    if (mine)
+      for (int i = it > STAGES ? it - STAGES : 0; i < it; ++i) tc::mbar_wait(&sm.full[w][i % STAGES], (i / STAGES) & 1);
     return;
   }
 
   // ------------------------------------------------------------------ consumers
-  const int wk = warp / WR, wr = warp % WR;
   const int g = lane >> 2, t4 = lane & 3;
-  for (; at < at1; ++seg) {
-    int nt = seq_tiles(p, b);
-    while (nt == 0 || at >= begin + units * nt) {
-      begin += units * nt;
-      nt = seq_tiles(p, ++b);
-    }
-    const int len = seq_len(p, b);
-    const int u = (int)((at - begin) / nt), t0 = (int)((at - begin) % nt);
-    const int t1 = (int)min((int64_t)nt, t0 + (at1 - at));
-    const int h = u / p.rblocks, rb = u % p.rblocks;
-
-    // Q^T operands of this warp's rows: row n = g of each 8-row tile, this lane's D / 4
-    // channels (t4 * 32 + ... for D = 128), as f16 under a power of two per row.
-    constexpr int CH = D / 64;             // 16-byte code chunks per lane and row
-    uint32_t qf[NT][CH * 8];
-    float qs[NT][2];                       // log2-domain score factors of the rows 2 t4, 2 t4 + 1
+  int it = 0;
+  constexpr int CH = D / 64;               // 16-byte code chunks per lane and row
+  uint32_t raw[NT][CH * 8];                // the segment's Q, read while the one before is joined
+  auto load_q = [&]() {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int r = rb * p.rows + (wr * NT + n) * 8 + g;
-      float amax = 0.f;
-      uint32_t raw[CH * 8];
+      const int r = seg.rb * ROWS + n * 8 + g;
       const bool in = r < p.R;
       const char* src = reinterpret_cast<const char*>(p.q);
-      if (in) src += 2 * ((int64_t)b * p.q_bs + (int64_t)(r / p.G) * p.q_ts + (int64_t)(h * p.G + r % p.G) * p.q_hs +
+      if (in) src += 2 * ((int64_t)seg.b * p.q_bs + (int64_t)(r / p.G) * p.q_ts + (int64_t)(seg.h * p.G + r % p.G) * p.q_hs +
                           t4 * (CH * 16));
 #pragma unroll
       for (int c = 0; c < CH * 2; ++c) {
         const uint4 x = in ? __ldg(reinterpret_cast<const uint4*>(src) + c) : make_uint4(0, 0, 0, 0);
-        raw[4 * c] = x.x; raw[4 * c + 1] = x.y; raw[4 * c + 2] = x.z; raw[4 * c + 3] = x.w;
+        raw[n][4 * c] = x.x; raw[n][4 * c + 1] = x.y; raw[n][4 * c + 2] = x.z; raw[n][4 * c + 3] = x.w;
       }
+    }
+  };
+  bool live = seg.next(p, (int)units);
+  if (live) load_q();
+  while (live) {
+    const int b = seg.b, h = seg.h, rb = seg.rb, len = seg.len, g0 = seg.g0, count = seg.count;
+    const bool whole = g0 == 0 && count == seg.ng;
+    const int gi0 = warp >= rot ? warp - rot : warp + WK - rot;   // this warp's first group
+    rot = (rot + count) % WK;
+
+    // Q^T operands: row n = g of each 8-row tile, this lane's D / 4 channels from t4 * D / 4, as
+    // f16 under a power of two per row.
+    uint32_t qf[NT][CH * 8];
+    float qs[NT][2];                       // log2-domain score factors of the rows 2 t4, 2 t4 + 1
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
       float f = 1.f;
       if constexpr (F16) {
 #pragma unroll
-        for (int c = 0; c < CH * 8; ++c) qf[n][c] = raw[c];
+        for (int c = 0; c < CH * 8; ++c) qf[n][c] = raw[n][c];
       } else {
+        float amax = 0.f;
 #pragma unroll
         for (int c = 0; c < CH * 8; ++c) {
-          const float2 x = unpack_bf16(raw[c]);
+          const float2 x = unpack_bf16(raw[n][c]);
           if (fabsf(x.x) < INFINITY) amax = fmaxf(amax, fabsf(x.x));
           if (fabsf(x.y) < INFINITY) amax = fmaxf(amax, fabsf(x.y));
         }
@@ -294,7 +388,7 @@ __global__ void __launch_bounds__(THREADS, OCC) attn_cached_kernel(const __grid_
         f = kv::pow2(e);
 #pragma unroll
         for (int c = 0; c < CH * 8; ++c) {
-          const float2 x = unpack_bf16(raw[c]);
+          const float2 x = unpack_bf16(raw[n][c]);
           qf[n][c] = kv::pack16<true>(x.x * down, x.y * down);
         }
       }
@@ -312,7 +406,7 @@ __global__ void __launch_bounds__(THREADS, OCC) attn_cached_kernel(const __grid_
       for (int c = 0; c < 2; ++c) {
         m[n][c] = -INFINITY;
         l[n][c] = 0.f;
-        const int r = rb * p.rows + (wr * NT + n) * 8 + 2 * t4 + c;
+        const int r = rb * ROWS + n * 8 + 2 * t4 + c;
         seen[n][c] = r < p.R ? len - p.Sq + 1 + r / p.G : len;
       }
 #pragma unroll
@@ -322,84 +416,107 @@ __global__ void __launch_bounds__(THREADS, OCC) attn_cached_kernel(const __grid_
     }
     const int all_seen = len - p.Sq + 1;   // keys below are seen by every row
 
-    for (int t = t0; t < t1; ++t, ++st) {
-      const int s = st % STAGES;
-      const bool ok = tc::mbar_wait(&sm.full[s], (st / STAGES) & 1);
+    int held = -1;
+    for (int gi = gi0; gi < count; gi += WK, ++it) {
+      const int s = it % STAGES;
+      const bool ok = tc::mbar_wait(&sm.full[warp][s], (it / STAGES) & 1);
       if (!ok) sm.abort_flag = 1;
-      if (__any_sync(0xffffffffu, !ok)) break;
-#pragma unroll 1
-      for (int kg = wk; kg < TK / 16; kg += WK) {
-        const int tok0 = t * TK + kg * 16;
-        const float sk = sm.sk[s][kg], sv = sm.sv[s][kg];
-        if (tok0 >= len || sk < 0.f) continue;
-        // ---- S^T = K Q^T
-        float acc[NT][4];
+      if (__any_sync(0xffffffffu, !ok || aborted())) break;
+      const typename SM::Slot& sl = sm.slot[warp][s];
+      const int base = (g0 + gi) * GT;
+      float sk[NT], sv[NT];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-        const uint8_t* kb = sm.k[s];
+      for (int j = 0; j < NT; ++j) {
+        const float2 sc = sm.scale[warp][s][j * 16 / p.box];
+        sk[j] = sc.x;
+        sv[j] = sc.y;
+      }
+      // ---- S^T = K Q^T of the group's 16-token parts
+      float acc[NT][NT][4];                // [part][row tile]
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[j][n][0] = acc[j][n][1] = acc[j][n][2] = acc[j][n][3] = 0.f;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-          const int r0 = kg * 16 + g;
-          const uint4 x0 = *reinterpret_cast<const uint4*>(kb + swz<D>(r0, t4 * CH + c));
-          const uint4 x1 = *reinterpret_cast<const uint4*>(kb + swz<D>(r0 + 8, t4 * CH + c));
+          const int r0 = j * 16 + g;
+          const uint4 x0 = *reinterpret_cast<const uint4*>(sl.k + swz<D>(r0, t4 * CH + c));
+          const uint4 x1 = *reinterpret_cast<const uint4*>(sl.k + swz<D>(r0 + 8, t4 * CH + c));
           const uint32_t w0[4] = {x0.x, x0.y, x0.z, x0.w}, w1[4] = {x1.x, x1.y, x1.z, x1.w};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const uint32_t a[4] = {kv::decode2(w0[e] & 0xffff), kv::decode2(w1[e] & 0xffff), kv::decode2(w0[e] >> 16),
-                                   kv::decode2(w1[e] >> 16)};
+            uint32_t a[4];
+            kv::decode4(w0[e], a[0], a[2]);
+            kv::decode4(w1[e], a[1], a[3]);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) mma_f16(acc[n], a, qf[n][c * 8 + 2 * e], qf[n][c * 8 + 2 * e + 1]);
+            for (int n = 0; n < NT; ++n) mma_f16(acc[j][n], a, qf[n][c * 8 + 2 * e], qf[n][c * 8 + 2 * e + 1]);
           }
         }
-        // ---- softmax; lane: tokens g, g + 8 of rows 2 t4, 2 t4 + 1
-        const bool edge = tok0 + 16 > all_seen;
-        uint32_t pf[NT][2];
+      }
+      // ---- softmax; lane: tokens g, g + 8 of each part, rows 2 t4, 2 t4 + 1
+      const bool edge = base + GT > all_seen;
+      uint32_t pf[NT][NT][2];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float x[4];
+      for (int n = 0; n < NT; ++n) {
+        float t0m = -INFINITY, t1m = -INFINITY;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = acc[n][e] * (sk * qs[n][e & 1]);
+        for (int j = 0; j < NT; ++j) {
+          float* x = acc[j][n];
+          const bool gone = sk[j] < 0.f;   // a missing page
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[e] *= sk[j] * qs[n][e & 1];
+            if (gone) x[e] = -INFINITY;
+          }
           if (edge) {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if (tok0 + g + (e >> 1) * 8 >= seen[n][e & 1]) x[e] = -INFINITY;
+              if (base + j * 16 + g + (e >> 1) * 8 >= seen[n][e & 1]) x[e] = -INFINITY;
           }
-          float t0m = fmaxf(x[0], x[2]), t1m = fmaxf(x[1], x[3]);
+          t0m = fmaxf(t0m, fmaxf(x[0], x[2]));
+          t1m = fmaxf(t1m, fmaxf(x[1], x[3]));
+        }
 #pragma unroll
-          for (int w = 4; w < 32; w <<= 1) {
-            t0m = fmaxf(t0m, __shfl_xor_sync(0xffffffffu, t0m, w));
-            t1m = fmaxf(t1m, __shfl_xor_sync(0xffffffffu, t1m, w));
-          }
-          const bool grow = t0m > m[n][0] + TAU || t1m > m[n][1] + TAU;
-          if (__any_sync(0xffffffffu, grow)) {
-            const float n0 = fmaxf(m[n][0], t0m), n1 = fmaxf(m[n][1], t1m);
-            const float a0 = n0 == -INFINITY ? 1.f : ex2(m[n][0] - n0), a1 = n1 == -INFINITY ? 1.f : ex2(m[n][1] - n1);
-            m[n][0] = n0; m[n][1] = n1;
-            l[n][0] *= a0; l[n][1] *= a1;
+        for (int w = 4; w < 32; w <<= 1) {
+          t0m = fmaxf(t0m, __shfl_xor_sync(0xffffffffu, t0m, w));
+          t1m = fmaxf(t1m, __shfl_xor_sync(0xffffffffu, t1m, w));
+        }
+        const bool grow = t0m > m[n][0] + TAU || t1m > m[n][1] + TAU;
+        if (__any_sync(0xffffffffu, grow)) {
+          const float n0 = fmaxf(m[n][0], t0m), n1 = fmaxf(m[n][1], t1m);
+          const float a0 = n0 == -INFINITY ? 1.f : ex2(m[n][0] - n0), a1 = n1 == -INFINITY ? 1.f : ex2(m[n][1] - n1);
+          m[n][0] = n0; m[n][1] = n1;
+          l[n][0] *= a0; l[n][1] *= a1;
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-              o[n][i][0] *= a0; o[n][i][1] *= a1; o[n][i][2] *= a0; o[n][i][3] *= a1;
-            }
+          for (int i = 0; i < MT; ++i) {
+            o[n][i][0] *= a0; o[n][i][1] *= a1; o[n][i][2] *= a0; o[n][i][3] *= a1;
           }
-          const float b0 = m[n][0] == -INFINITY ? 0.f : SHIFT - m[n][0], b1 = m[n][1] == -INFINITY ? 0.f : SHIFT - m[n][1];
+        }
+        const float b0 = m[n][0] == -INFINITY ? 0.f : SHIFT - m[n][0], b1 = m[n][1] == -INFINITY ? 0.f : SHIFT - m[n][1];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const float* x = acc[j][n];
           const float p0 = ex2(x[0] + b0), p1 = ex2(x[1] + b1), p2 = ex2(x[2] + b0), p3 = ex2(x[3] + b1);
           l[n][0] += p0 + p2;
           l[n][1] += p1 + p3;
-          pf[n][0] = transpose8(kv::pack16<true>(p0, p1));
-          pf[n][1] = transpose8(kv::pack16<true>(p2, p3));
+          pf[j][n][0] = transpose8(kv::pack16<true>(p0, p1));
+          pf[j][n][1] = transpose8(kv::pack16<true>(p2, p3));
         }
-        // ---- O^T += sv V^T P^T; lane: tokens 2 t4, +1, +8, +9, channels g * D/8 ...
-        const uint8_t* vb = sm.v[s];
-        constexpr int VW = D / 32;         // 32-bit words of channels per lane
+      }
+      // ---- O^T += sv V^T P^T; lane: tokens 2 t4, +1, +8, +9, channels g * D/8 ...
+      constexpr int VW = D / 32;           // 32-bit words of channels per lane
+#pragma unroll
+      for (int part = 0; part < NT; ++part) {
+        if (sk[part] < 0.f) continue;
         uint32_t vr[4][VW];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int r = kg * 16 + 2 * t4 + (j & 1) + (j >> 1) * 8;
+          const int r = part * 16 + 2 * t4 + (j & 1) + (j >> 1) * 8;
           if constexpr (D == 128) {
-            const uint4 x = *reinterpret_cast<const uint4*>(vb + swz<D>(r, g));
+            const uint4 x = *reinterpret_cast<const uint4*>(sl.v + swz<D>(r, g));
             vr[j][0] = x.x; vr[j][1] = x.y; vr[j][2] = x.z; vr[j][3] = x.w;
           } else {
-            const uint2 x = *reinterpret_cast<const uint2*>(vb + swz<D>(r, g >> 1) + (g & 1) * 8);
+            const uint2 x = *reinterpret_cast<const uint2*>(sl.v + swz<D>(r, g >> 1) + (g & 1) * 8);
             vr[j][0] = x.x; vr[j][1] = x.y;
           }
         }
@@ -407,7 +524,7 @@ __global__ void __launch_bounds__(THREADS, OCC) attn_cached_kernel(const __grid_
         if (edge) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const int tok = tok0 + 2 * t4 + (j & 1) + (j >> 1) * 8;
+            const int tok = base + part * 16 + 2 * t4 + (j & 1) + (j >> 1) * 8;
 #pragma unroll
             for (int w = 0; w < VW; ++w) {
               if (tok >= len) vr[j][w] = 0;      // behind the sequence: never looked at
@@ -424,7 +541,9 @@ __global__ void __launch_bounds__(THREADS, OCC) attn_cached_kernel(const __grid_
 #pragma unroll
           for (int z = 0; z < 2; ++z) {
             const uint32_t u01 = z ? hi01 : lo01, u89 = z ? hi89 : lo89;
-            uint32_t a[4] = {kv::decode2(u01 & 0xffff), kv::decode2(u01 >> 16), kv::decode2(u89 & 0xffff), kv::decode2(u89 >> 16)};
+            uint32_t a[4];
+            kv::decode4(u01, a[0], a[1]);
+            kv::decode4(u89, a[2], a[3]);
             if (poison) {
               // a NaN value reaches only the rows that see its token: it is taken out of the
               // product, and a second product counts the NaNs each row sees
@@ -440,7 +559,7 @@ __global__ void __launch_bounds__(THREADS, OCC) attn_cached_kernel(const __grid_
                 float cnt[4] = {0.f, 0.f, 0.f, 0.f};
                 float vis[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) vis[e] = tok0 + g + (e >> 1) * 8 < seen[n][e & 1] ? 1.f : 0.f;
+                for (int e = 0; e < 4; ++e) vis[e] = base + part * 16 + g + (e >> 1) * 8 < seen[n][e & 1] ? 1.f : 0.f;
                 mma_f16(cnt, bad, transpose8(kv::pack16<true>(vis[0], vis[1])), transpose8(kv::pack16<true>(vis[2], vis[3])));
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
@@ -450,96 +569,115 @@ __global__ void __launch_bounds__(THREADS, OCC) attn_cached_kernel(const __grid_
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               float d[4] = {0.f, 0.f, 0.f, 0.f};
-              mma_f16(d, a, pf[n][0], pf[n][1]);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) o[n][2 * w + z][e] = fmaf(d[e], sv, o[n][2 * w + z][e]);
+              mma_f16(d, a, pf[part][n][0], pf[part][n][1]);
+              float* oo = o[n][2 * w + z];
+              const float2 s2 = make_float2(sv[part], sv[part]);
+              const float2 o01 = ffma2(make_float2(d[0], d[1]), s2, make_float2(oo[0], oo[1]));
+              const float2 o23 = ffma2(make_float2(d[2], d[3]), s2, make_float2(oo[2], oo[3]));
+              oo[0] = o01.x; oo[1] = o01.y; oo[2] = o23.x; oo[3] = o23.y;
             }
           }
         }
       }
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&sm.empty[s]);
+      // the last slot of the segment is kept: it takes the warp's O
+      if (gi + WK < count) {
+        if (lane == 0) tc::mbar_arrive(&sm.empty[warp][s]);
+      } else {
+        held = s;
+      }
     }
-    at += t1 - t0;
-
-    // ---- the warps' partial results join: O of key group wk at sm.o[wk]
+    // ---- the warps' partial results join: each one's O in the slot it kept
+    if (held >= 0) {
+      float* mo = reinterpret_cast<float*>(&sm.slot[warp][held]);
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
+      for (int n = 0; n < NT; ++n) {
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        float x = l[n][c];
+        for (int c = 0; c < 2; ++c) {
+          float x = l[n][c];
 #pragma unroll
-        for (int w = 4; w < 32; w <<= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
-        const int r = (wr * NT + n) * 8 + 2 * t4 + c;
-        if (g == 0) {
-          sm.ml[wk][r][0] = m[n][c];
-          sm.ml[wk][r][1] = x;
-        }
+          for (int w = 4; w < 32; w <<= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
+          const int r = n * 8 + 2 * t4 + c;
+          if (g == 0) {
+            sm.ml[warp][r][0] = m[n][c];
+            sm.ml[warp][r][1] = x;
+          }
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          // channels g * D/8 + 2 i, + 1
-          *reinterpret_cast<float2*>(&sm.o[wk][r][g * (D / 8) + 2 * i]) = make_float2(o[n][i][c], o[n][i][2 + c]);
+          for (int i = 0; i < MT; ++i)       // channels g * D/8 + 2 i, + 1
+            *reinterpret_cast<float2*>(mo + r * D + g * (D / 8) + 2 * i) = make_float2(o[n][i][c], o[n][i][2 + c]);
         }
       }
     }
-    tc::bar_sync_named(1, NW * 32);
-    const bool whole = t0 == 0 && t1 == nt;
-    const bool bad = aborted();
-    const int slot = 2 * blockIdx.x + (t0 > 0 ? 0 : 1);   // a share's first segment may end a unit, its last may begin one
-    for (int i = tid; i < ROWS * (D / 4); i += NW * 32) {
+    if (lane == 0) sm.held[warp] = held;
+    live = seg.next(p, (int)units);
+    if (live) load_q();
+    tc::bar_sync_named(1, WK * 32);
+    const bool dead = aborted();
+    const int slot = 2 * blockIdx.x + (g0 > 0 ? 0 : 1);   // a share's first segment may end a unit, its last may begin one
+    for (int i = tid; i < ROWS * (D / 4); i += WK * 32) {
       const int r = i / (D / 4), c = i % (D / 4);
-      float mx = -INFINITY;
+      if (rb * ROWS + r >= p.R) break;     // rows in order: no more of them
+      float mk[WK], mx = -INFINITY;
 #pragma unroll
-      for (int k = 0; k < WK; ++k) mx = fmaxf(mx, sm.ml[k][r][0]);
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int k = 0; k < WK; ++k) {
+        mk[k] = sm.ml[k][r][0];
+        if (sm.held[k] >= 0) mx = fmaxf(mx, mk[k]);
+      }
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
       float ls = 0.f;
 #pragma unroll
       for (int k = 0; k < WK; ++k) {
-        // (m = -inf: no visible key, O and l are 0, or all of its scores are NaN, and so are they)
-        const float f = sm.ml[k][r][0] == -INFINITY ? 1.f : ex2(sm.ml[k][r][0] - mx);
-        const float4 x = *reinterpret_cast<const float4*>(&sm.o[k][r][c * 4]);
-        acc.x += f * x.x; acc.y += f * x.y; acc.z += f * x.z; acc.w += f * x.w;
-        ls += f * sm.ml[k][r][1];
+        const int hs = sm.held[k];
+        if (hs >= 0) {
+          // (m = -inf: no visible key, O and l are 0, or all of its scores are NaN, and so are they)
+          const float f = mk[k] == -INFINITY ? 1.f : ex2(mk[k] - mx);
+          const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(&sm.slot[k][hs]) + r * D + c * 4);
+          a.x += f * x.x; a.y += f * x.y; a.z += f * x.z; a.w += f * x.w;
+          ls += f * sm.ml[k][r][1];
+        }
       }
-      if (bad) acc = make_float4(NAN, NAN, NAN, NAN);
+      if (dead) a = make_float4(NAN, NAN, NAN, NAN);
       if (!whole) {
         float* dst = p.part + ((int64_t)slot * ROWS + r) * D + c * 4;
-        *reinterpret_cast<float4*>(dst) = acc;
+        *reinterpret_cast<float4*>(dst) = a;
         if (c == 0) {
           float* ml = p.part + (int64_t)2 * gridDim.x * ROWS * D + ((int64_t)slot * ROWS + r) * 2;
           ml[0] = mx;
-          ml[1] = ls;
+          ml[1] = dead ? 1.f : ls;
         }
       } else {
-        const int rr = rb * p.rows + r;
+        const int rr = rb * ROWS + r;
         if (rr < p.R) {
-          const float inv = ls > 0.f || ls != ls ? 1.f / ls : 0.f;
+          const float inv = dead || ls > 0.f || ls != ls ? 1.f / ls : 0.f;
           const int64_t orow = ((int64_t)b * p.Sq + rr / p.G) * p.Hq + h * p.G + rr % p.G;
           uint2 w;
-          w.x = kv::pack16<F16>(acc.x * inv, acc.y * inv);
-          w.y = kv::pack16<F16>(acc.z * inv, acc.w * inv);
+          w.x = kv::pack16<F16>(a.x * inv, a.y * inv);
+          w.y = kv::pack16<F16>(a.z * inv, a.w * inv);
           *reinterpret_cast<uint2*>(reinterpret_cast<char*>(p.o) + 2 * (orow * D + c * 4)) = w;
           if (c == 0 && p.lse) p.lse[orow] = ls == 0.f ? -INFINITY : (mx - SHIFT + log2f(ls)) * 0.6931471805599453f;
         }
       }
     }
-    tc::bar_sync_named(1, NW * 32);
+    tc::fence_proxy_async_smem();          // O's slots go back to the TMA
+    tc::bar_sync_named(1, WK * 32);
+    if (held >= 0 && lane == 0) tc::mbar_arrive(&sm.empty[warp][held]);
   }
 }
 
 // Joins the partials of the units that cross shares, and writes the empty sequences.
 // One block per (sequence, kv head, row block).
-template <int D, bool F16, int ROWS>
+template <int D, bool F16, int NT>
 __global__ void __launch_bounds__(128) attn_cached_join_kernel(Params p, int ctas) {
+  constexpr int GT = Shape<D, NT>::GT, ROWS = Shape<D, NT>::ROWS;
   const int lane = threadIdx.x & 31;
   const int64_t units = (int64_t)p.H * p.rblocks;
   const int b = (int)(blockIdx.x / units), u = (int)(blockIdx.x % units);
   const int h = u / p.rblocks, rb = u % p.rblocks;
-  const int nt = seq_tiles(p, b);
-  // tiles of the sequences before b, and of all (every warp for itself)
+  const int ng = seq_groups<GT>(p, b), span = seq_span<GT>(p, b);
+  // flat lengths of the sequences before b, and of all (every warp for itself)
   int64_t before = 0, sum = 0;
   for (int i = lane; i < p.B; i += 32) {
-    const int x = seq_tiles(p, i);
+    const int x = seq_span<GT>(p, i);
     sum += x;
     if (i < b) before += x;
   }
@@ -548,18 +686,19 @@ __global__ void __launch_bounds__(128) attn_cached_join_kernel(Params p, int cta
     sum += __shfl_xor_sync(0xffffffffu, sum, o);
     before += __shfl_xor_sync(0xffffffffu, before, o);
   }
-  const Share sh = share_of(p, units, sum, ctas);
+  const Share sh = share_of(units, sum, ctas, Shape<D, NT>::WK);
   int c0 = 0, c1 = -1;                     // CTAs whose shares hold a part of this unit
   int64_t begin = 0;
-  if (nt > 0) {
-    begin = before * units + (int64_t)u * nt;
+  if (ng > 0) {
+    begin = before * units + (int64_t)u * span;
     c0 = (int)(begin / sh.per);
-    c1 = (int)((begin + nt - 1) / sh.per);
+    c1 = (int)((begin + ng - 1) / sh.per);
     if (c0 == c1) return;                  // finished there
   }
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
   const float* mlp = p.part + (int64_t)2 * ctas * ROWS * D;
   for (int i = threadIdx.x; i < ROWS * (D / 4); i += 128) {
-    const int r = i / (D / 4), c = i % (D / 4), rr = rb * p.rows + r;
+    const int r = i / (D / 4), c = i % (D / 4), rr = rb * ROWS + r;
     if (rr >= p.R) break;
     float mx = -INFINITY, ls = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -585,51 +724,61 @@ __global__ void __launch_bounds__(128) attn_cached_join_kernel(Params p, int cta
   }
 }
 
-// Rows that a CTA takes: 8, 16, 32 or 64 of the R = Sq * Hq / Hkv.
-static int block_rows(int64_t R) { return R <= 8 ? 8 : R <= 16 ? 16 : R <= 32 ? 32 : 64; }
+// 8-row tiles that a CTA takes of the R = Sq * Hq / Hkv rows: rows above 16 form blocks that
+// read the cache again, mostly from L2 (more tiles per warp would not fit the registers).
+static int row_tiles(int64_t R) { return R <= 8 ? 1 : 2; }
 
 static int sm_count() {
+  static int counts[64];             // per device; written with the same value by every thread that gets there
   int dev = 0, n = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-  else cudaGetLastError();
+  if (cudaGetDevice(&dev) != cudaSuccess) { cudaGetLastError(); return n; }
+  if (dev < 64 && counts[dev]) return counts[dev];
+  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  if (dev < 64) counts[dev] = n;
   return n;
 }
 
-// CTAs of the main kernel: as many as fit on the GPU at once, no more than there can be tiles.
+// CTAs of the main kernel: as many as fit on the GPU at once, no more than can have work.
+template <int D, int NT>
 static int grid_of(int64_t B, int64_t H, int64_t R, int64_t max_tokens) {
-  const int rows = block_rows(R);
-  const int64_t most = B * H * ((R + rows - 1) / rows) * ((max_tokens + TK - 1) / TK);
-  const int64_t fit = (int64_t)sm_count() * (rows == 8 ? 2 : 1);
+  using S = Shape<D, NT>;
+  const int64_t most = (B * H * ((R + S::ROWS - 1) / S::ROWS) * ((max_tokens + S::GT - 1) / S::GT + PAD) + S::WK - 1) / S::WK;
+  const int64_t fit = (int64_t)sm_count() * S::OCC;
   return (int)(most < 1 ? 1 : most < fit ? most : fit);
 }
+static int grid_of(int64_t D, int64_t B, int64_t H, int64_t R, int64_t max_tokens) {
+  if (D == 64) return row_tiles(R) == 1 ? grid_of<64, 1>(B, H, R, max_tokens) : grid_of<64, 2>(B, H, R, max_tokens);
+  return row_tiles(R) == 1 ? grid_of<128, 1>(B, H, R, max_tokens) : grid_of<128, 2>(B, H, R, max_tokens);
+}
 
-template <int D, bool F16, int NT, int WR, int STAGES, int OCC>
+template <int D, bool F16, int NT>
 static int launch(const Maps& maps, const Params& p, int grid, cudaStream_t st) {
-  using SM = Smem<D, NT, WR, STAGES>;
-  const size_t smem = sizeof(SM) + 1024;
-  auto* kern = attn_cached_kernel<D, F16, NT, WR, STAGES, OCC>;
-  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  kern<<<grid, THREADS, smem, st>>>(maps, p);
+  using S = Shape<D, NT>;
+  const size_t smem = sizeof(Smem<D, NT>) + 1024;
+  auto* kern = attn_cached_kernel<D, F16, NT>;
+  static std::atomic<uint64_t> done{0};
+  if (int e = allow_smem((const void*)kern, smem, done)) return e;
+  kern<<<grid, S::THREADS, smem, st>>>(maps, p);
   if (int e = check_launch("attn_cached_kernel")) return e;
-  attn_cached_join_kernel<D, F16, SM::ROWS><<<(unsigned)((int64_t)p.B * p.H * p.rblocks), 128, 0, st>>>(p, grid);
+  cudaLaunchAttribute overlap{};
+  overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  overlap.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)((int64_t)p.B * p.H * p.rblocks));
+  cfg.blockDim = dim3(128);
+  cfg.stream = st;
+  cfg.attrs = &overlap;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, attn_cached_join_kernel<D, F16, NT>, p, grid);
   return check_launch("attn_cached_join_kernel");
 }
 
-template <int D, bool F16>
-static int launch_rows(const Maps& maps, const Params& p, int grid, cudaStream_t st) {
-  constexpr int S8 = D == 128 ? 2 : 4, S16 = D == 128 ? 4 : 6;
-  if (p.rows == 8) return launch<D, F16, 1, 1, S8, 2>(maps, p, grid, st);
-  if (p.rows == 16) return launch<D, F16, 2, 1, S16, 1>(maps, p, grid, st);
-  if (p.rows == 32) return launch<D, F16, 2, 2, S16, 1>(maps, p, grid, st);
-  return launch<D, F16, 2, 4, S16, 1>(maps, p, grid, st);
-}
-
-static int make_map(CUtensorMap* m, const void* base, uint64_t rows, int D, int page) {
+static int make_map(CUtensorMap* m, const void* base, uint64_t rows, int D, int box_rows) {
   tc::EncodeTiledFn fn = tc::encode_tiled_fn();
   if (!fn) return set_error(KB200_ERR_LAUNCH, "attn_cached: cuTensorMapEncodeTiled unavailable");
   cuuint64_t dims[2] = {(cuuint64_t)D, rows};
   cuuint64_t strides[1] = {(cuuint64_t)D};
-  cuuint32_t box[2] = {(cuuint32_t)D, (cuuint32_t)page};
+  cuuint32_t box[2] = {(cuuint32_t)D, (cuuint32_t)box_rows};
   cuuint32_t estr[2] = {1, 1};
   const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
@@ -655,8 +804,8 @@ extern "C" size_t kb200_attn_cached_workspace_size(int64_t B, int64_t Sq, int64_
   if (check_shape(B, Sq, Hq, Hkv, max_pages) || page < 1 || page > 128) return 0;
   if (B == 0 || Sq == 0) return 256;
   const int64_t R = Sq * (Hq / Hkv);
-  const int grid = grid_of(B, Hkv, R, max_pages * page);
-  return (size_t)2 * grid * block_rows(R) * (D + 2) * sizeof(float);
+  const int grid = grid_of(D, B, Hkv, R, max_pages * page);
+  return (size_t)2 * grid * row_tiles(R) * 8 * (D + 2) * sizeof(float);
 }
 
 extern "C" int kb200_attn_cached_fwd(const void* q, int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride,
@@ -675,7 +824,7 @@ extern "C" int kb200_attn_cached_fwd(const void* q, int64_t q_batch_stride, int6
   if (!workspace || workspace_bytes < need || !aligned16(workspace))
     return set_error(KB200_ERR_WORKSPACE, "attn_cached: workspace of %zu bytes needed, got %zu", need, workspace_bytes);
   const int64_t G = Hq / c->H, R = Sq * G;
-  const int rows = cached::block_rows(R);
+  const int nt = cached::row_tiles(R), rows = nt * 8;
   const int64_t rblocks = (R + rows - 1) / rows;
   if (B * c->H * rblocks > 0x7fffffffLL) return set_error(KB200_ERR_INVALID, "attn_cached: too many rows");
   cached::Params p{};
@@ -683,16 +832,21 @@ extern "C" int kb200_attn_cached_fwd(const void* q, int64_t q_batch_stride, int6
   p.k_scale = c->k_scale; p.v_scale = c->v_scale; p.part = (float*)workspace;
   p.q_bs = q_batch_stride; p.q_ts = q_token_stride; p.q_hs = q_head_stride;
   p.B = (int)B; p.Sq = (int)Sq; p.Hq = (int)Hq; p.H = (int)c->H; p.G = (int)G; p.R = (int)R;
-  p.rblocks = (int)rblocks; p.rows = rows;
+  p.rblocks = (int)rblocks;
   p.num_pages = (int)c->num_pages; p.max_pages = (int)max_pages; p.page = (int)c->page;
+  p.page_log2 = c->page == 16 ? 4 : c->page == 32 ? 5 : c->page == 64 ? 6 : 7;
+  p.box = c->page < nt * 16 ? (int)c->page : nt * 16;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   cached::Maps maps;
   const uint64_t mrows = (uint64_t)c->num_pages * c->H * c->page;
-  if (int e = cached::make_map(&maps.k, c->k_pages, mrows, (int)c->D, (int)c->page)) return e;
-  if (int e = cached::make_map(&maps.v, c->v_pages, mrows, (int)c->D, (int)c->page)) return e;
-  const int grid = cached::grid_of(B, c->H, R, max_pages * c->page);
+  if (int e = cached::make_map(&maps.k, c->k_pages, mrows, (int)c->D, p.box)) return e;
+  if (int e = cached::make_map(&maps.v, c->v_pages, mrows, (int)c->D, p.box)) return e;
+  const int grid = cached::grid_of(c->D, B, c->H, R, max_pages * c->page);
   cudaStream_t st = (cudaStream_t)stream;
-  if (c->D == 64)
-    return dtype ? cached::launch_rows<64, true>(maps, p, grid, st) : cached::launch_rows<64, false>(maps, p, grid, st);
-  return dtype ? cached::launch_rows<128, true>(maps, p, grid, st) : cached::launch_rows<128, false>(maps, p, grid, st);
+  if (c->D == 64) {
+    if (nt == 1) return dtype ? cached::launch<64, true, 1>(maps, p, grid, st) : cached::launch<64, false, 1>(maps, p, grid, st);
+    return dtype ? cached::launch<64, true, 2>(maps, p, grid, st) : cached::launch<64, false, 2>(maps, p, grid, st);
+  }
+  if (nt == 1) return dtype ? cached::launch<128, true, 1>(maps, p, grid, st) : cached::launch<128, false, 1>(maps, p, grid, st);
+  return dtype ? cached::launch<128, true, 2>(maps, p, grid, st) : cached::launch<128, false, 2>(maps, p, grid, st);
 }

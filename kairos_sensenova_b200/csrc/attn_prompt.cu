@@ -620,7 +620,8 @@ static int make_map(CUtensorMap* m, const void* base, const Params& p, int D, in
 template <int D, bool F16>
 static int launch(const Maps& maps, const Params& p, cudaStream_t st) {
   const size_t smem = sizeof(Smem<D>) + 1024;
-  cudaFuncSetAttribute(attn_prompt_kernel<D, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static std::atomic<uint64_t> done{0};
+  if (int e = allow_smem((const void*)attn_prompt_kernel<D, F16>, smem, done)) return e;
   const int64_t tiles = p.Tq * p.G / ROWS + p.N;             // no fewer than the sequences have
   attn_prompt_kernel<D, F16><<<(unsigned)(tiles * p.H), THREADS, smem, st>>>(maps, p);
   return check_launch("attn_prompt_kernel");

@@ -14,6 +14,20 @@ int set_error(int code, const char* fmt, ...) {
   return code;
 }
 
+int allow_smem(const void* kernel, size_t bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (e == cudaSuccess && (done.load(std::memory_order_relaxed) & bit)) return KB200_OK;
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return set_error(KB200_ERR_LAUNCH, "shared memory of %zu bytes: %s", bytes, cudaGetErrorString(e));
+  }
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return KB200_OK;
+}
+
 int check_launch(const char* what) {
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess)

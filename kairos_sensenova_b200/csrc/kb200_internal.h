@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 #include <stddef.h>
+#include <atomic>
 #include "../../include/kb200.h"
 
 namespace kb {
@@ -10,6 +11,9 @@ namespace kb {
 int set_error(int code, const char* fmt, ...);
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline size_t align_up(size_t x, size_t a = 256) { return (x + a - 1) / a * a; }
+// Lets `kernel` use `bytes` of dynamic shared memory on the current device.  `done` is the
+// kernel's own mask of the devices where that is set already (setting it twice does no harm).
+int allow_smem(const void* kernel, size_t bytes, std::atomic<uint64_t>& done);
 // Checks the result of the launches just issued.
 int check_launch(const char* what);
 }  // namespace kb

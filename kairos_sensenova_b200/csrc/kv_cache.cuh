@@ -38,6 +38,12 @@ KB_DEVI uint32_t decode2(uint32_t c) {
   asm("{.reg .b16 t;\n cvt.u16.u32 t, %1;\n cvt.rn.f16x2.e4m3x2 %0, t;}\n" : "=r"(r) : "r"(c));
   return r;
 }
+// The four codes of a word as two f16 pairs.  (Both halves in one statement: the conversion can
+// take either half of its register, where extracting them first costs an instruction each.)
+KB_DEVI void decode4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{.reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.rn.f16x2.e4m3x2 %0, a;\n cvt.rn.f16x2.e4m3x2 %1, b;}\n"
+      : "=r"(lo), "=r"(hi) : "r"(w));
+}
 KB_DEVI float2 half2_to_float2(uint32_t h) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }

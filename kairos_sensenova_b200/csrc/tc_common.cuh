@@ -21,6 +21,10 @@ KB_DEVI void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(smem_u32(bar)), "r"(bytes)
                : "memory");
 }
+// Adds to the phase's expected bytes without arriving.
+KB_DEVI void mbar_expect_tx_only(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;\n" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
 // try_wait with a suspend-time hint: the thread is suspended in hardware until
 // the phase completes or ~hint ns pass, instead of polling and taking issue slots.
 KB_DEVI bool mbar_try_wait(uint64_t* bar, uint32_t parity) {

@@ -20,6 +20,7 @@ and the table on the host first (it synchronises) and raises ``ValueError``.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -35,7 +36,7 @@ class KVCache:
     (``torch.float8_e4m3fn`` or ``uint8`` codes), ``k_scale``, ``v_scale`` ``[num_pages, heads]``
     fp32 powers of two, all contiguous.  A value is ``code * scale``."""
 
-    __slots__ = ('k_pages', 'v_pages', 'k_scale', 'v_scale', '_args')
+    __slots__ = ('_tensors', '_args', '_ref', '_shape', '_device')
 
     def __init__(self, k_pages, v_pages, k_scale, v_scale):
         if k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
@@ -59,9 +60,11 @@ class KVCache:
                 raise ValueError('KVCache: pages and scales must be on one device')
             if not t.is_contiguous():
                 raise ValueError('KVCache: pages and scales must be contiguous')
-        self.k_pages, self.v_pages, self.k_scale, self.v_scale = k_pages, v_pages, k_scale, v_scale
+        self._tensors = (k_pages, v_pages, k_scale, v_scale)
+        self._shape, self._device = (P, H, page, D), k_pages.device
         self._args = _lib.KvCacheArgs(k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                                       P, H, page, D)
+        self._ref = ctypes.byref(self._args)
 
     @classmethod
     def empty(cls, num_pages: int, num_heads: int, head_dim: int, page_size: int = 64, device='cuda'):
@@ -70,56 +73,66 @@ class KVCache:
                  .view(torch.float8_e4m3fn) for _ in range(2)]
         return cls(*codes, *(torch.ones(num_pages, num_heads, device=device) for _ in range(2)))
 
-    @property
-    def num_pages(self):
-        return self._args.num_pages
-
-    @property
-    def num_heads(self):
-        return self._args.H
-
-    @property
-    def page_size(self):
-        return self._args.page
-
-    @property
-    def head_dim(self):
-        return self._args.D
-
-    @property
-    def device(self):
-        return self.k_pages.device
+    k_pages = property(lambda self: self._tensors[0])
+    v_pages = property(lambda self: self._tensors[1])
+    k_scale = property(lambda self: self._tensors[2])
+    v_scale = property(lambda self: self._tensors[3])
+    num_pages = property(lambda self: self._shape[0])
+    num_heads = property(lambda self: self._shape[1])
+    page_size = property(lambda self: self._shape[2])
+    head_dim = property(lambda self: self._shape[3])
+    device = property(lambda self: self._device)
 
 
 def _index(t, shape, what, name, dev):
     """An int32 contiguous tensor of that shape on `dev` (None: any extent)."""
+    got = t.shape
+    if got != shape and (len(got) != len(shape) or any([n != m and n is not None for n, m in zip(shape, got)])):
+        raise ValueError(f'{what}: {name} must be {list(shape)}, got {tuple(got)}')
     if t.device != dev:
         raise ValueError(f'{what}: {name} must be on {dev}, got {t.device}')
-    if t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)):
-        raise ValueError(f'{what}: {name} must be {list(shape)}, got {tuple(t.shape)}')
-    if t.dtype != torch.int32:
-        if t.dtype != torch.int64:
+    if t.dtype is not torch.int32:
+        if t.dtype is not torch.int64:
             raise ValueError(f'{what}: {name} must be int32, got {t.dtype}')
         t = t.to(torch.int32)
     return t if t.is_contiguous() else t.contiguous()
 
 
 def _rows(t):
-    """`t` itself if its rows can be read in 16-byte steps in place, else a contiguous copy."""
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 and s > 0 for s in t.stride()[:-1]):
-        return t
-    return t.contiguous()
+    """(tensor, address, strides) of `t` if its rows can be read in 16-byte steps in place, else of a contiguous copy."""
+    strides, ptr = t.stride(), t.data_ptr()
+    bits = ptr >> 1                                 # 16-byte aligned, strides positive multiples of 8, channels contiguous
+    for s in strides[:-1]:
+        bits |= s if s > 0 else 1
+    if bits & 7 or strides[-1] != 1:
+        t = t.contiguous()
+        return t, t.data_ptr(), t.stride()
+    return t, ptr, strides
 
 
-def _forward_only(what, *tensors):
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+def _forward_only(what, a, b=None, c=None):
+    if torch.is_grad_enabled() and (a.requires_grad or (b is not None and b.requires_grad)
+                                    or (c is not None and c.requires_grad)):
         raise NotImplementedError(f'kairos_sensenova_b200.{what} is forward-only')
 
 
 def _cuda(what, cache):
-    if cache.device.type != 'cuda':
+    dev = cache._device
+    if dev.type != 'cuda':
         raise RuntimeError(f'{what}: the cache must be on a CUDA device (no CPU path)')
-    return cache.device
+    return dev
+
+
+def _launch(dev, what, fn, *args):
+    """``fn(*args, stream)`` on `dev`'s current stream, with `dev` the current device."""
+    index = dev.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _lib.check(rc, what)
 
 
 def check_tables(cache: KVCache, page_table, last, what='kv_cache', first=None, unique=False):
@@ -156,10 +169,12 @@ def kv_cache_append(cache: KVCache, k: torch.Tensor, v: torch.Tensor, page_table
     sequence (``check=True`` raises otherwise)."""
     what = 'kv_cache_append'
     dev = _cuda(what, cache)
-    H, D = cache.num_heads, cache.head_dim
-    if k.dim() != 3 or k.shape[1:] != (H, D) or v.shape != k.shape:
+    _, H, _, D = cache._shape
+    shape = k.shape
+    if len(shape) != 3 or shape[1] != H or shape[2] != D or v.shape != shape:
         raise ValueError(f'{what}: k and v must be [T, {H}, {D}], got {tuple(k.shape)}, {tuple(v.shape)}')
-    if k.dtype not in _DTYPES or v.dtype != k.dtype:
+    dtype = _DTYPES.get(k.dtype)
+    if dtype is None or v.dtype is not k.dtype:
         raise ValueError(f'{what}: k and v must both be bfloat16 or float16, got {k.dtype}, {v.dtype}')
     if k.device != dev or v.device != dev:
         raise ValueError(f'{what}: k and v must be on {dev}')
@@ -170,14 +185,12 @@ def kv_cache_append(cache: KVCache, k: torch.Tensor, v: torch.Tensor, page_table
     cu = _index(cu_seqlens, (B + 1,), what, 'cu_seqlens', dev)
     if check:
         check_tables(cache, page_table, lengths, what, lengths - (cu[1:] - cu[:-1]), unique=True)
-        if int(cu[0]) != 0 or int(cu[-1]) > k.shape[0]:
-            raise ValueError(f'{what}: cu_seqlens runs from {int(cu[0])} to {int(cu[-1])}, there are {k.shape[0]} tokens')
-    k, v = _rows(k), _rows(v)
-    with torch.cuda.device(dev):
-        _lib.check(_lib.lib().kb200_kv_append(
-            ctypes.byref(cache._args), k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-            page_table.data_ptr(), max_pages, lengths.data_ptr(), cu.data_ptr(), B, k.shape[0], _DTYPES[k.dtype],
-            torch.cuda.current_stream(dev).cuda_stream), what)
+        if int(cu[0]) != 0 or int(cu[-1]) > shape[0]:
+            raise ValueError(f'{what}: cu_seqlens runs from {int(cu[0])} to {int(cu[-1])}, there are {shape[0]} tokens')
+    k, kp, ks = _rows(k)
+    v, vp, vs = _rows(v)
+    _launch(dev, what, _lib.lib().kb200_kv_append, cache._ref, kp, vp, ks[0], ks[1], vs[0], vs[1],
+            page_table.data_ptr(), max_pages, lengths.data_ptr(), cu.data_ptr(), B, shape[0], dtype)
 
 
 def kv_cache_gather(cache: KVCache, page_table: torch.Tensor, starts: torch.Tensor, cu_seqlens: torch.Tensor, total: int,
@@ -188,31 +201,40 @@ def kv_cache_gather(cache: KVCache, page_table: torch.Tensor, starts: torch.Tens
     ``(k, v)`` to write into, contiguous."""
     what = 'kv_cache_gather'
     dev = _cuda(what, cache)
-    if dtype not in _DTYPES:
+    code = _DTYPES.get(dtype)
+    if code is None:
         raise ValueError(f'{what}: dtype must be bfloat16 or float16, got {dtype}')
     page_table = _index(page_table, (None, None), what, 'page_table', dev)
     B, max_pages = page_table.shape
     starts = _index(starts, (B,), what, 'starts', dev)
     cu = _index(cu_seqlens, (B + 1,), what, 'cu_seqlens', dev)
-    shape = (int(total), cache.num_heads, cache.head_dim)
+    shape = (int(total), cache._shape[1], cache._shape[3])
     if shape[0] < 0:
         raise ValueError(f'{what}: total {total}')
     if check:
         check_tables(cache, page_table, starts + cu[1:] - cu[:-1], what, starts)
         if int(cu[0]) != 0 or int(cu[-1]) > shape[0]:
             raise ValueError(f'{what}: cu_seqlens runs from {int(cu[0])} to {int(cu[-1])}, total is {shape[0]}')
-    with torch.cuda.device(dev):
-        if out is None:
-            k, v = torch.empty(shape, device=dev, dtype=dtype), torch.empty(shape, device=dev, dtype=dtype)
-        else:
-            k, v = out
-            for t in (k, v):
-                if t.shape != shape or t.dtype != dtype or t.device != dev or not t.is_contiguous() or t.data_ptr() % 16:
-                    raise ValueError(f'{what}: out must be contiguous 16-byte aligned {dtype} {list(shape)} on {dev}')
-        _lib.check(_lib.lib().kb200_kv_gather(
-            ctypes.byref(cache._args), page_table.data_ptr(), max_pages, starts.data_ptr(), cu.data_ptr(), B, shape[0],
-            k.data_ptr(), v.data_ptr(), _DTYPES[dtype], torch.cuda.current_stream(dev).cuda_stream), what)
+    if out is None:
+        k, v = torch.empty(shape, device=dev, dtype=dtype), torch.empty(shape, device=dev, dtype=dtype)
+    else:
+        k, v = out
+        for t in (k, v):
+            if t.shape != shape or t.dtype != dtype or t.device != dev or not t.is_contiguous() or t.data_ptr() % 16:
+                raise ValueError(f'{what}: out must be contiguous 16-byte aligned {dtype} {list(shape)} on {dev}')
+    _launch(dev, what, _lib.lib().kb200_kv_gather, cache._ref, page_table.data_ptr(), max_pages, starts.data_ptr(),
+            cu.data_ptr(), B, shape[0], k.data_ptr(), v.data_ptr(), code)
     return k, v
+
+
+@functools.lru_cache(maxsize=256)
+def _cached_workspace(device_index, *sizes):
+    """Workspace bytes for these sizes (they depend on the device's number of SMs)."""
+    with torch.cuda.device(device_index):
+        n = _lib.lib().kb200_attn_cached_workspace_size(*sizes)
+    if n == 0:
+        _lib.check(1, 'attention_cached')
+    return -(-n // 16) * 16
 
 
 def attention_cached(q: torch.Tensor, cache: KVCache, page_table: torch.Tensor, lengths: torch.Tensor,
@@ -228,15 +250,17 @@ def attention_cached(q: torch.Tensor, cache: KVCache, page_table: torch.Tensor, 
     the softmax sum ``[B, Sq, Hq]`` (-inf where nothing is seen)."""
     what = 'attention_cached'
     dev = _cuda(what, cache)
-    H, D = cache.num_heads, cache.head_dim
-    if q.dim() != 4 or q.shape[3] != D or q.shape[2] < 1 or q.shape[2] % H:
-        raise ValueError(f'{what}: q must be [B, Sq, Hq, {D}] with Hq a multiple of {H}, got {tuple(q.shape)}')
-    if q.dtype not in _DTYPES:
+    _, H, page, D = cache._shape
+    shape = q.shape
+    if len(shape) != 4 or shape[3] != D or shape[2] < 1 or shape[2] % H:
+        raise ValueError(f'{what}: q must be [B, Sq, Hq, {D}] with Hq a multiple of {H}, got {tuple(shape)}')
+    dtype = _DTYPES.get(q.dtype)
+    if dtype is None:
         raise ValueError(f'{what}: q must be bfloat16 or float16, got {q.dtype}')
     if q.device != dev:
         raise ValueError(f'{what}: q must be on {dev}, got {q.device}')
     _forward_only(what, q)
-    B, Sq, Hq, _ = q.shape
+    B, Sq, Hq, _ = shape
     page_table = _index(page_table, (B, None), what, 'page_table', dev)
     lengths = _index(lengths, (B,), what, 'lengths', dev)
     max_pages = page_table.shape[1]
@@ -244,20 +268,15 @@ def attention_cached(q: torch.Tensor, cache: KVCache, page_table: torch.Tensor, 
         check_tables(cache, page_table, lengths, what)
     if softmax_scale is None:
         softmax_scale = D ** -0.5
-    q = _rows(q)
-    L = _lib.lib()
-    with torch.cuda.device(dev):
-        if out is None:
-            out = torch.empty(q.shape, device=dev, dtype=q.dtype)
-        elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous() or out.data_ptr() % 16:
-            raise ValueError(f'{what}: out must be contiguous 16-byte aligned {q.dtype} {list(q.shape)} on {dev}')
-        lse = torch.empty(q.shape[:3], device=dev, dtype=torch.float32) if return_lse else None
-        nbytes = L.kb200_attn_cached_workspace_size(B, Sq, Hq, H, D, cache.page_size, max_pages)
-        if nbytes == 0:
-            _lib.check(1, what)
-        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-        _lib.check(L.kb200_attn_cached_fwd(
-            q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), ctypes.byref(cache._args), page_table.data_ptr(), max_pages,
-            lengths.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(), B, Sq, Hq, float(softmax_scale),
-            _DTYPES[q.dtype], ws.data_ptr(), nbytes, torch.cuda.current_stream(dev).cuda_stream), what)
+    q, qp, qs = _rows(q)
+    if out is None:
+        out = q.new_empty(shape)
+    elif out.shape != shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous() or out.data_ptr() % 16:
+        raise ValueError(f'{what}: out must be contiguous 16-byte aligned {q.dtype} {list(shape)} on {dev}')
+    lse = torch.empty(shape[:3], device=dev, dtype=torch.float32) if return_lse else None
+    nbytes = _cached_workspace(dev.index, B, Sq, Hq, H, D, page, max_pages)
+    ws = lengths.new_empty(nbytes >> 2)
+    _launch(dev, what, _lib.lib().kb200_attn_cached_fwd, qp, qs[0], qs[1], qs[2], cache._ref,
+            page_table.data_ptr(), max_pages, lengths.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else None, B, Sq,
+            Hq, float(softmax_scale), dtype, ws.data_ptr(), nbytes)
     return (out, lse) if return_lse else out

@@ -43,8 +43,12 @@ def test_index_and_rows():
         with pytest.raises(ValueError, match='x: y'):
             _index(bad, (3,), 'x', 'y', cpu)
     x = torch.zeros(10, 6, 64, dtype=torch.bfloat16)
-    assert _rows(x[:, 2:4]) .data_ptr() == x[:, 2:4].data_ptr()
-    assert _rows(x[..., 1:]).is_contiguous() and _rows(x.transpose(1, 2)).is_contiguous()
+    rows = lambda t: _rows(t)[0]  # noqa: E731
+    assert rows(x[:, 2:4]).data_ptr() == x[:, 2:4].data_ptr()
+    assert rows(x[..., 1:]).is_contiguous() and rows(x.transpose(1, 2)).is_contiguous()
+    assert rows(x[:, :1].expand(10, 3, 64)).is_contiguous()
+    t, ptr, strides = _rows(x[:, 1:, ::2])
+    assert t.is_contiguous() and strides == t.stride() and ptr == t.data_ptr()
 
 
 def test_check_tables():
