@@ -79,7 +79,7 @@ KB_DEVI int seq_len(const Params& p, int b) {
 // Groups of GT tokens of sequence b, and the length that each of its units takes in the flat
 // order: PAD more, positions without work that stand for what a segment costs apart from
 // its groups (Q, the join, the stores), so that shares of many short units balance too.
-constexpr int PAD = 8;
+constexpr int PAD = 16;
 template <int GT>
 KB_DEVI int seq_groups(const Params& p, int b) { return (seq_len(p, b) + GT - 1) / GT; }
 template <int GT>
@@ -135,6 +135,7 @@ struct Shape {
   static constexpr int OCC = D == 128 ? (NT == 1 ? 2 : 1) : (NT == 1 ? 3 : 2);
   static constexpr int STAGES = D == 128 ? (NT == 1 ? 3 : 2) : (NT == 1 ? 4 : 3);
   static constexpr int THREADS = (WK + 1) * 32;
+  static constexpr int JOIN = ROWS * D / 4 < 256 ? ROWS * D / 4 : 256;   // threads of a joining block
   static constexpr int MAXBOX = NT;          // boxes of a group: GT / box, box at least 16
 };
 
@@ -667,7 +668,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
 // Joins the partials of the units that cross shares, and writes the empty sequences.
 // One block per (sequence, kv head, row block).
 template <int D, bool F16, int NT>
-__global__ void __launch_bounds__(128) attn_cached_join_kernel(Params p, int ctas) {
+__global__ void __launch_bounds__(Shape<D, NT>::JOIN) attn_cached_join_kernel(Params p, int ctas) {
+  constexpr int THREADS = Shape<D, NT>::JOIN;
   constexpr int GT = Shape<D, NT>::GT, ROWS = Shape<D, NT>::ROWS;
   const int lane = threadIdx.x & 31;
   const int64_t units = (int64_t)p.H * p.rblocks;
@@ -696,31 +698,66 @@ __global__ void __launch_bounds__(128) attn_cached_join_kernel(Params p, int cta
     if (c0 == c1) return;                  // finished there
   }
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
-  const float* mlp = p.part + (int64_t)2 * ctas * ROWS * D;
-  for (int i = threadIdx.x; i < ROWS * (D / 4); i += 128) {
-    const int r = i / (D / 4), c = i % (D / 4), rr = rb * ROWS + r;
-    if (rr >= p.R) break;
-    float mx = -INFINITY, ls = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    // the part that begins the unit is its CTA's last segment (slot 1), the later ones
-    // continue it (slot 0)
-    for (int k = c0; k <= c1; ++k) {
-      const int64_t slot = 2 * (int64_t)k + (k == c0 ? 1 : 0);
-      const float m = mlp[(slot * ROWS + r) * 2], l = mlp[(slot * ROWS + r) * 2 + 1];
-      const float mn = fmaxf(mx, m), f0 = mx == -INFINITY ? 1.f : ex2(mx - mn), f1 = m == -INFINITY ? 1.f : ex2(m - mn);
-      const float4 x = *reinterpret_cast<const float4*>(p.part + (slot * ROWS + r) * D + c * 4);
-      acc.x = acc.x * f0 + x.x * f1; acc.y = acc.y * f0 + x.y * f1;
-      acc.z = acc.z * f0 + x.z * f1; acc.w = acc.w * f0 + x.w * f1;
-      ls = ls * f0 + l * f1;
-      mx = mn;
+  // Partials in share order: the part that begins the unit is its CTA's last segment (slot 1),
+  // the later ones continue it (slot 0).  A chunk's m and l are read together, then its O with
+  // all loads in flight: what the join costs is the two latencies.
+  constexpr int CHUNK = 32, ITEMS = ROWS * (D / 4) / THREADS;
+  __shared__ float fac[CHUNK][ROWS], run_m[ROWS], run_l[ROWS], scale_old[ROWS];
+  const float2* mlp = reinterpret_cast<const float2*>(p.part + (int64_t)2 * ctas * ROWS * D);
+  float4 acc[ITEMS];
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (threadIdx.x < ROWS) {
+    run_m[threadIdx.x] = -INFINITY;
+    run_l[threadIdx.x] = 0.f;
+  }
+  __syncthreads();
+  for (int k0 = c0; k0 <= c1; k0 += CHUNK) {
+    const int n = min(CHUNK, c1 + 1 - k0);
+    // a warp per row, a lane per part: the parts' factors, and that of what is joined so far
+    for (int r = threadIdx.x >> 5; r < ROWS; r += THREADS / 32) {
+      float2 x = make_float2(-INFINITY, 0.f);
+      if (lane < n) x = __ldcg(mlp + (2 * (int64_t)(k0 + lane) + (k0 + lane == c0 ? 1 : 0)) * ROWS + r);
+      const float before = run_m[r], mx = fmaxf(before, warp_max(x.x));
+      // (m = -inf: no visible key, O and l are 0, or all of its scores are NaN, and so are they)
+      const float f = x.x == -INFINITY ? 1.f : ex2(x.x - mx), f0 = before == -INFINITY ? 1.f : ex2(before - mx);
+      const float l = warp_sum(f * x.y) + run_l[r] * f0;
+      fac[lane][r] = f;
+      __syncwarp();
+      if (lane == 0) {
+        scale_old[r] = f0;
+        run_m[r] = mx;
+        run_l[r] = l;
+      }
     }
-    const float inv = ls > 0.f || ls != ls ? 1.f / ls : 0.f;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int r = (threadIdx.x + i * THREADS) / (D / 4), c = (threadIdx.x + i * THREADS) % (D / 4);
+      if (rb * ROWS + r >= p.R) continue;
+      const float f0 = scale_old[r];
+      acc[i].x *= f0; acc[i].y *= f0; acc[i].z *= f0; acc[i].w *= f0;
+#pragma unroll 16
+      for (int k = 0; k < n; ++k) {
+        const float f = fac[k][r];
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(
+            p.part + ((2 * (int64_t)(k0 + k) + (k0 + k == c0 ? 1 : 0)) * ROWS + r) * D + c * 4));
+        acc[i].x += x.x * f; acc[i].y += x.y * f; acc[i].z += x.z * f; acc[i].w += x.w * f;
+      }
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int r = (threadIdx.x + i * THREADS) / (D / 4), c = (threadIdx.x + i * THREADS) % (D / 4), rr = rb * ROWS + r;
+    if (rr >= p.R) continue;
+    const float l = run_l[r], inv = l > 0.f || l != l ? 1.f / l : 0.f;
     const int64_t orow = ((int64_t)b * p.Sq + rr / p.G) * p.Hq + h * p.G + rr % p.G;
     uint2 w;
-    w.x = kv::pack16<F16>(acc.x * inv, acc.y * inv);
-    w.y = kv::pack16<F16>(acc.z * inv, acc.w * inv);
+    w.x = kv::pack16<F16>(acc[i].x * inv, acc[i].y * inv);
+    w.y = kv::pack16<F16>(acc[i].z * inv, acc[i].w * inv);
     *reinterpret_cast<uint2*>(reinterpret_cast<char*>(p.o) + 2 * (orow * D + c * 4)) = w;
-    if (c == 0 && p.lse) p.lse[orow] = ls == 0.f ? -INFINITY : (mx - SHIFT + log2f(ls)) * 0.6931471805599453f;
+    if (c == 0 && p.lse) p.lse[orow] = l == 0.f ? -INFINITY : (run_m[r] - SHIFT + log2f(l)) * 0.6931471805599453f;
   }
 }
 
@@ -765,7 +802,7 @@ static int launch(const Maps& maps, const Params& p, int grid, cudaStream_t st) 
   overlap.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)((int64_t)p.B * p.H * p.rblocks));
-  cfg.blockDim = dim3(128);
+  cfg.blockDim = dim3(S::JOIN);
   cfg.stream = st;
   cfg.attrs = &overlap;
   cfg.numAttrs = 1;
