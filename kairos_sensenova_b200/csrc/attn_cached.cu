@@ -13,8 +13,10 @@
 // shares leaves a partial (m, l, O) per CTA, joined in share order (no atomics: the
 // result does not depend on timing) by a second, dependent kernel.
 //
-// A CTA: one producer warp streams K and V by TMA; every consumer warp has a ring of its
-// own and takes every WK-th group, so a warp never waits for another one inside a unit.
+// Every warp has a ring of its own, fills it by 16-byte cp.async (swizzled, so that no load from
+// it conflicts) and takes every WK-th group: no warp waits for another inside a unit.  (One
+// TMA box per 16 tokens and head ran at 80-100 cycles a box whatever its size, 25 B a cycle
+// and SM at D = 128 and half of that at D = 64.)
 // Per 16 tokens:
 //   S^T = K Q^T  mma.m16n8k16 f16 (16 tokens x 8 rows), codes widened to f16 in
 //                registers (exact); the contraction index is permuted so that a lane's
@@ -26,7 +28,6 @@
 // bf16 queries are multiplied by a power of two per row into f16's range first (exact
 // but for elements 2^-29 below the row's largest).  P is rounded to f16 (2^-12).
 #include "kv_cache.cuh"
-#include "tc_common.cuh"
 
 namespace kb {
 namespace cached {
@@ -39,6 +40,7 @@ struct Params {
   void* o;
   float* lse;
   const int32_t *table, *lengths;
+  const uint8_t *k_pages, *v_pages;
   const float *k_scale, *v_scale;
   float* part;                     // [2 G][rows][D] partial O, then [2 G][rows][2] (m, l)
   int64_t q_bs, q_ts, q_hs;        // batch, token, head strides of q, elements
@@ -46,12 +48,7 @@ struct Params {
   int rblocks;                     // row blocks per (sequence, kv head)
   int num_pages, max_pages, page;
   int page_log2;
-  int box;                         // tokens of one TMA box: min(page, tokens of a group)
   float scale_log2;
-};
-
-struct Maps {
-  CUtensorMap k, v;
 };
 
 KB_DEVI float ex2(float x) {
@@ -125,18 +122,25 @@ KB_DEVI Share share_of(int64_t units, int64_t sum_spans, int ctas, int wk) {
   return s;
 }
 
+// Where 16-byte chunk `c` of token row `r` lies in a slot.  Eight lanes that load together (K: two
+// rows, V: every second row, one or two channel chunks) meet eight different chunks of a line.
+template <int D>
+KB_DEVI uint32_t swz(int r, int c) {
+  if constexpr (D == 128) return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4));
+  else return (uint32_t)((r >> 1) * 128 + (((((r & 1) << 2) | c) ^ (((r >> 1) & 3) << 1)) << 4));
+}
+
 // The launch shapes.  NT: 8-row tiles of a CTA (rows up to 8: 1, else 2); a group is NT * 16
-// tokens.  WK consumer warps and their producer, OCC CTAs per SM: as many warps as the
-// registers allow (8 rows need under 128 at D = 128, 16 rows under 168).
+// tokens.  WK warps, OCC CTAs per SM: as many warps as the registers allow (at D = 128, 8 rows
+// need under 128 and 16 rows under 168).
 template <int D, int NT>
 struct Shape {
   static constexpr int GT = NT * 16, ROWS = NT * 8;
-  static constexpr int WK = D == 128 && NT == 2 ? 11 : 7;
+  static constexpr int WK = D == 128 && NT == 2 ? 12 : 8;
   static constexpr int OCC = D == 128 ? (NT == 1 ? 2 : 1) : (NT == 1 ? 3 : 2);
   static constexpr int STAGES = D == 128 ? (NT == 1 ? 3 : 2) : (NT == 1 ? 4 : 3);
-  static constexpr int THREADS = (WK + 1) * 32;
+  static constexpr int THREADS = WK * 32;
   static constexpr int JOIN = ROWS * D / 4 < 256 ? ROWS * D / 4 : 256;   // threads of a joining block
-  static constexpr int MAXBOX = NT;          // boxes of a group: GT / box, box at least 16
 };
 
 // A CTA's segments, in order: the groups [g0, g0 + count) of unit (b, h, rb); `ng` are all of
@@ -145,8 +149,10 @@ template <int GT>
 struct Walk {
   int64_t left;                        // flat positions still to come
   int b, u, x;                         // the next one: sequence, unit, position in the unit
-  int h, rb, len, ng, g0, count;
-  KB_DEVI Walk(const Params& p, int64_t at, int64_t end, int b_, int64_t begin) : left(end - at), b(b_) {
+  int b_of, h, rb, len, ng, g0, count; // (b_of: the segment's sequence)
+  KB_DEVI void start(const Params& p, int64_t at, int64_t end, int b_, int64_t begin) {
+    left = end - at;
+    b = b_;
     const int span = seq_span<GT>(p, b);
     u = (int)((at - begin) / span);
     x = (int)((at - begin) - (int64_t)u * span);
@@ -164,6 +170,7 @@ struct Walk {
       left -= take;
       g0 = x;
       count = min(x + take, ng) - x;
+      b_of = b;
       h = u / p.rblocks;
       rb = u - h * p.rblocks;
       x += take;
@@ -177,6 +184,16 @@ struct Walk {
   }
 };
 
+// Where the loading side of a warp is: kept in shared memory, since it is touched once per
+// batch and the registers are short.
+template <int GT>
+struct Feed {
+  Walk<GT> seg;
+  int rot, first, done;                      // of the segment: rotation, the warp's first group, groups batched
+  int live;
+  int h, n, tok0;                            // the next batch: head, groups, first token of its first group
+};
+
 template <int D, int NT>
 struct Smem {
   using S = Shape<D, NT>;
@@ -186,46 +203,121 @@ struct Smem {
   static_assert(sizeof(Slot) == S::ROWS * D * sizeof(float), "a slot also holds a warp's O");
   Slot slot[S::WK][S::STAGES];
   float ml[S::WK][S::ROWS][2];
-  float2 scale[S::WK][S::STAGES][S::MAXBOX]; // page scales (k, v) of each box; k < 0: no such page
-  uint64_t full[S::WK][S::STAGES], empty[S::WK][S::STAGES];
+  float2 scale[S::WK][S::STAGES][NT];        // page scales (k, v) of 16 tokens each; k < 0: no such page
+  Feed<S::GT> feed[S::WK];
+  Walk<S::GT> walk[S::WK];
   int64_t total, begin;
   int first_b;
   int held[S::WK];                           // the slot that holds the warp's O, -1: none
-  int abort_flag;
 };
 
-// 16-byte chunk `c` of page row `r` in a swizzled stage.
-template <int D>
-KB_DEVI uint32_t swz(int r, int c) {
-  if constexpr (D == 128) return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4));
-  else return (uint32_t)(r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
-}
+// The loading side of one warp: its groups in the order of the segments, STAGES ahead of
+// their use.  Page ids and scales are read by lanes, a batch of 32 16-token parts at once and
+// a batch ahead; a batch lies in one segment.
+template <int D, int NT>
+struct Loader {
+  using S = Shape<D, NT>;
+  static constexpr int BATCH = 32 / NT;      // groups of a batch
+  Feed<S::GT>* feed;
+  int h, n, pos, tok0, pg;                   // current batch: head, groups, next one, first token, this lane's page
+  int pg2;                                   // the next batch's
+  float2 sc, sc2;
+  bool pending;                              // sc2 is still to be read
+
+  KB_DEVI void next_batch(const Params& p, int units, int warp, int lane) {
+    __syncwarp();
+    Feed<S::GT> f = *feed;
+    f.n = 0;
+    pg2 = -1;
+    pending = false;
+    while (f.live) {
+      const int mine = f.seg.count > f.first ? (f.seg.count - f.first + S::WK - 1) / S::WK : 0;   // this warp's groups of the segment
+      if (f.done < mine) {
+        f.n = min(BATCH, mine - f.done);
+        f.h = f.seg.h;
+        const int gi = f.first + (f.done + lane / NT) * S::WK;
+        if (gi < f.seg.count) {
+          const int tok = (f.seg.g0 + gi) * S::GT + (lane % NT) * 16;
+          if (tok < f.seg.len) pg2 = __ldg(p.table + (int64_t)f.seg.b_of * p.max_pages + (tok >> p.page_log2));
+        }
+        f.tok0 = (f.seg.g0 + f.first + f.done * S::WK) * S::GT;
+        f.done += f.n;
+        pending = true;
+        break;
+      }
+      f.rot = (f.rot + f.seg.count) % S::WK;
+      f.first = warp >= f.rot ? warp - f.rot : warp + S::WK - f.rot;
+      f.done = 0;
+      f.live = f.seg.next(p, units);
+    }
+    __syncwarp();
+    if (lane == 0) *feed = f;
+    __syncwarp();
+  }
+  KB_DEVI void read_scales(const Params& p) {
+    sc2 = make_float2(-1.f, 0.f);
+    if (pg2 >= 0 && pg2 < p.num_pages) {
+      const int64_t i = (int64_t)pg2 * p.H + feed->h;
+      sc2.x = __ldg(p.k_scale + i);
+      sc2.y = __ldg(p.v_scale + i);
+    } else {
+      pg2 = -1;
+    }
+    pending = false;
+  }
+  KB_DEVI Loader(Feed<S::GT>* at, const Params& p, int units, int warp, int lane) : feed(at), n(0), pos(0) {
+    next_batch(p, units, warp, lane);
+  }
+  // The next group into `slot`; always one cp.async group, empty when the work is over.
+  KB_DEVI void load(const Params& p, int units, int warp, int lane, typename Smem<D, NT>::Slot& slot, float2* scale) {
+    if (pos == n) {
+      if (pending) read_scales(p);
+      h = feed->h; n = feed->n; tok0 = feed->tok0;
+      pg = pg2; sc = sc2;
+      pos = 0;
+      if (n) next_batch(p, units, warp, lane);
+    } else if (pending) {
+      read_scales(p);
+    }
+    if (n) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const int src = pos * NT + j;
+        const int page = __shfl_sync(0xffffffffu, pg, src);
+        const float2 s = make_float2(__shfl_sync(0xffffffffu, sc.x, src), __shfl_sync(0xffffffffu, sc.y, src));
+        if (lane == 0) scale[j] = s;
+        if (page >= 0) {
+          const int tok = tok0 + pos * (S::WK * S::GT) + j * 16;
+          const int64_t row = ((int64_t)page * p.H + h) * p.page + (tok & (p.page - 1));
+          const uint8_t *ks = p.k_pages + row * D + lane * 16, *vs = p.v_pages + row * D + lane * 16;
+          constexpr int RPI = 512 / D;       // rows that the warp's 32 chunks cover
+#pragma unroll
+          for (int i = 0; i < 16 / RPI; ++i) {
+            const uint32_t dst = swz<D>(j * 16 + i * RPI + lane / (D / 16), lane % (D / 16));
+            cp_async16(slot.k + dst, ks + i * 512, true);
+            cp_async16(slot.v + dst, vs + i * 512, true);
+          }
+        }
+      }
+      ++pos;
+    }
+    cp_async_commit();
+  }
+};
 
 template <int D, bool F16, int NT>
 __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
-    attn_cached_kernel(const __grid_constant__ Maps maps, Params p) {
+    attn_cached_kernel(Params p) {
   using S = Shape<D, NT>;
   using SM = Smem<D, NT>;
   constexpr int WK = S::WK, STAGES = S::STAGES, GT = S::GT, ROWS = S::ROWS;
   constexpr int MT = D / 16;               // 16-wide tiles of D
-  extern __shared__ __align__(1024) unsigned char smem_raw[];
-  SM& sm = *reinterpret_cast<SM*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
+  extern __shared__ __align__(128) unsigned char smem_raw[];
+  SM& sm = *reinterpret_cast<SM*>(smem_raw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t units = (int64_t)p.H * p.rblocks;
-  const int boxes = GT / p.box;
 
-  if (warp == WK) {
-    for (int i = lane; i < WK * STAGES; i += 32) {
-      tc::mbar_init(&sm.full[0][0] + i, boxes);
-      tc::mbar_init(&sm.empty[0][0] + i, 1);
-    }
-    if (lane == 0) {
-      sm.abort_flag = 0;
-      tc::prefetch_tmap(&maps.k);
-      tc::prefetch_tmap(&maps.v);
-    }
-    tc::fence_barrier_init();
-  } else if (warp == 0) {
+  if (warp == 0) {
     int64_t sum = 0;
     for (int b = lane; b < p.B; b += 32) sum += seq_span<GT>(p, b);
 #pragma unroll
@@ -246,99 +338,31 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
   // the join may be scheduled as soon as CTAs leave; it waits for all of them before it reads
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   if (at0 >= at1) return;
-  auto aborted = [&]() { return *((volatile int*)&sm.abort_flag) != 0; };
 
   // Every warp walks the CTA's segments in the same order.  Group i of a segment goes to
-  // consumer warp (i + rot) % WK, so that short segments use all of them in turn.
-  Walk<GT> seg(p, at0, at1, sm.first_b, sm.begin);
-  int rot = 0;
-  if (warp == WK) {
-    // ---------------------------------------------------------------- producer
-    // Lane w * boxes + i loads box i of consumer warp w's groups.  A round gives every warp
-    // one group.  Page ids are read AHEAD rounds before their use and scales half of that,
-    // across segments: with one round ahead the producer took a loaded memory latency per
-    // round and the CTA no more than 4 KB * WK in that time.
-    constexpr int AHEAD = 6, HALF = 3;
-    struct Round {
-      int state;                           // 0: the work is over, 1: no group for this lane, 2: a group
-      int pg, h, off;                      // its page in the pool (-1: none), head, first row in the page
-    };
-    const int w = lane / boxes, bi = lane % boxes;
-    int i0 = 0, base = 0;                  // rounds of the current segment begin at group i0; rot at its start
-    bool live = seg.next(p, (int)units);
-    auto next_round = [&]() {
-      Round r{0, -1, 0, 0};
-      if (live && i0 >= seg.count) {
-        base = (base + seg.count) % WK;
-        i0 = 0;
-        live = seg.next(p, (int)units);
-      }
-      if (!live) return r;
-      r.state = 1;
-      const int i = i0 + (w >= base ? w - base : w + WK - base);
-      i0 += WK;
-      if (w < WK && i < seg.count) {
-        r.state = 2;
-        const int tok = (seg.g0 + i) * GT + bi * p.box, pi = tok >> p.page_log2;
-        r.off = tok & (p.page - 1);
-        r.h = seg.h;
-        if (tok < seg.len) r.pg = __ldg(p.table + (int64_t)seg.b * p.max_pages + pi);
-      }
-      return r;
-    };
-    auto scale_of = [&](const Round& r) {
-      float2 s = make_float2(-1.f, 0.f);
-      if (r.pg >= 0 && r.pg < p.num_pages) {
-        s.x = __ldg(p.k_scale + (int64_t)r.pg * p.H + r.h);
-        s.y = __ldg(p.v_scale + (int64_t)r.pg * p.H + r.h);
-      }
-      return s;
-    };
-    int it = 0;                            // groups of this lane's ring
-    bool ok = true;
-    Round r[AHEAD];
-    float2 sc[HALF];
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) r[i] = next_round();
-#pragma unroll
-    for (int i = 0; i < HALF; ++i) sc[i] = scale_of(r[i]);
-    while (r[0].state) {
-      if (r[0].state == 2 && ok) {
-        const int s = it % STAGES;
-        if (it >= STAGES && !tc::mbar_wait(&sm.empty[w][s], (it / STAGES - 1) & 1)) { sm.abort_flag = 1; ok = false; }
-        if (aborted()) ok = false;
-        if (ok) {
-          typename SM::Slot& sl = sm.slot[w][s];
-          if (r[0].pg >= 0 && r[0].pg < p.num_pages) {
-            const int y = (r[0].pg * p.H + r[0].h) * p.page + r[0].off;
-            tc::mbar_expect_tx_only(&sm.full[w][s], (uint32_t)(2 * p.box * D));
-            tc::tma_load_2d(sl.k + bi * p.box * D, &maps.k, &sm.full[w][s], 0, y);
-            tc::tma_load_2d(sl.v + bi * p.box * D, &maps.v, &sm.full[w][s], 0, y);
-          }
-          sm.scale[w][s][bi] = sc[0];
-          tc::mbar_arrive(&sm.full[w][s]);
-          ++it;
-        }
-      }
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-#pragma unroll
-      for (int i = 0; i + 1 < HALF; ++i) sc[i] = sc[i + 1];
-      sc[HALF - 1] = scale_of(r[HALF]);
-#pragma unroll
-      for (int i = 0; i + 1 < AHEAD; ++i) r[i] = r[i + 1];
-      r[AHEAD - 1] = next_round();
-    }
-    const bool mine = w < WK;
-    // every load lands before the CTA may exit
-    if (mine)
-      for (int i = it > STAGES ? it - STAGES : 0; i < it; ++i) tc::mbar_wait(&sm.full[w][i % STAGES], (i / STAGES) & 1);
-    return;
+  // warp (i + rot) % WK, so that short segments use all of them in turn.
+  if (lane == 0) {
+    Feed<GT> f{};
+    f.seg.start(p, at0, at1, sm.first_b, sm.begin);
+    sm.walk[warp] = f.seg;
+    f.first = warp;
+    f.live = f.seg.next(p, (int)units);
+    sm.feed[warp] = f;
   }
-
-  // ------------------------------------------------------------------ consumers
+  Loader<D, NT> loader(&sm.feed[warp], p, (int)units, warp, lane);
+  for (int s = 0; s < STAGES; ++s) loader.load(p, (int)units, warp, lane, sm.slot[warp][s], sm.scale[warp][s]);
+  Walk<GT> seg;
+  auto next_segment = [&]() {              // the using side's walk, in shared memory too
+    __syncwarp();
+    seg = sm.walk[warp];
+    const bool more = seg.next(p, (int)units);
+    __syncwarp();
+    if (lane == 0) sm.walk[warp] = seg;
+    return more;
+  };
+  int rot = 0;
   const int g = lane >> 2, t4 = lane & 3;
-  int it = 0;
+  int s = 0;                               // this warp's next slot
   constexpr int CH = D / 64;               // 16-byte code chunks per lane and row
   uint32_t raw[NT][CH * 8];                // the segment's Q, read while the one before is joined
   auto load_q = [&]() {
@@ -347,7 +371,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
       const int r = seg.rb * ROWS + n * 8 + g;
       const bool in = r < p.R;
       const char* src = reinterpret_cast<const char*>(p.q);
-      if (in) src += 2 * ((int64_t)seg.b * p.q_bs + (int64_t)(r / p.G) * p.q_ts + (int64_t)(seg.h * p.G + r % p.G) * p.q_hs +
+      if (in) src += 2 * ((int64_t)seg.b_of * p.q_bs + (int64_t)(r / p.G) * p.q_ts + (int64_t)(seg.h * p.G + r % p.G) * p.q_hs +
                           t4 * (CH * 16));
 #pragma unroll
       for (int c = 0; c < CH * 2; ++c) {
@@ -356,10 +380,10 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
       }
     }
   };
-  bool live = seg.next(p, (int)units);
+  bool live = next_segment();
   if (live) load_q();
   while (live) {
-    const int b = seg.b, h = seg.h, rb = seg.rb, len = seg.len, g0 = seg.g0, count = seg.count;
+    const int b = seg.b_of, h = seg.h, rb = seg.rb, len = seg.len, g0 = seg.g0, count = seg.count;
     const bool whole = g0 == 0 && count == seg.ng;
     const int gi0 = warp >= rot ? warp - rot : warp + WK - rot;   // this warp's first group
     rot = (rot + count) % WK;
@@ -418,17 +442,15 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
     const int all_seen = len - p.Sq + 1;   // keys below are seen by every row
 
     int held = -1;
-    for (int gi = gi0; gi < count; gi += WK, ++it) {
-      const int s = it % STAGES;
-      const bool ok = tc::mbar_wait(&sm.full[warp][s], (it / STAGES) & 1);
-      if (!ok) sm.abort_flag = 1;
-      if (__any_sync(0xffffffffu, !ok || aborted())) break;
+    for (int gi = gi0; gi < count; gi += WK) {
+      cp_async_wait<STAGES - 1>();         // the oldest group has landed, for every lane
+      __syncwarp();
       const typename SM::Slot& sl = sm.slot[warp][s];
       const int base = (g0 + gi) * GT;
       float sk[NT], sv[NT];
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        const float2 sc = sm.scale[warp][s][j * 16 / p.box];
+        const float2 sc = sm.scale[warp][s][j];
         sk[j] = sc.x;
         sv[j] = sc.y;
       }
@@ -582,11 +604,9 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
       }
       __syncwarp();
       // the last slot of the segment is kept: it takes the warp's O
-      if (gi + WK < count) {
-        if (lane == 0) tc::mbar_arrive(&sm.empty[warp][s]);
-      } else {
-        held = s;
-      }
+      if (gi + WK < count) loader.load(p, (int)units, warp, lane, sm.slot[warp][s], sm.scale[warp][s]);
+      else held = s;
+      s = s + 1 == STAGES ? 0 : s + 1;
     }
     // ---- the warps' partial results join: each one's O in the slot it kept
     if (held >= 0) {
@@ -610,10 +630,9 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
       }
     }
     if (lane == 0) sm.held[warp] = held;
-    live = seg.next(p, (int)units);
+    live = next_segment();
     if (live) load_q();
-    tc::bar_sync_named(1, WK * 32);
-    const bool dead = aborted();
+    __syncthreads();
     const int slot = 2 * blockIdx.x + (g0 > 0 ? 0 : 1);   // a share's first segment may end a unit, its last may begin one
     for (int i = tid; i < ROWS * (D / 4); i += WK * 32) {
       const int r = i / (D / 4), c = i % (D / 4);
@@ -637,19 +656,18 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
           ls += f * sm.ml[k][r][1];
         }
       }
-      if (dead) a = make_float4(NAN, NAN, NAN, NAN);
       if (!whole) {
         float* dst = p.part + ((int64_t)slot * ROWS + r) * D + c * 4;
         *reinterpret_cast<float4*>(dst) = a;
         if (c == 0) {
           float* ml = p.part + (int64_t)2 * gridDim.x * ROWS * D + ((int64_t)slot * ROWS + r) * 2;
           ml[0] = mx;
-          ml[1] = dead ? 1.f : ls;
+          ml[1] = ls;
         }
       } else {
         const int rr = rb * ROWS + r;
         if (rr < p.R) {
-          const float inv = dead || ls > 0.f || ls != ls ? 1.f / ls : 0.f;
+          const float inv = ls > 0.f || ls != ls ? 1.f / ls : 0.f;
           const int64_t orow = ((int64_t)b * p.Sq + rr / p.G) * p.Hq + h * p.G + rr % p.G;
           uint2 w;
           w.x = kv::pack16<F16>(a.x * inv, a.y * inv);
@@ -659,9 +677,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
         }
       }
     }
-    tc::fence_proxy_async_smem();          // O's slots go back to the TMA
-    tc::bar_sync_named(1, WK * 32);
-    if (held >= 0 && lane == 0) tc::mbar_arrive(&sm.empty[warp][held]);
+    __syncthreads();
+    if (held >= 0) loader.load(p, (int)units, warp, lane, sm.slot[warp][held], sm.scale[warp][held]);
   }
 }
 
@@ -789,13 +806,13 @@ static int grid_of(int64_t D, int64_t B, int64_t H, int64_t R, int64_t max_token
 }
 
 template <int D, bool F16, int NT>
-static int launch(const Maps& maps, const Params& p, int grid, cudaStream_t st) {
+static int launch(const Params& p, int grid, cudaStream_t st) {
   using S = Shape<D, NT>;
-  const size_t smem = sizeof(Smem<D, NT>) + 1024;
+  const size_t smem = sizeof(Smem<D, NT>);
   auto* kern = attn_cached_kernel<D, F16, NT>;
   static std::atomic<uint64_t> done{0};
   if (int e = allow_smem((const void*)kern, smem, done)) return e;
-  kern<<<grid, S::THREADS, smem, st>>>(maps, p);
+  kern<<<grid, S::THREADS, smem, st>>>(p);
   if (int e = check_launch("attn_cached_kernel")) return e;
   cudaLaunchAttribute overlap{};
   overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -808,20 +825,6 @@ static int launch(const Maps& maps, const Params& p, int grid, cudaStream_t st) 
   cfg.numAttrs = 1;
   cudaLaunchKernelEx(&cfg, attn_cached_join_kernel<D, F16, NT>, p, grid);
   return check_launch("attn_cached_join_kernel");
-}
-
-static int make_map(CUtensorMap* m, const void* base, uint64_t rows, int D, int box_rows) {
-  tc::EncodeTiledFn fn = tc::encode_tiled_fn();
-  if (!fn) return set_error(KB200_ERR_LAUNCH, "attn_cached: cuTensorMapEncodeTiled unavailable");
-  cuuint64_t dims[2] = {(cuuint64_t)D, rows};
-  cuuint64_t strides[1] = {(cuuint64_t)D};
-  cuuint32_t box[2] = {(cuuint32_t)D, (cuuint32_t)box_rows};
-  cuuint32_t estr[2] = {1, 1};
-  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return set_error(KB200_ERR_LAUNCH, "attn_cached: tensor map encode failed (%d)", (int)r);
-  return KB200_OK;
 }
 
 static int check_shape(int64_t B, int64_t Sq, int64_t Hq, int64_t H, int64_t max_pages) {
@@ -866,24 +869,20 @@ extern "C" int kb200_attn_cached_fwd(const void* q, int64_t q_batch_stride, int6
   if (B * c->H * rblocks > 0x7fffffffLL) return set_error(KB200_ERR_INVALID, "attn_cached: too many rows");
   cached::Params p{};
   p.q = q; p.o = o; p.lse = lse; p.table = page_table; p.lengths = lengths;
+  p.k_pages = (const uint8_t*)c->k_pages; p.v_pages = (const uint8_t*)c->v_pages;
   p.k_scale = c->k_scale; p.v_scale = c->v_scale; p.part = (float*)workspace;
   p.q_bs = q_batch_stride; p.q_ts = q_token_stride; p.q_hs = q_head_stride;
   p.B = (int)B; p.Sq = (int)Sq; p.Hq = (int)Hq; p.H = (int)c->H; p.G = (int)G; p.R = (int)R;
   p.rblocks = (int)rblocks;
   p.num_pages = (int)c->num_pages; p.max_pages = (int)max_pages; p.page = (int)c->page;
   p.page_log2 = c->page == 16 ? 4 : c->page == 32 ? 5 : c->page == 64 ? 6 : 7;
-  p.box = c->page < nt * 16 ? (int)c->page : nt * 16;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
-  cached::Maps maps;
-  const uint64_t mrows = (uint64_t)c->num_pages * c->H * c->page;
-  if (int e = cached::make_map(&maps.k, c->k_pages, mrows, (int)c->D, p.box)) return e;
-  if (int e = cached::make_map(&maps.v, c->v_pages, mrows, (int)c->D, p.box)) return e;
   const int grid = cached::grid_of(c->D, B, c->H, R, max_pages * c->page);
   cudaStream_t st = (cudaStream_t)stream;
   if (c->D == 64) {
-    if (nt == 1) return dtype ? cached::launch<64, true, 1>(maps, p, grid, st) : cached::launch<64, false, 1>(maps, p, grid, st);
-    return dtype ? cached::launch<64, true, 2>(maps, p, grid, st) : cached::launch<64, false, 2>(maps, p, grid, st);
+    if (nt == 1) return dtype ? cached::launch<64, true, 1>(p, grid, st) : cached::launch<64, false, 1>(p, grid, st);
+    return dtype ? cached::launch<64, true, 2>(p, grid, st) : cached::launch<64, false, 2>(p, grid, st);
   }
-  if (nt == 1) return dtype ? cached::launch<128, true, 1>(maps, p, grid, st) : cached::launch<128, false, 1>(maps, p, grid, st);
-  return dtype ? cached::launch<128, true, 2>(maps, p, grid, st) : cached::launch<128, false, 2>(maps, p, grid, st);
+  if (nt == 1) return dtype ? cached::launch<128, true, 1>(p, grid, st) : cached::launch<128, false, 1>(p, grid, st);
+  return dtype ? cached::launch<128, true, 2>(p, grid, st) : cached::launch<128, false, 2>(p, grid, st);
 }
