@@ -27,6 +27,7 @@
 //                fp32, so scales of any spread keep full precision.
 // bf16 queries are multiplied by a power of two per row into f16's range first (exact
 // but for elements 2^-29 below the row's largest).  P is rounded to f16 (2^-12).
+#include <math.h>
 #include "kv_cache.cuh"
 
 namespace kb {
@@ -48,7 +49,8 @@ struct Params {
   int rblocks;                     // row blocks per (sequence, kv head)
   int num_pages, max_pages, page;
   int page_log2;
-  float scale_log2;
+  float scale_log2;                // |softmax scale| log2 e; its sign goes into q (flip)
+  uint32_t flip;
 };
 
 KB_DEVI float ex2(float x) {
@@ -376,7 +378,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
 #pragma unroll
       for (int c = 0; c < CH * 2; ++c) {
         const uint4 x = in ? __ldg(reinterpret_cast<const uint4*>(src) + c) : make_uint4(0, 0, 0, 0);
-        raw[n][4 * c] = x.x; raw[n][4 * c + 1] = x.y; raw[n][4 * c + 2] = x.z; raw[n][4 * c + 3] = x.w;
+        raw[n][4 * c] = x.x ^ p.flip; raw[n][4 * c + 1] = x.y ^ p.flip; raw[n][4 * c + 2] = x.z ^ p.flip;
+        raw[n][4 * c + 3] = x.w ^ p.flip;
       }
     }
   };
@@ -476,36 +479,37 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
           }
         }
       }
-      // ---- softmax; lane: tokens g, g + 8 of each part, rows 2 t4, 2 t4 + 1
+      // ---- softmax; lane: tokens g, g + 8 of each part, rows 2 t4, 2 t4 + 1.  The rows' maxima
+      // are looked up over the warp only when some lane's score passes the reference by TAU.
       const bool edge = base + GT > all_seen;
       uint32_t pf[NT][NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         float t0m = -INFINITY, t1m = -INFINITY;
+        float f0[NT], f1[NT];              // score factors, kept above 0: a masked -inf stays one
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
           float* x = acc[j][n];
-          const bool gone = sk[j] < 0.f;   // a missing page
+          f0[j] = fmaxf(sk[j] * qs[n][0], 1e-37f);
+          f1[j] = fmaxf(sk[j] * qs[n][1], 1e-37f);
+          if (sk[j] < 0.f) {               // a missing page
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            x[e] *= sk[j] * qs[n][e & 1];
-            if (gone) x[e] = -INFINITY;
+            for (int e = 0; e < 4; ++e) x[e] = -INFINITY;
           }
           if (edge) {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               if (base + j * 16 + g + (e >> 1) * 8 >= seen[n][e & 1]) x[e] = -INFINITY;
           }
-          t0m = fmaxf(t0m, fmaxf(x[0], x[2]));
-          t1m = fmaxf(t1m, fmaxf(x[1], x[3]));
+          t0m = fmaxf(t0m, fmaxf(x[0], x[2]) * f0[j]);
+          t1m = fmaxf(t1m, fmaxf(x[1], x[3]) * f1[j]);
         }
+        if (__any_sync(0xffffffffu, t0m > m[n][0] + TAU || t1m > m[n][1] + TAU)) {
 #pragma unroll
-        for (int w = 4; w < 32; w <<= 1) {
-          t0m = fmaxf(t0m, __shfl_xor_sync(0xffffffffu, t0m, w));
-          t1m = fmaxf(t1m, __shfl_xor_sync(0xffffffffu, t1m, w));
-        }
-        const bool grow = t0m > m[n][0] + TAU || t1m > m[n][1] + TAU;
-        if (__any_sync(0xffffffffu, grow)) {
+          for (int w = 4; w < 32; w <<= 1) {
+            t0m = fmaxf(t0m, __shfl_xor_sync(0xffffffffu, t0m, w));
+            t1m = fmaxf(t1m, __shfl_xor_sync(0xffffffffu, t1m, w));
+          }
           const float n0 = fmaxf(m[n][0], t0m), n1 = fmaxf(m[n][1], t1m);
           const float a0 = n0 == -INFINITY ? 1.f : ex2(m[n][0] - n0), a1 = n1 == -INFINITY ? 1.f : ex2(m[n][1] - n1);
           m[n][0] = n0; m[n][1] = n1;
@@ -519,7 +523,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
           const float* x = acc[j][n];
-          const float p0 = ex2(x[0] + b0), p1 = ex2(x[1] + b1), p2 = ex2(x[2] + b0), p3 = ex2(x[3] + b1);
+          const float p0 = ex2(fmaf(x[0], f0[j], b0)), p1 = ex2(fmaf(x[1], f1[j], b1)), p2 = ex2(fmaf(x[2], f0[j], b0)),
+                      p3 = ex2(fmaf(x[3], f1[j], b1));
           l[n][0] += p0 + p2;
           l[n][1] += p1 + p3;
           pf[j][n][0] = transpose8(kv::pack16<true>(p0, p1));
@@ -876,7 +881,8 @@ extern "C" int kb200_attn_cached_fwd(const void* q, int64_t q_batch_stride, int6
   p.rblocks = (int)rblocks;
   p.num_pages = (int)c->num_pages; p.max_pages = (int)max_pages; p.page = (int)c->page;
   p.page_log2 = c->page == 16 ? 4 : c->page == 32 ? 5 : c->page == 64 ? 6 : 7;
-  p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  p.scale_log2 = fabsf(softmax_scale) * 1.4426950408889634f;
+  p.flip = softmax_scale < 0.f ? 0x80008000u : 0u;
   const int grid = cached::grid_of(c->D, B, c->H, R, max_pages * c->page);
   cudaStream_t st = (cudaStream_t)stream;
   if (c->D == 64) {

@@ -470,20 +470,24 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
         if (bad & 0x80008000u) sm.bad_v[qt] = 1;
         tc::fence_proxy_async_smem();
       }
-      // row maxima (scaled to log2 units; four lanes share a row)
+      // maxima of this lane's scores (log2 units); those of the rows, which four lanes share, are
+      // only looked up when one passes the reference by TAU
       float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
       for (int c = 0; c < 16; ++c) {
         mx0 = fmaxf(mx0, fmaxf(__uint_as_float(s[4 * c]), __uint_as_float(s[4 * c + 1])));
         mx1 = fmaxf(mx1, fmaxf(__uint_as_float(s[4 * c + 2]), __uint_as_float(s[4 * c + 3])));
       }
-      mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
-      mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
-      mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2)) * sl2;
-      mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2)) * sl2;
+      mx0 *= sl2;
+      mx1 *= sl2;
       const bool grow = __any_sync(0xffffffffu, mx0 > mref[0] + TAU || mx1 > mref[1] + TAU);
       float a0 = 1.f, a1 = 1.f;
       if (grow) {
+#pragma unroll
+        for (int w = 1; w < 4; w <<= 1) {
+          mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, w));
+          mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, w));
+        }
         const float n0 = fmaxf(mref[0], mx0), n1 = fmaxf(mref[1], mx1);
         if (n0 != -INFINITY) a0 = ex2(mref[0] - n0);
         if (n1 != -INFINITY) a1 = ex2(mref[1] - n1);

@@ -139,6 +139,21 @@ def test_prompt_extremes():
     assert (o == 0).all()
 
 
+@pytest.mark.parametrize('scale', [-0.3, 0.0, 1e-3, 2.0])
+def test_any_softmax_scale(scale):
+    g = gen(13)
+    q, k, v = (randn(g, 150, 2, 64) for _ in range(3))
+    o, lse = attention_prompt(q, k, v, i32([0, 20, 150]), softmax_scale=scale, return_lse=True)
+    want, wlse, A = ref.prompt(q, k, v, [0, 20, 150], [0, 20, 150], scale)
+    close(o, want, A * (1 + abs(scale)), torch.bfloat16)      # |q| |k| scale < 32 (1 + |scale|) * 8 here
+    assert ((lse.double() - wlse).abs() <= 2.0 ** -9 + wlse.abs() * 2.0 ** -22).all()
+    cache, table, _ = make_cache([33, 100], 2, 64, 16, 3)
+    q = randn(g, 2, 2, 2, 64)
+    o = attention_cached(q, cache, i32(table), i32([33, 100]), softmax_scale=scale)
+    want, _, A = ref.cached(q, values(cache.k_pages), values(cache.v_pages), cache.k_scale, cache.v_scale, table, [33, 100], scale)
+    close(o, want, A * (1 + abs(scale)), torch.bfloat16, u_p=2.0 ** -11)
+
+
 def test_prompt_rows_behind_the_last_sequence_and_out():
     g = gen(7)
     q, k, v = (randn(g, 300, 2, 128) for _ in range(3))
