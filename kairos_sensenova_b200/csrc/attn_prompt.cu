@@ -15,22 +15,28 @@
 // keys, most first (each CTA finds its own by a search over the levels: no host
 // knowledge of the lengths, no extra launch); the short ones fill the end of the run.
 //
-// One CTA, 18 warps (the schedule of the FP8 kernel, attn_fp8_tc.cu):
-//   warp 16    TMA producer: K and V tiles into their rings
-//   warp 17    MMA issuer:  S = Q_t K_j^T (TMEM S), O_t += P_t V_j (P_t from TMEM, V read
-//              MN-major from its TMA tile), order QK_1(j) PV_1(j-1) QK_0(j+1) PV_0(j)
-//   warps 0-15 softmax: query tile t = w / 8, 16 rows each, read as 16x256b fragments: four
-//              lanes share a row, so a row's maximum takes two shuffles and no other warp
+// One CTA, 12 warps (one idles: registers are dealt by warpgroups of four):
+//   warps 0-7  softmax: query tile t = w / 4, one row per thread (its 128 scores in registers)
+//   warp 8     TMA producer: K and V tiles into their rings
+//   warp 9     issues S = Q_t K_j^T, in the order QK_0(j) QK_1(j): the two query tiles share one
+//              TMEM score buffer, which a tile gives back as soon as its scores are in registers
+//   warp 10    issues O_t += P_t V_j (P_t from TMEM, V read MN-major from its TMA tile)
+// What a period of 256 rows x 128 keys takes is the chain QK_0 - load - QK_1 - load: each link
+// is 512 cycles of product, the two hand-offs and the load.  So the loads read whole lanes
+// (32x32b; the 16-lane shapes run at half the rate) and the two kinds of products have
+// an issuer each, so that no QK waits behind a PV's operands.
 // The row maximum is kept lazily: O and l are rescaled only when it grows by more than
 // TAU (log2 units), so P <= 2^(SHIFT + TAU) (inside f16) and most tiles rescale nothing.
 // P is rounded to the input type (half a step, as the output is); l sums the unrounded P.
 //
-// Keys that a row does not see score -inf.  In the tiles that some row does not see
-// fully, V rows behind the sequence are zeroed in shared memory, and V is looked over
-// for NaN and infinities, since 0 * NaN would reach rows that must not see them; a tile of
-// rows that meets one is computed again, row by row, over the visible keys alone.
+// Keys that a row does not see score -inf, so their P is 0.  V rows behind the sequence are
+// zeroed in shared memory before the product.  A NaN or an infinity in V at a key that a
+// row must not see still reaches it as 0 * NaN: so a row whose O is not finite is computed again,
+// by its warp, over its visible keys alone (and if one of those is the cause, the result is
+// what it should be).
 //
-// Every wait is bounded; if one gives up, the CTA drains what is in flight and writes NaN.
+// Every wait is bounded.  A warp whose wait gives up stops, so that the others' waits give up
+// too; what is in flight is drained, and the CTA writes NaN.
 #include <math.h>
 #include <string.h>
 #include "kb200_internal.h"
@@ -50,6 +56,7 @@ struct Params {
   int N, Hq, H, G;
   float scale_log2;        // |softmax scale| log2 e; its sign goes into q (flip)
   uint32_t flip;
+  uint64_t g_magic;        // ceil(2^32 / G): x / G = x g_magic >> 32 for x G < 2^32
   int causal;
 };
 
@@ -57,6 +64,24 @@ KB_DEVI float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// 2^x for a pair on the FMA pipe: x = j + f, f in [-1/2, 1/2], by adding and taking away 1.5 * 2^23;
+// 2^f by a polynomial of degree 4 (least squares on the relative error, reweighted towards the
+// largest: 2.9e-6), times 2^j by its exponent field, which is 0 at j = -127: x below -126 gives 0.
+// A NaN stays one.
+KB_DEVI float2 exp2_poly(float2 x) {
+  constexpr float C = 12582912.f;
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.x));      // -127
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.y));
+  const float2 t = fadd2(x, make_float2(C, C));
+  const float2 j = fadd2(t, make_float2(-C, -C));
+  const float2 f = ffma2(j, make_float2(-1.f, -1.f), x);
+  float2 q = ffma2(make_float2(0.00958285323f, 0.00958285323f), f, make_float2(0.055906426f, 0.055906426f));
+  q = ffma2(q, f, make_float2(0.240240986f, 0.240240986f));
+  q = ffma2(q, f, make_float2(0.693124193f, 0.693124193f));
+  q = ffma2(q, f, make_float2(1.f, 1.f));
+  return fmul2(q, make_float2(__int_as_float((__float_as_int(t.x) << 23) + 0x3f800000),
+                              __int_as_float((__float_as_int(t.y) << 23) + 0x3f800000)));
 }
 // [start, end) of sequence s in the packed tokens, inside [0, T].
 KB_DEVI int2 seq_range(const int32_t* cu, int s, int64_t T) {
@@ -113,7 +138,10 @@ KB_DEVI void attend_row(const Params& p, int64_t tq, int h, int64_t k0, int64_t 
 
 constexpr int BM = 128, BN = 128, QT = 2, ROWS = QT * BM;
 constexpr float SHIFT = 6.f, TAU = 8.f;      // P = 2^(s - m + SHIFT) <= 2^14
-constexpr int THREADS = 18 * 32;
+constexpr int THREADS = 12 * 32;
+// Registers: the launch gives each thread 168 (its 384 threads share the SM's 65536); the softmax
+// warpgroups take 208 and the third leaves itself 88, 2 * 208 + 88 = 3 * 168.
+constexpr int REGS_SOFTMAX = 208, REGS_OTHERS = 88;
 constexpr int SORTED = 64;                   // up to this many sequences the tiles are sorted by their keys
 constexpr uint32_t TM_O = 0, TM_S = 256, TM_P = 384;   // TMEM columns: O_t at 128 t, S, P_t at 64 t
 
@@ -130,10 +158,10 @@ struct Smem {
   uint8_t v[VS][ATOMS][BN * 128];
   uint64_t q_full;
   uint64_t k_full[KS], k_empty[KS], v_full[VS], v_empty[VS];
-  uint64_t s_full[QT], s_free[QT], p_full[QT], pv_done[QT], o_done, drain;
+  uint64_t s_full[QT], s_free[QT], p_full[QT], pv_done[QT], o_done, drain[2];
   uint32_t tmem_base;
   int seq, tile;                             // this CTA's sequence (-1: none) and row tile in it
-  int bad_v[QT];
+  int4 range;                                // its queries and keys
   int abort_flag, keep_tmem;
 };
 
@@ -211,9 +239,15 @@ KB_DEVI void warp_arrive(uint64_t* bar, int lane) {
   if (lane == 0) tc::mbar_arrive(bar);
 }
 
+// Which of every 8 pairs of exponentials go to the FMA pipe.
+#ifndef KB_POLY
+#define KB_POLY (D == 128 ? 0x88 : 0x88)
+#endif
+
 template <int D, bool F16>
 __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_constant__ Maps maps, Params p) {
   using SM = Smem<D>;
+  constexpr int POLY = KB_POLY;
   constexpr int KS = SM::KS, VS = SM::VS, ATOMS = SM::ATOMS;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   SM& sm = *reinterpret_cast<SM*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
@@ -226,10 +260,14 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
     if (lane == 0) {
       sm.seq = s;
       sm.tile = t;
+      if (s >= 0) {
+        const int2 q = seq_range(p.cu_q, s, p.Tq), k = seq_range(p.cu_k, s, p.Tk);
+        sm.range = make_int4(q.x, q.y, k.x, k.y);
+      }
     }
-  } else if (warp == 16) {
+  } else if (warp == 8) {
     if (lane == 0) {
-      tc::mbar_init(&sm.q_full, 16);
+      tc::mbar_init(&sm.q_full, 8);
       for (int s = 0; s < KS; ++s) {
         tc::mbar_init(&sm.k_full[s], 1);
         tc::mbar_init(&sm.k_empty[s], 1);
@@ -240,20 +278,20 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
       }
       for (int i = 0; i < QT; ++i) {
         tc::mbar_init(&sm.s_full[i], 1);
-        tc::mbar_init(&sm.s_free[i], 8);
-        tc::mbar_init(&sm.p_full[i], 8);
+        tc::mbar_init(&sm.s_free[i], 4);
+        tc::mbar_init(&sm.p_full[i], 4);
         tc::mbar_init(&sm.pv_done[i], 1);
-        sm.bad_v[i] = 0;
       }
       tc::mbar_init(&sm.o_done, 1);
-      tc::mbar_init(&sm.drain, 1);
+      tc::mbar_init(&sm.drain[0], 1);
+      tc::mbar_init(&sm.drain[1], 1);
       sm.abort_flag = 0;
       sm.keep_tmem = 0;
       tc::fence_barrier_init();
       tc::prefetch_tmap(&maps.k);
       tc::prefetch_tmap(&maps.v);
     }
-  } else if (warp == 17) {
+  } else if (warp == 9) {
     tc::tmem_alloc(&sm.tmem_base, 512);
     tc::tmem_relinquish();
   }
@@ -263,31 +301,32 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
   const uint32_t tmem = sm.tmem_base;
   const int seq = sm.seq;
   if (seq < 0) {
-    if (warp == 17) tc::tmem_dealloc(tmem, 512);
+    if (warp == 9) tc::tmem_dealloc(tmem, 512);
     return;
   }
-  const int2 rq = seq_range(p.cu_q, seq, p.Tq), rk = seq_range(p.cu_k, seq, p.Tk);
+  const int2 rq = make_int2(sm.range.x, sm.range.y), rk = make_int2(sm.range.z, sm.range.w);
   const int n = rq.y - rq.x, m = rk.y - rk.x;
   const int64_t row0 = (int64_t)sm.tile * ROWS;              // first row (token * G + head)
   const int64_t nrows = min((int64_t)ROWS, (int64_t)n * p.G - row0);
   // keys that token t of the sequence sees
   auto seen_by = [&](int64_t t) { return p.causal ? (int)min((int64_t)m, max((int64_t)0, t + 1 + m - n)) : m; };
   const int ntiles = (seen_by((row0 + nrows - 1) / p.G) + BN - 1) / BN;
+  const int full = seen_by(row0 / p.G) / BN;                 // key tiles below are seen fully by every row
   auto aborted = [&]() { return *((volatile int*)&sm.abort_flag) != 0; };
 
-  if (warp == 16) {
+  if (warp >= 8) {
+    tc::setmaxnreg_dec<REGS_OTHERS>();
+  if (warp == 8) {
     // ------------------------------------------------------------ TMA producer
     if (lane == 0 && ntiles > 0) {
       int kiss = 0, viss = 0;
       for (int j = 0; j < ntiles; ++j) {
         const int sk = j % KS, sv = j % VS, tok = rk.x + j * BN;
         if (j >= KS && !tc::mbar_wait(&sm.k_empty[sk], (j / KS - 1) & 1)) { sm.abort_flag = 1; break; }
-        if (aborted()) break;
         tc::mbar_expect_tx(&sm.k_full[sk], ATOMS * BN * 128);
         for (int a = 0; a < ATOMS; ++a) tc::tma_load_3d(sm.k[sk][a], &maps.k, &sm.k_full[sk], a * 64, hk, tok);
         ++kiss;
         if (j >= VS && !tc::mbar_wait(&sm.v_empty[sv], (j / VS - 1) & 1)) { sm.abort_flag = 1; break; }
-        if (aborted()) break;
         tc::mbar_expect_tx(&sm.v_full[sv], ATOMS * BN * 128);
         for (int a = 0; a < ATOMS; ++a) tc::tma_load_3d(sm.v[sv][a], &maps.v, &sm.v_full[sv], a * 64, hk, tok);
         ++viss;
@@ -298,309 +337,271 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
       for (int j = viss > VS ? viss - VS : 0; j < viss; ++j) drained &= tc::mbar_wait(&sm.v_full[j % VS], (j / VS) & 1);
       if (!drained) { sm.abort_flag = 1; sm.keep_tmem = 1; }
     }
-  } else if (warp == 17) {
-    // ------------------------------------------------------------ MMA issuer
+  } else if (warp == 9 || warp == 10) {
+    // ------------------------------------------------------------ MMA issuers
     // The whole warp runs the schedule, so every operand is warp-uniform; one elected lane issues.
     if (ntiles > 0) {
       const bool leader = tc::elect_one();
-      constexpr uint32_t IDESC_QK = tc::idesc_f32acc(F16 ? 0 : 1, BM, BN, 0, 0);
-      constexpr uint32_t IDESC_PV = tc::idesc_f32acc(F16 ? 0 : 1, BM, D, 0, 1);
       constexpr uint64_t ATOM = BN * 128 / 16;               // descriptor units between 64-channel atoms
       const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
-      const uint64_t dq0 = tc::sdesc_sw128_kmajor(sm.q[0][0]);
-      const uint64_t dk0 = tc::sdesc_sw128_kmajor(sm.k[0][0]);
-      const uint64_t dv0 = tc::sdesc_sw128_mnmajor(sm.v[0][0], BN * 128);
-      auto commit = [&](uint64_t* bar) {
-        if (leader) tc::tc_commit(bar);
-        __syncwarp();
-      };
-      auto qk = [&](int t, int j) {   // S = Q_t K_j^T
-        const uint64_t dq = dq0 + (uint64_t)(t * ATOMS) * ATOM, dk = dk0 + (uint64_t)((j % KS) * ATOMS) * ATOM;
-        if (leader) {
-#pragma unroll
-          for (int ks = 0; ks < D / 16; ++ks)
-            tc::mma_bf16(tmem_u + TM_S, dq + (ks >> 2) * ATOM + 2 * (ks & 3), dk + (ks >> 2) * ATOM + 2 * (ks & 3), IDESC_QK,
-                         ks > 0 ? 1u : 0u);
-          tc::tc_commit(&sm.s_full[t]);
-        }
-        __syncwarp();
-      };
-      auto pv = [&](int t, int j) {   // O_t += P_t V_j, 16 keys per instruction
-        const uint64_t dv = dv0 + (uint64_t)((j % VS) * ATOMS) * ATOM;
-        if (leader) {
-#pragma unroll
-          for (int ks = 0; ks < BN / 16; ++ks)
-            tc::mma_bf16_ts(tmem_u + TM_O + t * 128, tmem_u + TM_P + t * 64 + ks * 8, dv + ks * (16 * 128 / 16), IDESC_PV,
-                            (j > 0 || ks > 0) ? 1u : 0u);
-          tc::tc_commit(&sm.pv_done[t]);
-        }
-        __syncwarp();
-      };
-      // a probe of the next phase goes out before the current group, so its latency overlaps the issue
-      auto probe = [&](uint64_t* bar, uint32_t parity) { return tc::mbar_test_wait(bar, parity); };
-      auto finish = [&](uint64_t* bar, uint32_t parity, bool pre) {
-        const bool w = __all_sync(0xffffffffu, pre || tc::mbar_test_wait_loop(bar, parity));
-        if (!w) sm.abort_flag = 1;
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        const bool w = __all_sync(0xffffffffu, tc::mbar_wait(bar, parity));
+        tc::tc_fence_after();
         return w;
       };
-      bool ok = __all_sync(0xffffffffu, tc::mbar_wait(&sm.q_full, 0) && tc::mbar_wait(&sm.k_full[0], 0));
+      bool ok = true;
+      if (warp == 9) {
+        constexpr uint32_t IDESC_QK = tc::idesc_f32acc(F16 ? 0 : 1, BM, BN, 0, 0);
+        const uint64_t dq0 = tc::sdesc_sw128_kmajor(sm.q[0][0]);
+        const uint64_t dk0 = tc::sdesc_sw128_kmajor(sm.k[0][0]);
+        auto qk = [&](int t, int j) {   // S = Q_t K_j^T
+          const uint64_t dq = dq0 + (uint64_t)(t * ATOMS) * ATOM, dk = dk0 + (uint64_t)((j % KS) * ATOMS) * ATOM;
+          if (leader) {
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ++ks)
+              tc::mma_bf16(tmem_u + TM_S, dq + (ks >> 2) * ATOM + 2 * (ks & 3), dk + (ks >> 2) * ATOM + 2 * (ks & 3), IDESC_QK,
+                           ks > 0 ? 1u : 0u);
+            tc::tc_commit(&sm.s_full[t]);
+            if (t == 1) tc::tc_commit(&sm.k_empty[j % KS]);
+          }
+          __syncwarp();
+        };
+        ok = wait(&sm.q_full, 0) && wait(&sm.k_full[0], 0);
+        if (ok) qk(0, 0);
+        for (int j = 0; ok && j < ntiles; ++j) {
+          ok = wait(&sm.s_free[0], j & 1);
+          if (!ok) break;
+          qk(1, j);
+          if (j + 1 < ntiles) {
+            ok = wait(&sm.k_full[(j + 1) % KS], ((j + 1) / KS) & 1) && wait(&sm.s_free[1], j & 1);
+            if (ok) qk(0, j + 1);
+          }
+        }
+      } else {
+        constexpr uint32_t IDESC_PV = tc::idesc_f32acc(F16 ? 0 : 1, BM, D, 0, 1);
+        const uint64_t dv0 = tc::sdesc_sw128_mnmajor(sm.v[0][0], BN * 128);
+        for (int j = 0; ok && j < ntiles; ++j) {
+          ok = wait(&sm.v_full[j % VS], (j / VS) & 1);
+          if (ok && (j + 1) * BN > m) {                      // the sequence ends in this tile
+            uint4* v = reinterpret_cast<uint4*>(sm.v[j % VS][0]);
+            for (int a = 0; a < ATOMS; ++a)
+              for (int i = (m - j * BN) * 8 + lane; i < BN * 8; i += 32) v[a * BN * 8 + i] = make_uint4(0, 0, 0, 0);
+            tc::fence_proxy_async_smem();
+            __syncwarp();
+          }
+          const uint64_t dv = dv0 + (uint64_t)((j % VS) * ATOMS) * ATOM;
+          for (int t = 0; ok && t < QT; ++t) {               // O_t += P_t V_j, 16 keys per instruction
+            ok = wait(&sm.p_full[t], j & 1);
+            if (ok && leader) {
+#pragma unroll
+              for (int ks = 0; ks < BN / 16; ++ks)
+                tc::mma_bf16_ts(tmem_u + TM_O + t * 128, tmem_u + TM_P + t * 64 + ks * 8, dv + ks * (16 * 128 / 16), IDESC_PV,
+                                (j > 0 || ks > 0) ? 1u : 0u);
+              tc::tc_commit(&sm.pv_done[t]);
+              if (t == 1) tc::tc_commit(&sm.v_empty[j % VS]);
+            }
+            __syncwarp();
+          }
+        }
+        if (ok && leader) tc::tc_commit(&sm.o_done);
+        __syncwarp();
+      }
       if (!ok) sm.abort_flag = 1;
-      if (ok) {
-        tc::tc_fence_after();
-        qk(0, 0);
-      }
-      bool pre_s0 = probe(&sm.s_free[0], 0);
-      for (int j = 0; ok && j < ntiles; ++j) {
-        const bool last = j + 1 == ntiles;
-        const int kn = (j + 1) % KS, vn = j % VS;
-        if (!finish(&sm.s_free[0], j & 1, pre_s0) || aborted()) { ok = false; break; }
-        tc::tc_fence_after();
-        const bool pre_p1 = j >= 1 ? probe(&sm.p_full[1], (j - 1) & 1) : true;
-        qk(1, j);
-        commit(&sm.k_empty[j % KS]);
-        bool pre_s1 = false, pre_k = true;
-        if (j >= 1) {
-          if (!finish(&sm.p_full[1], (j - 1) & 1, pre_p1)) { ok = false; break; }
-          tc::tc_fence_after();
-          pre_s1 = probe(&sm.s_free[1], j & 1);
-          if (!last) pre_k = probe(&sm.k_full[kn], ((j + 1) / KS) & 1);
-          pv(1, j - 1);
-          commit(&sm.v_empty[(j - 1) % VS]);
-        } else if (!last) {
-          pre_s1 = probe(&sm.s_free[1], j & 1);
-          pre_k = probe(&sm.k_full[kn], ((j + 1) / KS) & 1);
-        }
-        bool pre_p0, pre_v;
-        if (!last) {
-          if (!finish(&sm.k_full[kn], ((j + 1) / KS) & 1, pre_k)) { ok = false; break; }
-          if (!finish(&sm.s_free[1], j & 1, pre_s1)) { ok = false; break; }
-          tc::tc_fence_after();
-          pre_p0 = probe(&sm.p_full[0], j & 1);
-          pre_v = probe(&sm.v_full[vn], (j / VS) & 1);
-          qk(0, j + 1);
-        } else {
-          pre_p0 = probe(&sm.p_full[0], j & 1);
-          pre_v = probe(&sm.v_full[vn], (j / VS) & 1);
-        }
-        if (!finish(&sm.v_full[vn], (j / VS) & 1, pre_v)) { ok = false; break; }
-        if (!finish(&sm.p_full[0], j & 1, pre_p0)) { ok = false; break; }
-        tc::tc_fence_after();
-        pre_s0 = last ? true : probe(&sm.s_free[0], (j + 1) & 1);
-        pv(0, j);
-      }
-      if (ok) {   // PV_1 of the last key tile
-        const int j = ntiles - 1;
-        if (finish(&sm.p_full[1], j & 1, false)) {
-          tc::tc_fence_after();
-          pv(1, j);
-          commit(&sm.o_done);
-        }
-      }
-      commit(&sm.drain);   // every MMA this warp issued must complete before TMEM is freed
-      if (!__all_sync(0xffffffffu, tc::mbar_wait(&sm.drain, 0))) {
+      // every MMA this warp issued must complete before TMEM is freed
+      if (leader) tc::tc_commit(&sm.drain[warp - 9]);
+      __syncwarp();
+      if (!__all_sync(0xffffffffu, tc::mbar_wait(&sm.drain[warp - 9], 0))) {
         sm.abort_flag = 1;
         sm.keep_tmem = 1;
       }
     }
+  }
   } else {
-    // ------------------------------------------------------------ softmax (warps 0..15)
+    // ------------------------------------------------------------ softmax
+    tc::setmaxnreg_inc<REGS_SOFTMAX>();
     // Q into shared memory: 256 rows of D channels, 16 bytes at a time
     const uint32_t flip = p.flip;                            // 0x80008000: a negative scale, moved into q
-    for (int i = tid; ntiles > 0 && i < ROWS * (D / 8); i += 512) {
-      const int r = i / (D / 8), c = i % (D / 8);
-      uint4 x = make_uint4(0, 0, 0, 0);
-      if (r < nrows) {
-        const int64_t R = row0 + r, tok = R / p.G;
-        x = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(p.q) +
-                                                 2 * ((rq.x + tok) * p.q_ts + (hk * p.G + (R - tok * p.G)) * p.q_hs + c * 8)));
-        x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
+    constexpr int CPR = D / 8, BATCH = 8;                    // 16-byte chunks of a row; loads in flight per thread
+    const int64_t tok0 = row0 / p.G;
+    const uint32_t rem0 = (uint32_t)(row0 - tok0 * p.G);
+    // token of row r of the tile (from tok0) and head in the group
+    auto split = [&](int r, int& dt, int& hg) {
+      const uint32_t x = rem0 + r;
+      dt = (int)((x * p.g_magic) >> 32);
+      hg = (int)(x - dt * p.G);
+    };
+    const char* qbase = reinterpret_cast<const char*>(p.q) + 2 * ((rq.x + tok0) * p.q_ts + (int64_t)hk * p.G * p.q_hs);
+    if (ntiles > 0) {
+#pragma unroll 1
+      for (int i0 = tid; i0 < ROWS * CPR; i0 += 256 * BATCH) {
+        uint4 x[BATCH];
+#pragma unroll
+        for (int z = 0; z < BATCH; ++z) {
+          const int i = i0 + z * 256, r = i / CPR, c = i % CPR;
+          x[z] = make_uint4(0, 0, 0, 0);
+          if (r < nrows) {
+            int dt, hg;
+            split(r, dt, hg);
+            x[z] = __ldg(reinterpret_cast<const uint4*>(qbase + 2 * (dt * p.q_ts + hg * p.q_hs + c * 8)));
+          }
+        }
+#pragma unroll
+        for (int z = 0; z < BATCH; ++z) {
+          const int i = i0 + z * 256, r = i / CPR, c = i % CPR, rr = r % BM;
+          x[z].x ^= flip; x[z].y ^= flip; x[z].z ^= flip; x[z].w ^= flip;
+          *reinterpret_cast<uint4*>(&sm.q[r / BM][c / 8][rr * 128 + (((c % 8) ^ (rr & 7)) << 4)]) = x[z];
+        }
       }
-      const int rr = r % BM;
-      *reinterpret_cast<uint4*>(&sm.q[r / BM][c / 8][rr * 128 + (((c % 8) ^ (rr & 7)) << 4)]) = x;
     }
     tc::fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) tc::mbar_arrive(&sm.q_full);
 
-    const int qt = warp >> 3, w8 = warp & 7;
-    const int rbase = (warp & 3) * 32 + (w8 >> 2) * 16;      // this warp's first row == TMEM lane
-    const int g = lane >> 2, t4 = lane & 3;
-    const uint32_t lane_off = (uint32_t)rbase << 16;
+    const int qt = warp >> 2, w4 = warp & 3;
+    const int r = qt * BM + w4 * 32 + lane;                  // this thread's row; its TMEM lane is r % 128
+    const uint32_t lane_off = (uint32_t)(w4 * 32) << 16;
     const uint32_t tS = tmem + TM_S + lane_off, tO = tmem + TM_O + qt * 128 + lane_off, tP = tmem + TM_P + qt * 64 + lane_off;
     const float sl2 = p.scale_log2;
-    int lim[2];                                              // keys that rows g, g + 8 see
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = qt * BM + rbase + g + 8 * i;
-      lim[i] = r < nrows ? seen_by((row0 + r) / p.G) : 0x7fffffff;
-    }
-    // key tiles below are seen fully by every row of this query tile
-    const int full = qt * BM < nrows ? seen_by((row0 + qt * BM) / p.G) / BN : 0x7fffffff;
-    float mref[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    const bool live = r < nrows;
+    int my_dt, my_hg;
+    split(r, my_dt, my_hg);
+    const int lim = live ? seen_by(tok0 + my_dt) : 0x7fffffff;   // keys that the row sees
+    float mref = -INFINITY, l = 0.f;
     bool ok = true;
     for (int j = 0; j < ntiles; ++j) {
       if (!tc::mbar_wait(&sm.s_full[qt], j & 1)) { sm.abort_flag = 1; ok = false; }
-      if (__any_sync(0xffffffffu, !ok || aborted())) { ok = false; break; }
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
       tc::tc_fence_after();
-      uint32_t s[64];                                        // [8-column group][row g: 2, row g + 8: 2]
-      tc::tmem_ld16x256b_x16(tS, s);
+      uint32_t s[128];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tc::tmem_ld32(tS + c * 32, s + c * 32);
       tc::tmem_wait_ld();
       warp_arrive(&sm.s_free[qt], lane);
       if (j >= full) {
-        const int key0 = j * BN + 2 * t4;
+        const int end = lim - j * BN;
 #pragma unroll
-        for (int c = 0; c < 64; ++c)
-          if (key0 + (c >> 2) * 8 + (c & 1) >= lim[(c >> 1) & 1]) s[c] = __float_as_uint(-INFINITY);
-        // V of this tile: rows behind the sequence become 0; NaN and infinities are reported
-        if (!tc::mbar_wait(&sm.v_full[j % VS], (j / VS) & 1)) { sm.abort_flag = 1; ok = false; }
-        if (__any_sync(0xffffffffu, !ok)) break;
-        constexpr uint32_t EXP = F16 ? 0x7c007c00u : 0x7f807f80u, ONE = F16 ? 0x04000400u : 0x00800080u;
-        uint32_t bad = 0;
-        uint8_t* vb = sm.v[j % VS][0];
-#pragma unroll 1
-        for (int i = w8 * 32 + lane; i < ATOMS * BN * 8; i += 256) {
-          uint4* x = reinterpret_cast<uint4*>(vb) + i;       // 8 chunks per 128-byte row
-          if (j * BN + ((i >> 3) & (BN - 1)) >= m) {
-            *x = make_uint4(0, 0, 0, 0);
-          } else {
-            const uint4 y = *x;
-            bad |= ((y.x & EXP) + ONE) | ((y.y & EXP) + ONE) | ((y.z & EXP) + ONE) | ((y.w & EXP) + ONE);
+        for (int c0 = 0; c0 < BN; c0 += 32)
+          if (__any_sync(0xffffffffu, end < c0 + 32)) {
+#pragma unroll
+            for (int c = c0; c < c0 + 32; ++c)
+              if (c >= end) s[c] = __float_as_uint(-INFINITY);
           }
-        }
-        if (bad & 0x80008000u) sm.bad_v[qt] = 1;
-        tc::fence_proxy_async_smem();
       }
-      // maxima of this lane's scores (log2 units); those of the rows, which four lanes share, are
-      // only looked up when one passes the reference by TAU
-      float mx0 = -INFINITY, mx1 = -INFINITY;
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        mx0 = fmaxf(mx0, fmaxf(__uint_as_float(s[4 * c]), __uint_as_float(s[4 * c + 1])));
-        mx1 = fmaxf(mx1, fmaxf(__uint_as_float(s[4 * c + 2]), __uint_as_float(s[4 * c + 3])));
-      }
-      mx0 *= sl2;
-      mx1 *= sl2;
-      const bool grow = __any_sync(0xffffffffu, mx0 > mref[0] + TAU || mx1 > mref[1] + TAU);
-      float a0 = 1.f, a1 = 1.f;
+      for (int c = 0; c < BN; c += 8)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          mx[i] = fmaxf(mx[i], fmaxf(__uint_as_float(s[c + 2 * i]), __uint_as_float(s[c + 2 * i + 1])));
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
+      const bool grow = __any_sync(0xffffffffu, top > mref + TAU);
+      float alpha = 1.f;
       if (grow) {
-#pragma unroll
-        for (int w = 1; w < 4; w <<= 1) {
-          mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, w));
-          mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, w));
-        }
-        const float n0 = fmaxf(mref[0], mx0), n1 = fmaxf(mref[1], mx1);
-        if (n0 != -INFINITY) a0 = ex2(mref[0] - n0);
-        if (n1 != -INFINITY) a1 = ex2(mref[1] - n1);
-        mref[0] = n0;
-        mref[1] = n1;
-        l[0] *= a0;
-        l[1] *= a1;
+        const float mn = fmaxf(mref, top);
+        if (mn != -INFINITY) alpha = ex2(mref - mn);
+        mref = mn;
+        l *= alpha;
       }
       // (no key of the row seen yet: every score here is -inf, and so is x)
-      const float b0 = mref[0] == -INFINITY ? 0.f : SHIFT - mref[0], b1 = mref[1] == -INFINITY ? 0.f : SHIFT - mref[1];
-      const float2 sc = make_float2(sl2, sl2), bias0 = make_float2(b0, b0), bias1 = make_float2(b1, b1);
-      float2 ls0 = make_float2(0.f, 0.f), ls1 = make_float2(0.f, 0.f);
-      uint32_t pk[32];
+      const float b0 = mref == -INFINITY ? 0.f : SHIFT - mref;
+      const float2 sc = make_float2(sl2, sl2), bias = make_float2(b0, b0);
+      float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        const float2 x = ffma2(make_float2(__uint_as_float(s[4 * c]), __uint_as_float(s[4 * c + 1])), sc, bias0);
-        const float2 y = ffma2(make_float2(__uint_as_float(s[4 * c + 2]), __uint_as_float(s[4 * c + 3])), sc, bias1);
-        const float2 e = make_float2(ex2(x.x), ex2(x.y)), f = make_float2(ex2(y.x), ex2(y.y));
-        ls0 = fadd2(ls0, e);
-        ls1 = fadd2(ls1, f);
-        pk[2 * c] = kv::pack16<F16>(e.x, e.y);
-        pk[2 * c + 1] = kv::pack16<F16>(f.x, f.y);
+      for (int h = 0; h < 2; ++h) {
+        uint32_t pk[32];
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          const int i = h * 64 + 2 * c;
+          const float2 x = ffma2(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), sc, bias);
+          const float2 e = ((POLY >> (c & 7)) & 1) ? exp2_poly(x) : make_float2(ex2(x.x), ex2(x.y));
+          ls[c & 1] = fadd2(ls[c & 1], e);
+          pk[c] = kv::pack16<F16>(e.x, e.y);
+        }
+        if (h == 0) {
+          // P_t(j) overwrites P_t(j-1) and O_t may be rescaled: PV_t(j-1) must have completed
+          if (j >= 1 && !tc::mbar_wait(&sm.pv_done[qt], (j - 1) & 1)) { sm.abort_flag = 1; ok = false; }
+          ok = __all_sync(0xffffffffu, ok);
+          tc::tc_fence_after();
+        }
+        if (ok) tc::tmem_st32(tP + h * 32, pk);
       }
-      l[0] += ls0.x + ls0.y;
-      l[1] += ls1.x + ls1.y;
-      // P_t(j) overwrites P_t(j-1) and O_t may be rescaled: PV_t(j-1) must have completed
-      if (j >= 1 && !tc::mbar_wait(&sm.pv_done[qt], (j - 1) & 1)) { sm.abort_flag = 1; ok = false; }
-      if (__any_sync(0xffffffffu, !ok)) break;
-      tc::tc_fence_after();
-      tc::tmem_st16x128b_x16(tP, pk);
+      if (!ok) break;
+      l += (ls[0].x + ls[0].y) + (ls[1].x + ls[1].y);
       if (grow && j >= 1) {
 #pragma unroll 1
-        for (int c = 0; c < D / 64; ++c) {
+        for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
-          tc::tmem_ld16x256b_x8(tO + c * 64, o);
+          tc::tmem_ld32(tO + c * 32, o);
           tc::tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * ((e & 2) ? a1 : a0));
-          tc::tmem_st16x256b_x8(tO + c * 64, o);
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+          tc::tmem_st32(tO + c * 32, o);
         }
       }
       tc::tmem_wait_st();
       warp_arrive(&sm.p_full[qt], lane);
     }
-    // ---- epilogue: this warp's 16 rows, through its part of the Q tile (every product has read Q)
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-    }
+    // ---- epilogue
     if (ok && ntiles > 0) ok = __all_sync(0xffffffffu, tc::mbar_wait(&sm.o_done, 0));
     if (!ok) sm.abort_flag = 1;
-    tc::bar_sync_named(1 + qt, 256);                         // bad_v of the whole query tile
-    const bool bad = *((volatile int*)&sm.bad_v[qt]) != 0;
-    if (bad) {
-      for (int i = 0; i < 16; ++i) {
-        const int r = qt * BM + rbase + i;
-        if (r >= nrows) break;
-        const int64_t R = row0 + r, tok = R / p.G;
-        attend_row<D, F16>(p, rq.x + tok, (int)(hk * p.G + (R - tok * p.G)), rk.x, seen_by(tok), lane);
-      }
-    } else {
-      tc::tc_fence_after();
-      static_assert(sizeof(sm.q[0]) == 8 * 16 * D * 2, "the staged rows are the Q tile's size");
-      const bool dead = aborted();
-      uint8_t* stage = sm.q[qt][0] + w8 * 16 * (D * 2);      // 16 rows of D * 2 bytes, chunks rotated by the row
+    tc::tc_fence_after();
+    const float f = !ok || aborted() ? NAN : l == 0.f ? 0.f : 1.f / l;
+    // through this warp's part of the Q tile (every product has read Q), so that rows are stored whole
+    uint8_t* stage = sm.q[qt][0] + w4 * 32 * (D * 2);
+    bool finite = true;
 #pragma unroll
-      for (int c = 0; c < D / 64; ++c) {
-        uint32_t o[32];
-        if (ntiles > 0 && ok) {
-          tc::tmem_ld16x256b_x8(tO + c * 64, o);
-          tc::tmem_wait_ld();
-        } else {
+    for (int c = 0; c < D / 32; ++c) {
+      uint32_t o[32];
+      if (ntiles > 0 && ok) {
+        tc::tmem_ld32(tO + c * 32, o);
+        tc::tmem_wait_ld();
+      } else {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0;
-        }
-        const float f0 = dead ? NAN : l[0] == 0.f ? 0.f : 1.f / l[0], f1 = dead ? NAN : l[1] == 0.f ? 0.f : 1.f / l[1];
+        for (int e = 0; e < 32; ++e) o[e] = 0;
+      }
+      float worst = 0.f;                                     // NaN if some value is not finite: inf - inf
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {                        // 16-byte chunk: 8 channels
-          const int ch = c * 8 + k;
-          *reinterpret_cast<uint32_t*>(stage + g * (D * 2) + (((ch ^ g) & (D / 8 - 1)) << 4) + t4 * 4) =
-              kv::pack16<F16>(__uint_as_float(o[4 * k]) * f0, __uint_as_float(o[4 * k + 1]) * f0);
-          *reinterpret_cast<uint32_t*>(stage + (g + 8) * (D * 2) + (((ch ^ g) & (D / 8 - 1)) << 4) + t4 * 4) =
-              kv::pack16<F16>(__uint_as_float(o[4 * k + 2]) * f1, __uint_as_float(o[4 * k + 3]) * f1);
-        }
-      }
-      __syncwarp();
-#pragma unroll 4
-      for (int i = lane; i < 16 * (D / 8); i += 32) {
-        const int rr = i / (D / 8), ch = i % (D / 8), r = qt * BM + rbase + rr;
-        if (r < nrows) {
-          const int64_t R = row0 + r, tok = R / p.G;
-          const uint4 x = *reinterpret_cast<const uint4*>(stage + rr * (D * 2) + (((ch ^ (rr & 7)) & (D / 8 - 1)) << 4));
-          *reinterpret_cast<uint4*>(reinterpret_cast<char*>(p.o) +
-                                    2 * ((rq.x + tok) * p.o_ts + (hk * p.G + (R - tok * p.G)) * p.o_hs + ch * 8)) = x;
-        }
-      }
-      if (p.lse && t4 == 0) {
+      for (int e = 0; e < 32; ++e) worst = fmaf(__uint_as_float(o[e]), 0.f, worst);
+      finite &= worst == 0.f;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int r = qt * BM + rbase + g + 8 * i;
-          if (r < nrows) {
-            const int64_t R = row0 + r, tok = R / p.G;
-            p.lse[(rq.x + tok) * p.Hq + hk * p.G + (R - tok * p.G)] =
-                l[i] == 0.f ? -INFINITY : (mref[i] - SHIFT + log2f(l[i])) * 0.6931471805599453f;
-          }
-        }
+      for (int z = 0; z < 4; ++z) {
+        uint4 x;
+        x.x = kv::pack16<F16>(__uint_as_float(o[8 * z + 0]) * f, __uint_as_float(o[8 * z + 1]) * f);
+        x.y = kv::pack16<F16>(__uint_as_float(o[8 * z + 2]) * f, __uint_as_float(o[8 * z + 3]) * f);
+        x.z = kv::pack16<F16>(__uint_as_float(o[8 * z + 4]) * f, __uint_as_float(o[8 * z + 5]) * f);
+        x.w = kv::pack16<F16>(__uint_as_float(o[8 * z + 6]) * f, __uint_as_float(o[8 * z + 7]) * f);
+        *reinterpret_cast<uint4*>(stage + lane * (D * 2) + (((c * 4 + z) ^ (lane & 7)) << 4)) = x;
       }
+    }
+    __syncwarp();
+    char* obase = reinterpret_cast<char*>(p.o) + 2 * ((rq.x + tok0) * p.o_ts + (int64_t)hk * p.G * p.o_hs);
+#pragma unroll 8
+    for (int z = 0; z < CPR; ++z) {                          // 32 / CPR rows at a time
+      const int i = z * 32 + lane, rr = i / CPR, ch = i % CPR, ri = qt * BM + w4 * 32 + rr;
+      const uint4 x = *reinterpret_cast<const uint4*>(stage + rr * (D * 2) + ((ch ^ (rr & 7)) << 4));
+      if (ri < nrows) {
+        int dt, hg;
+        split(ri, dt, hg);
+        *reinterpret_cast<uint4*>(obase + 2 * (dt * p.o_ts + hg * p.o_hs + ch * 8)) = x;
+      }
+    }
+    if (p.lse && live)
+      p.lse[(rq.x + tok0 + my_dt) * p.Hq + hk * p.G + my_hg] =
+          l == 0.f ? -INFINITY : (mref - SHIFT + log2f(l)) * 0.6931471805599453f;
+    uint32_t again = __ballot_sync(0xffffffffu, live && ok && !finite);
+    __syncwarp();
+    while (again) {
+      const int i = __ffs(again) - 1;
+      again &= again - 1;
+      int dt, hg;
+      split(qt * BM + w4 * 32 + i, dt, hg);
+      attend_row<D, F16>(p, rq.x + tok0 + dt, hk * p.G + hg, rk.x, seen_by(tok0 + dt), lane);
     }
   }
   tc::tc_fence_before();
   __syncthreads();
-  if (warp == 17 && !sm.keep_tmem) {
+  if (warp == 9 && !sm.keep_tmem) {
     tc::tc_fence_after();
     tc::tmem_dealloc(tmem, 512);
   }
@@ -638,7 +639,7 @@ extern "C" int kb200_attn_prompt_fwd(const KB200PromptArgs* a, void* stream) {
   using namespace kb;
   if (!a) return set_error(KB200_ERR_INVALID, "attn_prompt: null arguments");
   if (a->N < 0 || a->Tq < 0 || a->Tk < 0 || a->N > (1 << 20) || a->Tq > 0x7fffff00LL || a->Tk > 0x7fffff00LL || a->Hq < 1 ||
-      a->Hkv < 1 || a->Hq % a->Hkv || a->Hq > (1 << 16) || (a->dtype != 0 && a->dtype != 1))
+      a->Hkv < 1 || a->Hq % a->Hkv || a->Hq > (1 << 14) || (a->dtype != 0 && a->dtype != 1))
     return set_error(KB200_ERR_INVALID, "attn_prompt: N=%lld Tq=%lld Tk=%lld Hq=%lld Hkv=%lld dtype=%d", (long long)a->N,
                      (long long)a->Tq, (long long)a->Tk, (long long)a->Hq, (long long)a->Hkv, a->dtype);
   if (a->D != 64 && a->D != 128) return set_error(KB200_ERR_INVALID, "attn_prompt: head dim %lld (64 or 128)", (long long)a->D);
@@ -656,7 +657,7 @@ extern "C" int kb200_attn_prompt_fwd(const KB200PromptArgs* a, void* stream) {
   prompt::Params p{a->q, a->k, a->v, a->o, a->lse, a->cu_q, a->cu_k, a->q_token_stride, a->q_head_stride,
                    a->k_token_stride, a->k_head_stride, a->v_token_stride, a->v_head_stride, a->o_token_stride,
                    a->o_head_stride, a->Tq, a->Tk, (int)a->N, (int)a->Hq, (int)a->Hkv, (int)G,
-                   sl2, a->softmax_scale < 0.f ? 0x80008000u : 0u, a->causal};
+                   sl2, a->softmax_scale < 0.f ? 0x80008000u : 0u, ((1ull << 32) + G - 1) / G, a->causal};
   prompt::Maps maps;
   memset(&maps, 0, sizeof(maps));
   if (a->Tk > 0) {                                           // (without keys nothing is loaded)
