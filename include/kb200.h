@@ -269,23 +269,49 @@ typedef struct KB200KvCache {
  * magnitude of its tokens within 448; when it grows, the codes already in the page
  * are re-encoded.  NaN and infinities become NaN codes and set no scale.  Pages that
  * the call writes must belong to one sequence only. */
-int kb200_kv_append(const KB200KvCache* c, const void* k, const void* v, int64_t k_token_stride, int64_t k_head_stride,
-                    int64_t v_token_stride, int64_t v_head_stride, const int32_t* page_table, int64_t max_pages,
-                    const int32_t* lengths, const int32_t* cu_new, int64_t B, int64_t T, int dtype, void* stream);
+typedef struct KB200KvAppendArgs {
+  KB200KvCache cache;
+  const void* k; const void* v;       /* [T, H, D]                                */
+  const int32_t* page_table;          /* [B, max_pages]                           */
+  const int32_t* lengths;             /* [B]                                      */
+  const int32_t* cu_new;              /* [B+1]                                    */
+  int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  int64_t max_pages, B, T;
+  int64_t dtype;
+} KB200KvAppendArgs;
+int kb200_kv_append(const KB200KvAppendArgs* a, void* stream);
 /* Dequantises tokens starts[b] .. starts[b] + cu[b+1] - cu[b] of each sequence into the
  * packed rows cu[b] .. of k, v [T, H, D]; rows at and behind cu[B] are left as they were. */
-int kb200_kv_gather(const KB200KvCache* c, const int32_t* page_table, int64_t max_pages, const int32_t* starts,
-                    const int32_t* cu, int64_t B, int64_t T, void* k, void* v, int dtype, void* stream);
+typedef struct KB200KvGatherArgs {
+  KB200KvCache cache;
+  void* k; void* v;                   /* out [T, H, D] contiguous                 */
+  const int32_t* page_table;          /* [B, max_pages]                           */
+  const int32_t* starts;              /* [B]                                      */
+  const int32_t* cu;                  /* [B+1]                                    */
+  int64_t max_pages, B, T;
+  int64_t dtype;
+} KB200KvGatherArgs;
+int kb200_kv_gather(const KB200KvGatherArgs* a, void* stream);
 /* Attention of the last Sq tokens of each sequence over the cache: q [B, Sq, Hq, D]
  * (strides in elements, multiples of 8), o [B, Sq, Hq, D] contiguous, lse [B, Sq, Hq] or
  * NULL.  Query i sees the sequence's keys j < lengths[b] - Sq + 1 + i; none: o = 0,
  * lse = -inf.  Lengths are clamped to max_pages * page. */
 size_t kb200_attn_cached_workspace_size(int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv, int64_t D, int64_t page,
                                         int64_t max_pages);
-int kb200_attn_cached_fwd(const void* q, int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride,
-                          const KB200KvCache* c, const int32_t* page_table, int64_t max_pages, const int32_t* lengths,
-                          void* o, float* lse, int64_t B, int64_t Sq, int64_t Hq, float softmax_scale, int dtype,
-                          void* workspace, size_t workspace_bytes, void* stream);
+typedef struct KB200AttnCachedArgs {
+  KB200KvCache cache;
+  const void* q;                      /* [B, Sq, Hq, D]                           */
+  void* o; float* lse;
+  const int32_t* page_table;          /* [B, max_pages]                           */
+  const int32_t* lengths;             /* [B]                                      */
+  void* workspace;                    /* 16-byte aligned                          */
+  size_t workspace_bytes;
+  int64_t q_batch_stride, q_token_stride, q_head_stride;
+  int64_t max_pages, B, Sq, Hq;
+  double softmax_scale;
+  int64_t dtype;
+} KB200AttnCachedArgs;
+int kb200_attn_cached_fwd(const KB200AttnCachedArgs* a, void* stream);
 
 /* ---------------------------------------------------------------------
  * Failure-path test hooks (no counterpart in the reference).

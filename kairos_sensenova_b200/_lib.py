@@ -82,6 +82,34 @@ class KvCacheArgs(ctypes.Structure):
     ]
 
 
+class KvAppendArgs(ctypes.Structure):
+    """Mirror of ``KB200KvAppendArgs`` (include/kb200.h)."""
+    _fields_ = [('cache', KvCacheArgs)] + [(n, ctypes.c_void_p) for n in ('k', 'v', 'page_table', 'lengths', 'cu_new')] + [
+        (n, ctypes.c_int64) for n in ('k_token_stride', 'k_head_stride', 'v_token_stride', 'v_head_stride', 'max_pages',
+                                      'B', 'T', 'dtype')]
+
+
+class KvGatherArgs(ctypes.Structure):
+    """Mirror of ``KB200KvGatherArgs`` (include/kb200.h)."""
+    _fields_ = [('cache', KvCacheArgs)] + [(n, ctypes.c_void_p) for n in ('k', 'v', 'page_table', 'starts', 'cu')] + [
+        (n, ctypes.c_int64) for n in ('max_pages', 'B', 'T', 'dtype')]
+
+
+class AttnCachedArgs(ctypes.Structure):
+    """Mirror of ``KB200AttnCachedArgs`` (include/kb200.h)."""
+    _fields_ = [('cache', KvCacheArgs)] + [(n, ctypes.c_void_p) for n in ('q', 'o', 'lse', 'page_table', 'lengths',
+                                                                          'workspace')] + [
+        (n, ctypes.c_int64) for n in ('workspace_bytes', 'q_batch_stride', 'q_token_stride', 'q_head_stride', 'max_pages',
+                                      'B', 'Sq', 'Hq')] + [('softmax_scale', ctypes.c_double), ('dtype', ctypes.c_int64)]
+
+
+# what follows the cache (packed once per KVCache), packed
+KV_CACHE_ARGS = struct.Struct('@4P4q')
+KV_APPEND_ARGS, KV_GATHER_ARGS, ATTN_CACHED_ARGS = struct.Struct('@5P8q'), struct.Struct('@5P4q'), struct.Struct('@6P8qdq')
+for _s, _c in ((KV_APPEND_ARGS, KvAppendArgs), (KV_GATHER_ARGS, KvGatherArgs), (ATTN_CACHED_ARGS, AttnCachedArgs)):
+    assert KV_CACHE_ARGS.size + _s.size == ctypes.sizeof(_c)
+
+
 _ATTN_SIG = (ctypes.c_int, [ctypes.c_void_p] * 4 + [ctypes.c_int64] * 5 +
              [ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p])
 
@@ -112,17 +140,12 @@ SIGNATURES = {
                             [ctypes.c_float, ctypes.c_void_p]),
     'kb200_residual_ln_mod': (ctypes.c_int, [ctypes.c_void_p] * 2 + [ctypes.c_int64] * 3 +
                               [ctypes.c_void_p] * 3 + [ctypes.c_int, ctypes.c_float] + [ctypes.c_void_p] * 2),
-    'kb200_attn_prompt_fwd': (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),   # PromptArgs or its packed bytes
-    'kb200_kv_append': (ctypes.c_int, [ctypes.POINTER(KvCacheArgs)] + [ctypes.c_void_p] * 2 + [ctypes.c_int64] * 4 +
-                        [ctypes.c_void_p, ctypes.c_int64] + [ctypes.c_void_p] * 2 + [ctypes.c_int64] * 2 +
-                        [ctypes.c_int, ctypes.c_void_p]),
-    'kb200_kv_gather': (ctypes.c_int, [ctypes.POINTER(KvCacheArgs), ctypes.c_void_p, ctypes.c_int64] +
-                        [ctypes.c_void_p] * 2 + [ctypes.c_int64] * 2 + [ctypes.c_void_p] * 2 +
-                        [ctypes.c_int, ctypes.c_void_p]),
+    # these four take their argument structure or its packed bytes
+    'kb200_attn_prompt_fwd': (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
+    'kb200_kv_append': (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
+    'kb200_kv_gather': (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
     'kb200_attn_cached_workspace_size': (ctypes.c_size_t, [ctypes.c_int64] * 7),
-    'kb200_attn_cached_fwd': (ctypes.c_int, [ctypes.c_void_p] + [ctypes.c_int64] * 3 + [ctypes.POINTER(KvCacheArgs),
-                              ctypes.c_void_p, ctypes.c_int64] + [ctypes.c_void_p] * 3 + [ctypes.c_int64] * 3 +
-                              [ctypes.c_float, ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    'kb200_attn_cached_fwd': (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
 }
 
 

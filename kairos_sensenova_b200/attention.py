@@ -21,7 +21,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib
-from .kv_cache import _DTYPES, _forward_only, _index, _launch, _rows
+from .kv_cache import _DTYPES, _int32, _launch, _refuse_grad, _rows
 
 
 def attention_fp8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, num_heads: int,
@@ -115,25 +115,26 @@ def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     ``return_lse`` also the fp32 log of the softmax sum ``[Tq, Hq]``.  ``check=True`` looks at
     the offsets on the host first (it synchronises) and raises ``ValueError``."""
     what = 'attention_prompt'
-    dev = q.device
-    if dev.type != 'cuda':
+    index = q.get_device()
+    if index < 0:
         raise RuntimeError(f'{what}: inputs must be CUDA tensors (no CPU path)')
-    shape, kshape = q.shape, k.shape
+    shape, kshape, qd = q.shape, k.shape, q.dtype
     if len(shape) != 3 or len(kshape) != 3 or v.shape != kshape or kshape[2] != shape[2] or kshape[1] < 1 \
             or shape[1] < 1 or shape[1] % kshape[1]:
         raise ValueError(f'{what}: q must be [Tq, Hq, D] and k, v [Tk, Hkv, D] with Hq a multiple of Hkv, got '
                          f'{tuple(shape)}, {tuple(kshape)}, {tuple(v.shape)}')
-    dtype = _DTYPES.get(q.dtype)
-    if dtype is None or k.dtype is not q.dtype or v.dtype is not q.dtype:
+    dtype = _DTYPES.get(qd)
+    if dtype is None or k.dtype is not qd or v.dtype is not qd:
         raise ValueError(f'{what}: q, k and v must all be bfloat16 or all float16, got {q.dtype}, {k.dtype}, {v.dtype}')
-    if k.device != dev or v.device != dev:
+    if k.get_device() != index or v.get_device() != index:
         raise ValueError(f'{what}: q, k and v must be on one device')
-    _forward_only(what, q, k, v)
-    N = cu_seqlens_q.shape[0] - 1 if cu_seqlens_q.dim() == 1 else -1
+    if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
+        _refuse_grad(what)
+    cu_q = _int32(cu_seqlens_q, (None,), what, 'cu_seqlens_q', index)
+    N = cu_q.shape[0] - 1
     if N < 0:
-        raise ValueError(f'{what}: cu_seqlens_q must be [N + 1], got {tuple(cu_seqlens_q.shape)}')
-    cu_q = _index(cu_seqlens_q, (N + 1,), what, 'cu_seqlens_q', dev)
-    cu_k = cu_q if cu_seqlens_k is None else _index(cu_seqlens_k, (N + 1,), what, 'cu_seqlens_k', dev)
+        raise ValueError(f'{what}: cu_seqlens_q must be [N + 1], got [0]')
+    cu_k = cu_q if cu_seqlens_k is None else _int32(cu_seqlens_k, (N + 1,), what, 'cu_seqlens_k', index)
     Tq, Hq, D = shape
     Tk, Hkv, _ = kshape
     if check:
@@ -141,8 +142,6 @@ def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
             at = cu.tolist()
             if at[0] != 0 or at[-1] > T or any(b < a for a, b in zip(at, at[1:])):
                 raise ValueError(f'{what}: {name} must rise from 0 to at most {T}')
-    if softmax_scale is None:
-        softmax_scale = D ** -0.5
     q, qp, qs = _rows(q)
     k, kp, ks = _rows(k)
     v, vp, vs = _rows(v)
@@ -151,12 +150,12 @@ def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         op, os = out.data_ptr(), (Hq * D, D)
     else:
         same, op, os = _rows(out)
-        if out.shape != shape or out.dtype != q.dtype or out.device != dev or same is not out:
-            raise ValueError(f'{what}: out must be {q.dtype} {list(shape)} on {dev}, its rows 16-byte aligned')
-    lse = torch.empty((Tq, Hq), device=dev, dtype=torch.float32) if return_lse else None
+        if out.shape != shape or out.dtype != qd or out.get_device() != index or same is not out:
+            raise ValueError(f'{what}: out must be {q.dtype} {list(shape)} on {q.device}, its rows 16-byte aligned')
+    lse = torch.empty((Tq, Hq), device=q.device, dtype=torch.float32) if return_lse else None
     args = _lib.PROMPT_ARGS.pack(
-        qp, kp, vp, op, lse.data_ptr() if return_lse else 0, cu_q.data_ptr(),
-        cu_k.data_ptr(), Tq, Tk, N, Hq, Hkv, D, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1], float(softmax_scale),
+        qp, kp, vp, op, lse.data_ptr() if return_lse else 0, cu_q.data_ptr(), cu_k.data_ptr(), Tq, Tk, N, Hq, Hkv, D,
+        qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1], D ** -0.5 if softmax_scale is None else softmax_scale,
         1 if causal else 0, dtype)
-    _launch(dev, what, _lib.lib().kb200_attn_prompt_fwd, args)
+    _launch(index, what, _lib.lib().kb200_attn_prompt_fwd, args)
     return (out, lse) if return_lse else out

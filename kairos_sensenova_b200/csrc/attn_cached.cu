@@ -853,36 +853,38 @@ extern "C" size_t kb200_attn_cached_workspace_size(int64_t B, int64_t Sq, int64_
   return (size_t)2 * grid * row_tiles(R) * 8 * (D + 2) * sizeof(float);
 }
 
-extern "C" int kb200_attn_cached_fwd(const void* q, int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride,
-                                     const KB200KvCache* c, const int32_t* page_table, int64_t max_pages,
-                                     const int32_t* lengths, void* o, float* lse, int64_t B, int64_t Sq, int64_t Hq,
-                                     float softmax_scale, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+extern "C" int kb200_attn_cached_fwd(const KB200AttnCachedArgs* a, void* stream) {
   using namespace kb;
+  if (!a) return set_error(KB200_ERR_INVALID, "attn_cached: null arguments");
+  const KB200KvCache* c = &a->cache;
+  const int64_t B = a->B, Sq = a->Sq, Hq = a->Hq, max_pages = a->max_pages;
+  const bool dtype = a->dtype == 1;
   if (int e = kv::check_cache(c, "attn_cached")) return e;
   if (int e = cached::check_shape(B, Sq, Hq, c->H, max_pages)) return e;
-  if (dtype != 0 && dtype != 1) return set_error(KB200_ERR_INVALID, "attn_cached: dtype=%d", dtype);
+  if (a->dtype != 0 && a->dtype != 1) return set_error(KB200_ERR_INVALID, "attn_cached: dtype=%lld", (long long)a->dtype);
   if (B == 0 || Sq == 0) return KB200_OK;
-  if (!q || !o || !lengths || (max_pages > 0 && !page_table)) return set_error(KB200_ERR_INVALID, "attn_cached: null pointer");
-  if (!aligned16(q) || !aligned16(o) || ((q_batch_stride | q_token_stride | q_head_stride) & 7))
+  if (!a->q || !a->o || !a->lengths || (max_pages > 0 && !a->page_table))
+    return set_error(KB200_ERR_INVALID, "attn_cached: null pointer");
+  if (!aligned16(a->q) || !aligned16(a->o) || ((a->q_batch_stride | a->q_token_stride | a->q_head_stride) & 7))
     return set_error(KB200_ERR_ALIGN, "attn_cached: q and o rows must be 16-byte aligned");
   const size_t need = kb200_attn_cached_workspace_size(B, Sq, Hq, c->H, c->D, c->page, max_pages);
-  if (!workspace || workspace_bytes < need || !aligned16(workspace))
-    return set_error(KB200_ERR_WORKSPACE, "attn_cached: workspace of %zu bytes needed, got %zu", need, workspace_bytes);
+  if (!a->workspace || a->workspace_bytes < need || !aligned16(a->workspace))
+    return set_error(KB200_ERR_WORKSPACE, "attn_cached: workspace of %zu bytes needed, got %zu", need, a->workspace_bytes);
   const int64_t G = Hq / c->H, R = Sq * G;
   const int nt = cached::row_tiles(R), rows = nt * 8;
   const int64_t rblocks = (R + rows - 1) / rows;
   if (B * c->H * rblocks > 0x7fffffffLL) return set_error(KB200_ERR_INVALID, "attn_cached: too many rows");
   cached::Params p{};
-  p.q = q; p.o = o; p.lse = lse; p.table = page_table; p.lengths = lengths;
+  p.q = a->q; p.o = a->o; p.lse = a->lse; p.table = a->page_table; p.lengths = a->lengths;
   p.k_pages = (const uint8_t*)c->k_pages; p.v_pages = (const uint8_t*)c->v_pages;
-  p.k_scale = c->k_scale; p.v_scale = c->v_scale; p.part = (float*)workspace;
-  p.q_bs = q_batch_stride; p.q_ts = q_token_stride; p.q_hs = q_head_stride;
+  p.k_scale = c->k_scale; p.v_scale = c->v_scale; p.part = (float*)a->workspace;
+  p.q_bs = a->q_batch_stride; p.q_ts = a->q_token_stride; p.q_hs = a->q_head_stride;
   p.B = (int)B; p.Sq = (int)Sq; p.Hq = (int)Hq; p.H = (int)c->H; p.G = (int)G; p.R = (int)R;
   p.rblocks = (int)rblocks;
   p.num_pages = (int)c->num_pages; p.max_pages = (int)max_pages; p.page = (int)c->page;
   p.page_log2 = c->page == 16 ? 4 : c->page == 32 ? 5 : c->page == 64 ? 6 : 7;
-  p.scale_log2 = fabsf(softmax_scale) * 1.4426950408889634f;
-  p.flip = softmax_scale < 0.f ? 0x80008000u : 0u;
+  p.scale_log2 = fabsf((float)a->softmax_scale) * 1.4426950408889634f;
+  p.flip = a->softmax_scale < 0.0 ? 0x80008000u : 0u;
   const int grid = cached::grid_of(c->D, B, c->H, R, max_pages * c->page);
   cudaStream_t st = (cudaStream_t)stream;
   if (c->D == 64) {

@@ -24,19 +24,19 @@ struct AppendParams {
 // values in registers (32 each), so that they are read once: amax over the group,
 // exponent, codes.  Tokens that were in the page before keep their codes unless the
 // exponent grows; then they are re-encoded under the new one.
-// Bound: HBM.  2 B read and 1 B written per value.
+// Bound: HBM.  2 B read and 1 B written per value.  A block takes several of a unit's
+// (head, k|v) items, the next one's loads under way while one is encoded: the three
+// dependent reads that find the page are paid once.
 template <int D, int PAGE, bool F16>
 __global__ void __launch_bounds__(PAGE * D / 32 > 256 ? 512 : 256) kv_append_kernel(AppendParams p) {
-  constexpr int GROUP = PAGE * D / 32;                 // threads of one (unit, head, k|v)
+  constexpr int GROUP = PAGE * D / 32;                 // threads of one item
   constexpr int THREADS = GROUP > 256 ? GROUP : 256;
   constexpr int PER_BLOCK = THREADS / GROUP;
   constexpr int CPT = D / 8;                           // 8-value chunks of a token
-  __shared__ float wmax[THREADS / 32];
+  __shared__ float wmax[2][THREADS / 32];
   const int grp = threadIdx.x / GROUP, t = threadIdx.x % GROUP;
-  const int item = blockIdx.y * PER_BLOCK + grp;       // (head, k|v)
-  const bool is_v = item & 1;
-  const int h = item >> 1;
   const int64_t unit = blockIdx.x;
+  const int part = blockIdx.y;
 
   // the unit's sequence: largest b with cu[b] / PAGE + 2 b <= unit
   int lo = 0, hi = p.B - 1;
@@ -48,91 +48,95 @@ __global__ void __launch_bounds__(PAGE * D / 32 > 256 ? 512 : 256) kv_append_ker
   const int64_t c0 = min((int64_t)max(0, p.cu[b]), p.T), c1 = min((int64_t)p.cu[b + 1], p.T);
   const int64_t n = c1 - c0, len = p.lengths[b], first = len - n;
   const int64_t pi = unit - (c0 / PAGE + 2 * b);       // index among the pages that b writes
-  bool live = n > 0 && first >= 0 && pi >= 0 && len <= (int64_t)p.max_pages * PAGE && h < p.H;
+  if (n <= 0 || first < 0 || pi < 0 || len > (int64_t)p.max_pages * PAGE) return;
   const int64_t slot = first / PAGE + pi;              // index into b's table row
-  live = live && slot * PAGE < len;
-  int pg = 0;
-  if (live) {
-    pg = p.table[(int64_t)b * p.max_pages + slot];
-    live = pg >= 0 && pg < p.num_pages;
-  }
+  if (slot * PAGE >= len) return;
+  const int pg = p.table[(int64_t)b * p.max_pages + slot];
+  if (pg < 0 || pg >= p.num_pages) return;
   const int64_t pos0 = slot * PAGE;                    // position of the page's first token
   const int keep = (int)max((int64_t)0, min((int64_t)PAGE, first - pos0));   // tokens that were there
   const int end = (int)min((int64_t)PAGE, len - pos0);
+  const int64_t row0 = c0 + pos0 - first;              // packed row of the page's first token
 
-  const char* src = reinterpret_cast<const char*>(is_v ? p.v : p.k);
-  const int64_t ts = is_v ? p.v_ts : p.k_ts, hs = is_v ? p.v_hs : p.k_hs;
-  uint4 x[4];
-  float amax = 0.f;
+  auto fetch = [&](int item, uint4* x) {
+    const bool is_v = item & 1;
+    const char* src = reinterpret_cast<const char*>(is_v ? p.v : p.k);
+    const int64_t ts = is_v ? p.v_ts : p.k_ts, hs = is_v ? p.v_hs : p.k_hs;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int c = t + i * GROUP, tok = c / CPT, d0 = (c % CPT) * 8;
-    x[i] = make_uint4(0, 0, 0, 0);
-    if (live && tok >= keep && tok < end)
-      x[i] = __ldg(reinterpret_cast<const uint4*>(src + 2 * ((c0 + pos0 + tok - first) * ts + h * hs + d0)));
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 f = unpack16<F16>(w[e]);
-      const float a = fabsf(f.x), c = fabsf(f.y);
-      if (a < INFINITY) amax = fmaxf(amax, a);         // NaN and infinities do not set the scale
-      if (c < INFINITY) amax = fmaxf(amax, c);
+    for (int i = 0; i < 4; ++i) {
+      const int c = t + i * GROUP, tok = c / CPT, d0 = (c % CPT) * 8;
+      x[i] = make_uint4(0, 0, 0, 0);
+      if (item < 2 * p.H && tok >= keep && tok < end)
+        x[i] = __ldg(reinterpret_cast<const uint4*>(src + 2 * ((row0 + tok) * ts + (item >> 1) * hs + d0)));
     }
-  }
-  amax = warp_max(amax);
-  if constexpr (GROUP > 32) {
-    if ((threadIdx.x & 31) == 0) wmax[threadIdx.x >> 5] = amax;
-    __syncthreads();
+  };
+  const int stride = gridDim.y * PER_BLOCK;
+  uint4 x[4], nx[4];
+  fetch(part * PER_BLOCK + grp, x);
+  int turn = 0;
+  for (int base = part * PER_BLOCK; base < 2 * p.H; base += stride, turn ^= 1) {   // (items: head, k|v)
+    const int item = base + grp;
+    fetch(item + stride, nx);
+    float amax = 0.f;
 #pragma unroll
-    for (int w = 0; w < GROUP / 32; ++w) amax = fmaxf(amax, wmax[grp * (GROUP / 32) + w]);
-  }
-  if (!live) return;
-
-  float* scale = (is_v ? p.v_scale : p.k_scale) + (int64_t)pg * p.H + h;
-  uint8_t* page = (is_v ? p.v_pages : p.k_pages) + ((int64_t)pg * p.H + h) * (PAGE * D);
-  int e = scale_exponent(amax), e_old = 0;
-  bool grown = false;
-  if (keep > 0) {
-    e_old = exponent_of(*scale);
-    grown = e > e_old;
-    e = max(e, e_old);
-  }
-  // x 2^-e in one product: e is at most 120, so 2^-e is normal
-  const float inv = pow2(-e), up = grown ? pow2(e_old - e) : 1.f;
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int c = t + i * GROUP, tok = c / CPT;
-    uint2* dst = reinterpret_cast<uint2*>(page) + c;
-    if (tok < keep) {
-      if (grown) {
-        const uint2 o = *dst;
-        uint2 r;
-        float2 f0 = half2_to_float2(decode2(o.x & 0xffff)), f1 = half2_to_float2(decode2(o.x >> 16));
-        r.x = encode2(f0.x * up, f0.y * up) | encode2(f1.x * up, f1.y * up) << 16;
-        f0 = half2_to_float2(decode2(o.y & 0xffff)), f1 = half2_to_float2(decode2(o.y >> 16));
-        r.y = encode2(f0.x * up, f0.y * up) | encode2(f1.x * up, f1.y * up) << 16;
-        *dst = r;
+      for (int e = 0; e < 4; ++e) {
+        const float2 f = unpack16<F16>(w[e]);
+        const float a = fabsf(f.x), c = fabsf(f.y);
+        if (a < INFINITY) amax = fmaxf(amax, a);         // NaN and infinities do not set the scale
+        if (c < INFINITY) amax = fmaxf(amax, c);
       }
-    } else if (tok < end) {
-      const float2 f0 = unpack16<F16>(x[i].x), f1 = unpack16<F16>(x[i].y), f2 = unpack16<F16>(x[i].z),
-                   f3 = unpack16<F16>(x[i].w);
-      uint2 r;
-      r.x = encode2(f0.x * inv, f0.y * inv) | encode2(f1.x * inv, f1.y * inv) << 16;
-      r.y = encode2(f2.x * inv, f2.y * inv) | encode2(f3.x * inv, f3.y * inv) << 16;
-      *dst = r;
     }
+    const bool is_v = item & 1, live = item < 2 * p.H;
+    const int h = item >> 1;
+    float* scale = (is_v ? p.v_scale : p.k_scale) + (int64_t)pg * p.H + h;
+    int e_old = 0;
+    if (keep > 0 && live) e_old = exponent_of(*scale);   // (every thread reads it before the barrier, one writes it after)
+    amax = warp_max(amax);
+    if constexpr (GROUP > 32) {
+      if ((threadIdx.x & 31) == 0) wmax[turn][threadIdx.x >> 5] = amax;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < GROUP / 32; ++w) amax = fmaxf(amax, wmax[turn][grp * (GROUP / 32) + w]);
+    }
+    if (live) {
+      uint8_t* page = (is_v ? p.v_pages : p.k_pages) + ((int64_t)pg * p.H + h) * (PAGE * D);
+      int e = scale_exponent(amax);
+      const bool grown = keep > 0 && e > e_old;
+      if (keep > 0) e = max(e, e_old);
+      // x 2^-e in one product: e is at most 120, so 2^-e is normal
+      const float inv = pow2(-e), up = grown ? pow2(e_old - e) : 1.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = t + i * GROUP, tok = c / CPT;
+        uint2* dst = reinterpret_cast<uint2*>(page) + c;
+        if (tok < keep) {
+          if (grown) {
+            const uint2 o = *dst;
+            uint2 r;
+            float2 f0 = half2_to_float2(decode2(o.x & 0xffff)), f1 = half2_to_float2(decode2(o.x >> 16));
+            r.x = encode2(f0.x * up, f0.y * up) | encode2(f1.x * up, f1.y * up) << 16;
+            f0 = half2_to_float2(decode2(o.y & 0xffff)), f1 = half2_to_float2(decode2(o.y >> 16));
+            r.y = encode2(f0.x * up, f0.y * up) | encode2(f1.x * up, f1.y * up) << 16;
+            *dst = r;
+          }
+        } else if (tok < end) {
+          const float2 f0 = unpack16<F16>(x[i].x), f1 = unpack16<F16>(x[i].y), f2 = unpack16<F16>(x[i].z),
+                       f3 = unpack16<F16>(x[i].w);
+          uint2 r;
+          r.x = encode2(f0.x * inv, f0.y * inv) | encode2(f1.x * inv, f1.y * inv) << 16;
+          r.y = encode2(f2.x * inv, f2.y * inv) | encode2(f3.x * inv, f3.y * inv) << 16;
+          *dst = r;
+        }
+      }
+      if constexpr (GROUP <= 32) __syncwarp();
+      if (t == 0) *scale = pow2(e);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = nx[i];
   }
-  // every thread of the group has read the old scale before it changes
-  if constexpr (GROUP > 32) {
-    // (whole blocks only: the groups of a block can differ in `live`)
-    asm volatile("bar.sync %0, %1;\n" ::"r"(1 + grp), "r"(GROUP) : "memory");
-  } else {
-    __syncwarp();
-  }
-  if (t == 0) *scale = pow2(e);
 }
 
 struct GatherParams {
@@ -152,7 +156,7 @@ struct GatherParams {
 // cu[B] are left as they were.
 template <int D, bool F16>
 __global__ void __launch_bounds__(256) kv_gather_kernel(GatherParams p) {
-  constexpr int TOK = 32, CPR = D / 16;
+  constexpr int TOK = 32, CPR = D / 16, UNROLL = 4;
   __shared__ int64_t row[TOK];     // code row of head 0 (a row has D codes), -1: no such token, -2: missing page
   __shared__ int pgs[TOK];
   const int64_t t0 = (int64_t)blockIdx.x * TOK;
@@ -170,34 +174,55 @@ __global__ void __launch_bounds__(256) kv_gather_kernel(GatherParams p) {
       }
     }
     row[threadIdx.x] = r;
-    pgs[threadIdx.x] = pg;
+    pgs[threadIdx.x] = r >= 0 ? pg : 0;
   }
   __syncthreads();
-  const int per_tok = p.H * CPR;
-  for (int it = threadIdx.x; it < TOK * per_tok; it += 256) {
-    const int tok = it / per_tok, rest = it % per_tok, h = rest / CPR, c = rest % CPR;
-    const int64_t r = row[tok];
-    if (r == -1) continue;
-    const int64_t dst = ((t0 + tok) * p.H + h) * D + c * 16;
+  // a thread keeps its (head, chunk) and goes through the tokens, `lanes` of which are taken at once
+  const int per_tok = p.H * CPR, lanes = per_tok >= 256 ? 1 : 256 / per_tok;
+  const int tok0 = per_tok >= 256 ? 0 : threadIdx.x / per_tok;
+  if (tok0 >= lanes) return;
+  for (int rest = per_tok >= 256 ? threadIdx.x : threadIdx.x % per_tok; rest < per_tok; rest += 256) {
+    const int h = rest / CPR, c = rest % CPR;
+    const int64_t hoff = (int64_t)h * p.page;
+    for (int tok = tok0; tok < TOK; tok += lanes * UNROLL) {
+      uint4 codes[UNROLL][2];
+      float s[UNROLL][2];
 #pragma unroll
-    for (int kv = 0; kv < 2; ++kv) {
-      uint4 codes = make_uint4(0, 0, 0, 0);
-      float s = 0.f;
-      if (r >= 0) {
-        codes = __ldg(reinterpret_cast<const uint4*>((kv ? p.v_pages : p.k_pages) + (r + (int64_t)h * p.page) * D + c * 16));
-        s = __ldg((kv ? p.v_scale : p.k_scale) + (int64_t)pgs[tok] * p.H + h);
-      }
-      const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
-      uint32_t o[8];
+      for (int z = 0; z < UNROLL; ++z) {
+        const int tt = tok + z * lanes;
+        const int64_t r = tt < TOK ? row[tt] : -1;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 f0 = half2_to_float2(decode2(w[e] & 0xffff)), f1 = half2_to_float2(decode2(w[e] >> 16));
-        o[2 * e] = pack16<F16>(f0.x * s, f0.y * s);
-        o[2 * e + 1] = pack16<F16>(f1.x * s, f1.y * s);
+        for (int kv = 0; kv < 2; ++kv) {
+          codes[z][kv] = make_uint4(0, 0, 0, 0);
+          s[z][kv] = 0.f;
+          if (r >= 0) {
+            codes[z][kv] = __ldg(reinterpret_cast<const uint4*>((kv ? p.v_pages : p.k_pages) + (r + hoff) * D + c * 16));
+            s[z][kv] = __ldg((kv ? p.v_scale : p.k_scale) + (int64_t)pgs[tt] * p.H + h);
+          }
+        }
       }
-      uint4* d = reinterpret_cast<uint4*>(reinterpret_cast<char*>(kv ? p.v : p.k) + 2 * dst);
-      d[0] = make_uint4(o[0], o[1], o[2], o[3]);
-      d[1] = make_uint4(o[4], o[5], o[6], o[7]);
+#pragma unroll
+      for (int z = 0; z < UNROLL; ++z) {
+        const int tt = tok + z * lanes;
+        if (tt >= TOK || row[tt] == -1) continue;
+        const int64_t dst = ((t0 + tt) * p.H + h) * D + c * 16;
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          const uint32_t w[4] = {codes[z][kv].x, codes[z][kv].y, codes[z][kv].z, codes[z][kv].w};
+          uint32_t o[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t lo, hi;
+            decode4(w[e], lo, hi);
+            const float2 f0 = half2_to_float2(lo), f1 = half2_to_float2(hi);
+            o[2 * e] = pack16<F16>(f0.x * s[z][kv], f0.y * s[z][kv]);
+            o[2 * e + 1] = pack16<F16>(f1.x * s[z][kv], f1.y * s[z][kv]);
+          }
+          uint4* d = reinterpret_cast<uint4*>(reinterpret_cast<char*>(kv ? p.v : p.k) + 2 * dst);
+          d[0] = make_uint4(o[0], o[1], o[2], o[3]);
+          d[1] = make_uint4(o[4], o[5], o[6], o[7]);
+        }
+      }
     }
   }
 }
@@ -217,67 +242,77 @@ int check_cache(const KB200KvCache* c, const char* what) {
 }
 
 template <int D, int PAGE, bool F16>
-static void launch_append(const AppendParams& p, cudaStream_t st) {
+static int launch_append(const AppendParams& p, cudaStream_t st) {
   constexpr int GROUP = PAGE * D / 32, THREADS = GROUP > 256 ? GROUP : 256, PER = THREADS / GROUP;
-  const int64_t units = p.T / PAGE + 2 * (int64_t)p.B;
-  kv_append_kernel<D, PAGE, F16><<<dim3((unsigned)units, (unsigned)((2 * p.H + PER - 1) / PER)), THREADS, 0, st>>>(p);
+  // few units: a block for every item group of a unit; many: four of them one after the other
+  // (32760 tokens of 8 heads: 46.8 us with four, 49 with two, 47.5 with eight; a unit's blocks next to
+  // each other in a one-dimensional grid: 53.8)
+  const int64_t units = p.T / PAGE + 2 * (int64_t)p.B, groups = (2 * p.H + PER - 1) / PER;
+  const int64_t items = units * groups <= 148 * 8 ? 1 : 4;
+  kv_append_kernel<D, PAGE, F16><<<dim3((unsigned)units, (unsigned)((groups + items - 1) / items)), THREADS, 0, st>>>(p);
+  return check_launch("kv_append_kernel");
 }
 
 template <int D, bool F16>
-static void launch_append_page(const AppendParams& p, int page, cudaStream_t st) {
-  if (page == 16) launch_append<D, 16, F16>(p, st);
-  else if (page == 32) launch_append<D, 32, F16>(p, st);
-  else if (page == 64) launch_append<D, 64, F16>(p, st);
-  else launch_append<D, 128, F16>(p, st);
+static int launch_append_page(const AppendParams& p, int page, cudaStream_t st) {
+  if (page == 16) return launch_append<D, 16, F16>(p, st);
+  if (page == 32) return launch_append<D, 32, F16>(p, st);
+  if (page == 64) return launch_append<D, 64, F16>(p, st);
+  return launch_append<D, 128, F16>(p, st);
 }
 
 }  // namespace kv
 }  // namespace kb
 
-extern "C" int kb200_kv_append(const KB200KvCache* c, const void* k, const void* v, int64_t k_token_stride,
-                               int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride,
-                               const int32_t* page_table, int64_t max_pages, const int32_t* lengths,
-                               const int32_t* cu_new, int64_t B, int64_t T, int dtype, void* stream) {
+extern "C" int kb200_kv_append(const KB200KvAppendArgs* a, void* stream) {
   using namespace kb;
+  if (!a) return set_error(KB200_ERR_INVALID, "kv_append: null arguments");
+  const KB200KvCache* c = &a->cache;
   if (int e = kv::check_cache(c, "kv_append")) return e;
-  if (B < 0 || T < 0 || max_pages < 0 || B > (1 << 24) || T > 0x7fffffffLL || (dtype != 0 && dtype != 1))
-    return set_error(KB200_ERR_INVALID, "kv_append: B=%lld T=%lld max_pages=%lld dtype=%d", (long long)B, (long long)T,
-                     (long long)max_pages, dtype);
-  if (B == 0 || T == 0) return KB200_OK;
-  if (!k || !v || !page_table || !lengths || !cu_new) return set_error(KB200_ERR_INVALID, "kv_append: null pointer");
-  if (!aligned16(k) || !aligned16(v) || ((k_token_stride | k_head_stride | v_token_stride | v_head_stride) & 7))
+  if (a->B < 0 || a->T < 0 || a->max_pages < 0 || a->B > (1 << 24) || a->max_pages > (1 << 26) || a->T > 0x7fffffffLL ||
+      (a->dtype != 0 && a->dtype != 1))
+    return set_error(KB200_ERR_INVALID, "kv_append: B=%lld T=%lld max_pages=%lld dtype=%lld", (long long)a->B,
+                     (long long)a->T, (long long)a->max_pages, (long long)a->dtype);
+  if (a->B == 0 || a->T == 0) return KB200_OK;
+  if (!a->k || !a->v || (a->max_pages > 0 && !a->page_table) || !a->lengths || !a->cu_new)
+    return set_error(KB200_ERR_INVALID, "kv_append: null pointer");
+  if (!aligned16(a->k) || !aligned16(a->v) ||
+      ((a->k_token_stride | a->k_head_stride | a->v_token_stride | a->v_head_stride) & 7))
     return set_error(KB200_ERR_ALIGN, "kv_append: k and v rows must be 16-byte aligned");
-  kv::AppendParams p{(uint8_t*)c->k_pages, (uint8_t*)c->v_pages, c->k_scale, c->v_scale, k, v, k_token_stride,
-                     k_head_stride, v_token_stride, v_head_stride, page_table, lengths, cu_new, (int)c->num_pages,
-                     (int)c->H, (int)max_pages, (int)B, T};
+  kv::AppendParams p{(uint8_t*)c->k_pages, (uint8_t*)c->v_pages, c->k_scale, c->v_scale, a->k, a->v, a->k_token_stride,
+                     a->k_head_stride, a->v_token_stride, a->v_head_stride, a->page_table, a->lengths, a->cu_new,
+                     (int)c->num_pages, (int)c->H, (int)a->max_pages, (int)a->B, a->T};
   cudaStream_t st = (cudaStream_t)stream;
   const int page = (int)c->page;
   if (c->D == 64) {
-    if (dtype) kv::launch_append_page<64, true>(p, page, st); else kv::launch_append_page<64, false>(p, page, st);
+    if (a->dtype) kv::launch_append_page<64, true>(p, page, st); else kv::launch_append_page<64, false>(p, page, st);
   } else {
-    if (dtype) kv::launch_append_page<128, true>(p, page, st); else kv::launch_append_page<128, false>(p, page, st);
+    if (a->dtype) kv::launch_append_page<128, true>(p, page, st); else kv::launch_append_page<128, false>(p, page, st);
   }
   return check_launch("kv_append_kernel");
 }
 
-extern "C" int kb200_kv_gather(const KB200KvCache* c, const int32_t* page_table, int64_t max_pages, const int32_t* starts,
-                               const int32_t* cu, int64_t B, int64_t T, void* k, void* v, int dtype, void* stream) {
+extern "C" int kb200_kv_gather(const KB200KvGatherArgs* a, void* stream) {
   using namespace kb;
+  if (!a) return set_error(KB200_ERR_INVALID, "kv_gather: null arguments");
+  const KB200KvCache* c = &a->cache;
   if (int e = kv::check_cache(c, "kv_gather")) return e;
-  if (B < 0 || T < 0 || max_pages < 0 || B > (1 << 24) || T > 0x7fffffffLL || (dtype != 0 && dtype != 1))
-    return set_error(KB200_ERR_INVALID, "kv_gather: B=%lld T=%lld max_pages=%lld dtype=%d", (long long)B, (long long)T,
-                     (long long)max_pages, dtype);
-  if (B == 0 || T == 0) return KB200_OK;
-  if (!k || !v || !page_table || !starts || !cu) return set_error(KB200_ERR_INVALID, "kv_gather: null pointer");
-  if (!aligned16(k) || !aligned16(v)) return set_error(KB200_ERR_ALIGN, "kv_gather: outputs must be 16-byte aligned");
-  kv::GatherParams p{(const uint8_t*)c->k_pages, (const uint8_t*)c->v_pages, c->k_scale, c->v_scale, page_table, starts,
-                     cu, k, v, (int)c->num_pages, (int)c->H, (int)max_pages, (int)B, (int)c->page, T};
+  if (a->B < 0 || a->T < 0 || a->max_pages < 0 || a->B > (1 << 24) || a->max_pages > (1 << 26) || a->T > 0x7fffffffLL ||
+      (a->dtype != 0 && a->dtype != 1))
+    return set_error(KB200_ERR_INVALID, "kv_gather: B=%lld T=%lld max_pages=%lld dtype=%lld", (long long)a->B,
+                     (long long)a->T, (long long)a->max_pages, (long long)a->dtype);
+  if (a->B == 0 || a->T == 0) return KB200_OK;
+  if (!a->k || !a->v || (a->max_pages > 0 && !a->page_table) || !a->starts || !a->cu)
+    return set_error(KB200_ERR_INVALID, "kv_gather: null pointer");
+  if (!aligned16(a->k) || !aligned16(a->v)) return set_error(KB200_ERR_ALIGN, "kv_gather: outputs must be 16-byte aligned");
+  kv::GatherParams p{(const uint8_t*)c->k_pages, (const uint8_t*)c->v_pages, c->k_scale, c->v_scale, a->page_table, a->starts,
+                     a->cu, a->k, a->v, (int)c->num_pages, (int)c->H, (int)a->max_pages, (int)a->B, (int)c->page, a->T};
   cudaStream_t st = (cudaStream_t)stream;
-  const unsigned grid = (unsigned)((T + 31) / 32);
+  const unsigned grid = (unsigned)((a->T + 31) / 32);
   if (c->D == 64) {
-    if (dtype) kv::kv_gather_kernel<64, true><<<grid, 256, 0, st>>>(p); else kv::kv_gather_kernel<64, false><<<grid, 256, 0, st>>>(p);
+    if (a->dtype) kv::kv_gather_kernel<64, true><<<grid, 256, 0, st>>>(p); else kv::kv_gather_kernel<64, false><<<grid, 256, 0, st>>>(p);
   } else {
-    if (dtype) kv::kv_gather_kernel<128, true><<<grid, 256, 0, st>>>(p); else kv::kv_gather_kernel<128, false><<<grid, 256, 0, st>>>(p);
+    if (a->dtype) kv::kv_gather_kernel<128, true><<<grid, 256, 0, st>>>(p); else kv::kv_gather_kernel<128, false><<<grid, 256, 0, st>>>(p);
   }
   return check_launch("kv_gather_kernel");
 }

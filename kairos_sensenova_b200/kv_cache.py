@@ -19,7 +19,6 @@ and the table on the host first (it synchronises) and raises ``ValueError``.
 """
 from __future__ import annotations
 
-import ctypes
 import functools
 
 import torch
@@ -36,7 +35,7 @@ class KVCache:
     (``torch.float8_e4m3fn`` or ``uint8`` codes), ``k_scale``, ``v_scale`` ``[num_pages, heads]``
     fp32 powers of two, all contiguous.  A value is ``code * scale``."""
 
-    __slots__ = ('_tensors', '_args', '_ref', '_shape', '_device')
+    __slots__ = ('_tensors', '_args', '_shape', '_row', '_device', '_index')
 
     def __init__(self, k_pages, v_pages, k_scale, v_scale):
         if k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
@@ -61,10 +60,10 @@ class KVCache:
             if not t.is_contiguous():
                 raise ValueError('KVCache: pages and scales must be contiguous')
         self._tensors = (k_pages, v_pages, k_scale, v_scale)
-        self._shape, self._device = (P, H, page, D), k_pages.device
-        self._args = _lib.KvCacheArgs(k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-                                      P, H, page, D)
-        self._ref = ctypes.byref(self._args)
+        self._shape, self._row, self._device = (P, H, page, D), (H, D), k_pages.device
+        self._index = k_pages.get_device()              # -1 on the CPU
+        self._args = _lib.KV_CACHE_ARGS.pack(k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                                             P, H, page, D)
 
     @classmethod
     def empty(cls, num_pages: int, num_heads: int, head_dim: int, page_size: int = 64, device='cuda'):
@@ -84,13 +83,13 @@ class KVCache:
     device = property(lambda self: self._device)
 
 
-def _index(t, shape, what, name, dev):
-    """An int32 contiguous tensor of that shape on `dev` (None: any extent)."""
+def _int32(t, shape, what, name, index):
+    """`t` as a contiguous int32 tensor of that shape on device `index` (None: any extent)."""
     got = t.shape
     if got != shape and (len(got) != len(shape) or any([n != m and n is not None for n, m in zip(shape, got)])):
         raise ValueError(f'{what}: {name} must be {list(shape)}, got {tuple(got)}')
-    if t.device != dev:
-        raise ValueError(f'{what}: {name} must be on {dev}, got {t.device}')
+    if t.get_device() != index:
+        raise ValueError(f'{what}: {name} must be on device {index}, got {t.device}')
     if t.dtype is not torch.int32:
         if t.dtype is not torch.int64:
             raise ValueError(f'{what}: {name} must be int32, got {t.dtype}')
@@ -110,27 +109,23 @@ def _rows(t):
     return t, ptr, strides
 
 
-def _forward_only(what, a, b=None, c=None):
-    if torch.is_grad_enabled() and (a.requires_grad or (b is not None and b.requires_grad)
-                                    or (c is not None and c.requires_grad)):
-        raise NotImplementedError(f'kairos_sensenova_b200.{what} is forward-only')
+def _refuse_grad(what):
+    raise NotImplementedError(f'kairos_sensenova_b200.{what} is forward-only')
 
 
-def _cuda(what, cache):
-    dev = cache._device
-    if dev.type != 'cuda':
+def _cuda_index(what, cache):
+    if cache._index < 0:
         raise RuntimeError(f'{what}: the cache must be on a CUDA device (no CPU path)')
-    return dev
+    return cache._index
 
 
-def _launch(dev, what, fn, *args):
-    """``fn(*args, stream)`` on `dev`'s current stream, with `dev` the current device."""
-    index = dev.index
-    if index == torch.cuda.current_device():
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+def _launch(index, what, fn, args):
+    """``fn(args, stream)`` on device `index`'s current stream, with that the current device."""
+    if index == torch._C._cuda_getDevice():
+        rc = fn(args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+        with torch.cuda.device(index):
+            rc = fn(args, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         _lib.check(rc, what)
 
@@ -168,29 +163,30 @@ def kv_cache_append(cache: KVCache, k: torch.Tensor, v: torch.Tensor, page_table
     are stored as NaN and set no scale.  The pages a call writes must each belong to one
     sequence (``check=True`` raises otherwise)."""
     what = 'kv_cache_append'
-    dev = _cuda(what, cache)
-    _, H, _, D = cache._shape
-    shape = k.shape
-    if len(shape) != 3 or shape[1] != H or shape[2] != D or v.shape != shape:
-        raise ValueError(f'{what}: k and v must be [T, {H}, {D}], got {tuple(k.shape)}, {tuple(v.shape)}')
-    dtype = _DTYPES.get(k.dtype)
-    if dtype is None or v.dtype is not k.dtype:
+    index = _cuda_index(what, cache)
+    shape, kd = k.shape, k.dtype
+    if len(shape) != 3 or shape[1:] != cache._row or v.shape != shape:
+        raise ValueError(f'{what}: k and v must be {["T", *cache._row]}, got {tuple(k.shape)}, {tuple(v.shape)}')
+    dtype = _DTYPES.get(kd)
+    if dtype is None or v.dtype is not kd:
         raise ValueError(f'{what}: k and v must both be bfloat16 or float16, got {k.dtype}, {v.dtype}')
-    if k.device != dev or v.device != dev:
-        raise ValueError(f'{what}: k and v must be on {dev}')
-    _forward_only(what, k, v)
-    page_table = _index(page_table, (None, None), what, 'page_table', dev)
+    if k.get_device() != index or v.get_device() != index:
+        raise ValueError(f'{what}: k and v must be on {cache.device}')
+    if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
+        _refuse_grad(what)
+    page_table = _int32(page_table, (None, None), what, 'page_table', index)
     B, max_pages = page_table.shape
-    lengths = _index(lengths, (B,), what, 'lengths', dev)
-    cu = _index(cu_seqlens, (B + 1,), what, 'cu_seqlens', dev)
+    lengths = _int32(lengths, (B,), what, 'lengths', index)
+    cu = _int32(cu_seqlens, (B + 1,), what, 'cu_seqlens', index)
     if check:
         check_tables(cache, page_table, lengths, what, lengths - (cu[1:] - cu[:-1]), unique=True)
         if int(cu[0]) != 0 or int(cu[-1]) > shape[0]:
             raise ValueError(f'{what}: cu_seqlens runs from {int(cu[0])} to {int(cu[-1])}, there are {shape[0]} tokens')
     k, kp, ks = _rows(k)
     v, vp, vs = _rows(v)
-    _launch(dev, what, _lib.lib().kb200_kv_append, cache._ref, kp, vp, ks[0], ks[1], vs[0], vs[1],
-            page_table.data_ptr(), max_pages, lengths.data_ptr(), cu.data_ptr(), B, shape[0], dtype)
+    _launch(index, what, _lib.lib().kb200_kv_append, cache._args + _lib.KV_APPEND_ARGS.pack(
+        kp, vp, page_table.data_ptr(), lengths.data_ptr(), cu.data_ptr(), ks[0], ks[1], vs[0], vs[1], max_pages, B,
+        shape[0], dtype))
 
 
 def kv_cache_gather(cache: KVCache, page_table: torch.Tensor, starts: torch.Tensor, cu_seqlens: torch.Tensor, total: int,
@@ -200,15 +196,15 @@ def kv_cache_gather(cache: KVCache, page_table: torch.Tensor, starts: torch.Tens
     the host (``cu_seqlens[-1]``, or more: rows behind it are left as they were).  ``out``:
     ``(k, v)`` to write into, contiguous."""
     what = 'kv_cache_gather'
-    dev = _cuda(what, cache)
+    index = _cuda_index(what, cache)
     code = _DTYPES.get(dtype)
     if code is None:
         raise ValueError(f'{what}: dtype must be bfloat16 or float16, got {dtype}')
-    page_table = _index(page_table, (None, None), what, 'page_table', dev)
+    page_table = _int32(page_table, (None, None), what, 'page_table', index)
     B, max_pages = page_table.shape
-    starts = _index(starts, (B,), what, 'starts', dev)
-    cu = _index(cu_seqlens, (B + 1,), what, 'cu_seqlens', dev)
-    shape = (int(total), cache._shape[1], cache._shape[3])
+    starts = _int32(starts, (B,), what, 'starts', index)
+    cu = _int32(cu_seqlens, (B + 1,), what, 'cu_seqlens', index)
+    shape = (int(total), *cache._row)
     if shape[0] < 0:
         raise ValueError(f'{what}: total {total}')
     if check:
@@ -216,14 +212,15 @@ def kv_cache_gather(cache: KVCache, page_table: torch.Tensor, starts: torch.Tens
         if int(cu[0]) != 0 or int(cu[-1]) > shape[0]:
             raise ValueError(f'{what}: cu_seqlens runs from {int(cu[0])} to {int(cu[-1])}, total is {shape[0]}')
     if out is None:
-        k, v = torch.empty(shape, device=dev, dtype=dtype), torch.empty(shape, device=dev, dtype=dtype)
+        k = torch.empty(shape, device=cache._device, dtype=dtype)
+        v = torch.empty_like(k)
     else:
         k, v = out
         for t in (k, v):
-            if t.shape != shape or t.dtype != dtype or t.device != dev or not t.is_contiguous() or t.data_ptr() % 16:
-                raise ValueError(f'{what}: out must be contiguous 16-byte aligned {dtype} {list(shape)} on {dev}')
-    _launch(dev, what, _lib.lib().kb200_kv_gather, cache._ref, page_table.data_ptr(), max_pages, starts.data_ptr(),
-            cu.data_ptr(), B, shape[0], k.data_ptr(), v.data_ptr(), code)
+            if t.shape != shape or t.dtype != dtype or t.get_device() != index or not t.is_contiguous() or t.data_ptr() % 16:
+                raise ValueError(f'{what}: out must be contiguous 16-byte aligned {dtype} {list(shape)} on {cache.device}')
+    _launch(index, what, _lib.lib().kb200_kv_gather, cache._args + _lib.KV_GATHER_ARGS.pack(
+        k.data_ptr(), v.data_ptr(), page_table.data_ptr(), starts.data_ptr(), cu.data_ptr(), max_pages, B, shape[0], code))
     return k, v
 
 
@@ -249,7 +246,7 @@ def attention_cached(q: torch.Tensor, cache: KVCache, page_table: torch.Tensor, 
     q's type (``out``: contiguous, to write into); with ``return_lse`` also the fp32 log of
     the softmax sum ``[B, Sq, Hq]`` (-inf where nothing is seen)."""
     what = 'attention_cached'
-    dev = _cuda(what, cache)
+    index = _cuda_index(what, cache)
     _, H, page, D = cache._shape
     shape = q.shape
     if len(shape) != 4 or shape[3] != D or shape[2] < 1 or shape[2] % H:
@@ -257,26 +254,25 @@ def attention_cached(q: torch.Tensor, cache: KVCache, page_table: torch.Tensor, 
     dtype = _DTYPES.get(q.dtype)
     if dtype is None:
         raise ValueError(f'{what}: q must be bfloat16 or float16, got {q.dtype}')
-    if q.device != dev:
-        raise ValueError(f'{what}: q must be on {dev}, got {q.device}')
-    _forward_only(what, q)
+    if q.get_device() != index:
+        raise ValueError(f'{what}: q must be on {cache.device}, got {q.device}')
+    if q.requires_grad and torch.is_grad_enabled():
+        _refuse_grad(what)
     B, Sq, Hq, _ = shape
-    page_table = _index(page_table, (B, None), what, 'page_table', dev)
-    lengths = _index(lengths, (B,), what, 'lengths', dev)
+    page_table = _int32(page_table, (B, None), what, 'page_table', index)
+    lengths = _int32(lengths, (B,), what, 'lengths', index)
     max_pages = page_table.shape[1]
     if check:
         check_tables(cache, page_table, lengths, what)
-    if softmax_scale is None:
-        softmax_scale = D ** -0.5
     q, qp, qs = _rows(q)
     if out is None:
         out = q.new_empty(shape)
-    elif out.shape != shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous() or out.data_ptr() % 16:
-        raise ValueError(f'{what}: out must be contiguous 16-byte aligned {q.dtype} {list(shape)} on {dev}')
-    lse = torch.empty(shape[:3], device=dev, dtype=torch.float32) if return_lse else None
-    nbytes = _cached_workspace(dev.index, B, Sq, Hq, H, D, page, max_pages)
+    elif out.shape != shape or out.dtype != q.dtype or out.get_device() != index or not out.is_contiguous() or out.data_ptr() % 16:
+        raise ValueError(f'{what}: out must be contiguous 16-byte aligned {q.dtype} {list(shape)} on {cache.device}')
+    lse = torch.empty(shape[:3], device=cache._device, dtype=torch.float32) if return_lse else None
+    nbytes = _cached_workspace(index, B, Sq, Hq, H, D, page, max_pages)
     ws = lengths.new_empty(nbytes >> 2)
-    _launch(dev, what, _lib.lib().kb200_attn_cached_fwd, qp, qs[0], qs[1], qs[2], cache._ref,
-            page_table.data_ptr(), max_pages, lengths.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else None, B, Sq,
-            Hq, float(softmax_scale), dtype, ws.data_ptr(), nbytes)
+    _launch(index, what, _lib.lib().kb200_attn_cached_fwd, cache._args + _lib.ATTN_CACHED_ARGS.pack(
+        qp, out.data_ptr(), lse.data_ptr() if return_lse else 0, page_table.data_ptr(), lengths.data_ptr(), ws.data_ptr(),
+        nbytes, qs[0], qs[1], qs[2], max_pages, B, Sq, Hq, D ** -0.5 if softmax_scale is None else softmax_scale, dtype))
     return (out, lse) if return_lse else out

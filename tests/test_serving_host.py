@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from kairos_sensenova_b200 import KVCache, _lib, attention_cached, attention_prompt, kv_cache_append, kv_cache_gather
-from kairos_sensenova_b200.kv_cache import _index, _rows, check_tables
+from kairos_sensenova_b200.kv_cache import _int32, _rows, check_tables
 from oracle import serving as ref
 
 i32 = lambda x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
@@ -37,11 +37,12 @@ def test_operators_refuse_cpu_tensors():
 
 
 def test_index_and_rows():
-    cpu = torch.device('cpu')
-    assert _index(torch.tensor([1, 2]), (2,), 'x', 'y', cpu).dtype == torch.int32
+    assert _int32(torch.tensor([1, 2]), (2,), 'x', 'y', -1).dtype == torch.int32
     for bad in (torch.zeros(3), torch.zeros(2, 2, dtype=torch.int32), torch.zeros(3, dtype=torch.int16)):
         with pytest.raises(ValueError, match='x: y'):
-            _index(bad, (3,), 'x', 'y', cpu)
+            _int32(bad, (3,), 'x', 'y', -1)
+    with pytest.raises(ValueError, match='device 0'):
+        _int32(i32([1, 2]), (2,), 'x', 'y', 0)
     x = torch.zeros(10, 6, 64, dtype=torch.bfloat16)
     rows = lambda t: _rows(t)[0]  # noqa: E731
     assert rows(x[:, 2:4]).data_ptr() == x[:, 2:4].data_ptr()
@@ -66,23 +67,36 @@ def test_check_tables():
 
 def test_c_entries_refuse():
     L = _lib.lib()
-    cache = lambda **kw: ctypes.byref(_lib.KvCacheArgs(**{**dict(k_pages=16, v_pages=16, k_scale=16, v_scale=16, num_pages=4, H=2,  # noqa: E731
-                                                                page=16, D=64), **kw}))
-    app = lambda c, k=16, B=1, T=1, dt=0, ts=64: L.kb200_kv_append(c, k, 16, ts, 64, ts, 64, 16, 4, 16, 16, B, T, dt, None)  # noqa: E731
-    assert app(cache(), T=0) == 0 and app(cache(), B=0) == 0
+    cache = lambda **kw: _lib.KvCacheArgs(**{**dict(k_pages=16, v_pages=16, k_scale=16, v_scale=16, num_pages=4, H=2, page=16,  # noqa: E731
+                                                   D=64), **kw})
+    tables = dict(page_table=16, lengths=16, max_pages=4, B=1)
+
+    def app(c=None, **kw):
+        a = dict(cache=c or cache(), k=16, v=16, cu_new=16, k_token_stride=64, v_token_stride=64, T=1, **tables)
+        return L.kb200_kv_append(ctypes.byref(_lib.KvAppendArgs(**{**a, **kw})), None)
+    assert app(T=0) == 0 and app(B=0) == 0
     for bad in (dict(D=96), dict(page=8), dict(page=48), dict(H=0), dict(num_pages=0), dict(k_pages=0), dict(num_pages=1 << 40)):
         assert app(cache(**bad)) == 1, bad
-    assert app(cache(k_pages=8)) == 2 and app(cache(), k=24) == 2 and app(cache(), ts=65) == 2
-    assert app(cache(), dt=2) == 1 and app(cache(), T=-1) == 1 and app(cache(), k=None) == 1
-    assert L.kb200_kv_gather(cache(), 16, 4, 16, 16, 1, 0, None, None, 0, None) == 0
-    assert L.kb200_kv_gather(cache(), 16, 4, 16, 16, 1, 5, None, None, 0, None) == 1
-    assert L.kb200_kv_gather(cache(), 16, 4, 16, 16, 1, 5, 24, 16, 0, None) == 2
+    assert app(cache(k_pages=8)) == 2 and app(k=24) == 2 and app(k_token_stride=65) == 2
+    assert app(dtype=2) == 1 and app(T=-1) == 1 and app(k=None) == 1 and app(lengths=None) == 1
+    assert L.kb200_kv_append(None, None) == 1 and L.kb200_kv_gather(None, None) == 1 and L.kb200_attn_cached_fwd(None, None) == 1
+
+    def gather(**kw):
+        a = dict(cache=cache(), k=16, v=16, page_table=16, starts=16, cu=16, max_pages=4, B=1, T=5)
+        return L.kb200_kv_gather(ctypes.byref(_lib.KvGatherArgs(**{**a, **kw})), None)
+    assert gather(T=0, k=None) == 0 and gather(k=None) == 1 and gather(k=24) == 2 and gather(dtype=3) == 1
+
     size = lambda *a: L.kb200_attn_cached_workspace_size(*a)  # noqa: E731
     assert size(1, 1, 8, 2, 64, 16, 4) > 0 and size(1, 1, 7, 2, 64, 16, 4) == 0 and size(-1, 1, 8, 2, 64, 16, 4) == 0
-    att = lambda q=16, B=1, Hq=4, dt=0, ws=None, n=0, qs=64: L.kb200_attn_cached_fwd(  # noqa: E731
-        q, qs, qs, qs, cache(), 16, 4, 16, 16, None, B, 1, Hq, 1.0, dt, ws, n, None)
-    assert att(B=0) == 0 and att(Hq=3) == 1 and att(dt=5) == 1 and att(q=None) == 1 and att(q=8) == 2 and att(qs=4) == 2
+
+    def att(**kw):
+        a = dict(cache=cache(), q=16, o=16, q_batch_stride=64, q_token_stride=64, q_head_stride=64, Sq=1, Hq=4, softmax_scale=1.0,
+                 **tables)
+        return L.kb200_attn_cached_fwd(ctypes.byref(_lib.AttnCachedArgs(**{**a, **kw})), None)
+    assert att(B=0) == 0 and att(Hq=3) == 1 and att(dtype=5) == 1 and att(q=None) == 1 and att(q=8) == 2
+    assert att(q_head_stride=4) == 2
     assert att() == 3 and b'workspace' in L.kb200_last_error()
+    assert att(workspace=16, workspace_bytes=64) == 3
     base = dict(q=16, k=16, v=16, o=16, cu_q=16, cu_k=16, Tq=4, Tk=4, N=1, Hq=4, Hkv=2, D=64, q_token_stride=64, softmax_scale=1.0)
     pr = lambda **kw: L.kb200_attn_prompt_fwd(ctypes.byref(_lib.PromptArgs(**{**base, **kw})), None)  # noqa: E731
     assert pr(N=0) == 0 and pr(Tq=0) == 0
