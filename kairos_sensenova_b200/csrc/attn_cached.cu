@@ -28,6 +28,7 @@
 // bf16 queries are multiplied by a power of two per row into f16's range first (exact
 // but for elements 2^-29 below the row's largest).  P is rounded to f16 (2^-12).
 #include <math.h>
+#include <type_traits>
 #include "kv_cache.cuh"
 
 namespace kb {
@@ -63,6 +64,13 @@ KB_DEVI void mma_f16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// The same from zero.  (As an output alone: a zeroed accumulator passed in would cost four moves.)
+KB_DEVI void mma_f16_first(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 KB_DEVI uint32_t transpose8(uint32_t x) {   // 8x8 matrix of 16-bit values over the warp
   uint32_t r;
@@ -457,12 +465,14 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
         sk[j] = sc.x;
         sv[j] = sc.y;
       }
+      // Groups in which some row does not see some token, or a page is missing, take a body of their
+      // own, so that the others' is free of the tests.
+      auto body = [&](auto edge_group) {
+      constexpr bool EDGE = decltype(edge_group)::value;
       // ---- S^T = K Q^T of the group's 16-token parts
       float acc[NT][NT][4];                // [part][row tile]
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n) acc[j][n][0] = acc[j][n][1] = acc[j][n][2] = acc[j][n][3] = 0.f;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
           const int r0 = j * 16 + g;
@@ -475,13 +485,14 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
             kv::decode4(w0[e], a[0], a[2]);
             kv::decode4(w1[e], a[1], a[3]);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) mma_f16(acc[j][n], a, qf[n][c * 8 + 2 * e], qf[n][c * 8 + 2 * e + 1]);
+            for (int n = 0; n < NT; ++n)
+              if (c == 0 && e == 0) mma_f16_first(acc[j][n], a, qf[n][0], qf[n][1]);
+              else mma_f16(acc[j][n], a, qf[n][c * 8 + 2 * e], qf[n][c * 8 + 2 * e + 1]);
           }
         }
       }
       // ---- softmax; lane: tokens g, g + 8 of each part, rows 2 t4, 2 t4 + 1.  The rows' maxima
       // are looked up over the warp only when some lane's score passes the reference by TAU.
-      const bool edge = base + GT > all_seen;
       uint32_t pf[NT][NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -492,11 +503,11 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
           float* x = acc[j][n];
           f0[j] = fmaxf(sk[j] * qs[n][0], 1e-37f);
           f1[j] = fmaxf(sk[j] * qs[n][1], 1e-37f);
-          if (sk[j] < 0.f) {               // a missing page
+          if (EDGE && sk[j] < 0.f) {       // a missing page
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[e] = -INFINITY;
           }
-          if (edge) {
+          if (EDGE) {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               if (base + j * 16 + g + (e >> 1) * 8 >= seen[n][e & 1]) x[e] = -INFINITY;
@@ -535,7 +546,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
       constexpr int VW = D / 32;           // 32-bit words of channels per lane
 #pragma unroll
       for (int part = 0; part < NT; ++part) {
-        if (sk[part] < 0.f) continue;
+        if (EDGE && sk[part] < 0.f) continue;
         uint32_t vr[4][VW];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -549,7 +560,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
           }
         }
         bool poison = false;               // a NaN code that some rows must not see
-        if (edge) {
+        if (EDGE) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int tok = base + part * 16 + 2 * t4 + (j & 1) + (j >> 1) * 8;
@@ -572,7 +583,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
             uint32_t a[4];
             kv::decode4(u01, a[0], a[1]);
             kv::decode4(u89, a[2], a[3]);
-            if (poison) {
+            if (EDGE && poison) {
               // a NaN value reaches only the rows that see its token: it is taken out of the
               // product, and a second product counts the NaNs each row sees
               uint32_t bad[4];
@@ -584,11 +595,10 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
               }
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
-                float cnt[4] = {0.f, 0.f, 0.f, 0.f};
-                float vis[4];
+                float cnt[4], vis[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) vis[e] = base + part * 16 + g + (e >> 1) * 8 < seen[n][e & 1] ? 1.f : 0.f;
-                mma_f16(cnt, bad, transpose8(kv::pack16<true>(vis[0], vis[1])), transpose8(kv::pack16<true>(vis[2], vis[3])));
+                mma_f16_first(cnt, bad, transpose8(kv::pack16<true>(vis[0], vis[1])), transpose8(kv::pack16<true>(vis[2], vis[3])));
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                   if (cnt[e] > 0.f) o[n][2 * w + z][e] = __uint_as_float(0x7fffffffu);
@@ -596,8 +606,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
             }
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              float d[4] = {0.f, 0.f, 0.f, 0.f};
-              mma_f16(d, a, pf[part][n][0], pf[part][n][1]);
+              float d[4];
+              mma_f16_first(d, a, pf[part][n][0], pf[part][n][1]);
               float* oo = o[n][2 * w + z];
               const float2 s2 = make_float2(sv[part], sv[part]);
               const float2 o01 = ffma2(make_float2(d[0], d[1]), s2, make_float2(oo[0], oo[1]));
@@ -607,6 +617,12 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
           }
         }
       }
+      };
+      bool edge = base + GT > all_seen;
+#pragma unroll
+      for (int j = 0; j < NT; ++j) edge |= sk[j] < 0.f;
+      if (edge) body(std::true_type{});
+      else body(std::false_type{});
       __syncwarp();
       // the last slot of the segment is kept: it takes the warp's O
       if (gi + WK < count) loader.load(p, (int)units, warp, lane, sm.slot[warp][s], sm.scale[warp][s]);
