@@ -140,6 +140,14 @@ KB_DEVI uint32_t swz(int r, int c) {
   else return (uint32_t)((r >> 1) * 128 + (((((r & 1) << 2) | c) ^ (((r >> 1) & 3) << 1)) << 4));
 }
 
+// Where 16-byte chunk `c` of row `r` of a warp's O lies in the slot it kept: the eight lanes that store
+// together (two chunk groups, four rows r = 2 t) meet eight different chunks of a line.
+template <int D>
+KB_DEVI int o_chunk(int r, int c) {
+  const int t = (r >> 1) & 3;
+  return r * (D / 4) + (c ^ (D == 128 ? t : (t & 1) | (t & 2) << 1));
+}
+
 // The launch shapes.  NT: 8-row tiles of a CTA (rows up to 8: 1, else 2); a group is NT * 16
 // tokens.  WK warps, OCC CTAs per SM: as many warps as the registers allow (at D = 128, 8 rows
 // need under 128 and 16 rows under 168).
@@ -216,8 +224,8 @@ struct Smem {
   float2 scale[S::WK][S::STAGES][NT];        // page scales (k, v) of 16 tokens each; k < 0: no such page
   Feed<S::GT> feed[S::WK];
   Walk<S::GT> walk[S::WK];
-  int64_t total, begin;
-  int first_b;
+  Walk<S::GT> start;
+  int64_t total;
   int held[S::WK];                           // the slot that holds the warp's O, -1: none
 };
 
@@ -233,7 +241,21 @@ struct Loader {
   int pg2;                                   // the next batch's
   float2 sc, sc2;
   bool pending;                              // sc2 is still to be read
+  float2* owed;                              // where the last group's scales are still to be written (null: nowhere)
 
+  // The scales of the group loaded last.  They are written one call later, so that the copies
+  // of a group do not wait for them.
+  KB_DEVI void pay(int lane) {
+    if (owed) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const int src = (pos - 1) * NT + j;
+        const float2 s = make_float2(__shfl_sync(0xffffffffu, sc.x, src), __shfl_sync(0xffffffffu, sc.y, src));
+        if (lane == 0) owed[j] = s;
+      }
+    }
+    owed = nullptr;
+  }
   KB_DEVI void next_batch(const Params& p, int units, int warp, int lane) {
     __syncwarp();
     Feed<S::GT> f = *feed;
@@ -275,12 +297,13 @@ struct Loader {
     }
     pending = false;
   }
-  KB_DEVI Loader(Feed<S::GT>* at, const Params& p, int units, int warp, int lane) : feed(at), n(0), pos(0) {
+  KB_DEVI Loader(Feed<S::GT>* at, const Params& p, int units, int warp, int lane) : feed(at), n(0), pos(0), owed(nullptr) {
     next_batch(p, units, warp, lane);
   }
   // The next group into `slot`; always one cp.async group, empty when the work is over.
   KB_DEVI void load(const Params& p, int units, int warp, int lane, typename Smem<D, NT>::Slot& slot, float2* scale) {
     if (pos == n) {
+      pay(lane);
       if (pending) read_scales(p);
       h = feed->h; n = feed->n; tok0 = feed->tok0;
       pg = pg2; sc = sc2;
@@ -289,13 +312,11 @@ struct Loader {
     } else if (pending) {
       read_scales(p);
     }
+    float2* now = nullptr;
     if (n) {
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        const int src = pos * NT + j;
-        const int page = __shfl_sync(0xffffffffu, pg, src);
-        const float2 s = make_float2(__shfl_sync(0xffffffffu, sc.x, src), __shfl_sync(0xffffffffu, sc.y, src));
-        if (lane == 0) scale[j] = s;
+        const int page = __shfl_sync(0xffffffffu, pg, pos * NT + j);
         if (page >= 0) {
           const int tok = tok0 + pos * (S::WK * S::GT) + j * 16;
           const int64_t row = ((int64_t)page * p.H + h) * p.page + (tok & (p.page - 1));
@@ -309,9 +330,12 @@ struct Loader {
           }
         }
       }
-      ++pos;
+      now = scale;
     }
     cp_async_commit();
+    pay(lane);
+    pos += n ? 1 : 0;
+    owed = now;
   }
 };
 
@@ -338,8 +362,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
     if ((int64_t)blockIdx.x * sh.per < sh.total) warp_find<GT>(p, units, blockIdx.x * sh.per, lane, b, begin);
     if (lane == 0) {
       sm.total = sum;
-      sm.first_b = b;
-      sm.begin = begin;
+      if ((int64_t)blockIdx.x * sh.per < sh.total)
+        sm.start.start(p, blockIdx.x * sh.per, min((blockIdx.x + 1) * sh.per, sh.total), b, begin);
     }
   }
   __syncthreads();
@@ -353,7 +377,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
   // warp (i + rot) % WK, so that short segments use all of them in turn.
   if (lane == 0) {
     Feed<GT> f{};
-    f.seg.start(p, at0, at1, sm.first_b, sm.begin);
+    f.seg = sm.start;
     sm.walk[warp] = f.seg;
     f.first = warp;
     f.live = f.seg.next(p, (int)units);
@@ -631,7 +655,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
     }
     // ---- the warps' partial results join: each one's O in the slot it kept
     if (held >= 0) {
-      float* mo = reinterpret_cast<float*>(&sm.slot[warp][held]);
+      float4* mo = reinterpret_cast<float4*>(&sm.slot[warp][held]);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -645,8 +669,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
             sm.ml[warp][r][1] = x;
           }
 #pragma unroll
-          for (int i = 0; i < MT; ++i)       // channels g * D/8 + 2 i, + 1
-            *reinterpret_cast<float2*>(mo + r * D + g * (D / 8) + 2 * i) = make_float2(o[n][i][c], o[n][i][2 + c]);
+          for (int i = 0; i < MT; i += 2)    // channels g * D/8 + 2 i .. + 3
+            mo[o_chunk<D>(r, g * (D / 32) + i / 2)] = make_float4(o[n][i][c], o[n][i][2 + c], o[n][i + 1][c], o[n][i + 1][2 + c]);
         }
       }
     }
@@ -672,7 +696,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
         if (hs >= 0) {
           // (m = -inf: no visible key, O and l are 0, or all of its scores are NaN, and so are they)
           const float f = mk[k] == -INFINITY ? 1.f : ex2(mk[k] - mx);
-          const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(&sm.slot[k][hs]) + r * D + c * 4);
+          const float4 x = reinterpret_cast<const float4*>(&sm.slot[k][hs])[o_chunk<D>(r, c)];
           a.x += f * x.x; a.y += f * x.y; a.z += f * x.z; a.w += f * x.w;
           ls += f * sm.ml[k][r][1];
         }
@@ -752,6 +776,19 @@ __global__ void __launch_bounds__(Shape<D, NT>::JOIN) attn_cached_join_kernel(Pa
   __syncthreads();
   for (int k0 = c0; k0 <= c1; k0 += CHUNK) {
     const int n = min(CHUNK, c1 + 1 - k0);
+    // the first parts' O is on its way while the factors are formed
+    constexpr int EARLY = 8;
+    float4 first[ITEMS][EARLY];
+    auto part_of = [&](int k, int r, int c) {
+      return reinterpret_cast<const float4*>(p.part + ((2 * (int64_t)(k0 + k) + (k0 + k == c0 ? 1 : 0)) * ROWS + r) * D + c * 4);
+    };
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int r = (threadIdx.x + i * THREADS) / (D / 4), c = (threadIdx.x + i * THREADS) % (D / 4);
+#pragma unroll
+      for (int k = 0; k < EARLY; ++k)
+        first[i][k] = k < n && rb * ROWS + r < p.R ? __ldcg(part_of(k, r, c)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
     // a warp per row, a lane per part: the parts' factors, and that of what is joined so far
     for (int r = threadIdx.x >> 5; r < ROWS; r += THREADS / 32) {
       float2 x = make_float2(-INFINITY, 0.f);
@@ -775,11 +812,17 @@ __global__ void __launch_bounds__(Shape<D, NT>::JOIN) attn_cached_join_kernel(Pa
       if (rb * ROWS + r >= p.R) continue;
       const float f0 = scale_old[r];
       acc[i].x *= f0; acc[i].y *= f0; acc[i].z *= f0; acc[i].w *= f0;
-#pragma unroll 16
-      for (int k = 0; k < n; ++k) {
+#pragma unroll
+      for (int k = 0; k < EARLY; ++k)
+        if (k < n) {
+          const float f = fac[k][r];
+          const float4 x = first[i][k];
+          acc[i].x += x.x * f; acc[i].y += x.y * f; acc[i].z += x.z * f; acc[i].w += x.w * f;
+        }
+#pragma unroll 8
+      for (int k = EARLY; k < n; ++k) {
         const float f = fac[k][r];
-        const float4 x = __ldcg(reinterpret_cast<const float4*>(
-            p.part + ((2 * (int64_t)(k0 + k) + (k0 + k == c0 ? 1 : 0)) * ROWS + r) * D + c * 4));
+        const float4 x = __ldcg(part_of(k, r, c));
         acc[i].x += x.x * f; acc[i].y += x.y * f; acc[i].z += x.z * f; acc[i].w += x.w * f;
       }
     }
