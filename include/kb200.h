@@ -246,7 +246,12 @@ typedef struct KB200PromptArgs {
   float softmax_scale;
   int causal;
   int dtype;
+  void* workspace;            /* 16-byte aligned, or NULL (below)                 */
+  size_t workspace_bytes;
 } KB200PromptArgs;
+/* Bytes with which few queries over many keys are shared out over all SMs; 0 where that
+ * is of no use.  Without a workspace the result is the same, slower in those cases. */
+size_t kb200_attn_prompt_workspace_size(int64_t Tq, int64_t Tk, int64_t N, int64_t Hq, int64_t Hkv, int64_t D);
 int kb200_attn_prompt_fwd(const KB200PromptArgs* a, void* stream);
 
 /* ---------------------------------------------------------------------

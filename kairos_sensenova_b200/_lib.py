@@ -65,11 +65,12 @@ class PromptArgs(ctypes.Structure):
         ('v_token_stride', ctypes.c_int64), ('v_head_stride', ctypes.c_int64),
         ('o_token_stride', ctypes.c_int64), ('o_head_stride', ctypes.c_int64),
         ('softmax_scale', ctypes.c_float), ('causal', ctypes.c_int), ('dtype', ctypes.c_int),
+        ('workspace', ctypes.c_void_p), ('workspace_bytes', ctypes.c_size_t),
     ]
 
 
 # the same bytes packed directly (a ctypes structure of this many fields costs several times as much to fill)
-PROMPT_ARGS = struct.Struct('@7P14qfii4x')
+PROMPT_ARGS = struct.Struct('@7P14qfiiPN')
 assert PROMPT_ARGS.size == ctypes.sizeof(PromptArgs)
 
 
@@ -142,6 +143,7 @@ SIGNATURES = {
                               [ctypes.c_void_p] * 3 + [ctypes.c_int, ctypes.c_float] + [ctypes.c_void_p] * 2),
     # these four take their argument structure or its packed bytes
     'kb200_attn_prompt_fwd': (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
+    'kb200_attn_prompt_workspace_size': (ctypes.c_size_t, [ctypes.c_int64] * 6),
     'kb200_kv_append': (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
     'kb200_kv_gather': (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
     'kb200_attn_cached_workspace_size': (ctypes.c_size_t, [ctypes.c_int64] * 7),

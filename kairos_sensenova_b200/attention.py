@@ -17,6 +17,8 @@ dilation is a rearrangement before this call); key tiles outside every window of
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 import torch.nn as nn
 
@@ -99,6 +101,13 @@ class AttentionModule(nn.Module):
 FP8AttentionModule = AttentionModule
 
 
+@functools.lru_cache(maxsize=256)
+def _prompt_workspace(device_index, *sizes):
+    """Workspace bytes for these sizes (they depend on the device's number of SMs)."""
+    with torch.cuda.device(device_index):
+        return _lib.lib().kb200_attn_prompt_workspace_size(*sizes)
+
+
 def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens_q: torch.Tensor,
                      cu_seqlens_k: torch.Tensor | None = None, softmax_scale: float | None = None,
                      causal: bool = True, out: torch.Tensor | None = None, return_lse: bool = False, check: bool = False):
@@ -153,9 +162,11 @@ def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         if out.shape != shape or out.dtype != qd or out.get_device() != index or same is not out:
             raise ValueError(f'{what}: out must be {q.dtype} {list(shape)} on {q.device}, its rows 16-byte aligned')
     lse = torch.empty((Tq, Hq), device=q.device, dtype=torch.float32) if return_lse else None
+    nbytes = _prompt_workspace(index, Tq, Tk, N, Hq, Hkv, D)
+    ws = cu_q.new_empty(nbytes >> 2) if nbytes else None
     args = _lib.PROMPT_ARGS.pack(
         qp, kp, vp, op, lse.data_ptr() if return_lse else 0, cu_q.data_ptr(), cu_k.data_ptr(), Tq, Tk, N, Hq, Hkv, D,
         qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1], D ** -0.5 if softmax_scale is None else softmax_scale,
-        1 if causal else 0, dtype)
+        1 if causal else 0, dtype, ws.data_ptr() if nbytes else 0, nbytes)
     _launch(index, what, _lib.lib().kb200_attn_prompt_fwd, args)
     return (out, lse) if return_lse else out

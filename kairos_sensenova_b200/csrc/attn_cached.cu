@@ -757,9 +757,10 @@ __global__ void __launch_bounds__(Shape<D, NT>::JOIN) attn_cached_join_kernel(Pa
     begin = before * units + (int64_t)u * span;
     c0 = (int)(begin / sh.per);
     c1 = (int)((begin + ng - 1) / sh.per);
-    if (c0 == c1) return;                  // finished there
   }
+  // (every block waits, those without work too: this grid must not end before the one it follows)
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  if (ng > 0 && c0 == c1) return;          // finished there
   // Partials in share order: the part that begins the unit is its CTA's last segment (slot 1),
   // the later ones continue it (slot 0).  A chunk's m and l are read together, then its O with
   // all loads in flight: what the join costs is the two latencies.
@@ -845,16 +846,6 @@ __global__ void __launch_bounds__(Shape<D, NT>::JOIN) attn_cached_join_kernel(Pa
 // 8-row tiles that a CTA takes of the R = Sq * Hq / Hkv rows: rows above 16 form blocks that
 // read the cache again, mostly from L2 (more tiles per warp would not fit the registers).
 static int row_tiles(int64_t R) { return R <= 8 ? 1 : 2; }
-
-static int sm_count() {
-  static int counts[64];             // per device; written with the same value by every thread that gets there
-  int dev = 0, n = 148;
-  if (cudaGetDevice(&dev) != cudaSuccess) { cudaGetLastError(); return n; }
-  if (dev < 64 && counts[dev]) return counts[dev];
-  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-  if (dev < 64) counts[dev] = n;
-  return n;
-}
 
 // CTAs of the main kernel: as many as fit on the GPU at once, no more than can have work.
 template <int D, int NT>

@@ -6,21 +6,29 @@
 // Bound: the tensor pipe and the exponentials together.  A tile of 256 rows x 128 keys is
 // 4 * 256 * 128 * D flops (2048 cycles at D = 128) and 32768 exponentials (2048 cycles of MUFU).
 //
-// Rows.  The G = Hq / Hkv heads that share a kv head are rows of one matrix, row
-// r = token * G + head in group, so a CTA of 256 rows reads each key tile once for all of
-// them, and short prompts still fill the tile.  Any G works: Q is fetched with plain
-// loads, K and V by TMA (boxes of 64 channels x 128 tokens of one head, any token stride).
+// Rows.  The G = Hq / Hkv heads that share a kv head are rows of one matrix: a query tile of 128
+// rows holds T = 128 / G tokens (rounded down) with G heads each, row = token * G + head, so a
+// CTA reads each key tile once for all of them, and short prompts still fill the tile.  That is a
+// TMA box of T tokens x G heads; with G not a divisor of 128 a few rows stay empty.  (G
+// over 128: the heads are taken in equal parts of at most 128.)  K and V come in boxes of 64
+// channels x 128 tokens of one head; any token and head stride works.
 //
-// Order.  CTA c takes tile c / Hkv of all sequences' tiles sorted by their number of
-// keys, most first (each CTA finds its own by a search over the levels: no host
-// knowledge of the lengths, no extra launch); the short ones fill the end of the run.
+// Items.  The kernel is persistent, a CTA per SM.  An item is a tile of rows with the key tiles
+// that it sees; K, V and the next item's Q are on their way while one is computed.
+//   * Many items: sorted by their number of keys, most first, CTA c takes them in turns (c, then
+//     2 S - 1 - c, 2 S + c, ... of S CTAs), so that every CTA gets long and short ones.
+//   * Few items for the SMs and many keys: the key tiles of all items are laid end to end and
+//     every CTA takes an equal share, as in attn_cached.cu; an item that crosses shares leaves
+//     fp32 partials (m, l, O), joined in share order by a second kernel.
+// Both are found on the device from the offsets: the host need not know the lengths.
 //
-// One CTA, 12 warps (one idles: registers are dealt by warpgroups of four):
+// One CTA, 12 warps (registers are dealt by warpgroups of four):
 //   warps 0-7  softmax: query tile t = w / 4, one row per thread (its 128 scores in registers)
 //   warp 8     TMA producer: K and V tiles into their rings
 //   warp 9     issues S = Q_t K_j^T, in the order QK_0(j) QK_1(j): the two query tiles share one
 //              TMEM score buffer, which a tile gives back as soon as its scores are in registers
 //   warp 10    issues O_t += P_t V_j (P_t from TMEM, V read MN-major from its TMA tile)
+//   warp 11    finds the items and loads their Q
 // What a period of 256 rows x 128 keys takes is the chain QK_0 - load - QK_1 - load: each link
 // is 512 cycles of product, the two hand-offs and the load.  So the loads read whole lanes
 // (32x32b; the 16-lane shapes run at half the rate) and the two kinds of products have
@@ -36,7 +44,7 @@
 // what it should be).
 //
 // Every wait is bounded.  A warp whose wait gives up stops, so that the others' waits give up
-// too; what is in flight is drained, and the CTA writes NaN.
+// too; what is in flight is drained, and the CTA writes NaN into all of its rows.
 #include <math.h>
 #include <string.h>
 #include "kb200_internal.h"
@@ -53,10 +61,12 @@ struct Params {
   const int32_t *cu_q, *cu_k;
   int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, o_ts, o_hs;
   int64_t Tq, Tk;
-  int N, Hq, H, G;
+  int N, Hq, H, G;         // H kv heads times parts, G query heads of each
+  int parts, tq;           // parts of a kv head's query heads; tokens of a query tile
   float scale_log2;        // |softmax scale| log2 e; its sign goes into q (flip)
   uint32_t flip;
-  uint64_t g_magic;        // ceil(2^32 / G): x / G = x g_magic >> 32 for x G < 2^32
+  int split;               // equal shares of the key tiles (else whole items)
+  float* part;             // shares: [2 CTAs][rows][D] partial O, then [2 CTAs][rows][2] (m, l)
   int causal;
 };
 
@@ -104,7 +114,7 @@ KB_DEVI void store16(void* base, int64_t i, float x) {
 template <int D, bool F16>
 KB_DEVI void attend_row(const Params& p, int64_t tq, int h, int64_t k0, int64_t seen, int lane) {
   constexpr int C = D / 32;
-  const int hk = h / p.G;
+  const int hk = h / (p.G * p.parts);
   float q[C], acc[C];
 #pragma unroll
   for (int c = 0; c < C; ++c) {
@@ -146,7 +156,24 @@ constexpr int SORTED = 64;                   // up to this many sequences the ti
 constexpr uint32_t TM_O = 0, TM_S = 256, TM_P = 384;   // TMEM columns: O_t at 128 t, S, P_t at 64 t
 
 struct Maps {
-  CUtensorMap k, v;
+  CUtensorMap q, k, v;
+};
+
+constexpr int TABLE = 128;                   // shares: at most this many row tiles
+constexpr int PAD = 3;                       // shares: what an item costs besides its key tiles, in key tiles
+constexpr int LEAST = 8;                     // shares: at least this many key tiles
+
+// The row tiles of all sequences, and the flat length of those before each (key tiles + PAD).
+struct Table {
+  int before[TABLE + 1];
+  uint8_t seq[TABLE], tile[TABLE];
+};
+
+struct Item {
+  int q0, n, k0, m;                          // packed queries and keys of the sequence
+  int tile, hk;                              // row tile in it, kv head
+  int j0, j1, all;                           // key tiles [j0, j1) of the `all` that the tile sees
+  int slot;                                  // where the partial goes; -1: the item is whole, -2: no more items
 };
 
 template <int D>
@@ -156,22 +183,33 @@ struct Smem {
   uint8_t q[QT][ATOMS][BM * 128];
   uint8_t k[KS][ATOMS][BN * 128];
   uint8_t v[VS][ATOMS][BN * 128];
-  uint64_t q_full;
+  uint64_t item_full[2], item_free[2];       // an item is published / every warp has read it
+  uint64_t q_full, q_free;
   uint64_t k_full[KS], k_empty[KS], v_full[VS], v_empty[VS];
-  uint64_t s_full[QT], s_free[QT], p_full[QT], pv_done[QT], o_done, drain[2];
+  uint64_t s_full[QT], s_free[QT], p_full[QT], pv_done[QT], drain[2];
+  Item item[2];
+  Table table;
   uint32_t tmem_base;
-  int seq, tile;                             // this CTA's sequence (-1: none) and row tile in it
-  int4 range;                                // its queries and keys
   int abort_flag, keep_tmem;
 };
+
+// Keys that query `t` of n sees, of m.
+KB_DEVI int seen_by(const Params& p, int64_t t, int n, int m) {
+  return p.causal ? (int)min((int64_t)m, max((int64_t)0, t + 1 + m - n)) : m;
+}
+// Key tiles that row tile `tile` sees.
+KB_DEVI int key_tiles(const Params& p, int tile, int n, int m) {
+  const int64_t last = min((int64_t)n, (int64_t)(tile + 1) * QT * p.tq) - 1;
+  return (seen_by(p, last, n, m) + BN - 1) / BN;
+}
 
 // Tile `r` of the order above: sequence and tile in it, by one warp (seq = -1: there is none).
 KB_DEVI void find_tile(const Params& p, int64_t r, int lane, int& seq, int& tile) {
   auto tiles_of = [&](int s, int& level) {   // row tiles of sequence s; level of its first one
     const int2 q = seq_range(p.cu_q, s, p.Tq), k = seq_range(p.cu_k, s, p.Tk);
     const int n = q.y - q.x;
-    level = p.causal ? (int)(max(k.y - k.x - n, 0) * (int64_t)p.G / ROWS) : 0;
-    return (int)(((int64_t)n * p.G + ROWS - 1) / ROWS);
+    level = p.causal ? max(k.y - k.x - n, 0) / (QT * p.tq) : 0;
+    return (n + QT * p.tq - 1) / (QT * p.tq);
   };
   seq = -1;
   tile = 0;
@@ -232,6 +270,118 @@ KB_DEVI void find_tile(const Params& p, int64_t r, int lane, int& seq, int& tile
   }
 }
 
+// Fills the table, by one warp; returns the number of row tiles.
+KB_DEVI int build_table(const Params& p, Table& tb, int lane) {
+  int base = 0;
+  for (int s0 = 0; s0 < p.N; s0 += 32) {
+    const int s = s0 + lane;
+    int nt = 0;
+    if (s < p.N) {
+      const int2 q = seq_range(p.cu_q, s, p.Tq);
+      nt = min(TABLE, (q.y - q.x + QT * p.tq - 1) / (QT * p.tq));
+    }
+    int inc = nt;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += y;
+    }
+    for (int i = 0; i < nt && base + inc - nt + i < TABLE; ++i) {
+      tb.seq[base + inc - nt + i] = (uint8_t)s;
+      tb.tile[base + inc - nt + i] = (uint8_t)i;
+    }
+    base = min(TABLE, base + __shfl_sync(0xffffffffu, inc, 31));
+  }
+  __syncwarp();
+  int before = 0;
+  for (int f0 = 0; f0 < base; f0 += 32) {
+    int cost = 0;
+    if (f0 + lane < base) {
+      const int s = tb.seq[f0 + lane];
+      const int2 q = seq_range(p.cu_q, s, p.Tq), k = seq_range(p.cu_k, s, p.Tk);
+      cost = key_tiles(p, tb.tile[f0 + lane], q.y - q.x, k.y - k.x) + PAD;
+    }
+    int inc = cost;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += y;
+    }
+    if (f0 + lane < base) tb.before[f0 + lane + 1] = before + inc;
+    before += __shfl_sync(0xffffffffu, inc, 31);
+  }
+  if (lane == 0) tb.before[0] = 0;
+  __syncwarp();
+  return base;
+}
+// Flat positions of a share: those of all kv heads, [hk][row tile][key tile + PAD].
+KB_DEVI int64_t share_size(const Params& p, int flat, int ctas) {
+  return max((int64_t)LEAST, ((int64_t)flat * p.H + ctas - 1) / ctas);
+}
+
+// The items of a CTA, one after the other; by one warp, every lane has them.
+struct Items {
+  int64_t turn, left;
+  int tiles, flat, hk, f, x;                 // shares: row tiles, their flat length; the next position
+  KB_DEVI void start(const Params& p, Table& tb, int lane) {
+    turn = 0;
+    left = 0;
+    if (!p.split) return;
+    tiles = build_table(p, tb, lane);
+    flat = tb.before[tiles];
+    if (flat == 0) return;
+    const int64_t all = (int64_t)flat * p.H, per = share_size(p, flat, gridDim.x), at = blockIdx.x * per;
+    left = min(per, all - at);
+    if (left <= 0) return;
+    hk = (int)(at / flat);
+    const int rem = (int)(at - (int64_t)hk * flat);
+    f = 0;
+    while (tb.before[f + 1] <= rem) ++f;
+    x = rem - tb.before[f];
+  }
+  KB_DEVI Item next(const Params& p, const Table& tb, int lane) {
+    Item it{};
+    it.slot = -2;
+    int seq, tile;
+    if (!p.split) {
+      const int64_t S = gridDim.x, r = turn * S + ((turn & 1) ? S - 1 - blockIdx.x : blockIdx.x);
+      ++turn;
+      find_tile(p, r / p.H, lane, seq, tile);
+      if (seq < 0) return it;
+      it.hk = (int)(r % p.H);
+    } else {
+      int take, span;
+      do {
+        if (left <= 0) return it;
+        if (f == tiles) {
+          f = 0;
+          ++hk;
+        }
+        span = tb.before[f + 1] - tb.before[f];
+        take = (int)min((int64_t)(span - x), left);
+        left -= take;
+        it.j0 = x;
+        it.j1 = min(x + take, span - PAD);
+        seq = tb.seq[f];
+        tile = tb.tile[f];
+        it.hk = hk;
+        x += take;
+        if (x == span) {
+          x = 0;
+          ++f;
+        }
+      } while (it.j1 <= it.j0 && !(it.j0 == 0 && span == PAD));   // (an item that sees no key is written too)
+    }
+    const int2 q = seq_range(p.cu_q, seq, p.Tq), k = seq_range(p.cu_k, seq, p.Tk);
+    it.q0 = q.x; it.n = q.y - q.x; it.k0 = k.x; it.m = k.y - k.x;
+    it.tile = tile;
+    it.all = key_tiles(p, tile, it.n, it.m);
+    if (!p.split) it.j1 = it.all;
+    it.slot = it.j0 == 0 && it.j1 == it.all ? -1 : 2 * (int)blockIdx.x + (it.j0 > 0 ? 0 : 1);
+    return it;
+  }
+};
+
 // One arrival per warp, after its TMEM reads or writes.
 KB_DEVI void warp_arrive(uint64_t* bar, int lane) {
   tc::tc_fence_before();
@@ -239,35 +389,31 @@ KB_DEVI void warp_arrive(uint64_t* bar, int lane) {
   if (lane == 0) tc::mbar_arrive(bar);
 }
 
-// Which of every 8 pairs of exponentials go to the FMA pipe.
-#ifndef KB_POLY
-#define KB_POLY (D == 128 ? 0x88 : 0x88)
-#endif
+// Which of every 8 pairs of exponentials go to the FMA pipe (measured with none, 1, 2, 3 and 4 of 8;
+// 2 of 8 was fastest for D = 128: 170, 161, 156, 165 and 166 us for two pieces of prompts).
+constexpr int POLY = 0x88;
 
 template <int D, bool F16>
 __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_constant__ Maps maps, Params p) {
   using SM = Smem<D>;
-  constexpr int POLY = KB_POLY;
   constexpr int KS = SM::KS, VS = SM::VS, ATOMS = SM::ATOMS;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   SM& sm = *reinterpret_cast<SM*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int hk = blockIdx.x % p.H;
 
-  if (warp == 0) {
-    int s, t;
-    find_tile(p, blockIdx.x / p.H, lane, s, t);
+  if (warp == 8) {
     if (lane == 0) {
-      sm.seq = s;
-      sm.tile = t;
-      if (s >= 0) {
-        const int2 q = seq_range(p.cu_q, s, p.Tq), k = seq_range(p.cu_k, s, p.Tk);
-        sm.range = make_int4(q.x, q.y, k.x, k.y);
+      for (int i = 0; i < 2; ++i) {
+        tc::mbar_init(&sm.item_full[i], 1);
+        tc::mbar_init(&sm.item_free[i], 11);
+        tc::mbar_init(&sm.s_full[i], 1);
+        tc::mbar_init(&sm.s_free[i], 4);
+        tc::mbar_init(&sm.p_full[i], 4);
+        tc::mbar_init(&sm.pv_done[i], 1);
+        tc::mbar_init(&sm.drain[i], 1);
       }
-    }
-  } else if (warp == 8) {
-    if (lane == 0) {
-      tc::mbar_init(&sm.q_full, 8);
+      tc::mbar_init(&sm.q_full, 1);
+      tc::mbar_init(&sm.q_free, 1);
       for (int s = 0; s < KS; ++s) {
         tc::mbar_init(&sm.k_full[s], 1);
         tc::mbar_init(&sm.k_empty[s], 1);
@@ -276,18 +422,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
         tc::mbar_init(&sm.v_full[s], 1);
         tc::mbar_init(&sm.v_empty[s], 1);
       }
-      for (int i = 0; i < QT; ++i) {
-        tc::mbar_init(&sm.s_full[i], 1);
-        tc::mbar_init(&sm.s_free[i], 4);
-        tc::mbar_init(&sm.p_full[i], 4);
-        tc::mbar_init(&sm.pv_done[i], 1);
-      }
-      tc::mbar_init(&sm.o_done, 1);
-      tc::mbar_init(&sm.drain[0], 1);
-      tc::mbar_init(&sm.drain[1], 1);
       sm.abort_flag = 0;
       sm.keep_tmem = 0;
       tc::fence_barrier_init();
+      tc::prefetch_tmap(&maps.q);
       tc::prefetch_tmap(&maps.k);
       tc::prefetch_tmap(&maps.v);
     }
@@ -299,48 +437,90 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = sm.tmem_base;
-  const int seq = sm.seq;
-  if (seq < 0) {
-    if (warp == 9) tc::tmem_dealloc(tmem, 512);
-    return;
-  }
-  const int2 rq = make_int2(sm.range.x, sm.range.y), rk = make_int2(sm.range.z, sm.range.w);
-  const int n = rq.y - rq.x, m = rk.y - rk.x;
-  const int64_t row0 = (int64_t)sm.tile * ROWS;              // first row (token * G + head)
-  const int64_t nrows = min((int64_t)ROWS, (int64_t)n * p.G - row0);
-  // keys that token t of the sequence sees
-  auto seen_by = [&](int64_t t) { return p.causal ? (int)min((int64_t)m, max((int64_t)0, t + 1 + m - n)) : m; };
-  const int ntiles = (seen_by((row0 + nrows - 1) / p.G) + BN - 1) / BN;
-  const int full = seen_by(row0 / p.G) / BN;                 // key tiles below are seen fully by every row
-  auto aborted = [&]() { return *((volatile int*)&sm.abort_flag) != 0; };
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");   // the join, if any: it waits for this grid's end
+
+  // Item number `c` of the CTA; false: no more (or its wait gave up).
+  auto get_item = [&](int c, Item& it, bool& ok) {
+    ok = __all_sync(0xffffffffu, tc::mbar_wait(&sm.item_full[c & 1], (c >> 1) & 1));
+    if (!ok) {
+      sm.abort_flag = 1;
+      return false;
+    }
+    it = sm.item[c & 1];
+    __syncwarp();
+    if (lane == 0) tc::mbar_arrive(&sm.item_free[c & 1]);
+    return it.slot != -2;
+  };
 
   if (warp >= 8) {
     tc::setmaxnreg_dec<REGS_OTHERS>();
-  if (warp == 8) {
-    // ------------------------------------------------------------ TMA producer
-    if (lane == 0 && ntiles > 0) {
-      int kiss = 0, viss = 0;
-      for (int j = 0; j < ntiles; ++j) {
-        const int sk = j % KS, sv = j % VS, tok = rk.x + j * BN;
-        if (j >= KS && !tc::mbar_wait(&sm.k_empty[sk], (j / KS - 1) & 1)) { sm.abort_flag = 1; break; }
-        tc::mbar_expect_tx(&sm.k_full[sk], ATOMS * BN * 128);
-        for (int a = 0; a < ATOMS; ++a) tc::tma_load_3d(sm.k[sk][a], &maps.k, &sm.k_full[sk], a * 64, hk, tok);
-        ++kiss;
-        if (j >= VS && !tc::mbar_wait(&sm.v_empty[sv], (j / VS - 1) & 1)) { sm.abort_flag = 1; break; }
-        tc::mbar_expect_tx(&sm.v_full[sv], ATOMS * BN * 128);
-        for (int a = 0; a < ATOMS; ++a) tc::tma_load_3d(sm.v[sv][a], &maps.v, &sm.v_full[sv], a * 64, hk, tok);
-        ++viss;
+    Item it;
+    bool ok = true;
+    if (warp == 8) {
+      // ---------------------------------------------------------- TMA producer
+      int g = 0;                                             // key tiles so far: ring positions
+      for (int c = 0; get_item(c, it, ok); ++c) {
+        for (int j = it.j0; ok && j < it.j1; ++j, ++g) {
+          const int sk = g % KS, sv = g % VS, tok = it.k0 + j * BN;
+          if (g >= KS) ok = __all_sync(0xffffffffu, tc::mbar_wait(&sm.k_empty[sk], (g / KS - 1) & 1));
+          if (!ok) break;
+          if (lane == 0) {
+            tc::mbar_expect_tx(&sm.k_full[sk], ATOMS * BN * 128);
+            for (int a = 0; a < ATOMS; ++a) tc::tma_load_3d(sm.k[sk][a], &maps.k, &sm.k_full[sk], a * 64, it.hk / p.parts, tok);
+          }
+          if (g >= VS) ok = __all_sync(0xffffffffu, tc::mbar_wait(&sm.v_empty[sv], (g / VS - 1) & 1));
+          if (!ok) {                                         // (K of this tile is under way, V is not)
+            ok = tc::mbar_wait(&sm.k_full[sk], (g / KS) & 1) && false;
+            break;
+          }
+          if (lane == 0) {
+            tc::mbar_expect_tx(&sm.v_full[sv], ATOMS * BN * 128);
+            for (int a = 0; a < ATOMS; ++a) tc::tma_load_3d(sm.v[sv][a], &maps.v, &sm.v_full[sv], a * 64, it.hk / p.parts, tok);
+          }
+        }
+        if (!ok) break;
       }
-      // before the CTA may exit, every load it issued must have landed
+      if (!ok) sm.abort_flag = 1;
+      // before the CTA may exit, every load must have landed
       bool drained = true;
-      for (int j = kiss > KS ? kiss - KS : 0; j < kiss; ++j) drained &= tc::mbar_wait(&sm.k_full[j % KS], (j / KS) & 1);
-      for (int j = viss > VS ? viss - VS : 0; j < viss; ++j) drained &= tc::mbar_wait(&sm.v_full[j % VS], (j / VS) & 1);
+      for (int i = g > KS ? g - KS : 0; i < g; ++i) drained &= tc::mbar_wait(&sm.k_full[i % KS], (i / KS) & 1);
+      for (int i = g > VS ? g - VS : 0; i < g; ++i) drained &= tc::mbar_wait(&sm.v_full[i % VS], (i / VS) & 1);
       if (!drained) { sm.abort_flag = 1; sm.keep_tmem = 1; }
-    }
-  } else if (warp == 9 || warp == 10) {
-    // ------------------------------------------------------------ MMA issuers
-    // The whole warp runs the schedule, so every operand is warp-uniform; one elected lane issues.
-    if (ntiles > 0) {
+    } else if (warp == 11) {
+      // ---------------------------------------------------------- items, and their Q
+      Items items;
+      items.start(p, sm.table, lane);
+      int uses = 0;                                          // of the Q tile
+      for (int c = 0; ok; ++c) {
+        it = items.next(p, sm.table, lane);
+        if (c >= 2) ok = __all_sync(0xffffffffu, tc::mbar_wait(&sm.item_free[c & 1], ((c >> 1) - 1) & 1));
+        if (!ok) break;
+        if (lane == 0) {
+          sm.item[c & 1] = it;
+          tc::mbar_arrive(&sm.item_full[c & 1]);
+        }
+        __syncwarp();
+        if (it.slot == -2) break;
+        if (it.j1 <= it.j0) continue;
+        if (uses > 0) ok = __all_sync(0xffffffffu, tc::mbar_wait(&sm.q_free, (uses - 1) & 1));
+        if (!ok) break;
+        ++uses;
+        if (lane == 0) {                                     // (tokens behind the sequence: rows that are not stored)
+          tc::mbar_expect_tx(&sm.q_full, QT * ATOMS * p.tq * p.G * 128);
+          for (int t = 0; t < QT; ++t)
+            for (int a = 0; a < ATOMS; ++a)
+              tc::tma_load_3d(sm.q[t][a], &maps.q, &sm.q_full, a * 64, it.hk * p.G, it.q0 + (it.tile * QT + t) * p.tq);
+        }
+        __syncwarp();
+      }
+      if (uses > 0 && !__all_sync(0xffffffffu, tc::mbar_wait(&sm.q_full, (uses - 1) & 1))) {   // Q must land before the exit
+        ok = false;
+        sm.keep_tmem = 1;
+      }
+      if (!ok) sm.abort_flag = 1;
+    } else {
+      // ---------------------------------------------------------- MMA issuers
+      // The whole warp runs the schedule, so every operand is warp-uniform; one elected lane issues.
       const bool leader = tc::elect_one();
       constexpr uint64_t ATOM = BN * 128 / 16;               // descriptor units between 64-channel atoms
       const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
@@ -349,62 +529,72 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
         tc::tc_fence_after();
         return w;
       };
-      bool ok = true;
+      int g = 0;                                             // key tiles so far
       if (warp == 9) {
-        constexpr uint32_t IDESC_QK = tc::idesc_f32acc(F16 ? 0 : 1, BM, BN, 0, 0);
+        // (bit 13 of the descriptor negates A: the sign of the scale)
+        const uint32_t idesc = tc::idesc_f32acc(F16 ? 0 : 1, BM, BN, 0, 0) | (p.flip ? 1u << 13 : 0u);
         const uint64_t dq0 = tc::sdesc_sw128_kmajor(sm.q[0][0]);
         const uint64_t dk0 = tc::sdesc_sw128_kmajor(sm.k[0][0]);
-        auto qk = [&](int t, int j) {   // S = Q_t K_j^T
-          const uint64_t dq = dq0 + (uint64_t)(t * ATOMS) * ATOM, dk = dk0 + (uint64_t)((j % KS) * ATOMS) * ATOM;
+        auto qk = [&](int t, int slot) {                     // S = Q_t K^T
+          const uint64_t dq = dq0 + (uint64_t)(t * ATOMS) * ATOM, dk = dk0 + (uint64_t)(slot * ATOMS) * ATOM;
           if (leader) {
 #pragma unroll
             for (int ks = 0; ks < D / 16; ++ks)
-              tc::mma_bf16(tmem_u + TM_S, dq + (ks >> 2) * ATOM + 2 * (ks & 3), dk + (ks >> 2) * ATOM + 2 * (ks & 3), IDESC_QK,
+              tc::mma_bf16(tmem_u + TM_S, dq + (ks >> 2) * ATOM + 2 * (ks & 3), dk + (ks >> 2) * ATOM + 2 * (ks & 3), idesc,
                            ks > 0 ? 1u : 0u);
             tc::tc_commit(&sm.s_full[t]);
-            if (t == 1) tc::tc_commit(&sm.k_empty[j % KS]);
+            if (t == 1) tc::tc_commit(&sm.k_empty[slot]);
           }
           __syncwarp();
         };
-        ok = wait(&sm.q_full, 0) && wait(&sm.k_full[0], 0);
-        if (ok) qk(0, 0);
-        for (int j = 0; ok && j < ntiles; ++j) {
-          ok = wait(&sm.s_free[0], j & 1);
-          if (!ok) break;
-          qk(1, j);
-          if (j + 1 < ntiles) {
-            ok = wait(&sm.k_full[(j + 1) % KS], ((j + 1) / KS) & 1) && wait(&sm.s_free[1], j & 1);
-            if (ok) qk(0, j + 1);
+        int uses = 0;
+        for (int c = 0; get_item(c, it, ok); ++c) {
+          if (it.j1 <= it.j0) continue;
+          ok = wait(&sm.q_full, uses & 1);
+          ++uses;
+          for (int j = it.j0; ok && j < it.j1; ++j, ++g) {
+            ok = wait(&sm.k_full[g % KS], (g / KS) & 1);
+            if (ok && g > 0) ok = wait(&sm.s_free[1], (g - 1) & 1);
+            if (!ok) break;
+            qk(0, g % KS);
+            ok = wait(&sm.s_free[0], g & 1);
+            if (ok) qk(1, g % KS);
           }
+          if (!ok) break;
+          if (leader) tc::tc_commit(&sm.q_free);
+          __syncwarp();
         }
       } else {
         constexpr uint32_t IDESC_PV = tc::idesc_f32acc(F16 ? 0 : 1, BM, D, 0, 1);
         const uint64_t dv0 = tc::sdesc_sw128_mnmajor(sm.v[0][0], BN * 128);
-        for (int j = 0; ok && j < ntiles; ++j) {
-          ok = wait(&sm.v_full[j % VS], (j / VS) & 1);
-          if (ok && (j + 1) * BN > m) {                      // the sequence ends in this tile
-            uint4* v = reinterpret_cast<uint4*>(sm.v[j % VS][0]);
-            for (int a = 0; a < ATOMS; ++a)
-              for (int i = (m - j * BN) * 8 + lane; i < BN * 8; i += 32) v[a * BN * 8 + i] = make_uint4(0, 0, 0, 0);
-            tc::fence_proxy_async_smem();
-            __syncwarp();
-          }
-          const uint64_t dv = dv0 + (uint64_t)((j % VS) * ATOMS) * ATOM;
-          for (int t = 0; ok && t < QT; ++t) {               // O_t += P_t V_j, 16 keys per instruction
-            ok = wait(&sm.p_full[t], j & 1);
-            if (ok && leader) {
-#pragma unroll
-              for (int ks = 0; ks < BN / 16; ++ks)
-                tc::mma_bf16_ts(tmem_u + TM_O + t * 128, tmem_u + TM_P + t * 64 + ks * 8, dv + ks * (16 * 128 / 16), IDESC_PV,
-                                (j > 0 || ks > 0) ? 1u : 0u);
-              tc::tc_commit(&sm.pv_done[t]);
-              if (t == 1) tc::tc_commit(&sm.v_empty[j % VS]);
+        for (int c = 0; get_item(c, it, ok); ++c) {
+          for (int j = it.j0; ok && j < it.j1; ++j, ++g) {
+            const int slot = g % VS;
+            ok = wait(&sm.v_full[slot], (g / VS) & 1);
+            if (ok && (j + 1) * BN > it.m) {                 // the sequence ends in this tile
+              uint4* v = reinterpret_cast<uint4*>(sm.v[slot][0]);
+              for (int a = 0; a < ATOMS; ++a)
+                for (int i = (it.m - j * BN) * 8 + lane; i < BN * 8; i += 32) v[a * BN * 8 + i] = make_uint4(0, 0, 0, 0);
+              tc::fence_proxy_async_smem();
+              __syncwarp();
             }
-            __syncwarp();
+            const uint64_t dv = dv0 + (uint64_t)(slot * ATOMS) * ATOM;
+            for (int t = 0; ok && t < QT; ++t) {             // O_t += P_t V_j, 16 keys per instruction
+              // (the softmax publishes an item's first P_t when it has read the O_t before)
+              ok = wait(&sm.p_full[t], g & 1);
+              if (ok && leader) {
+#pragma unroll
+                for (int ks = 0; ks < BN / 16; ++ks)
+                  tc::mma_bf16_ts(tmem_u + TM_O + t * 128, tmem_u + TM_P + t * 64 + ks * 8, dv + ks * (16 * 128 / 16), IDESC_PV,
+                                  (j > it.j0 || ks > 0) ? 1u : 0u);
+                tc::tc_commit(&sm.pv_done[t]);
+                if (t == 1) tc::tc_commit(&sm.v_empty[slot]);
+              }
+              __syncwarp();
+            }
           }
+          if (!ok) break;
         }
-        if (ok && leader) tc::tc_commit(&sm.o_done);
-        __syncwarp();
       }
       if (!ok) sm.abort_flag = 1;
       // every MMA this warp issued must complete before TMEM is freed
@@ -415,189 +605,158 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
         sm.keep_tmem = 1;
       }
     }
-  }
   } else {
     // ------------------------------------------------------------ softmax
     tc::setmaxnreg_inc<REGS_SOFTMAX>();
-    // Q into shared memory: 256 rows of D channels, 16 bytes at a time
-    const uint32_t flip = p.flip;                            // 0x80008000: a negative scale, moved into q
-    constexpr int CPR = D / 8, BATCH = 8;                    // 16-byte chunks of a row; loads in flight per thread
-    const int64_t tok0 = row0 / p.G;
-    const uint32_t rem0 = (uint32_t)(row0 - tok0 * p.G);
-    // token of row r of the tile (from tok0) and head in the group
-    auto split = [&](int r, int& dt, int& hg) {
-      const uint32_t x = rem0 + r;
-      dt = (int)((x * p.g_magic) >> 32);
-      hg = (int)(x - dt * p.G);
-    };
-    const char* qbase = reinterpret_cast<const char*>(p.q) + 2 * ((rq.x + tok0) * p.q_ts + (int64_t)hk * p.G * p.q_hs);
-    if (ntiles > 0) {
-#pragma unroll 1
-      for (int i0 = tid; i0 < ROWS * CPR; i0 += 256 * BATCH) {
-        uint4 x[BATCH];
-#pragma unroll
-        for (int z = 0; z < BATCH; ++z) {
-          const int i = i0 + z * 256, r = i / CPR, c = i % CPR;
-          x[z] = make_uint4(0, 0, 0, 0);
-          if (r < nrows) {
-            int dt, hg;
-            split(r, dt, hg);
-            x[z] = __ldg(reinterpret_cast<const uint4*>(qbase + 2 * (dt * p.q_ts + hg * p.q_hs + c * 8)));
-          }
-        }
-#pragma unroll
-        for (int z = 0; z < BATCH; ++z) {
-          const int i = i0 + z * 256, r = i / CPR, c = i % CPR, rr = r % BM;
-          x[z].x ^= flip; x[z].y ^= flip; x[z].z ^= flip; x[z].w ^= flip;
-          *reinterpret_cast<uint4*>(&sm.q[r / BM][c / 8][rr * 128 + (((c % 8) ^ (rr & 7)) << 4)]) = x[z];
-        }
-      }
-    }
-    tc::fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) tc::mbar_arrive(&sm.q_full);
-
     const int qt = warp >> 2, w4 = warp & 3;
-    const int r = qt * BM + w4 * 32 + lane;                  // this thread's row; its TMEM lane is r % 128
+    const int row = w4 * 32 + lane, r = qt * BM + row;       // this thread's row; its TMEM lane is `row`
+    const int dt = qt * p.tq + row / p.G, hg = row % p.G;    // its token in the tile and head
+    const bool in_tile = row < p.tq * p.G;
     const uint32_t lane_off = (uint32_t)(w4 * 32) << 16;
     const uint32_t tS = tmem + TM_S + lane_off, tO = tmem + TM_O + qt * 128 + lane_off, tP = tmem + TM_P + qt * 64 + lane_off;
     const float sl2 = p.scale_log2;
-    const bool live = r < nrows;
-    int my_dt, my_hg;
-    split(r, my_dt, my_hg);
-    const int lim = live ? seen_by(tok0 + my_dt) : 0x7fffffff;   // keys that the row sees
-    float mref = -INFINITY, l = 0.f;
+    int g = 0;                                               // key tiles so far
     bool ok = true;
-    for (int j = 0; j < ntiles; ++j) {
-      if (!tc::mbar_wait(&sm.s_full[qt], j & 1)) { sm.abort_flag = 1; ok = false; }
-      ok = __all_sync(0xffffffffu, ok);
+    Item it;
+    for (int c = 0; get_item(c, it, ok); ++c) {
+      const int tok = it.tile * QT * p.tq + dt;              // in the sequence
+      const bool live = in_tile && tok < it.n;
+      const int lim = live ? seen_by(p, tok, it.n, it.m) : 0x7fffffff;   // keys that the row sees
+      const int full = seen_by(p, it.tile * QT * p.tq, it.n, it.m) / BN;   // key tiles below are seen fully by every row
+      float mref = -INFINITY, l = 0.f;
+      for (int j = it.j0; j < it.j1; ++j, ++g) {
+        ok = __all_sync(0xffffffffu, tc::mbar_wait(&sm.s_full[qt], g & 1));
+        if (!ok) break;
+        tc::tc_fence_after();
+        uint32_t s[128];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tc::tmem_ld32(tS + i * 32, s + i * 32);
+        tc::tmem_wait_ld();
+        warp_arrive(&sm.s_free[qt], lane);
+        if (j >= full) {
+          const int end = lim - j * BN;
+#pragma unroll
+          for (int c0 = 0; c0 < BN; c0 += 32)
+            if (__any_sync(0xffffffffu, end < c0 + 32)) {
+#pragma unroll
+              for (int i = c0; i < c0 + 32; ++i)
+                if (i >= end) s[i] = __float_as_uint(-INFINITY);
+            }
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < BN; i += 8)
+#pragma unroll
+          for (int z = 0; z < 4; ++z)
+            mx[z] = fmaxf(mx[z], fmaxf(__uint_as_float(s[i + 2 * z]), __uint_as_float(s[i + 2 * z + 1])));
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
+        // (rows that are not stored have no say: what they hold must not change how others round)
+        const bool grow = __any_sync(0xffffffffu, live && top > mref + TAU);
+        float alpha = 1.f;
+        if (grow) {
+          const float mn = fmaxf(mref, top);
+          if (mn != -INFINITY) alpha = ex2(mref - mn);
+          mref = mn;
+          l *= alpha;
+        }
+        // (no key of the row seen yet: every score here is -inf, and so is x)
+        const float b0 = mref == -INFINITY ? 0.f : SHIFT - mref;
+        const float2 sc = make_float2(sl2, sl2), bias = make_float2(b0, b0);
+        float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t pk[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const int e0 = h * 64 + 2 * i;
+            const float2 x = ffma2(make_float2(__uint_as_float(s[e0]), __uint_as_float(s[e0 + 1])), sc, bias);
+            const float2 e = ((POLY >> (i & 7)) & 1) ? exp2_poly(x) : make_float2(ex2(x.x), ex2(x.y));
+            ls[i & 1] = fadd2(ls[i & 1], e);
+            pk[i] = kv::pack16<F16>(e.x, e.y);
+          }
+          if (h == 0) {
+            // P_t(j) overwrites P_t(j-1) and O_t may be rescaled: PV_t(j-1) must have completed
+            if (g > 0) ok = __all_sync(0xffffffffu, tc::mbar_wait(&sm.pv_done[qt], (g - 1) & 1));
+            tc::tc_fence_after();
+          }
+          if (ok) tc::tmem_st32(tP + h * 32, pk);
+        }
+        if (!ok) break;
+        l += (ls[0].x + ls[0].y) + (ls[1].x + ls[1].y);
+        if (grow && j > it.j0) {
+#pragma unroll 1
+          for (int i = 0; i < D / 32; ++i) {
+            uint32_t o[32];
+            tc::tmem_ld32(tO + i * 32, o);
+            tc::tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tc::tmem_st32(tO + i * 32, o);
+          }
+        }
+        tc::tmem_wait_st();
+        warp_arrive(&sm.p_full[qt], lane);
+      }
+      // ---- the item's end: O_t of this row
+      const bool any = it.j1 > it.j0;
+      if (ok && any) ok = __all_sync(0xffffffffu, tc::mbar_wait(&sm.pv_done[qt], (g - 1) & 1));
       if (!ok) break;
       tc::tc_fence_after();
-      uint32_t s[128];
+      if (it.slot >= 0) {                                    // a partial: O and l under this row's m
+        float* dst = p.part + ((int64_t)it.slot * ROWS + r) * D;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tc::tmem_ld32(tS + c * 32, s + c * 32);
-      tc::tmem_wait_ld();
-      warp_arrive(&sm.s_free[qt], lane);
-      if (j >= full) {
-        const int end = lim - j * BN;
-#pragma unroll
-        for (int c0 = 0; c0 < BN; c0 += 32)
-          if (__any_sync(0xffffffffu, end < c0 + 32)) {
-#pragma unroll
-            for (int c = c0; c < c0 + 32; ++c)
-              if (c >= end) s[c] = __float_as_uint(-INFINITY);
-          }
-      }
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int c = 0; c < BN; c += 8)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          mx[i] = fmaxf(mx[i], fmaxf(__uint_as_float(s[c + 2 * i]), __uint_as_float(s[c + 2 * i + 1])));
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
-      const bool grow = __any_sync(0xffffffffu, top > mref + TAU);
-      float alpha = 1.f;
-      if (grow) {
-        const float mn = fmaxf(mref, top);
-        if (mn != -INFINITY) alpha = ex2(mref - mn);
-        mref = mn;
-        l *= alpha;
-      }
-      // (no key of the row seen yet: every score here is -inf, and so is x)
-      const float b0 = mref == -INFINITY ? 0.f : SHIFT - mref;
-      const float2 sc = make_float2(sl2, sl2), bias = make_float2(b0, b0);
-      float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t pk[32];
-#pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          const int i = h * 64 + 2 * c;
-          const float2 x = ffma2(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), sc, bias);
-          const float2 e = ((POLY >> (c & 7)) & 1) ? exp2_poly(x) : make_float2(ex2(x.x), ex2(x.y));
-          ls[c & 1] = fadd2(ls[c & 1], e);
-          pk[c] = kv::pack16<F16>(e.x, e.y);
-        }
-        if (h == 0) {
-          // P_t(j) overwrites P_t(j-1) and O_t may be rescaled: PV_t(j-1) must have completed
-          if (j >= 1 && !tc::mbar_wait(&sm.pv_done[qt], (j - 1) & 1)) { sm.abort_flag = 1; ok = false; }
-          ok = __all_sync(0xffffffffu, ok);
-          tc::tc_fence_after();
-        }
-        if (ok) tc::tmem_st32(tP + h * 32, pk);
-      }
-      if (!ok) break;
-      l += (ls[0].x + ls[0].y) + (ls[1].x + ls[1].y);
-      if (grow && j >= 1) {
-#pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
+        for (int i = 0; i < D / 32; ++i) {
           uint32_t o[32];
-          tc::tmem_ld32(tO + c * 32, o);
+          tc::tmem_ld32(tO + i * 32, o);
           tc::tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-          tc::tmem_st32(tO + c * 32, o);
+          for (int z = 0; z < 32; z += 4) *reinterpret_cast<uint4*>(dst + i * 32 + z) = make_uint4(o[z], o[z + 1], o[z + 2], o[z + 3]);
+        }
+        *reinterpret_cast<float2*>(p.part + (int64_t)2 * gridDim.x * ROWS * D + ((int64_t)it.slot * ROWS + r) * 2) =
+            make_float2(mref, l);
+        continue;
+      }
+      const float f = l == 0.f ? 0.f : 1.f / l;
+      const int64_t gt = (int64_t)it.q0 + tok;
+      const int head = it.hk * p.G + hg;
+      char* orow = reinterpret_cast<char*>(p.o) + 2 * (gt * p.o_ts + head * p.o_hs);
+      bool finite = true;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        uint32_t o[32];
+        if (any) {
+          tc::tmem_ld32(tO + i * 32, o);
+          tc::tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0;
+        }
+        float worst = 0.f;                                   // NaN if some value is not finite
+#pragma unroll
+        for (int e = 0; e < 32; ++e) worst = fmaf(__uint_as_float(o[e]), 0.f, worst);
+        finite &= worst == 0.f;
+        if (live) {
+#pragma unroll
+          for (int z = 0; z < 4; ++z) {
+            uint4 x;
+            x.x = kv::pack16<F16>(__uint_as_float(o[8 * z + 0]) * f, __uint_as_float(o[8 * z + 1]) * f);
+            x.y = kv::pack16<F16>(__uint_as_float(o[8 * z + 2]) * f, __uint_as_float(o[8 * z + 3]) * f);
+            x.z = kv::pack16<F16>(__uint_as_float(o[8 * z + 4]) * f, __uint_as_float(o[8 * z + 5]) * f);
+            x.w = kv::pack16<F16>(__uint_as_float(o[8 * z + 6]) * f, __uint_as_float(o[8 * z + 7]) * f);
+            *reinterpret_cast<uint4*>(orow + 2 * (i * 32 + z * 8)) = x;
+          }
         }
       }
-      tc::tmem_wait_st();
-      warp_arrive(&sm.p_full[qt], lane);
+      if (p.lse && live) p.lse[gt * p.Hq + head] = l == 0.f ? -INFINITY : (mref - SHIFT + log2f(l)) * 0.6931471805599453f;
+      uint32_t again = __ballot_sync(0xffffffffu, live && !finite);
+      while (again) {
+        const int i = __ffs(again) - 1;
+        again &= again - 1;
+        const int ti = __shfl_sync(0xffffffffu, tok, i), hi = __shfl_sync(0xffffffffu, head, i);
+        attend_row<D, F16>(p, it.q0 + ti, hi, it.k0, seen_by(p, ti, it.n, it.m), lane);
+      }
     }
-    // ---- epilogue
-    if (ok && ntiles > 0) ok = __all_sync(0xffffffffu, tc::mbar_wait(&sm.o_done, 0));
     if (!ok) sm.abort_flag = 1;
-    tc::tc_fence_after();
-    const float f = !ok || aborted() ? NAN : l == 0.f ? 0.f : 1.f / l;
-    // through this warp's part of the Q tile (every product has read Q), so that rows are stored whole
-    uint8_t* stage = sm.q[qt][0] + w4 * 32 * (D * 2);
-    bool finite = true;
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c) {
-      uint32_t o[32];
-      if (ntiles > 0 && ok) {
-        tc::tmem_ld32(tO + c * 32, o);
-        tc::tmem_wait_ld();
-      } else {
-#pragma unroll
-        for (int e = 0; e < 32; ++e) o[e] = 0;
-      }
-      float worst = 0.f;                                     // NaN if some value is not finite: inf - inf
-#pragma unroll
-      for (int e = 0; e < 32; ++e) worst = fmaf(__uint_as_float(o[e]), 0.f, worst);
-      finite &= worst == 0.f;
-#pragma unroll
-      for (int z = 0; z < 4; ++z) {
-        uint4 x;
-        x.x = kv::pack16<F16>(__uint_as_float(o[8 * z + 0]) * f, __uint_as_float(o[8 * z + 1]) * f);
-        x.y = kv::pack16<F16>(__uint_as_float(o[8 * z + 2]) * f, __uint_as_float(o[8 * z + 3]) * f);
-        x.z = kv::pack16<F16>(__uint_as_float(o[8 * z + 4]) * f, __uint_as_float(o[8 * z + 5]) * f);
-        x.w = kv::pack16<F16>(__uint_as_float(o[8 * z + 6]) * f, __uint_as_float(o[8 * z + 7]) * f);
-        *reinterpret_cast<uint4*>(stage + lane * (D * 2) + (((c * 4 + z) ^ (lane & 7)) << 4)) = x;
-      }
-    }
-    __syncwarp();
-    char* obase = reinterpret_cast<char*>(p.o) + 2 * ((rq.x + tok0) * p.o_ts + (int64_t)hk * p.G * p.o_hs);
-#pragma unroll 8
-    for (int z = 0; z < CPR; ++z) {                          // 32 / CPR rows at a time
-      const int i = z * 32 + lane, rr = i / CPR, ch = i % CPR, ri = qt * BM + w4 * 32 + rr;
-      const uint4 x = *reinterpret_cast<const uint4*>(stage + rr * (D * 2) + ((ch ^ (rr & 7)) << 4));
-      if (ri < nrows) {
-        int dt, hg;
-        split(ri, dt, hg);
-        *reinterpret_cast<uint4*>(obase + 2 * (dt * p.o_ts + hg * p.o_hs + ch * 8)) = x;
-      }
-    }
-    if (p.lse && live)
-      p.lse[(rq.x + tok0 + my_dt) * p.Hq + hk * p.G + my_hg] =
-          l == 0.f ? -INFINITY : (mref - SHIFT + log2f(l)) * 0.6931471805599453f;
-    uint32_t again = __ballot_sync(0xffffffffu, live && ok && !finite);
-    __syncwarp();
-    while (again) {
-      const int i = __ffs(again) - 1;
-      again &= again - 1;
-      int dt, hg;
-      split(qt * BM + w4 * 32 + i, dt, hg);
-      attend_row<D, F16>(p, rq.x + tok0 + dt, hk * p.G + hg, rk.x, seen_by(tok0 + dt), lane);
-    }
   }
   tc::tc_fence_before();
   __syncthreads();
@@ -605,35 +764,167 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
     tc::tc_fence_after();
     tc::tmem_dealloc(tmem, 512);
   }
+  if (sm.abort_flag && warp == 0) {                          // a wait gave up: no result is better than a wrong one
+    Items items;
+    items.start(p, sm.table, lane);
+    for (Item it = items.next(p, sm.table, lane); it.slot != -2; it = items.next(p, sm.table, lane)) {
+      for (int i = lane; i < ROWS; i += 32) {
+        const int row = i % BM, tok = (it.tile * QT + i / BM) * p.tq + row / p.G;
+        if (it.slot >= 0) {
+          p.part[(int64_t)2 * gridDim.x * ROWS * D + ((int64_t)it.slot * ROWS + i) * 2 + 1] = NAN;
+        } else if (row < p.tq * p.G && tok < it.n) {
+          for (int d = 0; d < D; ++d)
+            store16<F16>(p.o, (it.q0 + tok) * p.o_ts + (it.hk * p.G + row % p.G) * p.o_hs + d, NAN);
+        }
+      }
+    }
+  }
 }
 
-// [T, H, D] 16-bit with the given strides (elements): boxes of 64 channels x 1 head x 128 tokens.
-static int make_map(CUtensorMap* m, const void* base, const Params& p, int D, int64_t ts, int64_t hs, int f16) {
+// Joins the partials of the items that cross shares.  A block per item and 32 rows, a warp per row.
+template <int D, bool F16>
+__global__ void __launch_bounds__(256) attn_prompt_join_kernel(Params p, int ctas) {
+  __shared__ Table tb;
+  __shared__ int count;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp == 0) {
+    const int n = build_table(p, tb, lane);
+    if (lane == 0) count = n;
+  }
+  __syncthreads();
+  const int f = blockIdx.x / p.H, hk = blockIdx.x % p.H;
+  // (every block waits, those without work too: this grid must not end before the one it follows)
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  if (f >= count) return;
+  const int flat = tb.before[count], all = tb.before[f + 1] - tb.before[f] - PAD;
+  if (all == 0) return;
+  const int64_t per = share_size(p, flat, ctas), begin = (int64_t)hk * flat + tb.before[f];
+  const int c0 = (int)(begin / per), c1 = (int)((begin + all - 1) / per);
+  if (c0 == c1) return;                                      // finished there
+  const int seq = tb.seq[f], tile = tb.tile[f];
+  const int2 q = seq_range(p.cu_q, seq, p.Tq), k = seq_range(p.cu_k, seq, p.Tk);
+  const int n = q.y - q.x, m = k.y - k.x;
+  constexpr int V = D / 32;                                  // channels of a lane
+  const float* mlp = p.part + (int64_t)2 * ctas * ROWS * D;
+  for (int r = blockIdx.y * 32 + warp; r < blockIdx.y * 32 + 32; r += 8) {
+    const int row = r % BM, tok = (tile * QT + r / BM) * p.tq + row / p.G, head = hk * p.G + row % p.G;
+    if (row >= p.tq * p.G || tok >= n) continue;
+    float mx = -INFINITY, l = 0.f, acc[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) acc[v] = 0.f;
+    for (int c = c0; c <= c1; ++c) {
+      const int64_t row = (2 * (int64_t)c + (c == c0 ? 1 : 0)) * ROWS + r;
+      const float2 ml = __ldcg(reinterpret_cast<const float2*>(mlp + row * 2));
+      float x[V];
+      if constexpr (V == 4) {
+        const float4 y = __ldcg(reinterpret_cast<const float4*>(p.part + row * D) + lane);
+        x[0] = y.x; x[1] = y.y; x[2] = y.z; x[3] = y.w;
+      } else {
+        const float2 y = __ldcg(reinterpret_cast<const float2*>(p.part + row * D) + lane);
+        x[0] = y.x; x[1] = y.y;
+      }
+      // (m = -inf: no visible key, O and l are 0, or all of its scores are NaN, and so are they)
+      const float mn = fmaxf(mx, ml.x), f0 = mx == -INFINITY ? 1.f : ex2(mx - mn), f1 = ml.x == -INFINITY ? 1.f : ex2(ml.x - mn);
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc[v] = acc[v] * f0 + x[v] * f1;
+      l = l * f0 + ml.y * f1;
+      mx = mn;
+    }
+    const int64_t gt = (int64_t)q.x + tok;
+    float worst = 0.f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) worst = fmaf(acc[v], 0.f, worst);
+    if (__any_sync(0xffffffffu, worst != 0.f)) {             // not finite: over the visible keys alone
+      attend_row<D, F16>(p, gt, head, k.x, seen_by(p, tok, n, m), lane);
+      continue;
+    }
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+    char* orow = reinterpret_cast<char*>(p.o) + 2 * (gt * p.o_ts + head * p.o_hs + lane * V);
+    if constexpr (V == 4)
+      *reinterpret_cast<uint2*>(orow) = make_uint2(kv::pack16<F16>(acc[0] * inv, acc[1] * inv), kv::pack16<F16>(acc[2] * inv, acc[3] * inv));
+    else
+      *reinterpret_cast<uint32_t*>(orow) = kv::pack16<F16>(acc[0] * inv, acc[1] * inv);
+    if (lane == 0 && p.lse) p.lse[gt * p.Hq + head] = l == 0.f ? -INFINITY : (mx - SHIFT + log2f(l)) * 0.6931471805599453f;
+  }
+}
+
+// [T, H, D] 16-bit with the given strides (elements): boxes of 64 channels x `heads` x `tokens`.
+static int make_map(CUtensorMap* m, const void* base, int64_t T, int64_t H, int D, int64_t ts, int64_t hs, int heads, int tokens,
+                    int f16) {
   tc::EncodeTiledFn fn = tc::encode_tiled_fn();
   if (!fn) return set_error(KB200_ERR_LAUNCH, "attn_prompt: cuTensorMapEncodeTiled unavailable");
-  cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)p.H, (cuuint64_t)p.Tk};
+  cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)H, (cuuint64_t)T};
   cuuint64_t strides[2] = {(cuuint64_t)hs * 2, (cuuint64_t)ts * 2};
-  cuuint32_t box[3] = {64, 1, BN};
+  cuuint32_t box[3] = {64, (cuuint32_t)heads, (cuuint32_t)tokens};
   cuuint32_t estr[3] = {1, 1, 1};
   const CUresult r = fn(m, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base),
                         dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return set_error(KB200_ERR_INVALID, "attn_prompt: k or v cannot be read by TMA (%d)", (int)r);
+  if (r != CUDA_SUCCESS) return set_error(KB200_ERR_INVALID, "attn_prompt: q, k or v cannot be read by TMA (%d)", (int)r);
   return KB200_OK;
 }
 
+// How the G query heads of a kv head are taken: in `parts` equal parts of `g` <= 128 heads, `tq`
+// tokens to a query tile.
+struct Split {
+  int64_t parts, g, tq;
+};
+static Split split_heads(int64_t G) {
+  Split s{1, G, 0};
+  while (s.g > BM || G % s.parts) {
+    ++s.parts;
+    s.g = G / s.parts;
+  }
+  s.tq = BM / s.g;
+  return s;
+}
+
+// Row tiles that the sequences have at most.
+static int64_t most_tiles(int64_t Tq, int64_t N, int64_t tq) { return Tq / (QT * tq) + N; }
+
+// Whether the key tiles are shared out: when whole items would leave SMs idle (up to 3 items for 2
+// SMs; beyond that the sorted order balances) and there are enough keys for the partials and the
+// second kernel to pay.  512 + 300 queries over 12345 + 8000 keys, 32/8 heads, 104 items: SPLIT_US
+static bool shares(int64_t Tq, int64_t Tk, int64_t N, int64_t H, const Split& s, int sms) {
+  const int64_t tiles = most_tiles(Tq, N, s.tq);
+  return tiles <= TABLE && 2 * tiles * H * s.parts <= 3 * sms && Tk >= 2048;
+}
+
 template <int D, bool F16>
-static int launch(const Maps& maps, const Params& p, cudaStream_t st) {
+static int launch(const Maps& maps, const Params& p, int sms, cudaStream_t st) {
   const size_t smem = sizeof(Smem<D>) + 1024;
   static std::atomic<uint64_t> done{0};
   if (int e = allow_smem((const void*)attn_prompt_kernel<D, F16>, smem, done)) return e;
-  const int64_t tiles = p.Tq * p.G / ROWS + p.N;             // no fewer than the sequences have
-  attn_prompt_kernel<D, F16><<<(unsigned)(tiles * p.H), THREADS, smem, st>>>(maps, p);
-  return check_launch("attn_prompt_kernel");
+  const int64_t items = most_tiles(p.Tq, p.N, p.tq) * p.H;
+  const int grid = p.split || items > sms ? sms : (int)items;
+  attn_prompt_kernel<D, F16><<<grid, THREADS, smem, st>>>(maps, p);
+  if (int e = check_launch("attn_prompt_kernel")) return e;
+  if (!p.split) return KB200_OK;
+  cudaLaunchAttribute overlap{};
+  overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  overlap.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)items, ROWS / 32);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cfg.attrs = &overlap;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, attn_prompt_join_kernel<D, F16>, p, grid);
+  return check_launch("attn_prompt_join_kernel");
 }
 
 }  // namespace prompt
 }  // namespace kb
+
+extern "C" size_t kb200_attn_prompt_workspace_size(int64_t Tq, int64_t Tk, int64_t N, int64_t Hq, int64_t Hkv, int64_t D) {
+  using namespace kb;
+  if (Tq <= 0 || Tk < 0 || N <= 0 || Hq < 1 || Hkv < 1 || Hq % Hkv || Hq > (1 << 14) || N > (1 << 20) || Tq > 0x7fffff00LL ||
+      (D != 64 && D != 128))
+    return 0;
+  const int sms = sm_count();
+  if (!prompt::shares(Tq, Tk, N, Hkv, prompt::split_heads(Hq / Hkv), sms)) return 0;
+  return (size_t)2 * sms * prompt::ROWS * (D + 2) * sizeof(float);
+}
 
 extern "C" int kb200_attn_prompt_fwd(const KB200PromptArgs* a, void* stream) {
   using namespace kb;
@@ -650,21 +941,33 @@ extern "C" int kb200_attn_prompt_fwd(const KB200PromptArgs* a, void* stream) {
       ((a->q_token_stride | a->q_head_stride | a->k_token_stride | a->k_head_stride | a->v_token_stride | a->v_head_stride |
         a->o_token_stride | a->o_head_stride) & 7))
     return set_error(KB200_ERR_ALIGN, "attn_prompt: q, k, v and o rows must be 16-byte aligned");
-  const int64_t G = a->Hq / a->Hkv;
-  if ((a->Tq * G / prompt::ROWS + a->N) * a->Hkv > 0x7fffffffLL) return set_error(KB200_ERR_INVALID, "attn_prompt: too many rows");
+  const prompt::Split sp = prompt::split_heads(a->Hq / a->Hkv);
+  if (prompt::most_tiles(a->Tq, a->N, sp.tq) * a->Hkv * sp.parts > 0x7fffffffLL)
+    return set_error(KB200_ERR_INVALID, "attn_prompt: too many rows");
   // a scale of 0 becomes one too small to matter, so that a masked score stays -inf
   const float sl2 = fmaxf(fabsf(a->softmax_scale) * 1.4426950408889634f, 1e-30f);
+  const int sms = sm_count();
+  const bool split = a->workspace && a->workspace_bytes > 0 && prompt::shares(a->Tq, a->Tk, a->N, a->Hkv, sp, sms);
+  if (split && (a->workspace_bytes < kb200_attn_prompt_workspace_size(a->Tq, a->Tk, a->N, a->Hq, a->Hkv, a->D) ||
+                !aligned16(a->workspace)))
+    return set_error(KB200_ERR_WORKSPACE, "attn_prompt: workspace of %zu bytes given, %zu needed (or none)", a->workspace_bytes,
+                     kb200_attn_prompt_workspace_size(a->Tq, a->Tk, a->N, a->Hq, a->Hkv, a->D));
   prompt::Params p{a->q, a->k, a->v, a->o, a->lse, a->cu_q, a->cu_k, a->q_token_stride, a->q_head_stride,
                    a->k_token_stride, a->k_head_stride, a->v_token_stride, a->v_head_stride, a->o_token_stride,
-                   a->o_head_stride, a->Tq, a->Tk, (int)a->N, (int)a->Hq, (int)a->Hkv, (int)G,
-                   sl2, a->softmax_scale < 0.f ? 0x80008000u : 0u, ((1ull << 32) + G - 1) / G, a->causal};
+                   a->o_head_stride, a->Tq, a->Tk, (int)a->N, (int)a->Hq, (int)(a->Hkv * sp.parts), (int)sp.g,
+                   (int)sp.parts, (int)sp.tq, sl2, a->softmax_scale < 0.f ? 0x80008000u : 0u, split, (float*)a->workspace,
+                   a->causal};
   prompt::Maps maps;
   memset(&maps, 0, sizeof(maps));
+  const int D = (int)a->D;
+  if (int e = prompt::make_map(&maps.q, a->q, a->Tq, a->Hq, D, a->q_token_stride, a->q_head_stride, p.G, p.tq, a->dtype)) return e;
   if (a->Tk > 0) {                                           // (without keys nothing is loaded)
-    if (int e = prompt::make_map(&maps.k, a->k, p, (int)a->D, a->k_token_stride, a->k_head_stride, a->dtype)) return e;
-    if (int e = prompt::make_map(&maps.v, a->v, p, (int)a->D, a->v_token_stride, a->v_head_stride, a->dtype)) return e;
+    if (int e = prompt::make_map(&maps.k, a->k, a->Tk, a->Hkv, D, a->k_token_stride, a->k_head_stride, 1, prompt::BN, a->dtype))
+      return e;
+    if (int e = prompt::make_map(&maps.v, a->v, a->Tk, a->Hkv, D, a->v_token_stride, a->v_head_stride, 1, prompt::BN, a->dtype))
+      return e;
   }
   cudaStream_t st = (cudaStream_t)stream;
-  if (a->D == 64) return a->dtype ? prompt::launch<64, true>(maps, p, st) : prompt::launch<64, false>(maps, p, st);
-  return a->dtype ? prompt::launch<128, true>(maps, p, st) : prompt::launch<128, false>(maps, p, st);
+  if (a->D == 64) return a->dtype ? prompt::launch<64, true>(maps, p, sms, st) : prompt::launch<64, false>(maps, p, sms, st);
+  return a->dtype ? prompt::launch<128, true>(maps, p, sms, st) : prompt::launch<128, false>(maps, p, sms, st);
 }

@@ -28,6 +28,16 @@ int allow_smem(const void* kernel, size_t bytes, std::atomic<uint64_t>& done) {
   return KB200_OK;
 }
 
+int sm_count() {
+  static int counts[64];             // per device; written with the same value by every thread that gets there
+  int dev = 0, n = 148;
+  if (cudaGetDevice(&dev) != cudaSuccess) { cudaGetLastError(); return n; }
+  if (dev < 64 && counts[dev]) return counts[dev];
+  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  if (dev < 64) counts[dev] = n;
+  return n;
+}
+
 int check_launch(const char* what) {
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess)

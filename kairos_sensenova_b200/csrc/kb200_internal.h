@@ -14,6 +14,8 @@ inline size_t align_up(size_t x, size_t a = 256) { return (x + a - 1) / a * a; }
 // Lets `kernel` use `bytes` of dynamic shared memory on the current device.  `done` is the
 // kernel's own mask of the devices where that is set already (setting it twice does no harm).
 int allow_smem(const void* kernel, size_t bytes, std::atomic<uint64_t>& done);
+// SMs of the current device (148 without one).
+int sm_count();
 // Checks the result of the launches just issued.
 int check_launch(const char* what);
 }  // namespace kb
