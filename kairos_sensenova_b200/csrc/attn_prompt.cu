@@ -15,8 +15,9 @@
 //
 // Items.  The kernel is persistent, a CTA per SM.  An item is a tile of rows with the key tiles
 // that it sees; K, V and the next item's Q are on their way while one is computed.
-//   * Many items: sorted by their number of keys, most first, CTA c takes them in turns (c, then
-//     2 S - 1 - c, 2 S + c, ... of S CTAs), so that every CTA gets long and short ones.
+//   * Many items: sorted by their number of keys, most first, one launched CTA for each.  A
+//     CTA that runs takes over the next CTA that has not started (cluster launch control), so
+//     the items go to the SMs as they become free, without a counter in memory.
 //   * Few items for the SMs and many keys: the key tiles of all items are laid end to end and
 //     every CTA takes an equal share, as in attn_cached.cu; an item that crosses shares leaves
 //     fp32 partials (m, l, O), joined in share order by a second kernel.
@@ -183,13 +184,16 @@ struct Smem {
   uint8_t q[QT][ATOMS][BM * 128];
   uint8_t k[KS][ATOMS][BN * 128];
   uint8_t v[VS][ATOMS][BN * 128];
-  uint64_t item_full[2], item_free[2];       // an item is published / every warp has read it
+  uint64_t item_full, item_free;             // an item is published / every warp has read it
+  uint64_t answered;
   uint64_t q_full, q_free;
   uint64_t k_full[KS], k_empty[KS], v_full[VS], v_empty[VS];
   uint64_t s_full[QT], s_free[QT], p_full[QT], pv_done[QT], drain[2];
-  Item item[2];
+  alignas(16) uint4 answer[2];
+  Item item;
   Table table;
   uint32_t tmem_base;
+  int took[3];                               // whole items: the last ones this CTA took
   int abort_flag, keep_tmem;
 };
 
@@ -319,12 +323,27 @@ KB_DEVI int64_t share_size(const Params& p, int flat, int ctas) {
   return max((int64_t)LEAST, ((int64_t)flat * p.H + ctas - 1) / ctas);
 }
 
+// The next CTA of the grid that has not started will not start, and this one does its work: asks
+// for it (the answer, 16 bytes, is counted on `bar`), and reads the answer (-1: there is none).
+KB_DEVI void take_over_ask(uint4* answer, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];\n"
+               ::"r"(smem_u32(answer)), "r"(smem_u32(bar)) : "memory");
+}
+KB_DEVI int take_over_answer(const uint4* answer) {
+  int block;
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b128 h;\n ld.shared.b128 h, [%1];\n"
+      " clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n mov.b32 %0, -1;\n"
+      " @p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%0, _, _, _}, h;\n}\n"
+      : "=r"(block) : "r"(smem_u32(answer)) : "memory");
+  return block;
+}
+
 // The items of a CTA, one after the other; by one warp, every lane has them.
 struct Items {
-  int64_t turn, left;
+  int64_t left;
   int tiles, flat, hk, f, x;                 // shares: row tiles, their flat length; the next position
   KB_DEVI void start(const Params& p, Table& tb, int lane) {
-    turn = 0;
     left = 0;
     if (!p.split) return;
     tiles = build_table(p, tb, lane);
@@ -339,16 +358,16 @@ struct Items {
     while (tb.before[f + 1] <= rem) ++f;
     x = rem - tb.before[f];
   }
-  KB_DEVI Item next(const Params& p, const Table& tb, int lane) {
+  // `block`: whole items, the one to take (-1: none).
+  KB_DEVI Item next(const Params& p, const Table& tb, int block, int lane) {
     Item it{};
     it.slot = -2;
     int seq, tile;
     if (!p.split) {
-      const int64_t S = gridDim.x, r = turn * S + ((turn & 1) ? S - 1 - blockIdx.x : blockIdx.x);
-      ++turn;
-      find_tile(p, r / p.H, lane, seq, tile);
+      if (block < 0) return it;
+      find_tile(p, block / p.H, lane, seq, tile);
       if (seq < 0) return it;
-      it.hk = (int)(r % p.H);
+      it.hk = block % p.H;
     } else {
       int take, span;
       do {
@@ -404,14 +423,15 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
   if (warp == 8) {
     if (lane == 0) {
       for (int i = 0; i < 2; ++i) {
-        tc::mbar_init(&sm.item_full[i], 1);
-        tc::mbar_init(&sm.item_free[i], 11);
         tc::mbar_init(&sm.s_full[i], 1);
         tc::mbar_init(&sm.s_free[i], 4);
         tc::mbar_init(&sm.p_full[i], 4);
         tc::mbar_init(&sm.pv_done[i], 1);
         tc::mbar_init(&sm.drain[i], 1);
       }
+      tc::mbar_init(&sm.item_full, 1);
+      tc::mbar_init(&sm.item_free, 11);
+      tc::mbar_init(&sm.answered, 1);
       tc::mbar_init(&sm.q_full, 1);
       tc::mbar_init(&sm.q_free, 1);
       for (int s = 0; s < KS; ++s) {
@@ -422,6 +442,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
         tc::mbar_init(&sm.v_full[s], 1);
         tc::mbar_init(&sm.v_empty[s], 1);
       }
+      sm.took[0] = sm.took[1] = sm.took[2] = -1;
       sm.abort_flag = 0;
       sm.keep_tmem = 0;
       tc::fence_barrier_init();
@@ -441,14 +462,14 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
 
   // Item number `c` of the CTA; false: no more (or its wait gave up).
   auto get_item = [&](int c, Item& it, bool& ok) {
-    ok = __all_sync(0xffffffffu, tc::mbar_wait(&sm.item_full[c & 1], (c >> 1) & 1));
+    ok = __all_sync(0xffffffffu, tc::mbar_wait(&sm.item_full, c & 1));
     if (!ok) {
       sm.abort_flag = 1;
       return false;
     }
-    it = sm.item[c & 1];
+    it = sm.item;
     __syncwarp();
-    if (lane == 0) tc::mbar_arrive(&sm.item_free[c & 1]);
+    if (lane == 0) tc::mbar_arrive(&sm.item_free);
     return it.slot != -2;
   };
 
@@ -490,14 +511,30 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
       // ---------------------------------------------------------- items, and their Q
       Items items;
       items.start(p, sm.table, lane);
-      int uses = 0;                                          // of the Q tile
+      int uses = 0, block = blockIdx.x;                      // of the Q tile; the CTA whose item is next
       for (int c = 0; ok; ++c) {
-        it = items.next(p, sm.table, lane);
-        if (c >= 2) ok = __all_sync(0xffffffffu, tc::mbar_wait(&sm.item_free[c & 1], ((c >> 1) - 1) & 1));
+        // (the next item is taken when every warp has this one: not earlier than it is needed)
+        if (c > 0) ok = __all_sync(0xffffffffu, tc::mbar_wait(&sm.item_free, (c - 1) & 1));
         if (!ok) break;
+        if (c > 0 && !p.split) {
+          if (lane == 0) {
+            tc::fence_proxy_async_smem();
+            tc::mbar_expect_tx(&sm.answered, 16);
+            take_over_ask(&sm.answer[c & 1], &sm.answered);
+          }
+          __syncwarp();
+          ok = __all_sync(0xffffffffu, tc::mbar_wait(&sm.answered, (c - 1) & 1));
+          if (!ok) {
+            sm.keep_tmem = 1;
+            break;
+          }
+          block = take_over_answer(&sm.answer[c & 1]);
+        }
+        it = items.next(p, sm.table, block, lane);
         if (lane == 0) {
-          sm.item[c & 1] = it;
-          tc::mbar_arrive(&sm.item_full[c & 1]);
+          sm.took[c % 3] = block;
+          sm.item = it;
+          tc::mbar_arrive(&sm.item_full);
         }
         __syncwarp();
         if (it.slot == -2) break;
@@ -767,7 +804,13 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
   if (sm.abort_flag && warp == 0) {                          // a wait gave up: no result is better than a wrong one
     Items items;
     items.start(p, sm.table, lane);
-    for (Item it = items.next(p, sm.table, lane); it.slot != -2; it = items.next(p, sm.table, lane)) {
+    // all of its shares, or the whole items that it may not have finished: the last three it took
+    for (int c = 0; p.split || c < 3; ++c) {
+      const Item it = items.next(p, sm.table, p.split ? 0 : sm.took[c], lane);
+      if (it.slot == -2) {
+        if (p.split) break;
+        continue;
+      }
       for (int i = lane; i < ROWS; i += 32) {
         const int row = i % BM, tok = (it.tile * QT + i / BM) * p.tq + row / p.G;
         if (it.slot >= 0) {
@@ -896,7 +939,7 @@ static int launch(const Maps& maps, const Params& p, int sms, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
   if (int e = allow_smem((const void*)attn_prompt_kernel<D, F16>, smem, done)) return e;
   const int64_t items = most_tiles(p.Tq, p.N, p.tq) * p.H;
-  const int grid = p.split || items > sms ? sms : (int)items;
+  const int grid = p.split ? sms : (int)items;
   attn_prompt_kernel<D, F16><<<grid, THREADS, smem, st>>>(maps, p);
   if (int e = check_launch("attn_prompt_kernel")) return e;
   if (!p.split) return KB200_OK;
