@@ -40,9 +40,10 @@
 //
 // Keys that a row does not see score -inf, so their P is 0.  V rows behind the sequence are
 // zeroed in shared memory before the product.  A NaN or an infinity in V at a key that a
-// row must not see still reaches it as 0 * NaN: so a row whose O is not finite is computed again,
-// by its warp, over its visible keys alone (and if one of those is the cause, the result is
-// what it should be).
+// row must not see still reaches it as 0 * NaN: so for a row whose O is not finite (and whose l
+// is: a NaN among its own scores makes all of it NaN) the keys that its last tiles hide from it
+// are looked at, and if V is not finite there the row is computed again, by its warp, over its
+// visible keys alone.
 //
 // Every wait is bounded.  A warp whose wait gives up stops, so that the others' waits give up
 // too; what is in flight is drained, and the CTA writes NaN into all of its rows.
@@ -111,6 +112,16 @@ KB_DEVI void store16(void* base, int64_t i, float x) {
   else reinterpret_cast<__nv_bfloat16*>(base)[i] = __float2bfloat16_rn(x);
 }
 
+// Whether V of kv head `hk` is not finite somewhere at the keys [from, to), by one warp.
+template <int D, bool F16>
+KB_DEVI bool not_finite_v(const Params& p, int hk, int64_t from, int64_t to, int lane) {
+  float worst = 0.f;
+  for (int64_t j = from; j < to; ++j)
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) worst = fmaf(load16<F16>(p.v, j * p.v_ts + hk * p.v_hs + c * 32 + lane), 0.f, worst);
+  return __any_sync(0xffffffffu, worst != 0.f);
+}
+
 // Query token `tq` of head `h`, which sees the keys [k0, k0 + seen), by one warp.
 template <int D, bool F16>
 KB_DEVI void attend_row(const Params& p, int64_t tq, int h, int64_t k0, int64_t seen, int lane) {
@@ -140,6 +151,10 @@ KB_DEVI void attend_row(const Params& p, int64_t tq, int h, int64_t k0, int64_t 
     l += e;
 #pragma unroll
     for (int c = 0; c < C; ++c) acc[c] = fmaf(e, load16<F16>(p.v, (k0 + j) * p.v_ts + hk * p.v_hs + c * 32 + lane), acc[c]);
+    bool settled = true;                                     // NaN in every channel stays so
+#pragma unroll
+    for (int c = 0; c < C; ++c) settled &= acc[c] != acc[c];
+    if (__all_sync(0xffffffffu, settled)) break;
   }
   const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
 #pragma unroll
@@ -785,12 +800,14 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
         }
       }
       if (p.lse && live) p.lse[gt * p.Hq + head] = l == 0.f ? -INFINITY : (mref - SHIFT + log2f(l)) * 0.6931471805599453f;
-      uint32_t again = __ballot_sync(0xffffffffu, live && !finite);
+      uint32_t again = __ballot_sync(0xffffffffu, live && !finite && l == l);
       while (again) {
         const int i = __ffs(again) - 1;
         again &= again - 1;
         const int ti = __shfl_sync(0xffffffffu, tok, i), hi = __shfl_sync(0xffffffffu, head, i);
-        attend_row<D, F16>(p, it.q0 + ti, hi, it.k0, seen_by(p, ti, it.n, it.m), lane);
+        const int seen = seen_by(p, ti, it.n, it.m);
+        if (not_finite_v<D, F16>(p, it.hk / p.parts, (int64_t)it.k0 + seen, (int64_t)it.k0 + min(it.m, it.j1 * BN), lane))
+          attend_row<D, F16>(p, it.q0 + ti, hi, it.k0, seen, lane);
       }
     }
     if (!ok) sm.abort_flag = 1;
@@ -877,8 +894,10 @@ __global__ void __launch_bounds__(256) attn_prompt_join_kernel(Params p, int cta
     float worst = 0.f;
 #pragma unroll
     for (int v = 0; v < V; ++v) worst = fmaf(acc[v], 0.f, worst);
-    if (__any_sync(0xffffffffu, worst != 0.f)) {             // not finite: over the visible keys alone
-      attend_row<D, F16>(p, gt, head, k.x, seen_by(p, tok, n, m), lane);
+    const int seen = seen_by(p, tok, n, m);
+    if (__any_sync(0xffffffffu, worst != 0.f) && l == l &&
+        not_finite_v<D, F16>(p, hk / p.parts, (int64_t)k.x + seen, (int64_t)k.x + min(m, all * BN), lane)) {
+      attend_row<D, F16>(p, gt, head, k.x, seen, lane);
       continue;
     }
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
@@ -1004,6 +1023,7 @@ extern "C" int kb200_attn_prompt_fwd(const KB200PromptArgs* a, void* stream) {
   memset(&maps, 0, sizeof(maps));
   const int D = (int)a->D;
   if (int e = prompt::make_map(&maps.q, a->q, a->Tq, a->Hq, D, a->q_token_stride, a->q_head_stride, p.G, p.tq, a->dtype)) return e;
+  maps.k = maps.v = maps.q;
   if (a->Tk > 0) {                                           // (without keys nothing is loaded)
     if (int e = prompt::make_map(&maps.k, a->k, a->Tk, a->Hkv, D, a->k_token_stride, a->k_head_stride, 1, prompt::BN, a->dtype))
       return e;

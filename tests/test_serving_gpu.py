@@ -121,6 +121,71 @@ def test_prompt_masked_values_do_not_leak(dtype, value):
     close(o[:350], want[:350], A[:350], dtype)
 
 
+@pytest.mark.parametrize('keys', [400, 9000])
+def test_prompt_nan_everywhere_and_no_keys(keys):
+    """All of V, or of K, is NaN: so is the result, in no unusual time; no keys at all: 0.  (9000 keys of 400 queries are
+    shared out over the SMs.)"""
+    g = gen(17)
+    q, k, v = randn(g, 400, 2, 128), randn(g, keys, 2, 128), randn(g, keys, 2, 128)
+    nan = torch.full_like(v, math.nan)
+    for a, b in ((k, nan), (nan, v)):
+        assert torch.isnan(attention_prompt(q, a, b, i32([0, 400]), i32([0, keys]))).all()
+    vb = v.clone()
+    vb[keys - 30, 1, 9] = -math.inf                          # seen by the last 30 queries
+    o, lse = attention_prompt(q, k, vb, i32([0, 400]), i32([0, keys]), return_lse=True)
+    want, wlse, A = ref.prompt(q, k, vb, [0, 400], [0, keys], 128 ** -0.5)
+    hit = torch.zeros_like(o, dtype=torch.bool)
+    hit[370:, 1, 9] = True
+    close(o[~hit], want[~hit], A[~hit], torch.bfloat16)
+    assert (o[hit] == -math.inf).all()
+    close_lse(lse, wlse)
+    o, lse = attention_prompt(q, k[:0], v[:0], i32([0, 400]), i32([0, 0]), return_lse=True)
+    assert (o == 0).all() and (lse == -math.inf).all()
+
+
+@pytest.mark.parametrize('heads,kv,dim,dtype', [(32, 8, 128, torch.bfloat16), (10, 2, 64, torch.float16), (2, 1, 128, torch.float16)])
+def test_prompt_shared_out(heads, kv, dim, dtype):
+    """Few rows and many keys: the key tiles go to all SMs in shares, sequences of other lengths and empty ones among them."""
+    g = gen(heads)
+    nq, nk = [70, 0, 1, 300, 5], [6000, 10, 2100, 4097, 3]
+    q, k, v = randn(g, sum(nq), heads, dim, dtype=dtype), randn(g, sum(nk), kv, dim, dtype=dtype), randn(g, sum(nk), kv, dim, dtype=dtype)
+    for causal in (True, False):
+        o, lse = attention_prompt(q, k, v, i32(cu(nq)), i32(cu(nk)), causal=causal, return_lse=True)
+        want, wlse, A = ref.prompt(q, k, v, cu(nq), cu(nk), dim ** -0.5, causal)
+        close(o, want, A, dtype)
+        close_lse(lse, wlse)
+        assert torch.equal(o, attention_prompt(q, k, v, i32(cu(nq)), i32(cu(nk)), causal=causal))
+
+
+def test_first_call_captured():
+    """A process whose first calls are made while a graph is captured."""
+    import subprocess
+    import sys
+    code = """
+import torch
+from kairos_sensenova_b200 import *
+i32 = lambda x: torch.tensor(x, dtype=torch.int32, device='cuda')
+x = torch.randn(40, 2, 64, device='cuda').bfloat16()
+c = KVCache.empty(4, 2, 64, 16)
+t, n, s, cu = i32([[0, 1, 2]]), i32([40]), i32([0]), i32([0, 40])
+out = []
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    kv_cache_append(c, x, x, t, n, cu)
+    k, v = kv_cache_gather(c, t, s, cu, 40)
+    out = [k, v, attention_prompt(x, k, v, cu), attention_cached(x[None, -1:], c, t, n)]
+g.replay()
+torch.cuda.synchronize()
+kv_cache_append(c, x, x, t, n, cu)
+k, v = kv_cache_gather(c, t, s, cu, 40)
+for a, b in zip(out, [k, v, attention_prompt(x, k, v, cu), attention_cached(x[None, -1:], c, t, n)]):
+    assert torch.equal(a, b)
+print('same')
+"""
+    r = subprocess.run([sys.executable, '-c', code], capture_output=True, text=True, timeout=200)
+    assert r.returncode == 0 and 'same' in r.stdout, r.stderr[-2000:]
+
+
 def test_prompt_extremes():
     """Scores up to the largest finite ones, equal scores, and a row maximum that keeps rising along the keys."""
     n, dt = 700, torch.bfloat16
