@@ -39,12 +39,7 @@ __global__ void __launch_bounds__(PAGE * D / 32 > 256 ? 512 : 256) kv_append_ker
   const int part = blockIdx.y;
 
   // the unit's sequence: largest b with cu[b] / PAGE + 2 b <= unit
-  int lo = 0, hi = p.B - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if ((int64_t)max(0, p.cu[mid]) / PAGE + 2 * mid <= unit) lo = mid; else hi = mid - 1;
-  }
-  const int b = lo;
+  const int b = warp_last(p.B, threadIdx.x & 31, [&](int i) { return (int64_t)max(0, p.cu[i]) / PAGE + 2 * i <= unit; });
   const int64_t c0 = min((int64_t)max(0, p.cu[b]), p.T), c1 = min((int64_t)p.cu[b + 1], p.T);
   const int64_t n = c1 - c0, len = p.lengths[b], first = len - n;
   const int64_t pi = unit - (c0 / PAGE + 2 * b);       // index among the pages that b writes
@@ -161,11 +156,18 @@ __global__ void __launch_bounds__(256) kv_gather_kernel(GatherParams p) {
   __shared__ int pgs[TOK];
   const int64_t t0 = (int64_t)blockIdx.x * TOK;
   if (threadIdx.x < TOK) {
-    const int64_t i = t0 + threadIdx.x;
+    const int lane = threadIdx.x;
+    const int64_t i = t0 + lane;
+    // the first token's sequence, and of the 32 that begin after it those that begin at or before each token
+    const int b0 = find_sequence(p.cu, p.B, t0, lane);
+    const int next = b0 + 1 + lane < p.B ? p.cu[b0 + 1 + lane] : 0x7fffffff;
+    int b = b0;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) b += __shfl_sync(0xffffffffu, next, j) <= i ? 1 : 0;
+    while (b - b0 >= 32 && b + 1 < p.B && p.cu[b + 1] <= i) ++b;   // (more of them: empty ones)
     int64_t r = -1;
     int pg = 0;
     if (i < p.T && i < p.cu[p.B] && i >= p.cu[0]) {
-      const int b = find_sequence(p.cu, p.B, i);
       const int64_t pos = p.starts[b] + i - p.cu[b];
       r = -2;
       if (pos >= 0 && pos < (int64_t)p.max_pages * p.page) {

@@ -64,14 +64,23 @@ KB_DEVI uint32_t pack16(float lo, float hi) {
   }
 }
 
-// Index of the sequence whose packed range holds token t: the last b < B with cu[b] <= t.
-KB_DEVI int find_sequence(const int32_t* cu, int B, int64_t t) {
-  int lo = 0, hi = B - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (cu[mid] <= t) lo = mid; else hi = mid - 1;
+// The last b < B for which below(b) holds (it holds up to some b, at 0 in any case), by one warp: 32
+// places are looked at together, so that 1024 sequences cost two loads' latencies and not ten.
+template <class F>
+KB_DEVI int warp_last(int B, int lane, F below) {
+  int lo = 0, n = B;                       // the answer is in [lo, lo + n)
+  while (n > 1) {
+    const int step = (n + 31) / 32, at = lo + lane * step;
+    const uint32_t m = __ballot_sync(0xffffffffu, lane * step < n && (lane == 0 || below(at)));
+    const int k = 31 - __clz(m);
+    lo += k * step;
+    n = min(step, n - k * step);
   }
   return lo;
+}
+// Index of the sequence whose packed range holds token t: the last b < B with cu[b] <= t.
+KB_DEVI int find_sequence(const int32_t* cu, int B, int64_t t, int lane) {
+  return warp_last(B, lane, [&](int b) { return cu[b] <= t; });
 }
 
 int check_cache(const KB200KvCache* c, const char* what);

@@ -26,6 +26,8 @@ import torch
 from . import _lib
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+_I32 = torch.int32
+_get_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 PAGE_SIZES = (16, 32, 64, 128)
 HEAD_DIMS = (64, 128)
 
@@ -85,12 +87,14 @@ class KVCache:
 
 def _int32(t, shape, what, name, index):
     """`t` as a contiguous int32 tensor of that shape on device `index` (None: any extent)."""
+    if t.dtype is _I32 and t.get_device() == index and t.shape == shape and t.is_contiguous():
+        return t
     got = t.shape
     if got != shape and (len(got) != len(shape) or any([n != m and n is not None for n, m in zip(shape, got)])):
         raise ValueError(f'{what}: {name} must be {list(shape)}, got {tuple(got)}')
     if t.get_device() != index:
         raise ValueError(f'{what}: {name} must be on device {index}, got {t.device}')
-    if t.dtype is not torch.int32:
+    if t.dtype is not _I32:
         if t.dtype is not torch.int64:
             raise ValueError(f'{what}: {name} must be int32, got {t.dtype}')
         t = t.to(torch.int32)
@@ -101,12 +105,16 @@ def _rows(t):
     """(tensor, address, strides) of `t` if its rows can be read in 16-byte steps in place, else of a contiguous copy."""
     strides, ptr = t.stride(), t.data_ptr()
     bits = ptr >> 1                                 # 16-byte aligned, strides positive multiples of 8, channels contiguous
-    for s in strides[:-1]:
-        bits |= s if s > 0 else 1
-    if bits & 7 or strides[-1] != 1:
-        t = t.contiguous()
-        return t, t.data_ptr(), t.stride()
-    return t, ptr, strides
+    if len(strides) == 3:
+        a, b, c = strides
+        if not (bits | a | b) & 7 and c == 1 and a > 0 and b > 0:
+            return t, ptr, strides
+    else:
+        a, b, c, d = strides
+        if not (bits | a | b | c) & 7 and d == 1 and a > 0 and b > 0 and c > 0:
+            return t, ptr, strides
+    t = t.clone(memory_format=torch.contiguous_format)   # (contiguous() would keep an unaligned start)
+    return t, t.data_ptr(), t.stride()
 
 
 def _refuse_grad(what):
@@ -121,13 +129,23 @@ def _cuda_index(what, cache):
 
 def _launch(index, what, fn, args):
     """``fn(args, stream)`` on device `index`'s current stream, with that the current device."""
-    if index == torch._C._cuda_getDevice():
-        rc = fn(args, torch._C._cuda_getCurrentRawStream(index))
+    if index == _get_device():
+        rc = fn(args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            rc = fn(args, torch._C._cuda_getCurrentRawStream(index))
+            rc = fn(args, _raw_stream(index))
     if rc:
         _lib.check(rc, what)
+
+
+def _table(t, rows, what, index):
+    """``(table, rows, max_pages)``: `t` as an int32 table ``[rows, max_pages]`` (rows None: any)."""
+    if t.dtype is not _I32 or t.get_device() != index or not t.is_contiguous():
+        t = _int32(t, (rows, None), what, 'page_table', index)
+    shape = t.shape
+    if len(shape) != 2 or (rows is not None and shape[0] != rows):
+        raise ValueError(f'{what}: page_table must be {[rows, None]}, got {tuple(shape)}')
+    return t, shape[0], shape[1]
 
 
 def check_tables(cache: KVCache, page_table, last, what='kv_cache', first=None, unique=False):
@@ -174,8 +192,7 @@ def kv_cache_append(cache: KVCache, k: torch.Tensor, v: torch.Tensor, page_table
         raise ValueError(f'{what}: k and v must be on {cache.device}')
     if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
         _refuse_grad(what)
-    page_table = _int32(page_table, (None, None), what, 'page_table', index)
-    B, max_pages = page_table.shape
+    page_table, B, max_pages = _table(page_table, None, what, index)
     lengths = _int32(lengths, (B,), what, 'lengths', index)
     cu = _int32(cu_seqlens, (B + 1,), what, 'cu_seqlens', index)
     if check:
@@ -200,8 +217,7 @@ def kv_cache_gather(cache: KVCache, page_table: torch.Tensor, starts: torch.Tens
     code = _DTYPES.get(dtype)
     if code is None:
         raise ValueError(f'{what}: dtype must be bfloat16 or float16, got {dtype}')
-    page_table = _int32(page_table, (None, None), what, 'page_table', index)
-    B, max_pages = page_table.shape
+    page_table, B, max_pages = _table(page_table, None, what, index)
     starts = _int32(starts, (B,), what, 'starts', index)
     cu = _int32(cu_seqlens, (B + 1,), what, 'cu_seqlens', index)
     shape = (int(total), *cache._row)
@@ -259,14 +275,13 @@ def attention_cached(q: torch.Tensor, cache: KVCache, page_table: torch.Tensor, 
     if q.requires_grad and torch.is_grad_enabled():
         _refuse_grad(what)
     B, Sq, Hq, _ = shape
-    page_table = _int32(page_table, (B, None), what, 'page_table', index)
+    page_table, _, max_pages = _table(page_table, B, what, index)
     lengths = _int32(lengths, (B,), what, 'lengths', index)
-    max_pages = page_table.shape[1]
     if check:
         check_tables(cache, page_table, lengths, what)
     q, qp, qs = _rows(q)
     if out is None:
-        out = q.new_empty(shape)
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
     elif out.shape != shape or out.dtype != q.dtype or out.get_device() != index or not out.is_contiguous() or out.data_ptr() % 16:
         raise ValueError(f'{what}: out must be contiguous 16-byte aligned {q.dtype} {list(shape)} on {cache.device}')
     lse = torch.empty(shape[:3], device=cache._device, dtype=torch.float32) if return_lse else None

@@ -342,6 +342,23 @@ def test_append_leaves_out_what_does_not_fit():
     assert (kg[12:16] == 1).all() and (kg[16:60] == 0).all()
 
 
+def test_append_and_gather_many_sequences():
+    """More sequences than a warp looks at together, runs of empty ones among them."""
+    n = [1, 0, 3] * 30 + [0] * 70 + [5] * 40 + [0] * 33 + [70] + [1] * 900
+    old = [i % 37 for i in range(len(n))]
+    lens = [a + b for a, b in zip(n, old)]
+    H, D, page = 1, 64, 16
+    cache, table, _ = make_cache(lens, H, D, page, seed=8)
+    g = gen(8)
+    k, v = randn(g, sum(n), H, D), randn(g, sum(n), H, D)
+    w, s = values(cache.k_pages), cache.k_scale.clone()
+    ref.append(w, s, k, table, lens, cu(n))
+    kv_cache_append(cache, k, v, i32(table), i32(lens), i32(cu(n)))
+    assert torch.equal(cache.k_scale, s) and torch.equal(values(cache.k_pages).nan_to_num(), w.nan_to_num())
+    kg, _ = kv_cache_gather(cache, i32(table), i32(old), i32(cu(n)), sum(n))
+    assert torch.equal(kg, ref.gather(w, s, table, old, n).bfloat16())
+
+
 def test_gather_leaves_other_rows():
     cache, table, _ = make_cache([30], 2, 128, 16, 1)
     out = [torch.full((50, 2, 128), 5.0, device='cuda', dtype=torch.bfloat16) for _ in range(2)]

@@ -48,6 +48,8 @@ def test_index_and_rows():
     assert rows(x[:, 2:4]).data_ptr() == x[:, 2:4].data_ptr()
     assert rows(x[..., 1:]).is_contiguous() and rows(x.transpose(1, 2)).is_contiguous()
     assert rows(x[:, :1].expand(10, 3, 64)).is_contiguous()
+    odd = torch.zeros(10 * 64 + 1, dtype=torch.bfloat16)[1:].view(10, 1, 64)    # contiguous, 2 bytes off
+    assert rows(odd).data_ptr() % 16 == 0 and rows(odd[None]).data_ptr() % 16 == 0
     t, ptr, strides = _rows(x[:, 1:, ::2])
     assert t.is_contiguous() and strides == t.stride() and ptr == t.data_ptr()
 
