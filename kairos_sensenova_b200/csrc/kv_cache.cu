@@ -72,18 +72,31 @@ __global__ void __launch_bounds__(PAGE * D / 32 > 256 ? 512 : 256) kv_append_ker
   for (int base = part * PER_BLOCK; base < 2 * p.H; base += stride, turn ^= 1) {   // (items: head, k|v)
     const int item = base + grp;
     fetch(item + stride, nx);
-    float amax = 0.f;
+    // the largest magnitude, as 16-bit integers in pairs (the order of the magnitudes; NaN and
+    // infinities come out on top, and only if there are some is it done again without them)
+    constexpr uint32_t INF = F16 ? 0x7c00u : 0x7f80u;
+    uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+    for (int i = 0; i < 4; ++i)
+      top = __vmaxu2(__vmaxu2(__vmaxu2(top, x[i].x & 0x7fff7fffu), __vmaxu2(x[i].y & 0x7fff7fffu, x[i].z & 0x7fff7fffu)),
+                     x[i].w & 0x7fff7fffu);
+    uint32_t mag = max(top & 0xffffu, top >> 16);
+    const bool odd = mag >= INF;                         // this thread has a value that is not finite
+    if (odd) {
+      mag = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 f = unpack16<F16>(w[e]);
-        const float a = fabsf(f.x), c = fabsf(f.y);
-        if (a < INFINITY) amax = fmaxf(amax, a);         // NaN and infinities do not set the scale
-        if (c < INFINITY) amax = fmaxf(amax, c);
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t lo = w[e] & 0x7fffu, hi = (w[e] >> 16) & 0x7fffu;
+          if (lo < INF) mag = max(mag, lo);
+          if (hi < INF) mag = max(mag, hi);
+        }
       }
     }
+    const float2 mag2 = unpack16<F16>(mag);
+    float amax = mag2.x;
     const bool is_v = item & 1, live = item < 2 * p.H;
     const int h = item >> 1;
     float* scale = (is_v ? p.v_scale : p.k_scale) + (int64_t)pg * p.H + h;
@@ -118,11 +131,17 @@ __global__ void __launch_bounds__(PAGE * D / 32 > 256 ? 512 : 256) kv_append_ker
             *dst = r;
           }
         } else if (tok < end) {
-          const float2 f0 = unpack16<F16>(x[i].x), f1 = unpack16<F16>(x[i].y), f2 = unpack16<F16>(x[i].z),
-                       f3 = unpack16<F16>(x[i].w);
+          const float2 s2 = make_float2(inv, inv);
+          const float2 f0 = fmul2(unpack16<F16>(x[i].x), s2), f1 = fmul2(unpack16<F16>(x[i].y), s2),
+                       f2 = fmul2(unpack16<F16>(x[i].z), s2), f3 = fmul2(unpack16<F16>(x[i].w), s2);
           uint2 r;
-          r.x = encode2(f0.x * inv, f0.y * inv) | encode2(f1.x * inv, f1.y * inv) << 16;
-          r.y = encode2(f2.x * inv, f2.y * inv) | encode2(f3.x * inv, f3.y * inv) << 16;
+          if (odd) {
+            r.x = encode2(f0.x, f0.y) | encode2(f1.x, f1.y) << 16;
+            r.y = encode2(f2.x, f2.y) | encode2(f3.x, f3.y) << 16;
+          } else {
+            r.x = encode2_finite(f0) | encode2_finite(f1) << 16;
+            r.y = encode2_finite(f2) | encode2_finite(f3) << 16;
+          }
           *dst = r;
         }
       }
@@ -145,13 +164,13 @@ struct GatherParams {
 
 // Packed token i of sequence b is its cached token starts[b] + i - cu[b]; out [T, H, D].
 // A block takes 32 packed tokens: a warp finds their pages, then every thread
-// dequantises 16 codes at a time (one 16-byte load, two 16-byte stores), heads of a
+// dequantises 8 codes at a time (an 8-byte load, a 16-byte store), heads of a
 // token next to each other so that the stores are contiguous.  Bound: HBM.  1 B read
 // and 2 B written per value.  Tokens of a missing page read as 0; rows at and behind
 // cu[B] are left as they were.
 template <int D, bool F16>
 __global__ void __launch_bounds__(256) kv_gather_kernel(GatherParams p) {
-  constexpr int TOK = 32, CPR = D / 16, UNROLL = 4;
+  constexpr int TOK = 32, CPR = D / 8, UNROLL = 8;
   __shared__ int64_t row[TOK];     // code row of head 0 (a row has D codes), -1: no such token, -2: missing page
   __shared__ int pgs[TOK];
   const int64_t t0 = (int64_t)blockIdx.x * TOK;
@@ -187,7 +206,7 @@ __global__ void __launch_bounds__(256) kv_gather_kernel(GatherParams p) {
     const int h = rest / CPR, c = rest % CPR;
     const int64_t hoff = (int64_t)h * p.page;
     for (int tok = tok0; tok < TOK; tok += lanes * UNROLL) {
-      uint4 codes[UNROLL][2];
+      uint2 codes[UNROLL][2];
       float s[UNROLL][2];
 #pragma unroll
       for (int z = 0; z < UNROLL; ++z) {
@@ -195,10 +214,10 @@ __global__ void __launch_bounds__(256) kv_gather_kernel(GatherParams p) {
         const int64_t r = tt < TOK ? row[tt] : -1;
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
-          codes[z][kv] = make_uint4(0, 0, 0, 0);
+          codes[z][kv] = make_uint2(0, 0);
           s[z][kv] = 0.f;
           if (r >= 0) {
-            codes[z][kv] = __ldg(reinterpret_cast<const uint4*>((kv ? p.v_pages : p.k_pages) + (r + hoff) * D + c * 16));
+            codes[z][kv] = __ldg(reinterpret_cast<const uint2*>((kv ? p.v_pages : p.k_pages) + (r + hoff) * D + c * 8));
             s[z][kv] = __ldg((kv ? p.v_scale : p.k_scale) + (int64_t)pgs[tt] * p.H + h);
           }
         }
@@ -207,22 +226,20 @@ __global__ void __launch_bounds__(256) kv_gather_kernel(GatherParams p) {
       for (int z = 0; z < UNROLL; ++z) {
         const int tt = tok + z * lanes;
         if (tt >= TOK || row[tt] == -1) continue;
-        const int64_t dst = ((t0 + tt) * p.H + h) * D + c * 16;
+        const int64_t dst = ((t0 + tt) * p.H + h) * D + c * 8;
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
-          const uint32_t w[4] = {codes[z][kv].x, codes[z][kv].y, codes[z][kv].z, codes[z][kv].w};
-          uint32_t o[8];
+          const uint32_t w[2] = {codes[z][kv].x, codes[z][kv].y};
+          uint32_t o[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
+          for (int e = 0; e < 2; ++e) {
             uint32_t lo, hi;
             decode4(w[e], lo, hi);
             const float2 f0 = half2_to_float2(lo), f1 = half2_to_float2(hi);
             o[2 * e] = pack16<F16>(f0.x * s[z][kv], f0.y * s[z][kv]);
             o[2 * e + 1] = pack16<F16>(f1.x * s[z][kv], f1.y * s[z][kv]);
           }
-          uint4* d = reinterpret_cast<uint4*>(reinterpret_cast<char*>(kv ? p.v : p.k) + 2 * dst);
-          d[0] = make_uint4(o[0], o[1], o[2], o[3]);
-          d[1] = make_uint4(o[4], o[5], o[6], o[7]);
+          *reinterpret_cast<uint4*>(reinterpret_cast<char*>(kv ? p.v : p.k) + 2 * dst) = make_uint4(o[0], o[1], o[2], o[3]);
         }
       }
     }

@@ -32,6 +32,8 @@ KB_DEVI uint32_t encode2(float a, float b) {
   if (fabsf(b) == INFINITY) b = __uint_as_float(0x7fffffffu);
   return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
 }
+// The same for values known not to be infinite.
+KB_DEVI uint32_t encode2_finite(float2 f) { return (uint32_t)__nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3); }
 // The two e4m3 codes in the low half of `c` as f16 pair (exact).
 KB_DEVI uint32_t decode2(uint32_t c) {
   uint32_t r;
