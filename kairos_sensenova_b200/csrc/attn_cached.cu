@@ -727,40 +727,45 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
   }
 }
 
-// Joins the partials of the units that cross shares, and writes the empty sequences.
-// One block per (sequence, kv head, row block).
+// Joins the partials of the units that cross shares, and writes the empty sequences.  Block c looks
+// at the border before share c; the block of a unit's first border joins it.  (So there are as many
+// blocks as shares, whatever the number of units.)
 template <int D, bool F16, int NT>
 __global__ void __launch_bounds__(Shape<D, NT>::JOIN) attn_cached_join_kernel(Params p, int ctas) {
   constexpr int THREADS = Shape<D, NT>::JOIN;
   constexpr int GT = Shape<D, NT>::GT, ROWS = Shape<D, NT>::ROWS;
   const int lane = threadIdx.x & 31;
   const int64_t units = (int64_t)p.H * p.rblocks;
-  const int b = (int)(blockIdx.x / units), u = (int)(blockIdx.x % units);
-  const int h = u / p.rblocks, rb = u % p.rblocks;
-  const int ng = seq_groups<GT>(p, b), span = seq_span<GT>(p, b);
-  // flat lengths of the sequences before b, and of all (every warp for itself)
-  int64_t before = 0, sum = 0;
-  for (int i = lane; i < p.B; i += 32) {
-    const int x = seq_span<GT>(p, i);
-    sum += x;
-    if (i < b) before += x;
-  }
+  int64_t sum = 0;
+  for (int i = lane; i < p.B; i += 32) sum += seq_span<GT>(p, i);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    before += __shfl_xor_sync(0xffffffffu, before, o);
-  }
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   const Share sh = share_of(units, sum, ctas, Shape<D, NT>::WK);
-  int c0 = 0, c1 = -1;                     // CTAs whose shares hold a part of this unit
-  int64_t begin = 0;
-  if (ng > 0) {
-    begin = before * units + (int64_t)u * span;
-    c0 = (int)(begin / sh.per);
-    c1 = (int)((begin + ng - 1) / sh.per);
+  const int64_t at = (int64_t)blockIdx.x * sh.per;
+  int b = 0, u = 0, c0 = 0, c1 = -1;       // the unit, and the CTAs whose shares hold a part of it (none: nothing to join)
+  if (blockIdx.x > 0 && at < sh.total) {
+    int64_t begin;
+    warp_find<GT>(p, units, at, lane, b, begin);
+    const int ng = seq_groups<GT>(p, b), span = seq_span<GT>(p, b);
+    u = (int)((at - begin) / span);
+    const int before = (int)(at - begin - (int64_t)u * span);   // the unit's groups on this side of the border
+    if (before > 0 && before < ng && (at - before) / sh.per == blockIdx.x - 1) {
+      c0 = (int)blockIdx.x - 1;
+      c1 = (int)((at - before + ng - 1) / sh.per);
+    }
   }
   // (every block waits, those without work too: this grid must not end before the one it follows)
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
-  if (ng > 0 && c0 == c1) return;          // finished there
+  const int64_t per_seq = (int64_t)p.Sq * p.Hq;
+  for (int i = blockIdx.x; i < p.B; i += gridDim.x)
+    if (seq_len(p, i) == 0) {
+      for (int64_t e = threadIdx.x; e < per_seq * (D / 8); e += THREADS)
+        reinterpret_cast<uint4*>(p.o)[i * per_seq * (D / 8) + e] = make_uint4(0, 0, 0, 0);
+      if (p.lse)
+        for (int64_t e = threadIdx.x; e < per_seq; e += THREADS) p.lse[i * per_seq + e] = -INFINITY;
+    }
+  if (c1 < c0) return;
+  const int h = u / p.rblocks, rb = u % p.rblocks;
   // Partials in share order: the part that begins the unit is its CTA's last segment (slot 1),
   // the later ones continue it (slot 0).  A chunk's m and l are read together, then its O with
   // all loads in flight: what the join costs is the two latencies.
@@ -873,7 +878,7 @@ static int launch(const Params& p, int grid, cudaStream_t st) {
   overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   overlap.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)((int64_t)p.B * p.H * p.rblocks));
+  cfg.gridDim = dim3((unsigned)grid);
   cfg.blockDim = dim3(S::JOIN);
   cfg.stream = st;
   cfg.attrs = &overlap;

@@ -5,6 +5,8 @@
     python -m kairos_sensenova_b200.profile_cases prologue T H  # gdn_prologue on a fused [T, 3*H*128 + 2H (+pad)] projection
     python -m kairos_sensenova_b200.profile_cases resln T C     # residual_ln_mod on [T, C] bf16 rows
     python -m kairos_sensenova_b200.profile_cases dit L         # one eager DiT step (config 4 shapes, L blocks)
+    python -m kairos_sensenova_b200.profile_cases prompt T H    # attention_prompt, one prompt of T tokens, H heads on H/3 kv heads
+    python -m kairos_sensenova_b200.profile_cases cache T H     # kv_cache_append, kv_cache_gather, attention_cached: 8 sequences of T tokens
 
 Each runs the operator twice (warm) on synthetic seeded inputs and exits, so an
 ``ncu -k <kernel> -s <n> -c 1`` capture sees a handful of launches of a
@@ -66,8 +68,33 @@ def main(argv):
         ctx = torch.randn(cfg.text_len, cfg.text_dim, generator=gen, device='cuda')
         with torch.no_grad():
             model(lat, torch.tensor([500.0], device='cuda'), ctx)
+    elif what == 'prompt':
+        from .attention import attention_prompt
+        gen = torch.Generator(device='cuda')
+        gen.manual_seed(3)
+        kv = max(1, h // 3)
+        x = torch.randn(n, h // kv * kv + 2 * kv, 128, generator=gen, device='cuda').to(torch.bfloat16)
+        q, k, v = x.split([h // kv * kv, kv, kv], 1)
+        cu = torch.tensor([0, n], dtype=torch.int32, device='cuda')
+        for _ in range(2):
+            attention_prompt(q, k, v, cu)
+    elif what == 'cache':
+        from .kv_cache import KVCache, attention_cached, kv_cache_append, kv_cache_gather
+        gen = torch.Generator(device='cuda')
+        gen.manual_seed(4)
+        B, kv, pages = 8, max(1, h // 3), -(-n // 64)
+        cache = KVCache.empty(B * pages, kv, 128, 64)
+        k, v = (torch.randn(B * n, kv, 128, generator=gen, device='cuda').to(torch.bfloat16) for _ in range(2))
+        q = torch.randn(B, 1, h // kv * kv, 128, generator=gen, device='cuda').to(torch.bfloat16)
+        i32 = dict(dtype=torch.int32, device='cuda')
+        table = torch.randperm(B * pages, generator=gen, device='cuda').to(torch.int32).view(B, pages)
+        lengths, cu = torch.full((B,), n, **i32), torch.arange(0, B * n + 1, n, **i32)
+        for _ in range(2):
+            kv_cache_append(cache, k, v, table, lengths, cu)
+            kv_cache_gather(cache, table, torch.zeros(B, **i32), cu, B * n)
+            attention_cached(q, cache, table, lengths)
     else:
-        raise SystemExit(f'unknown case {what!r} (attn | gdn | prologue | resln | dit)')
+        raise SystemExit(f'unknown case {what!r} (attn | gdn | prologue | resln | dit | prompt | cache)')
     torch.cuda.synchronize()
     print('ok')
 

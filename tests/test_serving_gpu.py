@@ -157,6 +157,35 @@ def test_prompt_shared_out(heads, kv, dim, dtype):
         assert torch.equal(o, attention_prompt(q, k, v, i32(cu(nq)), i32(cu(nk)), causal=causal))
 
 
+def test_prompt_many_sequences():
+    """Thousands of sequences, runs of empty ones among them."""
+    nq = [1, 0, 3, 130] * 40 + [0] * 500 + [2] * 3000 + [0, 300, 0]
+    g = gen(31)
+    q, k, v = randn(g, sum(nq), 3, 64), randn(g, sum(nq), 1, 64), randn(g, sum(nq), 1, 64)
+    for causal in (True, False):
+        o, lse = attention_prompt(q, k, v, i32(cu(nq)), causal=causal, return_lse=True)
+        some = [i for i, n in enumerate(nq) if n][::7] + [len(nq) - 2]
+        at = cu(nq)
+        for i in some:
+            a, b = at[i], at[i + 1]
+            want, wlse, A = ref.prompt(q[a:b], k[a:b], v[a:b], [0, b - a], [0, b - a], 64 ** -0.5, causal)
+            close(o[a:b], want, A, torch.bfloat16)
+            close_lse(lse[a:b], wlse)
+
+
+def test_cached_many_sequences():
+    """More units than shares, and thousands of empty sequences."""
+    lens = [0, 17, 0, 40, 1] * 300 + [0] * 1000 + [900, 0, 3]
+    H, D, page = 2, 64, 16
+    cache, table, _ = make_cache(lens, H, D, page, seed=12)
+    q = randn(gen(12), len(lens), 1, 4, D)
+    out = torch.full((len(lens), 1, 4, D), 3.0, device='cuda', dtype=torch.bfloat16)
+    _, lse = attention_cached(q, cache, i32(table), i32(lens), out=out, return_lse=True)
+    want, wlse, A = ref.cached(q, values(cache.k_pages), values(cache.v_pages), cache.k_scale, cache.v_scale, table, lens, D ** -0.5)
+    close(out, want, A, torch.bfloat16, u_p=2.0 ** -11)
+    close_lse(lse, wlse)
+
+
 def test_first_call_captured():
     """A process whose first calls are made while a graph is captured."""
     import subprocess
