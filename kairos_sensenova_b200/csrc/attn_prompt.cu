@@ -276,7 +276,8 @@ KB_DEVI void find_tile(const Params& p, int64_t r, int lane, int& seq, int& tile
   seq = kv::warp_last(p.N, lane, [&](int s) { return first(s) <= r; });
   int lv;
   const int nt = tiles_of(seq, lv);
-  tile = max(-1, nt - 1 - (int)min(r - first(seq), (int64_t)nt));
+  const int64_t off = r - first(seq);
+  tile = off >= 0 && off < nt ? nt - 1 - (int)off : -1;
 }
 
 // Fills the table, by one warp; returns the number of row tiles.
