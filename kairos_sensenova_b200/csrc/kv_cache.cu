@@ -303,12 +303,8 @@ extern "C" int kb200_kv_append(const KB200KvAppendArgs* a, void* stream) {
                      (int)c->num_pages, (int)c->H, (int)a->max_pages, (int)a->B, a->T};
   cudaStream_t st = (cudaStream_t)stream;
   const int page = (int)c->page;
-  if (c->D == 64) {
-    if (a->dtype) kv::launch_append_page<64, true>(p, page, st); else kv::launch_append_page<64, false>(p, page, st);
-  } else {
-    if (a->dtype) kv::launch_append_page<128, true>(p, page, st); else kv::launch_append_page<128, false>(p, page, st);
-  }
-  return check_launch("kv_append_kernel");
+  if (c->D == 64) return a->dtype ? kv::launch_append_page<64, true>(p, page, st) : kv::launch_append_page<64, false>(p, page, st);
+  return a->dtype ? kv::launch_append_page<128, true>(p, page, st) : kv::launch_append_page<128, false>(p, page, st);
 }
 
 extern "C" int kb200_kv_gather(const KB200KvGatherArgs* a, void* stream) {
