@@ -231,7 +231,9 @@ int kb200_residual_ln_mod(void* x, const void* r, int64_t rows, int64_t dim, int
  * rows at and behind cu_q[N] are left as they were.  A masked key's values reach no
  * output, whatever they are.  D = 64 or 128; dtype 0 bf16, 1 fp16.  Strides in
  * elements, multiples of 8; channels contiguous.  cu_q, cu_k are device arrays, not
- * read by the host; offsets are clamped to the tokens there are.
+ * read by the host; offsets are clamped to the tokens there are.  o may not overlap the
+ * inputs.  Hq up to 2^14, N up to 2^20 and N * Hkv up to 2^24 (Hkv times the parts, where
+ * more than 128 query heads share a kv head).
  * --------------------------------------------------------------------- */
 typedef struct KB200PromptArgs {
   const void* q;              /* [Tq, Hq, D]                                      */

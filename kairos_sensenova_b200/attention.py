@@ -120,9 +120,9 @@ def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     keys the queries are the last n of the m tokens: query i sees the first ``i + 1 + m - n``
     keys (``causal=False``: all m).  A query that sees none gets 0; the values of keys that a
     query does not see never reach it, NaN and infinities included.  Returns ``[Tq, Hq, D]``
-    (``out``: to write into; rows behind the last sequence are left as they were); with
-    ``return_lse`` also the fp32 log of the softmax sum ``[Tq, Hq]``.  ``check=True`` looks at
-    the offsets on the host first (it synchronises) and raises ``ValueError``."""
+    (``out``: to write into, apart from the inputs; rows behind the last sequence are left as they
+    were); with ``return_lse`` also the fp32 log of the softmax sum ``[Tq, Hq]``.  ``check=True``
+    looks at the offsets on the host first (it synchronises) and raises ``ValueError``."""
     what = 'attention_prompt'
     index = q.get_device()
     if index < 0:

@@ -100,7 +100,17 @@ KB_DEVI int seq_span(const Params& p, int b) {
 template <int GT>
 KB_DEVI void warp_find(const Params& p, int64_t units, int64_t at, int lane, int& b_out, int64_t& begin_out) {
   int64_t base = 0;
-  for (int b0 = 0; b0 < p.B; b0 += 32) {
+  int b0 = 0;
+  for (; b0 + 256 < p.B; b0 += 256) {      // many sequences: 256 are passed over at once
+    int64_t sum = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += seq_span<GT>(p, b0 + i * 32 + lane);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (base + units * sum > at) break;
+    base += units * sum;
+  }
+  for (; b0 < p.B; b0 += 32) {
     const int64_t mine = b0 + lane < p.B ? units * seq_span<GT>(p, b0 + lane) : 0;
     int64_t inc = mine;
 #pragma unroll
@@ -175,16 +185,22 @@ struct Walk {
     u = (int)((at - begin) / span);
     x = (int)((at - begin) - (int64_t)u * span);
   }
-  KB_DEVI bool next(const Params& p, int units) {
+  // (by a warp, whose lanes all have the same; 32 sequences are looked at for one that is not empty)
+  KB_DEVI bool next(const Params& p, int units, int lane) {
     while (left > 0) {
+      if (u == units) {
+        u = x = 0;
+        uint32_t some = 0;
+        for (++b; b < p.B; b += 32) {
+          some = __ballot_sync(0xffffffffu, b + lane < p.B && seq_len(p, b + lane) > 0);
+          if (some) break;
+        }
+        if (!some) return false;
+        b += __ffs(some) - 1;
+      }
       len = seq_len(p, b);
       ng = (len + GT - 1) / GT;
-      if (ng == 0 || u == units) {
-        ++b;
-        u = x = 0;
-        continue;
-      }
-      const int take = (int)min((int64_t)(ng + PAD - x), left);
+      const int take = (int)min((int64_t)max(ng + PAD - x, 1), left);
       left -= take;
       g0 = x;
       count = min(x + take, ng) - x;
@@ -192,7 +208,7 @@ struct Walk {
       h = u / p.rblocks;
       rb = u - h * p.rblocks;
       x += take;
-      if (x == ng + PAD) {
+      if (x >= ng + PAD) {
         x = 0;
         ++u;
       }
@@ -280,7 +296,7 @@ struct Loader {
       f.rot = (f.rot + f.seg.count) % S::WK;
       f.first = warp >= f.rot ? warp - f.rot : warp + S::WK - f.rot;
       f.done = 0;
-      f.live = f.seg.next(p, units);
+      f.live = f.seg.next(p, units, lane);
     }
     __syncwarp();
     if (lane == 0) *feed = f;
@@ -375,13 +391,13 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
 
   // Every warp walks the CTA's segments in the same order.  Group i of a segment goes to
   // warp (i + rot) % WK, so that short segments use all of them in turn.
-  if (lane == 0) {
+  {
     Feed<GT> f{};
     f.seg = sm.start;
-    sm.walk[warp] = f.seg;
+    if (lane == 0) sm.walk[warp] = f.seg;
     f.first = warp;
-    f.live = f.seg.next(p, (int)units);
-    sm.feed[warp] = f;
+    f.live = f.seg.next(p, (int)units, lane);
+    if (lane == 0) sm.feed[warp] = f;
   }
   Loader<D, NT> loader(&sm.feed[warp], p, (int)units, warp, lane);
   for (int s = 0; s < STAGES; ++s) loader.load(p, (int)units, warp, lane, sm.slot[warp][s], sm.scale[warp][s]);
@@ -389,7 +405,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
   auto next_segment = [&]() {              // the using side's walk, in shared memory too
     __syncwarp();
     seg = sm.walk[warp];
-    const bool more = seg.next(p, (int)units);
+    const bool more = seg.next(p, (int)units, lane);
     __syncwarp();
     if (lane == 0) sm.walk[warp] = seg;
     return more;
@@ -917,6 +933,8 @@ extern "C" int kb200_attn_cached_fwd(const KB200AttnCachedArgs* a, void* stream)
   if (int e = kv::check_cache(c, "attn_cached")) return e;
   if (int e = cached::check_shape(B, Sq, Hq, c->H, max_pages)) return e;
   if (a->dtype != 0 && a->dtype != 1) return set_error(KB200_ERR_INVALID, "attn_cached: dtype=%lld", (long long)a->dtype);
+  if (!(fabsf((float)a->softmax_scale) < INFINITY))
+    return set_error(KB200_ERR_INVALID, "attn_cached: softmax_scale=%f", a->softmax_scale);
   if (B == 0 || Sq == 0) return KB200_OK;
   if (!a->q || !a->o || !a->lengths || (max_pages > 0 && !a->page_table))
     return set_error(KB200_ERR_INVALID, "attn_cached: null pointer");

@@ -1004,8 +1004,11 @@ extern "C" int kb200_attn_prompt_fwd(const KB200PromptArgs* a, void* stream) {
         a->o_token_stride | a->o_head_stride) & 7))
     return set_error(KB200_ERR_ALIGN, "attn_prompt: q, k, v and o rows must be 16-byte aligned");
   const prompt::Split sp = prompt::split_heads(a->Hq / a->Hkv);
-  if (prompt::most_tiles(a->Tq, a->N, sp.tq) * a->Hkv * sp.parts > 0x7fffffffLL)
-    return set_error(KB200_ERR_INVALID, "attn_prompt: too many rows");
+  // (passing over a number that no tile has takes a CTA 1-2 us: the second limit keeps a run of them, 2^24 / SMs at
+  // most, far inside the bounds of the waits)
+  if (prompt::most_tiles(a->Tq, a->N, sp.tq) * a->Hkv * sp.parts > 0x7fffffffLL || a->N * a->Hkv * sp.parts > (1 << 24))
+    return set_error(KB200_ERR_INVALID, "attn_prompt: too many rows, or sequences times kv heads");
+  if (!(fabsf(a->softmax_scale) < INFINITY)) return set_error(KB200_ERR_INVALID, "attn_prompt: softmax_scale=%f", a->softmax_scale);
   // a scale of 0 becomes one too small to matter, so that a masked score stays -inf
   const float sl2 = fmaxf(fabsf(a->softmax_scale) * 1.4426950408889634f, 1e-30f);
   const int sms = sm_count();

@@ -29,7 +29,7 @@ int allow_smem(const void* kernel, size_t bytes, std::atomic<uint64_t>& done) {
 }
 
 int sm_count() {
-  static int counts[64];             // per device; written with the same value by every thread that gets there
+  static std::atomic<int> counts[64];   // per device
   int dev = 0, n = 148;
   if (cudaGetDevice(&dev) != cudaSuccess) { cudaGetLastError(); return n; }
   if (dev < 64 && counts[dev]) return counts[dev];

@@ -259,7 +259,7 @@ def attention_cached(q: torch.Tensor, cache: KVCache, page_table: torch.Tensor, 
     reads kv head ``h // (Hq / heads)``); ``lengths[b]`` counts the cached tokens, the Sq
     themselves included, and query i sees the first ``lengths[b] - Sq + 1 + i`` of them.  A
     query that sees none (an idle slot of length 0) gets 0.  Returns ``[B, Sq, Hq, D]`` in
-    q's type (``out``: contiguous, to write into); with ``return_lse`` also the fp32 log of
+    q's type (``out``: contiguous, to write into, apart from the inputs); with ``return_lse`` also the fp32 log of
     the softmax sum ``[B, Sq, Hq]`` (-inf where nothing is seen)."""
     what = 'attention_cached'
     index = _cuda_index(what, cache)

@@ -105,6 +105,9 @@ def test_c_entries_refuse():
     for bad in (dict(D=96), dict(Hq=3), dict(Hkv=0), dict(Tq=-1), dict(dtype=2), dict(q=None), dict(k=None), dict(cu_k=None)):
         assert pr(**bad) == 1, bad
     assert pr(v=8) == 2 and pr(o_head_stride=4) == 2
+    for scale in (float('nan'), float('inf'), -float('inf')):
+        assert pr(softmax_scale=scale) == 1 and att(softmax_scale=scale) == 1, scale
+    assert pr(N=1 << 20, Hq=32, Hkv=32) == 1 and pr(N=(1 << 20) + 1) == 1
 
 
 def test_oracle_rounds_as_torch_does():
