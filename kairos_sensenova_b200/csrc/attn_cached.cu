@@ -13,6 +13,8 @@
 // shares leaves a partial (m, l, O) per CTA, joined in share order (no atomics: the
 // result does not depend on timing) by a second, dependent kernel.
 //
+// A short unit in a share of several is one warp's alone, without a join (short_unit below).
+//
 // Every warp has a ring of its own, fills it by 16-byte cp.async (swizzled, so that no load from
 // it conflicts) and takes every WK-th group: no warp waits for another inside a unit.  (One
 // TMA box per 16 tokens and head ran at 80-100 cycles a box whatever its size, 25 B a cycle
@@ -171,22 +173,36 @@ struct Shape {
   static constexpr int JOIN = ROWS * D / 4 < 256 ? ROWS * D / 4 : 256;   // threads of a joining block
 };
 
+// A unit is short if a warp alone should take it.  Spread over the WK = 8 warps it costs ng / 8 groups and
+// about 2 more for the join, in which all warps wait; one warp's alone ng groups and no join, but the
+// share's U = per / (ng + PAD) units may not go evenly into the warps, which costs up to ng groups
+// once.  So units of up to 4 U groups are taken alone, if there are at least 4 to a share.  (1024
+// sequences of 100 tokens, 24/8 heads of 128: 78 us so, 161 us without; 256 of 300: 53 and 68 us.)
+KB_DEVI int short_unit(int64_t per) {      // ng <= per / 4 - PAD, ng (ng + PAD) <= 4 per
+  const float x = (float)per;
+  return (int)fminf(x * 0.25f - PAD, sqrtf(4.f * x + PAD * PAD / 4) - PAD / 2);
+}
+
 // A CTA's segments, in order: the groups [g0, g0 + count) of unit (b, h, rb); `ng` are all of
 // the unit's.  (Parts of a share that are padding alone are passed over.)
-template <int GT>
+template <int GT, int WK>
 struct Walk {
   int64_t left;                        // flat positions still to come
   int b, u, x;                         // the next one: sequence, unit, position in the unit
   int b_of, h, rb, len, ng, g0, count; // (b_of: the segment's sequence)
-  KB_DEVI void start(const Params& p, int64_t at, int64_t end, int b_, int64_t begin) {
+  int short_ng;                        // units of up to so many groups are short
+  int turn, solo;                      // the warp that takes the next short unit; that takes this segment, -1: all do
+  KB_DEVI void start(const Params& p, int64_t at, int64_t end, int64_t per, int b_, int64_t begin) {
     left = end - at;
+    short_ng = short_unit(per);
+    turn = 0;
     b = b_;
     const int span = seq_span<GT>(p, b);
     u = (int)((at - begin) / span);
     x = (int)((at - begin) - (int64_t)u * span);
   }
   // (by a warp, whose lanes all have the same; 32 sequences are looked at for one that is not empty)
-  KB_DEVI bool next(const Params& p, int units, int lane) {
+  KB_DEVI bool next(const Params& p, int units, int lane, int warp) {
     while (left > 0) {
       if (u == units) {
         u = x = 0;
@@ -200,6 +216,14 @@ struct Walk {
       }
       len = seq_len(p, b);
       ng = (len + GT - 1) / GT;
+      const bool alone = ng <= short_ng;
+      if (alone && x == 0) {           // the other warps' short units of this sequence are passed over at once
+        const int k = min(min(warp >= turn ? warp - turn : warp + WK - turn, units - u), (int)min(left, (int64_t)0x7fffffff) / (ng + PAD));
+        u += k;
+        left -= (int64_t)k * (ng + PAD);
+        turn = turn + k >= WK ? turn + k - WK : turn + k;
+        if (u == units || left <= 0) continue;
+      }
       const int take = (int)min((int64_t)max(ng + PAD - x, 1), left);
       left -= take;
       g0 = x;
@@ -212,18 +236,35 @@ struct Walk {
         x = 0;
         ++u;
       }
-      if (count > 0) return true;
+      if (count > 0) {
+        solo = -1;
+        if (alone && count == ng) {
+          solo = turn;
+          turn = turn + 1 == WK ? 0 : turn + 1;
+          if (solo != warp) continue;
+        }
+        return true;
+      }
     }
     return false;
   }
 };
 
+// The first of a segment's groups that `warp` takes, and with which it goes on: a short unit is one
+// warp's alone; else every WK-th group, beginning so that short segments use all warps in turn.
+template <int GT, int WK>
+KB_DEVI int first_group(const Walk<GT, WK>& seg, int rot, int warp) {
+  if (seg.solo >= 0) return 0;
+  return warp >= rot ? warp - rot : warp + WK - rot;
+}
+
 // Where the loading side of a warp is: kept in shared memory, since it is touched once per
 // batch and the registers are short.
-template <int GT>
+template <int GT, int WK>
 struct Feed {
-  Walk<GT> seg;
+  Walk<GT, WK> seg;
   int rot, first, done;                      // of the segment: rotation, the warp's first group, groups batched
+  int step;                                  // tokens from one of the warp's groups to the next
   int live;
   int h, n, tok0;                            // the next batch: head, groups, first token of its first group
 };
@@ -238,9 +279,9 @@ struct Smem {
   Slot slot[S::WK][S::STAGES];
   float ml[S::WK][S::ROWS][2];
   float2 scale[S::WK][S::STAGES][NT];        // page scales (k, v) of 16 tokens each; k < 0: no such page
-  Feed<S::GT> feed[S::WK];
-  Walk<S::GT> walk[S::WK];
-  Walk<S::GT> start;
+  Feed<S::GT, S::WK> feed[S::WK];
+  Walk<S::GT, S::WK> walk[S::WK];
+  Walk<S::GT, S::WK> start;
   int64_t total;
   int held[S::WK];                           // the slot that holds the warp's O, -1: none
 };
@@ -252,9 +293,9 @@ template <int D, int NT>
 struct Loader {
   using S = Shape<D, NT>;
   static constexpr int BATCH = 32 / NT;      // groups of a batch
-  Feed<S::GT>* feed;
-  int h, n, pos, tok0, pg;                   // current batch: head, groups, next one, first token, this lane's page
-  int pg2;                                   // the next batch's
+  Feed<S::GT, S::WK>* feed;
+  int n, pos, row;                           // current batch: groups, next one; this lane's part: its first code row, -1: no such page
+  int pg2;                                   // the next batch's: its row, or while `pending` the page that it is formed from
   float2 sc, sc2;
   bool pending;                              // sc2 is still to be read
   float2* owed;                              // where the last group's scales are still to be written (null: nowhere)
@@ -274,69 +315,72 @@ struct Loader {
   }
   KB_DEVI void next_batch(const Params& p, int units, int warp, int lane) {
     __syncwarp();
-    Feed<S::GT> f = *feed;
+    Feed<S::GT, S::WK> f = *feed;
     f.n = 0;
     pg2 = -1;
     pending = false;
     while (f.live) {
-      const int mine = f.seg.count > f.first ? (f.seg.count - f.first + S::WK - 1) / S::WK : 0;   // this warp's groups of the segment
+      const bool solo = f.seg.solo >= 0;
+      const int by = solo ? 1 : S::WK;
+      const int mine = f.seg.count > f.first ? (f.seg.count - f.first + by - 1) / by : 0;   // this warp's groups of the segment
       if (f.done < mine) {
         f.n = min(BATCH, mine - f.done);
         f.h = f.seg.h;
-        const int gi = f.first + (f.done + lane / NT) * S::WK;
+        const int gi = f.first + (f.done + lane / NT) * by;
         if (gi < f.seg.count) {
           const int tok = (f.seg.g0 + gi) * S::GT + (lane % NT) * 16;
           if (tok < f.seg.len) pg2 = __ldg(p.table + (int64_t)f.seg.b_of * p.max_pages + (tok >> p.page_log2));
         }
-        f.tok0 = (f.seg.g0 + f.first + f.done * S::WK) * S::GT;
+        f.tok0 = (f.seg.g0 + f.first + f.done * by) * S::GT;
+        f.step = by * S::GT;
         f.done += f.n;
         pending = true;
         break;
       }
-      f.rot = (f.rot + f.seg.count) % S::WK;
-      f.first = warp >= f.rot ? warp - f.rot : warp + S::WK - f.rot;
+      if (!solo) f.rot = (f.rot + f.seg.count) % S::WK;
       f.done = 0;
-      f.live = f.seg.next(p, units, lane);
+      f.live = f.seg.next(p, units, lane, warp);
+      f.first = first_group(f.seg, f.rot, warp);
     }
     __syncwarp();
     if (lane == 0) *feed = f;
     __syncwarp();
   }
-  KB_DEVI void read_scales(const Params& p) {
+  KB_DEVI void read_scales(const Params& p, int lane) {
     sc2 = make_float2(-1.f, 0.f);
     if (pg2 >= 0 && pg2 < p.num_pages) {
       const int64_t i = (int64_t)pg2 * p.H + feed->h;
       sc2.x = __ldg(p.k_scale + i);
       sc2.y = __ldg(p.v_scale + i);
+      const int tok = feed->tok0 + (lane / NT) * feed->step + (lane % NT) * 16;
+      pg2 = (int)i * p.page + (tok & (p.page - 1));   // (below 2^31: the pool's limit)
     } else {
       pg2 = -1;
     }
     pending = false;
   }
-  KB_DEVI Loader(Feed<S::GT>* at, const Params& p, int units, int warp, int lane) : feed(at), n(0), pos(0), owed(nullptr) {
+  KB_DEVI Loader(Feed<S::GT, S::WK>* at, const Params& p, int units, int warp, int lane) : feed(at), n(0), pos(0), owed(nullptr) {
     next_batch(p, units, warp, lane);
   }
   // The next group into `slot`; always one cp.async group, empty when the work is over.
   KB_DEVI void load(const Params& p, int units, int warp, int lane, typename Smem<D, NT>::Slot& slot, float2* scale) {
     if (pos == n) {
       pay(lane);
-      if (pending) read_scales(p);
-      h = feed->h; n = feed->n; tok0 = feed->tok0;
-      pg = pg2; sc = sc2;
+      if (pending) read_scales(p, lane);
+      n = feed->n;
+      row = pg2; sc = sc2;
       pos = 0;
       if (n) next_batch(p, units, warp, lane);
     } else if (pending) {
-      read_scales(p);
+      read_scales(p, lane);
     }
     float2* now = nullptr;
     if (n) {
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        const int page = __shfl_sync(0xffffffffu, pg, pos * NT + j);
-        if (page >= 0) {
-          const int tok = tok0 + pos * (S::WK * S::GT) + j * 16;
-          const int64_t row = ((int64_t)page * p.H + h) * p.page + (tok & (p.page - 1));
-          const uint8_t *ks = p.k_pages + row * D + lane * 16, *vs = p.v_pages + row * D + lane * 16;
+        const int from = __shfl_sync(0xffffffffu, row, pos * NT + j);
+        if (from >= 0) {
+          const uint8_t *ks = p.k_pages + (int64_t)from * D + lane * 16, *vs = p.v_pages + (int64_t)from * D + lane * 16;
           constexpr int RPI = 512 / D;       // rows that the warp's 32 chunks cover
 #pragma unroll
           for (int i = 0; i < 16 / RPI; ++i) {
@@ -379,7 +423,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
     if (lane == 0) {
       sm.total = sum;
       if ((int64_t)blockIdx.x * sh.per < sh.total)
-        sm.start.start(p, blockIdx.x * sh.per, min((blockIdx.x + 1) * sh.per, sh.total), b, begin);
+        sm.start.start(p, blockIdx.x * sh.per, min((blockIdx.x + 1) * sh.per, sh.total), sh.per, b, begin);
     }
   }
   __syncthreads();
@@ -392,22 +436,23 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
   // Every warp walks the CTA's segments in the same order.  Group i of a segment goes to
   // warp (i + rot) % WK, so that short segments use all of them in turn.
   {
-    Feed<GT> f{};
+    Feed<GT, WK> f{};
     f.seg = sm.start;
     if (lane == 0) sm.walk[warp] = f.seg;
-    f.first = warp;
-    f.live = f.seg.next(p, (int)units, lane);
+    f.live = f.seg.next(p, (int)units, lane, warp);
+    f.first = first_group(f.seg, 0, warp);
     if (lane == 0) sm.feed[warp] = f;
   }
   Loader<D, NT> loader(&sm.feed[warp], p, (int)units, warp, lane);
   for (int s = 0; s < STAGES; ++s) loader.load(p, (int)units, warp, lane, sm.slot[warp][s], sm.scale[warp][s]);
-  Walk<GT> seg;
+  Walk<GT, WK> seg;
   auto next_segment = [&]() {              // the using side's walk, in shared memory too
     __syncwarp();
     seg = sm.walk[warp];
-    const bool more = seg.next(p, (int)units, lane);
+    const bool more = seg.next(p, (int)units, lane, warp);
     __syncwarp();
     if (lane == 0) sm.walk[warp] = seg;
+    __syncwarp();
     return more;
   };
   int rot = 0;
@@ -434,10 +479,11 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
   bool live = next_segment();
   if (live) load_q();
   while (live) {
-    const int b = seg.b_of, h = seg.h, rb = seg.rb, len = seg.len, g0 = seg.g0, count = seg.count;
-    const bool whole = g0 == 0 && count == seg.ng;
-    const int gi0 = warp >= rot ? warp - rot : warp + WK - rot;   // this warp's first group
-    rot = (rot + count) % WK;
+    const bool solo = seg.solo >= 0;
+    const int len = seg.len, first = first_group(seg, rot, warp), step = (solo ? 1 : WK) * GT;
+    int left = first < seg.count ? solo ? seg.count : (seg.count - first + WK - 1) / WK : 0;   // this warp's groups
+    int base = (seg.g0 + first) * GT;
+    if (!solo) rot = (rot + seg.count) % WK;
 
     // Q^T operands: row n = g of each 8-row tile, this lane's D / 4 channels from t4 * D / 4, as
     // f16 under a power of two per row.
@@ -482,7 +528,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
       for (int c = 0; c < 2; ++c) {
         m[n][c] = -INFINITY;
         l[n][c] = 0.f;
-        const int r = rb * ROWS + n * 8 + 2 * t4 + c;
+        const int r = seg.rb * ROWS + n * 8 + 2 * t4 + c;
         seen[n][c] = r < p.R ? len - p.Sq + 1 + r / p.G : len;
       }
 #pragma unroll
@@ -493,11 +539,10 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
     const int all_seen = len - p.Sq + 1;   // keys below are seen by every row
 
     int held = -1;
-    for (int gi = gi0; gi < count; gi += WK) {
+    for (; left > 0; --left, base += step) {
       cp_async_wait<STAGES - 1>();         // the oldest group has landed, for every lane
       __syncwarp();
       const typename SM::Slot& sl = sm.slot[warp][s];
-      const int base = (g0 + gi) * GT;
       float sk[NT], sv[NT];
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
@@ -665,10 +710,13 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
       else body(std::false_type{});
       __syncwarp();
       // the last slot of the segment is kept: it takes the warp's O
-      if (gi + WK < count) loader.load(p, (int)units, warp, lane, sm.slot[warp][s], sm.scale[warp][s]);
+      if (left > 1 || step == GT) loader.load(p, (int)units, warp, lane, sm.slot[warp][s], sm.scale[warp][s]);
       else held = s;
       s = s + 1 == STAGES ? 0 : s + 1;
     }
+    const Walk<GT, WK> now = sm.walk[warp];      // (the segment again: read back, not kept over the loop)
+    const int b = now.b_of, h = now.h, rb = now.rb, g0 = now.g0;
+    const bool whole = now.count == now.ng;
     // ---- the warps' partial results join: each one's O in the slot it kept
     if (held >= 0) {
       float4* mo = reinterpret_cast<float4*>(&sm.slot[warp][held]);
@@ -690,9 +738,33 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
         }
       }
     }
-    if (lane == 0) sm.held[warp] = held;
+    if (lane == 0 && step != GT) sm.held[warp] = held;
     live = next_segment();
     if (live) load_q();
+    if (step == GT) {
+      // ---- this warp has all of the unit
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float x = l[n][c];
+#pragma unroll
+          for (int w = 4; w < 32; w <<= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
+          const int rr = rb * ROWS + n * 8 + 2 * t4 + c;
+          if (rr >= p.R) continue;
+          const float inv = x > 0.f || x != x ? 1.f / x : 0.f;
+          const int64_t orow = ((int64_t)b * p.Sq + rr / p.G) * p.Hq + h * p.G + rr % p.G;
+          uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<char*>(p.o) + 2 * (orow * D + g * (D / 8)));
+#pragma unroll
+          for (int i = 0; i < MT; i += 4)    // channels g * D/8 + 2 i .. + 7
+            dst[i / 4] = make_uint4(kv::pack16<F16>(o[n][i][c] * inv, o[n][i][2 + c] * inv),
+                                    kv::pack16<F16>(o[n][i + 1][c] * inv, o[n][i + 1][2 + c] * inv),
+                                    kv::pack16<F16>(o[n][i + 2][c] * inv, o[n][i + 2][2 + c] * inv),
+                                    kv::pack16<F16>(o[n][i + 3][c] * inv, o[n][i + 3][2 + c] * inv));
+          if (g == 0 && p.lse) p.lse[orow] = x == 0.f ? -INFINITY : (m[n][c] - SHIFT + log2f(x)) * 0.6931471805599453f;
+        }
+      continue;
+    }
     __syncthreads();
     const int slot = 2 * blockIdx.x + (g0 > 0 ? 0 : 1);   // a share's first segment may end a unit, its last may begin one
     for (int i = tid; i < ROWS * (D / 4); i += WK * 32) {

@@ -99,7 +99,7 @@ def gather(codes, scale, table, starts, counts):
 
 
 def cached(q, k_codes, v_codes, k_scale, v_scale, table, lengths, scale):
-    """q [B, Sq, Hq, D], codes as values -> (o, lse, A)."""
+    """q [B, Sq, Hq, D], codes as values -> (o, lse, A).  Tokens of pages outside the pool are left out."""
     B, Sq, Hq, D = q.shape
     P, H, page, _ = k_codes.shape
     g = Hq // H
@@ -110,10 +110,13 @@ def cached(q, k_codes, v_codes, k_scale, v_scale, table, lengths, scale):
         if m == 0:
             continue
         ids = torch.tensor(table[b][:-(-m // page)], device=q.device)
+        there = ((ids >= 0) & (ids < P)).repeat_interleave(page)[:m]
+        ids = ids.clamp(0, P - 1)
+        before = torch.cat([there.new_zeros(1, dtype=torch.int64), there.cumsum(0)])
         for h in range(H):
-            k, v = ((c[ids, h].double() * s[ids, h].double()[:, None, None]).reshape(-1, D)[:m]
+            k, v = ((c[ids, h].double() * s[ids, h].double()[:, None, None]).reshape(-1, D)[:m][there]
                     for c, s in ((k_codes, k_scale), (v_codes, v_scale)))
-            seen = (m - Sq + 1 + torch.arange(Sq, device=q.device)).repeat_interleave(g)
+            seen = before[(m - Sq + 1 + torch.arange(Sq, device=q.device)).clamp(0, m)].repeat_interleave(g)
             rows = attend(q[b, :, h * g:(h + 1) * g].reshape(Sq * g, D), k, v, seen, scale)
             o[b, :, h * g:(h + 1) * g] = rows[0].view(Sq, g, D)
             lse[b, :, h * g:(h + 1) * g] = rows[1].view(Sq, g)

@@ -186,6 +186,24 @@ def test_cached_many_sequences():
     close_lse(lse, wlse)
 
 
+@pytest.mark.parametrize('heads,H,D,sq,dtype', [(24, 8, 128, 1, torch.bfloat16), (6, 3, 64, 4, torch.float16),
+                                                (48, 12, 64, 8, torch.bfloat16), (12, 4, 128, 6, torch.float16)])
+def test_cached_short_sequences(heads, H, D, sq, dtype):
+    """Many units to a share: short ones, which a warp takes alone, with empty and long ones among them, an odd page
+    count and a page that is not there."""
+    lens = [1 + (i * 37) % 190 for i in range(260)] + [0, 5000, 0, 1] + [100] * 100 + [1111] + [16] * 60 + [0]
+    page = 32
+    cache, table, _ = make_cache(lens, H, D, page, seed=14)
+    table = [list(r) for r in table]
+    table[7][0] = -1
+    q = randn(gen(15), len(lens), sq, heads, D, dtype=dtype)
+    o, lse = attention_cached(q, cache, i32(table), i32(lens), return_lse=True)
+    want, wlse, A = ref.cached(q, values(cache.k_pages), values(cache.v_pages), cache.k_scale, cache.v_scale, table, lens, D ** -0.5)
+    close(o, want, A, dtype, u_p=2.0 ** -11)
+    close_lse(lse, wlse)
+    assert torch.equal(o, attention_cached(q, cache, i32(table), i32(lens)))
+
+
 def test_first_call_captured():
     """A process whose first calls are made while a graph is captured."""
     import subprocess
