@@ -161,16 +161,17 @@ KB_DEVI int o_chunk(int r, int c) {
 }
 
 // The launch shapes.  NT: 8-row tiles of a CTA (rows up to 8: 1, else 2); a group is NT * 16
-// tokens.  WK warps, OCC CTAs per SM: as many warps as the registers allow (at D = 128, 8 rows
-// need under 128 and 16 rows under 168).
+// tokens.  WK warps, OCC CTAs per SM: as many as the registers allow without spilling the loop (16 rows
+// at D = 128 take all 255; with 12 warps of 168, 32 queries of 32 sequences of 4000 tokens took 176 us
+// and not 133).
 template <int D, int NT>
 struct Shape {
   static constexpr int GT = NT * 16, ROWS = NT * 8;
-  static constexpr int WK = D == 128 && NT == 2 ? 12 : 8;
+  static constexpr int WK = 8;
   static constexpr int OCC = D == 128 ? (NT == 1 ? 2 : 1) : (NT == 1 ? 3 : 2);
-  static constexpr int STAGES = D == 128 ? (NT == 1 ? 3 : 2) : (NT == 1 ? 4 : 3);
+  static constexpr int STAGES = D == 64 && NT == 1 ? 4 : 3;
   static constexpr int THREADS = WK * 32;
-  static constexpr int JOIN = ROWS * D / 4 < 256 ? ROWS * D / 4 : 256;   // threads of a joining block
+  static constexpr int JOIN = ROWS * D / 4;  // threads of a joining block: four channels of a row each
 };
 
 // A unit is short if a warp alone should take it.  Spread over the WK = 8 warps it costs ng / 8 groups and
@@ -857,12 +858,11 @@ __global__ void __launch_bounds__(Shape<D, NT>::JOIN) attn_cached_join_kernel(Pa
   // Partials in share order: the part that begins the unit is its CTA's last segment (slot 1),
   // the later ones continue it (slot 0).  A chunk's m and l are read together, then its O with
   // all loads in flight: what the join costs is the two latencies.
-  constexpr int CHUNK = 32, ITEMS = ROWS * (D / 4) / THREADS;
+  constexpr int CHUNK = 32;
   __shared__ float fac[CHUNK][ROWS], run_m[ROWS], run_l[ROWS], scale_old[ROWS];
   const float2* mlp = reinterpret_cast<const float2*>(p.part + (int64_t)2 * ctas * ROWS * D);
-  float4 acc[ITEMS];
-#pragma unroll
-  for (int i = 0; i < ITEMS; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int r = threadIdx.x / (D / 4), c = threadIdx.x % (D / 4), rr = rb * ROWS + r;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   if (threadIdx.x < ROWS) {
     run_m[threadIdx.x] = -INFINITY;
     run_l[threadIdx.x] = 0.f;
@@ -872,17 +872,12 @@ __global__ void __launch_bounds__(Shape<D, NT>::JOIN) attn_cached_join_kernel(Pa
     const int n = min(CHUNK, c1 + 1 - k0);
     // the first parts' O is on its way while the factors are formed
     constexpr int EARLY = 8;
-    float4 first[ITEMS][EARLY];
-    auto part_of = [&](int k, int r, int c) {
+    float4 first[EARLY];
+    auto part_of = [&](int k) {
       return reinterpret_cast<const float4*>(p.part + ((2 * (int64_t)(k0 + k) + (k0 + k == c0 ? 1 : 0)) * ROWS + r) * D + c * 4);
     };
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-      const int r = (threadIdx.x + i * THREADS) / (D / 4), c = (threadIdx.x + i * THREADS) % (D / 4);
-#pragma unroll
-      for (int k = 0; k < EARLY; ++k)
-        first[i][k] = k < n && rb * ROWS + r < p.R ? __ldcg(part_of(k, r, c)) : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
+    for (int k = 0; k < EARLY; ++k) first[k] = k < n && rr < p.R ? __ldcg(part_of(k)) : make_float4(0.f, 0.f, 0.f, 0.f);
     // a warp per row, a lane per part: the parts' factors, and that of what is joined so far
     for (int r = threadIdx.x >> 5; r < ROWS; r += THREADS / 32) {
       float2 x = make_float2(-INFINITY, 0.f);
@@ -900,40 +895,33 @@ __global__ void __launch_bounds__(Shape<D, NT>::JOIN) attn_cached_join_kernel(Pa
       }
     }
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-      const int r = (threadIdx.x + i * THREADS) / (D / 4), c = (threadIdx.x + i * THREADS) % (D / 4);
-      if (rb * ROWS + r >= p.R) continue;
+    if (rr < p.R) {
       const float f0 = scale_old[r];
-      acc[i].x *= f0; acc[i].y *= f0; acc[i].z *= f0; acc[i].w *= f0;
+      acc.x *= f0; acc.y *= f0; acc.z *= f0; acc.w *= f0;
 #pragma unroll
       for (int k = 0; k < EARLY; ++k)
         if (k < n) {
           const float f = fac[k][r];
-          const float4 x = first[i][k];
-          acc[i].x += x.x * f; acc[i].y += x.y * f; acc[i].z += x.z * f; acc[i].w += x.w * f;
+          const float4 x = first[k];
+          acc.x += x.x * f; acc.y += x.y * f; acc.z += x.z * f; acc.w += x.w * f;
         }
 #pragma unroll 8
       for (int k = EARLY; k < n; ++k) {
         const float f = fac[k][r];
-        const float4 x = __ldcg(part_of(k, r, c));
-        acc[i].x += x.x * f; acc[i].y += x.y * f; acc[i].z += x.z * f; acc[i].w += x.w * f;
+        const float4 x = __ldcg(part_of(k));
+        acc.x += x.x * f; acc.y += x.y * f; acc.z += x.z * f; acc.w += x.w * f;
       }
     }
     __syncthreads();
   }
-#pragma unroll
-  for (int i = 0; i < ITEMS; ++i) {
-    const int r = (threadIdx.x + i * THREADS) / (D / 4), c = (threadIdx.x + i * THREADS) % (D / 4), rr = rb * ROWS + r;
-    if (rr >= p.R) continue;
-    const float l = run_l[r], inv = l > 0.f || l != l ? 1.f / l : 0.f;
-    const int64_t orow = ((int64_t)b * p.Sq + rr / p.G) * p.Hq + h * p.G + rr % p.G;
-    uint2 w;
-    w.x = kv::pack16<F16>(acc[i].x * inv, acc[i].y * inv);
-    w.y = kv::pack16<F16>(acc[i].z * inv, acc[i].w * inv);
-    *reinterpret_cast<uint2*>(reinterpret_cast<char*>(p.o) + 2 * (orow * D + c * 4)) = w;
-    if (c == 0 && p.lse) p.lse[orow] = l == 0.f ? -INFINITY : (run_m[r] - SHIFT + log2f(l)) * 0.6931471805599453f;
-  }
+  if (rr >= p.R) return;
+  const float l = run_l[r], inv = l > 0.f || l != l ? 1.f / l : 0.f;
+  const int64_t orow = ((int64_t)b * p.Sq + rr / p.G) * p.Hq + h * p.G + rr % p.G;
+  uint2 w;
+  w.x = kv::pack16<F16>(acc.x * inv, acc.y * inv);
+  w.y = kv::pack16<F16>(acc.z * inv, acc.w * inv);
+  *reinterpret_cast<uint2*>(reinterpret_cast<char*>(p.o) + 2 * (orow * D + c * 4)) = w;
+  if (c == 0 && p.lse) p.lse[orow] = l == 0.f ? -INFINITY : (run_m[r] - SHIFT + log2f(l)) * 0.6931471805599453f;
 }
 
 // 8-row tiles that a CTA takes of the R = Sq * Hq / Hkv rows: rows above 16 form blocks that
