@@ -879,19 +879,19 @@ __global__ void __launch_bounds__(Shape<D, NT>::JOIN) attn_cached_join_kernel(Pa
 #pragma unroll
     for (int k = 0; k < EARLY; ++k) first[k] = k < n && rr < p.R ? __ldcg(part_of(k)) : make_float4(0.f, 0.f, 0.f, 0.f);
     // a warp per row, a lane per part: the parts' factors, and that of what is joined so far
-    for (int r = threadIdx.x >> 5; r < ROWS; r += THREADS / 32) {
+    for (int w = threadIdx.x >> 5; w < ROWS; w += THREADS / 32) {
       float2 x = make_float2(-INFINITY, 0.f);
-      if (lane < n) x = __ldcg(mlp + (2 * (int64_t)(k0 + lane) + (k0 + lane == c0 ? 1 : 0)) * ROWS + r);
-      const float before = run_m[r], mx = fmaxf(before, warp_max(x.x));
+      if (lane < n) x = __ldcg(mlp + (2 * (int64_t)(k0 + lane) + (k0 + lane == c0 ? 1 : 0)) * ROWS + w);
+      const float before = run_m[w], mx = fmaxf(before, warp_max(x.x));
       // (m = -inf: no visible key, O and l are 0, or all of its scores are NaN, and so are they)
       const float f = x.x == -INFINITY ? 1.f : ex2(x.x - mx), f0 = before == -INFINITY ? 1.f : ex2(before - mx);
-      const float l = warp_sum(f * x.y) + run_l[r] * f0;
-      fac[lane][r] = f;
+      const float l = warp_sum(f * x.y) + run_l[w] * f0;
+      fac[lane][w] = f;
       __syncwarp();
       if (lane == 0) {
-        scale_old[r] = f0;
-        run_m[r] = mx;
-        run_l[r] = l;
+        scale_old[w] = f0;
+        run_m[w] = mx;
+        run_l[w] = l;
       }
     }
     __syncthreads();

@@ -183,7 +183,11 @@ __global__ void __launch_bounds__(256) kv_gather_kernel(GatherParams p) {
     int b = b0;
 #pragma unroll
     for (int j = 0; j < 32; ++j) b += __shfl_sync(0xffffffffu, next, j) <= i ? 1 : 0;
-    while (b - b0 >= 32 && b + 1 < p.B && p.cu[b + 1] <= i) ++b;   // (more of them: empty ones)
+    if (b - b0 >= 32)                // (more of them: empty ones)
+      for (int end = p.B; end - b > 1;) {
+        const int mid = b + (end - b) / 2;
+        if (p.cu[mid] <= i) b = mid; else end = mid;
+      }
     int64_t r = -1;
     int pg = 0;
     if (i < p.T && i < p.cu[p.B] && i >= p.cu[0]) {
