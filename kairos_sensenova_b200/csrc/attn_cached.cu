@@ -27,6 +27,9 @@
 //   O^T += V^T P^T, P transposed between the two by movmatrix.  The products of 16
 //                tokens are formed from zero and added times their page's V scale in
 //                fp32, so scales of any spread keep full precision.
+// Measured: 96 sequences of 2900 tokens, 24/24 heads of 128: 288 us, 5.9 TB/s; 131072 + 100001 tokens, 32/8
+// heads: 92 us, 5.2 TB/s; 64 rows (8 queries, 96/12 heads) of 28957 tokens: 82 us, bound by the issue slots of
+// its four row blocks.
 // bf16 queries are multiplied by a power of two per row into f16's range first (exact
 // but for elements 2^-29 below the row's largest).  P is rounded to f16 (2^-12).
 #include <math.h>

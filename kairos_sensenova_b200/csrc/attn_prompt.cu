@@ -6,6 +6,9 @@
 // Bound: the tensor pipe and the exponentials together.  A tile of 256 rows x 128 keys is
 // 4 * 256 * 128 * D flops (2048 cycles at D = 128) and 32768 exponentials (2048 cycles of MUFU).
 //
+// Measured: 16380 tokens, 24/24 heads of 128: 1.3-1.5 ms, 1.1-1.27 PFLOP/s as the clock goes; 8192 tokens of
+// 24/8 heads 341 us with the tensor pipe active 70 % of the time.
+//
 // Rows.  The G = Hq / Hkv heads that share a kv head are rows of one matrix: a query tile of 128
 // rows holds T = 128 / G tokens (rounded down) with G heads each, row = token * G + head, so a
 // CTA reads each key tile once for all of them, and short prompts still fill the tile.  That is a
