@@ -179,6 +179,7 @@ struct Maps {
 };
 
 constexpr int TABLE = 128;                   // shares: at most this many row tiles
+constexpr int SHORT = 8;                     // whole items: one of fewer key tiles is short
 constexpr int PAD = 3;                       // shares: what an item costs besides its key tiles, in key tiles
 // shares: at least this many key tiles (450 queries over 2365 keys, 4/1 heads of 128: 28.7 us, with eight 34.8;
 // 606 keys and 4339 of 4/4 heads: 38 and 39)
@@ -204,16 +205,16 @@ struct Smem {
   uint8_t q[QT][ATOMS][BM * 128];
   uint8_t k[KS][ATOMS][BN * 128];
   uint8_t v[VS][ATOMS][BN * 128];
-  uint64_t item_full, item_free;             // an item is published / every warp has read it
+  uint64_t item_full[2], item_free[2];       // an item is published / every warp has read it
   uint64_t answered;
   uint64_t q_full, q_free;
   uint64_t k_full[KS], k_empty[KS], v_full[VS], v_empty[VS];
   uint64_t s_full[QT], s_free[QT], p_full[QT], pv_done[QT], drain[2];
   alignas(16) uint4 answer[2];
-  Item item;
+  Item item[2];
   Table table;
   uint32_t tmem_base;
-  int took[3];                               // whole items: the last ones this CTA took
+  int took[4];                               // whole items: the last ones this CTA took
   int abort_flag, keep_tmem;
 };
 
@@ -444,8 +445,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
         tc::mbar_init(&sm.pv_done[i], 1);
         tc::mbar_init(&sm.drain[i], 1);
       }
-      tc::mbar_init(&sm.item_full, 1);
-      tc::mbar_init(&sm.item_free, 11);
+      for (int i = 0; i < 2; ++i) {
+        tc::mbar_init(&sm.item_full[i], 1);
+        tc::mbar_init(&sm.item_free[i], 11);
+      }
       tc::mbar_init(&sm.answered, 1);
       tc::mbar_init(&sm.q_full, 1);
       tc::mbar_init(&sm.q_free, 1);
@@ -457,7 +460,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
         tc::mbar_init(&sm.v_full[s], 1);
         tc::mbar_init(&sm.v_empty[s], 1);
       }
-      sm.took[0] = sm.took[1] = sm.took[2] = -1;
+      sm.took[0] = sm.took[1] = sm.took[2] = sm.took[3] = -1;
       sm.abort_flag = 0;
       sm.keep_tmem = 0;
       tc::fence_barrier_init();
@@ -477,14 +480,14 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
 
   // Item number `c` of the CTA; false: no more (or its wait gave up).
   auto get_item = [&](int c, Item& it, bool& ok) {
-    ok = __all_sync(0xffffffffu, tc::mbar_wait(&sm.item_full, c & 1));
+    ok = __all_sync(0xffffffffu, tc::mbar_wait(&sm.item_full[c & 1], (c >> 1) & 1));
     if (!ok) {
       sm.abort_flag = 1;
       return false;
     }
-    it = sm.item;
+    it = sm.item[c & 1];
     __syncwarp();
-    if (lane == 0) tc::mbar_arrive(&sm.item_free);
+    if (lane == 0) tc::mbar_arrive(&sm.item_free[c & 1]);
     return it.slot != -2;
   };
 
@@ -527,9 +530,13 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
       Items items;
       items.start(p, sm.table, lane);
       int uses = 0, asked = 0, block = blockIdx.x;           // of the Q tile; take-overs; the CTA whose item is next
+      bool ahead = false;
       for (int c = 0; ok; ++c) {
-        // (the next item is taken when every warp has this one: not earlier than it is needed)
-        if (c > 0) ok = __all_sync(0xffffffffu, tc::mbar_wait(&sm.item_free, (c - 1) & 1));
+        // The next item is taken when every warp has the last one, not earlier than it is needed; or, if that
+        // one is short, when every warp has the one before, so that it is there in time (64 sequences of
+        // 200 tokens, 24/8 heads: 76.9 us, 78.6 without; 512 + 300 queries over 12345 + 8000 keys, in shares: 134 and 136).
+        if (c > 1) ok = __all_sync(0xffffffffu, tc::mbar_wait(&sm.item_free[c & 1], ((c >> 1) - 1) & 1));
+        if (ok && c > 0 && !ahead) ok = __all_sync(0xffffffffu, tc::mbar_wait(&sm.item_free[(c - 1) & 1], ((c - 1) >> 1) & 1));
         for (bool own = c == 0; ok; own = false) {
           if (!own && !p.split) {
             if (lane == 0) {
@@ -551,11 +558,12 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
         }
         if (!ok) break;
         if (lane == 0) {
-          sm.took[c % 3] = block;
-          sm.item = it;
-          tc::mbar_arrive(&sm.item_full);
+          sm.took[c & 3] = block;
+          sm.item[c & 1] = it;
+          tc::mbar_arrive(&sm.item_full[c & 1]);
         }
         __syncwarp();
+        ahead = p.split || it.j1 - it.j0 < SHORT;
         if (it.slot == -2) break;
         if (it.j1 <= it.j0) continue;
         if (uses > 0) ok = __all_sync(0xffffffffu, tc::mbar_wait(&sm.q_free, (uses - 1) & 1));
@@ -825,8 +833,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
   if (sm.abort_flag && warp == 0) {                          // a wait gave up: no result is better than a wrong one
     Items items;
     items.start(p, sm.table, lane);
-    // all of its shares, or the whole items that it may not have finished: the last three it took
-    for (int c = 0; p.split || c < 3; ++c) {
+    // all of its shares, or the whole items that it may not have finished: the last four it took
+    for (int c = 0; p.split || c < 4; ++c) {
       const Item it = items.next(p, sm.table, p.split ? 0 : sm.took[c], lane);
       if (it.slot < -1) {
         if (p.split) break;
