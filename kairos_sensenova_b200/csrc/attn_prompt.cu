@@ -812,7 +812,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
         }
       }
       if (p.lse && live) p.lse[gt * p.Hq + head] = l == 0.f ? -INFINITY : (mref - SHIFT + log2f(l)) * 0.6931471805599453f;
+      // (a row's lane has stored it, and other lanes store it again: the votes and shuffles order no memory)
       uint32_t again = __ballot_sync(0xffffffffu, live && !finite && l == l);
+      __syncwarp();
       while (again) {
         const int i = __ffs(again) - 1;
         again &= again - 1;
