@@ -41,12 +41,15 @@
 // TAU (log2 units), so P <= 2^(SHIFT + TAU) (inside f16) and most tiles rescale nothing.
 // P is rounded to the input type (half a step, as the output is); l sums the unrounded P.
 //
-// Keys that a row does not see score -inf, so their P is 0.  V rows behind the sequence are
-// zeroed in shared memory before the product.  A NaN or an infinity in V at a key that a
-// row must not see still reaches it as 0 * NaN: so for a row whose O is not finite (and whose l
-// is: a NaN among its own scores makes all of it NaN) the keys that its last tiles hide from it
-// are looked at, and if V is not finite there the row is computed again, by its warp, over its
-// visible keys alone.
+// Keys that a row does not see score -inf, so their P is 0.  V rows behind the last that a row of the
+// item sees are left out of the product, or zeroed in shared memory before it.  A NaN or an infinity in
+// V at a key that a row must not see would still reach it as 0 * NaN.  So the warp that issues PV
+// looks over the V rows that are hidden from some row of a query tile (as many as it has tokens, in
+// the item's last tiles), in shared memory, while it waits for P: what is not finite there is zeroed
+// and its keys are noted, and at the item's end the rows that see such a key add its V, as it is in
+// memory, to O.  (The look costs 84.4 -> 87.7 us for 6696 tokens in prompts of 1 to 2600, 24/8 heads of
+// 128, since the products leave few of shared memory's cycles; done by the softmax warps, by the
+// producer or from global memory it cost 88 to 93.)
 //
 // Every wait is bounded.  A warp whose wait gives up stops, so that the others' waits give up
 // too; what is in flight is drained, and the CTA writes NaN into all of its rows.
@@ -105,64 +108,23 @@ KB_DEVI int2 seq_range(const int32_t* cu, int s, int64_t T) {
 }
 
 template <bool F16>
-KB_DEVI float load16(const void* base, int64_t i) {
-  if constexpr (F16) return __half2float(reinterpret_cast<const __half*>(base)[i]);
-  else return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(base)[i]);
-}
-template <bool F16>
 KB_DEVI void store16(void* base, int64_t i, float x) {
   if constexpr (F16) reinterpret_cast<__half*>(base)[i] = __float2half_rn(x);
   else reinterpret_cast<__nv_bfloat16*>(base)[i] = __float2bfloat16_rn(x);
 }
 
-// Whether V of kv head `hk` is not finite somewhere at the keys [from, to), by one warp.
-template <int D, bool F16>
-KB_DEVI bool not_finite_v(const Params& p, int hk, int64_t from, int64_t to, int lane) {
-  float worst = 0.f;
-  for (int64_t j = from; j < to; ++j)
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c) worst = fmaf(load16<F16>(p.v, j * p.v_ts + hk * p.v_hs + c * 32 + lane), 0.f, worst);
-  return __any_sync(0xffffffffu, worst != 0.f);
+// 0 if the 16-bit pairs looked at so far are all finite: 0 * x is NaN for the others, and stays.
+template <bool F16>
+KB_DEVI uint32_t not_finite(uint32_t x, uint32_t so_far) {
+  if constexpr (F16) asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(so_far) : "r"(x), "r"(0u));
+  else asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(so_far) : "r"(x), "r"(0u));
+  return so_far;
 }
-
-// Query token `tq` of head `h`, which sees the keys [k0, k0 + seen), by one warp.
-template <int D, bool F16>
-KB_DEVI void attend_row(const Params& p, int64_t tq, int h, int64_t k0, int64_t seen, int lane) {
-  constexpr int C = D / 32;
-  const int hk = h / (p.G * p.parts);
-  float q[C], acc[C];
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    q[c] = load16<F16>(p.q, tq * p.q_ts + h * p.q_hs + c * 32 + lane) * (p.flip ? -p.scale_log2 : p.scale_log2);
-    acc[c] = 0.f;
-  }
-  float m = -INFINITY, l = 0.f;
-  for (int64_t j = 0; j < seen; ++j) {
-    float s = 0.f;
-#pragma unroll
-    for (int c = 0; c < C; ++c) s = fmaf(q[c], load16<F16>(p.k, (k0 + j) * p.k_ts + hk * p.k_hs + c * 32 + lane), s);
-    s = warp_sum(s);
-    const float mn = fmaxf(m, s);
-    if (mn > m) {
-      const float a = ex2(m - mn);
-      l *= a;
-#pragma unroll
-      for (int c = 0; c < C; ++c) acc[c] *= a;
-      m = mn;
-    }
-    const float e = s == -INFINITY ? 0.f : ex2(s - m);
-    l += e;
-#pragma unroll
-    for (int c = 0; c < C; ++c) acc[c] = fmaf(e, load16<F16>(p.v, (k0 + j) * p.v_ts + hk * p.v_hs + c * 32 + lane), acc[c]);
-    bool settled = true;                                     // NaN in every channel stays so
-#pragma unroll
-    for (int c = 0; c < C; ++c) settled &= acc[c] != acc[c];
-    if (__all_sync(0xffffffffu, settled)) break;
-  }
-  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-#pragma unroll
-  for (int c = 0; c < C; ++c) store16<F16>(p.o, tq * p.o_ts + h * p.o_hs + c * 32 + lane, acc[c] * inv);
-  if (lane == 0 && p.lse) p.lse[tq * p.Hq + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+// The halves of a 16-bit pair that are not finite, as ones.
+template <bool F16>
+KB_DEVI uint32_t odd_halves(uint32_t x) {
+  constexpr uint32_t INF = F16 ? 0x7c00u : 0x7f80u;
+  return ((x & INF) == INF ? 0xffffu : 0u) | ((x >> 16 & INF) == INF ? 0xffff0000u : 0u);
 }
 
 constexpr int BM = 128, BN = 128, QT = 2, ROWS = QT * BM;
@@ -216,7 +178,62 @@ struct Smem {
   uint32_t tmem_base;
   int took[4];                               // whole items: the last ones this CTA took
   int abort_flag, keep_tmem;
+  // Keys with a V that is not finite, from the first that some row of the item does not see on (a row sees fewer than
+  // ROWS of these); the items with keys take the two in turn.
+  uint32_t odd[2][ROWS / 32];
+  int any_odd[2];
 };
+
+// What is not finite in the rows [r0, r1) of a V tile in shared memory becomes 0, by one warp; row r is key r + key0
+// of those that `odd` marks (`clear`: it has none yet).  (The two functions are not inlined: they are hardly ever
+// called, and in line their code alone cost 5 % of a packed batch's time.)
+template <int D, bool F16>
+__device__ __noinline__ void take_out(uint4* v, int r0, int r1, int key0, uint32_t* odd, bool clear, int lane) {
+  if (clear && lane < ROWS / 32) odd[lane] = 0;
+  __syncwarp();
+  for (int r = r0; r < r1; ++r) {            // (a row is 8 chunks of each atom: its channels, in some order)
+    bool mine = false;
+    if (lane < D / 8) {
+      uint4& x = v[(lane >> 3) * BN * 8 + r * 8 + (lane & 7)];
+      const uint4 z = make_uint4(odd_halves<F16>(x.x), odd_halves<F16>(x.y), odd_halves<F16>(x.z), odd_halves<F16>(x.w));
+      mine = (z.x | z.y | z.z | z.w) != 0;
+      if (mine) x = make_uint4(x.x & ~z.x, x.y & ~z.y, x.z & ~z.z, x.w & ~z.w);
+    }
+    const int k = r + key0;
+    if (__any_sync(0xffffffffu, mine) && lane == 0 && k < ROWS) odd[k >> 5] |= 1u << (k & 31);
+  }
+  tc::fence_proxy_async_smem();
+  __syncwarp();
+}
+// Adds to the O of each lane's row, in TMEM, what was taken out at the first `keys` keys of those that `odd` marks.
+template <int D, bool F16>
+__device__ __noinline__ void put_back(uint32_t tO, const char* v, int64_t v_bytes, int keys, const uint32_t* odd) {
+#pragma unroll 1
+  for (int i = 0; i < D / 32; ++i) {
+    uint32_t o[32];
+    tc::tmem_ld32(tO + i * 32, o);
+    tc::tmem_wait_ld();
+#pragma unroll 1
+    for (int k = 0; k < keys; ++k) {
+      if (!(odd[k >> 5] >> (k & 31) & 1)) continue;
+      const uint4* src = reinterpret_cast<const uint4*>(v + k * v_bytes + i * 64);
+#pragma unroll
+      for (int z = 0; z < 4; ++z) {
+        const uint4 x = __ldg(src + z);
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = kv::unpack16<F16>(w[e] & odd_halves<F16>(w[e]));
+          o[8 * z + 2 * e] = __float_as_uint(__uint_as_float(o[8 * z + 2 * e]) + f.x);
+          o[8 * z + 2 * e + 1] = __float_as_uint(__uint_as_float(o[8 * z + 2 * e + 1]) + f.y);
+        }
+      }
+    }
+    __syncwarp();
+    tc::tmem_st32(tO + i * 32, o);
+  }
+  tc::tmem_wait_st();
+}
 
 // Keys that query `t` of n sees, of m.
 KB_DEVI int seen_by(const Params& p, int64_t t, int n, int m) {
@@ -442,7 +459,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
         tc::mbar_init(&sm.s_full[i], 1);
         tc::mbar_init(&sm.s_free[i], 4);
         tc::mbar_init(&sm.p_full[i], 4);
-        tc::mbar_init(&sm.pv_done[i], 1);
+        tc::mbar_init(&sm.pv_done[i], 2);
         tc::mbar_init(&sm.drain[i], 1);
       }
       for (int i = 0; i < 2; ++i) {
@@ -631,33 +648,65 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
       } else {
         constexpr uint32_t IDESC_PV = tc::idesc_f32acc(F16 ? 0 : 1, BM, D, 0, 1);
         const uint64_t dv0 = tc::sdesc_sw128_mnmajor(sm.v[0][0], BN * 128);
+        int uses = 0;                                        // items with keys so far
         for (int c = 0; get_item(c, it, ok); ++c) {
+          // the first key that some row does not see; the first that no row of tile 0 sees, that none sees
+          const int hidden = seen_by(p, it.tile * QT * p.tq, it.n, it.m);
+          const int beyond0 = seen_by(p, min(it.n, it.tile * QT * p.tq + p.tq) - 1, it.n, it.m);
+          const int beyond = seen_by(p, min((int64_t)it.n, (int64_t)(it.tile + 1) * QT * p.tq) - 1, it.n, it.m);
+          bool odd = false;                                  // V is not finite somewhere from there on
           for (int j = it.j0; ok && j < it.j1; ++j, ++g) {
             const int slot = g % VS;
             ok = wait(&sm.v_full[slot], (g / VS) & 1);
-            if (ok && (j + 1) * BN > it.m) {                 // the sequence ends in this tile
-              uint4* v = reinterpret_cast<uint4*>(sm.v[slot][0]);
+            if (!ok) break;
+            uint4* v = reinterpret_cast<uint4*>(sm.v[slot][0]);
+            const int r0 = max(hidden - j * BN, 0), r1 = min(beyond - j * BN, BN), steps1 = (r1 + 15) / 16;
+            // (at least one, so that O_0 begins from zero)
+            const int steps0 = min(max((beyond0 - j * BN + 15) / 16, 1), steps1), mid = min(max(steps0 * 16, r0), r1);
+            if (r1 < steps1 * 16) {                          // (the product takes the keys by 16)
               for (int a = 0; a < ATOMS; ++a)
-                for (int i = (it.m - j * BN) * 8 + lane; i < BN * 8; i += 32) v[a * BN * 8 + i] = make_uint4(0, 0, 0, 0);
+                for (int i = r1 * 8 + lane; i < steps1 * 128; i += 32) v[a * BN * 8 + i] = make_uint4(0, 0, 0, 0);
               tc::fence_proxy_async_smem();
               __syncwarp();
             }
+            if (j == it.j0 && lane == 0) sm.any_odd[uses & 1] = 0;   // (two items on, this warp has had the P of the item
+                                                             // between, and so every softmax warp has read it)
             const uint64_t dv = dv0 + (uint64_t)(slot * ATOMS) * ATOM;
             for (int t = 0; ok && t < QT; ++t) {             // O_t += P_t V_j, 16 keys per instruction
+              const int from = t == 0 ? r0 : mid, to = t == 0 ? mid : r1, steps = t == 0 ? steps0 : steps1;
+              if (from < to) {                               // is V finite at the keys that some row of the tile does not see?
+                uint32_t x0 = 0, x1 = 0, x2 = 0, x3 = 0;
+                for (int a = 0; a < ATOMS; ++a)
+#pragma unroll 4
+                  for (int i = from * 8 + lane; i < to * 8; i += 32) {
+                    const uint4 x = v[a * BN * 8 + i];
+                    x0 = not_finite<F16>(x.x, x0); x1 = not_finite<F16>(x.y, x1);
+                    x2 = not_finite<F16>(x.z, x2); x3 = not_finite<F16>(x.w, x3);
+                  }
+                if (__any_sync(0xffffffffu, ((x0 | x1 | x2 | x3) & 0x7fff7fffu) != 0)) {
+                  take_out<D, F16>(v, from, to, j * BN - hidden, sm.odd[uses & 1], !odd, lane);
+                  odd = true;
+                  if (lane == 0) sm.any_odd[uses & 1] = 1;
+                }
+              }
               // (the softmax publishes an item's first P_t when it has read the O_t before)
               ok = wait(&sm.p_full[t], g & 1);
               if (ok && leader) {
 #pragma unroll
-                for (int ks = 0; ks < BN / 16; ++ks)
+                for (int ks = 0; ks < BN / 16; ++ks) {
+                  if (ks == steps) break;
                   tc::mma_bf16_ts(tmem_u + TM_O + t * 128, tmem_u + TM_P + t * 64 + ks * 8, dv + ks * (16 * 128 / 16), IDESC_PV,
                                   (j > it.j0 || ks > 0) ? 1u : 0u);
+                }
                 tc::tc_commit(&sm.pv_done[t]);
                 if (t == 1) tc::tc_commit(&sm.v_empty[slot]);
               }
               __syncwarp();
+              if (ok && lane == 0) tc::mbar_arrive(&sm.pv_done[t]);   // (counted too: it releases any_odd and odd)
             }
           }
           if (!ok) break;
+          uses += it.j1 > it.j0;
         }
       }
       if (!ok) sm.abort_flag = 1;
@@ -679,14 +728,14 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
     const uint32_t lane_off = (uint32_t)(w4 * 32) << 16;
     const uint32_t tS = tmem + TM_S + lane_off, tO = tmem + TM_O + qt * 128 + lane_off, tP = tmem + TM_P + qt * 64 + lane_off;
     const float sl2 = p.scale_log2;
-    int g = 0;                                               // key tiles so far
+    int g = 0, uses = 0;                                     // key tiles, and items with keys, so far
     bool ok = true;
     Item it;
     for (int c = 0; get_item(c, it, ok); ++c) {
       const int tok = it.tile * QT * p.tq + dt;              // in the sequence
       const bool live = in_tile && tok < it.n;
       const int lim = live ? seen_by(p, tok, it.n, it.m) : 0x7fffffff;   // keys that the row sees
-      const int full = seen_by(p, it.tile * QT * p.tq, it.n, it.m) / BN;   // key tiles below are seen fully by every row
+      const int hidden = seen_by(p, it.tile * QT * p.tq, it.n, it.m);    // the first key that some row does not see
       float mref = -INFINITY, l = 0.f;
       for (int j = it.j0; j < it.j1; ++j, ++g) {
         ok = __all_sync(0xffffffffu, tc::mbar_wait(&sm.s_full[qt], g & 1));
@@ -697,7 +746,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
         for (int i = 0; i < 4; ++i) tc::tmem_ld32(tS + i * 32, s + i * 32);
         tc::tmem_wait_ld();
         warp_arrive(&sm.s_free[qt], lane);
-        if (j >= full) {
+        if (j >= hidden / BN) {                              // (the tiles below are seen fully by every row)
           const int end = lim - j * BN;
 #pragma unroll
           for (int c0 = 0; c0 < BN; c0 += 32)
@@ -766,6 +815,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
       if (ok && any) ok = __all_sync(0xffffffffu, tc::mbar_wait(&sm.pv_done[qt], (g - 1) & 1));
       if (!ok) break;
       tc::tc_fence_after();
+      if (any && sm.any_odd[uses & 1]) {                     // V that was taken out of the product: added where the row sees it
+        const char* v = reinterpret_cast<const char*>(p.v) + 2 * (((int64_t)it.k0 + hidden) * p.v_ts + (it.hk / p.parts) * p.v_hs);
+        put_back<D, F16>(tO, v, 2 * p.v_ts, live ? lim - hidden : 0, sm.odd[uses & 1]);
+      }
+      uses += any;
       if (it.slot >= 0) {                                    // a partial: O and l under this row's m
         float* dst = p.part + ((int64_t)it.slot * ROWS + r) * D;
 #pragma unroll
@@ -784,7 +838,6 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
       const int64_t gt = (int64_t)it.q0 + tok;
       const int head = it.hk * p.G + hg;
       char* orow = reinterpret_cast<char*>(p.o) + 2 * (gt * p.o_ts + head * p.o_hs);
-      bool finite = true;
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) {
         uint32_t o[32];
@@ -795,10 +848,6 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = 0;
         }
-        float worst = 0.f;                                   // NaN if some value is not finite
-#pragma unroll
-        for (int e = 0; e < 32; ++e) worst = fmaf(__uint_as_float(o[e]), 0.f, worst);
-        finite &= worst == 0.f;
         if (live) {
 #pragma unroll
           for (int z = 0; z < 4; ++z) {
@@ -812,17 +861,6 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
         }
       }
       if (p.lse && live) p.lse[gt * p.Hq + head] = l == 0.f ? -INFINITY : (mref - SHIFT + log2f(l)) * 0.6931471805599453f;
-      // (a row's lane has stored it, and other lanes store it again: the votes and shuffles order no memory)
-      uint32_t again = __ballot_sync(0xffffffffu, live && !finite && l == l);
-      __syncwarp();
-      while (again) {
-        const int i = __ffs(again) - 1;
-        again &= again - 1;
-        const int ti = __shfl_sync(0xffffffffu, tok, i), hi = __shfl_sync(0xffffffffu, head, i);
-        const int seen = seen_by(p, ti, it.n, it.m);
-        if (not_finite_v<D, F16>(p, it.hk / p.parts, (int64_t)it.k0 + seen, (int64_t)it.k0 + min(it.m, it.j1 * BN), lane))
-          attend_row<D, F16>(p, it.q0 + ti, hi, it.k0, seen, lane);
-      }
     }
     if (!ok) sm.abort_flag = 1;
   }
@@ -876,8 +914,8 @@ __global__ void __launch_bounds__(256) attn_prompt_join_kernel(Params p, int cta
   const int c0 = (int)(begin / per), c1 = (int)((begin + all - 1) / per);
   if (c0 == c1) return;                                      // finished there
   const int seq = tb.seq[f], tile = tb.tile[f];
-  const int2 q = seq_range(p.cu_q, seq, p.Tq), k = seq_range(p.cu_k, seq, p.Tk);
-  const int n = q.y - q.x, m = k.y - k.x;
+  const int2 q = seq_range(p.cu_q, seq, p.Tq);
+  const int n = q.y - q.x;
   constexpr int V = D / 32;                                  // channels of a lane
   const float* mlp = p.part + (int64_t)2 * ctas * ROWS * D;
   for (int r = blockIdx.y * 32 + warp; r < blockIdx.y * 32 + 32; r += 8) {
@@ -905,15 +943,6 @@ __global__ void __launch_bounds__(256) attn_prompt_join_kernel(Params p, int cta
       mx = mn;
     }
     const int64_t gt = (int64_t)q.x + tok;
-    float worst = 0.f;
-#pragma unroll
-    for (int v = 0; v < V; ++v) worst = fmaf(acc[v], 0.f, worst);
-    const int seen = seen_by(p, tok, n, m);
-    if (__any_sync(0xffffffffu, worst != 0.f) && l == l &&
-        not_finite_v<D, F16>(p, hk / p.parts, (int64_t)k.x + seen, (int64_t)k.x + min(m, all * BN), lane)) {
-      attend_row<D, F16>(p, gt, head, k.x, seen, lane);
-      continue;
-    }
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
     char* orow = reinterpret_cast<char*>(p.o) + 2 * (gt * p.o_ts + head * p.o_hs + lane * V);
     if constexpr (V == 4)

@@ -143,6 +143,46 @@ def test_prompt_nan_everywhere_and_no_keys(keys):
     assert (o == 0).all() and (lse == -math.inf).all()
 
 
+def milliseconds(f, n=5):
+    """The median of n calls, after three."""
+    times = []
+    for i in range(n + 3):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        f()
+        b.record()
+        b.synchronize()
+        times.append(a.elapsed_time(b))
+    return sorted(times[3:])[n // 2]
+
+
+@pytest.mark.parametrize('nq,nk,heads,kv,dim,dtype', [
+    ([3000], [3000], 24, 24, 128, torch.bfloat16),            # whole items of 256 tokens
+    ([1000, 1, 333], [1500, 700, 300], 24, 8, 64, torch.float16),   # 84 tokens; more keys than queries, and fewer
+    ([90] * 3, [90] * 3, 300, 1, 64, torch.bfloat16),         # the heads of a kv head in three parts
+    ([200, 40], [9000, 2100], 6, 2, 128, torch.float16),      # key tiles in shares
+])
+def test_prompt_hidden_values_at_many_keys(nq, nk, heads, kv, dim, dtype):
+    """V not finite at the newest keys, some channels of one kv head and all of another: infinities of both signs and NaN reach the
+    rows that see them, no other, and do not slow the call down by more than the tiles at the diagonal."""
+    g = gen(41)
+    q, k, v = randn(g, sum(nq), heads, dim, dtype=dtype), randn(g, sum(nk), kv, dim, dtype=dtype), randn(g, sum(nk), kv, dim, dtype=dtype)
+    bad = v.clone()
+    for end, n in zip(cu(nk)[1:], nk):
+        bad[end - 1, 0] = math.nan
+        for back, ch, x in ((3, 5, math.inf), (3, 6, -math.inf), (40, 5, math.inf), (41, 6, math.inf), (70, 7, -math.inf)):
+            if back < n:
+                bad[end - back, kv - 1, ch] = x
+    cq, ck = i32(cu(nq)), i32(cu(nk))
+    o, lse = attention_prompt(q, k, bad, cq, ck, return_lse=True)
+    want, wlse, A = ref.prompt(q, k, bad, cu(nq), cu(nk), dim ** -0.5)
+    assert not torch.isfinite(want).all()
+    close(o, want, A, dtype)
+    close_lse(lse, wlse)
+    clean = milliseconds(lambda: attention_prompt(q, k, v, cq, ck))
+    assert milliseconds(lambda: attention_prompt(q, k, bad, cq, ck)) <= 2 * clean + 0.2
+
+
 @pytest.mark.parametrize('heads,kv,dim,dtype', [(32, 8, 128, torch.bfloat16), (10, 2, 64, torch.float16), (2, 1, 128, torch.float16)])
 def test_prompt_shared_out(heads, kv, dim, dtype):
     """Few rows and many keys: the key tiles go to all SMs in shares, sequences of other lengths and empty ones among them."""
