@@ -514,7 +514,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
     bool ok = true;
     if (warp == 8) {
       // ---------------------------------------------------------- TMA producer
-      int g = 0;                                             // key tiles so far: ring positions
+      int g = 0, ks = 0, vs = 0;                             // key tiles so far: ring positions; K and V tiles loaded
       for (int c = 0; get_item(c, it, ok); ++c) {
         for (int j = it.j0; ok && j < it.j1; ++j, ++g) {
           const int sk = g % KS, sv = g % VS, tok = it.k0 + j * BN;
@@ -524,23 +524,23 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
             tc::mbar_expect_tx(&sm.k_full[sk], ATOMS * BN * 128);
             for (int a = 0; a < ATOMS; ++a) tc::tma_load_3d(sm.k[sk][a], &maps.k, &sm.k_full[sk], a * 64, it.hk / p.parts, tok);
           }
+          ++ks;
           if (g >= VS) ok = __all_sync(0xffffffffu, tc::mbar_wait(&sm.v_empty[sv], (g / VS - 1) & 1));
-          if (!ok) {                                         // (K of this tile is under way, V is not)
-            ok = tc::mbar_wait(&sm.k_full[sk], (g / KS) & 1) && false;
-            break;
-          }
+          if (!ok) break;                                    // (K of this tile is under way, V is not)
           if (lane == 0) {
             tc::mbar_expect_tx(&sm.v_full[sv], ATOMS * BN * 128);
             for (int a = 0; a < ATOMS; ++a) tc::tma_load_3d(sm.v[sv][a], &maps.v, &sm.v_full[sv], a * 64, it.hk / p.parts, tok);
           }
+          ++vs;
         }
         if (!ok) break;
       }
       if (!ok) sm.abort_flag = 1;
-      // before the CTA may exit, every load must have landed
+      // before the CTA may exit, every load must have landed (of each slot the last one: a wait for an earlier phase
+      // would take the phase after for it)
       bool drained = true;
-      for (int i = g > KS ? g - KS : 0; i < g; ++i) drained &= tc::mbar_wait(&sm.k_full[i % KS], (i / KS) & 1);
-      for (int i = g > VS ? g - VS : 0; i < g; ++i) drained &= tc::mbar_wait(&sm.v_full[i % VS], (i / VS) & 1);
+      for (int i = max(ks - KS, 0); i < ks; ++i) drained &= tc::mbar_wait(&sm.k_full[i % KS], (i / KS) & 1);
+      for (int i = max(vs - VS, 0); i < vs; ++i) drained &= tc::mbar_wait(&sm.v_full[i % VS], (i / VS) & 1);
       if (!drained) { sm.abort_flag = 1; sm.keep_tmem = 1; }
     } else if (warp == 11) {
       // ---------------------------------------------------------- items, and their Q
