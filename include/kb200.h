@@ -250,6 +250,9 @@ typedef struct KB200PromptArgs {
   int dtype;
   void* workspace;            /* 16-byte aligned, or NULL (below)                 */
   size_t workspace_bytes;
+  int* status;                /* device word, or NULL: becomes the site of a wait that gave up (kb200_read_error_word);
+                               * the rows that were not finished are NaN then, in o and lse */
+  int64_t wait_clocks;        /* bound of each device-side wait in SM clocks, up to 4e9; 0: 4e9 */
 } KB200PromptArgs;
 /* Bytes with which few queries over many keys are shared out over all SMs; 0 where that
  * is of no use.  Without a workspace the result is the same, slower in those cases. */

@@ -66,11 +66,12 @@ class PromptArgs(ctypes.Structure):
         ('o_token_stride', ctypes.c_int64), ('o_head_stride', ctypes.c_int64),
         ('softmax_scale', ctypes.c_float), ('causal', ctypes.c_int), ('dtype', ctypes.c_int),
         ('workspace', ctypes.c_void_p), ('workspace_bytes', ctypes.c_size_t),
+        ('status', ctypes.c_void_p), ('wait_clocks', ctypes.c_int64),
     ]
 
 
 # the same bytes packed directly (a ctypes structure of this many fields costs several times as much to fill)
-PROMPT_ARGS = struct.Struct('@7P14qfiiPN')
+PROMPT_ARGS = struct.Struct('@7P14qfiiPNPq')
 assert PROMPT_ARGS.size == ctypes.sizeof(PromptArgs)
 
 

@@ -122,7 +122,8 @@ def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     query does not see never reach it, NaN and infinities included.  Returns ``[Tq, Hq, D]``
     (``out``: to write into, apart from the inputs; rows behind the last sequence are left as they
     were); with ``return_lse`` also the fp32 log of the softmax sum ``[Tq, Hq]``.  ``check=True``
-    looks at the offsets on the host first (it synchronises) and raises ``ValueError``."""
+    looks at the offsets on the host first (it synchronises) and raises ``ValueError``, and ``RuntimeError`` if a device-side
+    wait gave up (without it such rows are NaN)."""
     what = 'attention_prompt'
     index = q.get_device()
     if index < 0:
@@ -164,9 +165,12 @@ def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     lse = torch.empty((Tq, Hq), device=q.device, dtype=torch.float32) if return_lse else None
     nbytes = _prompt_workspace(index, Tq, Tk, N, Hq, Hkv, D)
     ws = cu_q.new_empty(nbytes >> 2) if nbytes else None
+    status = cu_q.new_zeros(1) if check else None
     args = _lib.PROMPT_ARGS.pack(
         qp, kp, vp, op, lse.data_ptr() if return_lse else 0, cu_q.data_ptr(), cu_k.data_ptr(), Tq, Tk, N, Hq, Hkv, D,
         qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1], D ** -0.5 if softmax_scale is None else softmax_scale,
-        1 if causal else 0, dtype, ws.data_ptr() if nbytes else 0, nbytes)
+        1 if causal else 0, dtype, ws.data_ptr() if nbytes else 0, nbytes, status.data_ptr() if check else 0, 0)
     _launch(index, what, _lib.lib().kb200_attn_prompt_fwd, args)
+    if check:
+        _launch(index, what, _lib.lib().kb200_read_error_word, status.data_ptr())
     return (out, lse) if return_lse else out

@@ -52,7 +52,8 @@
 // producer or from global memory it cost 88 to 93.)
 //
 // Every wait is bounded.  A warp whose wait gives up stops, so that the others' waits give up
-// too; what is in flight is drained, and the CTA writes NaN into all of its rows.
+// too; what is in flight is drained, the status word is set, and the CTA writes NaN into the outputs, o and lse, of
+// the items that it has taken and not finished.
 #include <math.h>
 #include <string.h>
 #include "kb200_internal.h"
@@ -76,6 +77,8 @@ struct Params {
   int split;               // equal shares of the key tiles (else whole items)
   float* part;             // shares: [2 CTAs][rows][D] partial O, then [2 CTAs][rows][2] (m, l)
   int causal;
+  int* status;             // set when a wait gives up, or null
+  long long wait_clocks;   // BOUNDED: bound of a wait
 };
 
 KB_DEVI float ex2(float x) {
@@ -130,6 +133,7 @@ KB_DEVI uint32_t odd_halves(uint32_t x) {
 constexpr int BM = 128, BN = 128, QT = 2, ROWS = QT * BM;
 constexpr float SHIFT = 6.f, TAU = 8.f;      // P = 2^(s - m + SHIFT) <= 2^14
 constexpr int THREADS = 12 * 32;
+constexpr int SITE = 50;                     // of a wait that gives up, in the status word
 // Registers: the launch gives each thread 168 (its 384 threads share the SM's 65536); the softmax
 // warpgroups take 208 and the third leaves itself 88, 2 * 208 + 88 = 3 * 168.
 constexpr int REGS_SOFTMAX = 208, REGS_OTHERS = 88;
@@ -176,7 +180,8 @@ struct Smem {
   Item item[2];
   Table table;
   uint32_t tmem_base;
-  int took[4];                               // whole items: the last ones this CTA took
+  int took[4], taken;                        // whole items: the CTAs whose items this one took last, and how many
+  int done[8];                               // items that each softmax warp has finished
   int abort_flag, keep_tmem;
   // Keys with a V that is not finite, from the first that some row of the item does not see on (a row sees fewer than
   // ROWS of these); the items with keys take the two in turn.
@@ -445,7 +450,8 @@ KB_DEVI void warp_arrive(uint64_t* bar, int lane) {
 // 2 of 8 was fastest for D = 128: 170, 161, 156, 165 and 166 us for two pieces of prompts).
 constexpr int POLY = 0x88;
 
-template <int D, bool F16>
+// (BOUNDED: with the caller's bound of a wait, instead of 4e9 clocks)
+template <int D, bool F16, bool BOUNDED>
 __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_constant__ Maps maps, Params p) {
   using SM = Smem<D>;
   constexpr int KS = SM::KS, VS = SM::VS, ATOMS = SM::ATOMS;
@@ -477,7 +483,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
         tc::mbar_init(&sm.v_full[s], 1);
         tc::mbar_init(&sm.v_empty[s], 1);
       }
-      sm.took[0] = sm.took[1] = sm.took[2] = sm.took[3] = -1;
+      sm.taken = 0;
+      for (int i = 0; i < 8; ++i) sm.done[i] = 0;
       sm.abort_flag = 0;
       sm.keep_tmem = 0;
       tc::fence_barrier_init();
@@ -495,9 +502,14 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
   const uint32_t tmem = sm.tmem_base;
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");   // the join, if any: it waits for this grid's end
 
+  auto wait_for = [&](uint64_t* bar, uint32_t parity) { 
+    // (a thread suspended in try_wait looks at no clock: short bounds need the polling loop)
+    if constexpr (BOUNDED) return tc::mbar_test_wait_loop(bar, parity, p.wait_clocks);
+    else return tc::mbar_wait(bar, parity);
+  };
   // Item number `c` of the CTA; false: no more (or its wait gave up).
   auto get_item = [&](int c, Item& it, bool& ok) {
-    ok = __all_sync(0xffffffffu, tc::mbar_wait(&sm.item_full[c & 1], (c >> 1) & 1));
+    ok = __all_sync(0xffffffffu, wait_for(&sm.item_full[c & 1], (c >> 1) & 1));
     if (!ok) {
       sm.abort_flag = 1;
       return false;
@@ -518,14 +530,14 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
       for (int c = 0; get_item(c, it, ok); ++c) {
         for (int j = it.j0; ok && j < it.j1; ++j, ++g) {
           const int sk = g % KS, sv = g % VS, tok = it.k0 + j * BN;
-          if (g >= KS) ok = __all_sync(0xffffffffu, tc::mbar_wait(&sm.k_empty[sk], (g / KS - 1) & 1));
+          if (g >= KS) ok = __all_sync(0xffffffffu, wait_for(&sm.k_empty[sk], (g / KS - 1) & 1));
           if (!ok) break;
           if (lane == 0) {
             tc::mbar_expect_tx(&sm.k_full[sk], ATOMS * BN * 128);
             for (int a = 0; a < ATOMS; ++a) tc::tma_load_3d(sm.k[sk][a], &maps.k, &sm.k_full[sk], a * 64, it.hk / p.parts, tok);
           }
           ++ks;
-          if (g >= VS) ok = __all_sync(0xffffffffu, tc::mbar_wait(&sm.v_empty[sv], (g / VS - 1) & 1));
+          if (g >= VS) ok = __all_sync(0xffffffffu, wait_for(&sm.v_empty[sv], (g / VS - 1) & 1));
           if (!ok) break;                                    // (K of this tile is under way, V is not)
           if (lane == 0) {
             tc::mbar_expect_tx(&sm.v_full[sv], ATOMS * BN * 128);
@@ -552,8 +564,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
         // The next item is taken when every warp has the last one, not earlier than it is needed; or, if that
         // one is short, when every warp has the one before, so that it is there in time (64 sequences of
         // 200 tokens, 24/8 heads: 76.9 us, 78.6 without; 512 + 300 queries over 12345 + 8000 keys, in shares: 134 and 136).
-        if (c > 1) ok = __all_sync(0xffffffffu, tc::mbar_wait(&sm.item_free[c & 1], ((c >> 1) - 1) & 1));
-        if (ok && c > 0 && !ahead) ok = __all_sync(0xffffffffu, tc::mbar_wait(&sm.item_free[(c - 1) & 1], ((c - 1) >> 1) & 1));
+        if (c > 1) ok = __all_sync(0xffffffffu, wait_for(&sm.item_free[c & 1], ((c >> 1) - 1) & 1));
+        if (ok && c > 0 && !ahead) ok = __all_sync(0xffffffffu, wait_for(&sm.item_free[(c - 1) & 1], ((c - 1) >> 1) & 1));
         for (bool own = c == 0; ok; own = false) {
           if (!own && !p.split) {
             if (lane == 0) {
@@ -562,13 +574,20 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
               take_over_ask(&sm.answer[asked & 1], &sm.answered);
             }
             __syncwarp();
-            ok = __all_sync(0xffffffffu, tc::mbar_wait(&sm.answered, asked & 1));
-            if (!ok) {
+            ok = __all_sync(0xffffffffu, wait_for(&sm.answered, asked & 1));
+            if (!ok && !__all_sync(0xffffffffu, tc::mbar_wait(&sm.answered, asked & 1))) {   // it must land before the exit
               sm.keep_tmem = 1;
               break;
             }
             block = take_over_answer(&sm.answer[asked & 1]);
             ++asked;
+            if (!ok) {                                       // (an item that this CTA has taken and will not finish)
+              if (lane == 0) {
+                sm.took[c & 3] = block;
+                sm.taken = c + 1;
+              }
+              break;
+            }
           }
           it = items.next(p, sm.table, block, lane);
           if (it.slot != -3) break;
@@ -576,6 +595,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
         if (!ok) break;
         if (lane == 0) {
           sm.took[c & 3] = block;
+          sm.taken = c + 1;
           sm.item[c & 1] = it;
           tc::mbar_arrive(&sm.item_full[c & 1]);
         }
@@ -583,7 +603,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
         ahead = p.split || it.j1 - it.j0 < SHORT;
         if (it.slot == -2) break;
         if (it.j1 <= it.j0) continue;
-        if (uses > 0) ok = __all_sync(0xffffffffu, tc::mbar_wait(&sm.q_free, (uses - 1) & 1));
+        if (uses > 0) ok = __all_sync(0xffffffffu, wait_for(&sm.q_free, (uses - 1) & 1));
         if (!ok) break;
         ++uses;
         if (lane == 0) {                                     // (tokens behind the sequence: rows that are not stored)
@@ -606,7 +626,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
       constexpr uint64_t ATOM = BN * 128 / 16;               // descriptor units between 64-channel atoms
       const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
       auto wait = [&](uint64_t* bar, uint32_t parity) {
-        const bool w = __all_sync(0xffffffffu, tc::mbar_wait(bar, parity));
+        const bool w = __all_sync(0xffffffffu, wait_for(bar, parity));
         tc::tc_fence_after();
         return w;
       };
@@ -738,7 +758,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
       const int hidden = seen_by(p, it.tile * QT * p.tq, it.n, it.m);    // the first key that some row does not see
       float mref = -INFINITY, l = 0.f;
       for (int j = it.j0; j < it.j1; ++j, ++g) {
-        ok = __all_sync(0xffffffffu, tc::mbar_wait(&sm.s_full[qt], g & 1));
+        ok = __all_sync(0xffffffffu, wait_for(&sm.s_full[qt], g & 1));
         if (!ok) break;
         tc::tc_fence_after();
         uint32_t s[128];
@@ -789,7 +809,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
           }
           if (h == 0) {
             // P_t(j) overwrites P_t(j-1) and O_t may be rescaled: PV_t(j-1) must have completed
-            if (g > 0) ok = __all_sync(0xffffffffu, tc::mbar_wait(&sm.pv_done[qt], (g - 1) & 1));
+            if (g > 0) ok = __all_sync(0xffffffffu, wait_for(&sm.pv_done[qt], (g - 1) & 1));
             tc::tc_fence_after();
           }
           if (ok) tc::tmem_st32(tP + h * 32, pk);
@@ -812,7 +832,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
       }
       // ---- the item's end: O_t of this row
       const bool any = it.j1 > it.j0;
-      if (ok && any) ok = __all_sync(0xffffffffu, tc::mbar_wait(&sm.pv_done[qt], (g - 1) & 1));
+      if (ok && any) ok = __all_sync(0xffffffffu, wait_for(&sm.pv_done[qt], (g - 1) & 1));
       if (!ok) break;
       tc::tc_fence_after();
       if (any && sm.any_odd[uses & 1]) {                     // V that was taken out of the product: added where the row sees it
@@ -832,6 +852,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
         }
         *reinterpret_cast<float2*>(p.part + (int64_t)2 * gridDim.x * ROWS * D + ((int64_t)it.slot * ROWS + r) * 2) =
             make_float2(mref, l);
+        if (lane == 0) sm.done[warp] = c + 1;
         continue;
       }
       const float f = l == 0.f ? 0.f : 1.f / l;
@@ -861,6 +882,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
         }
       }
       if (p.lse && live) p.lse[gt * p.Hq + head] = l == 0.f ? -INFINITY : (mref - SHIFT + log2f(l)) * 0.6931471805599453f;
+      if (lane == 0) sm.done[warp] = c + 1;
     }
     if (!ok) sm.abort_flag = 1;
   }
@@ -871,22 +893,26 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
     tc::tmem_dealloc(tmem, 512);
   }
   if (sm.abort_flag && warp == 0) {                          // a wait gave up: no result is better than a wrong one
+    if (lane == 0 && p.status) atomicCAS(p.status, 0, SITE);
+    int first = sm.done[0];
+    for (int i = 1; i < 8; ++i) first = min(first, sm.done[i]);
     Items items;
     items.start(p, sm.table, lane);
-    // all of its shares, or the whole items that it may not have finished: the last four it took
-    for (int c = 0; p.split || c < 4; ++c) {
-      const Item it = items.next(p, sm.table, p.split ? 0 : sm.took[c], lane);
-      if (it.slot < -1) {
-        if (p.split) break;
-        continue;
-      }
+    // its shares, or the whole items, from the first that some warp has not finished (a warp that takes an item has finished
+    // the one before, and the items are found two ahead: at most four)
+    for (int c = p.split ? 0 : first; p.split || c < sm.taken; ++c) {
+      const Item it = items.next(p, sm.table, p.split ? 0 : sm.took[c & 3], lane);
+      if (it.slot == -2 && p.split) break;
+      if (it.slot < -1 || c < first) continue;
       for (int i = lane; i < ROWS; i += 32) {
         const int row = i % BM, tok = (it.tile * QT + i / BM) * p.tq + row / p.G;
         if (it.slot >= 0) {
-          p.part[(int64_t)2 * gridDim.x * ROWS * D + ((int64_t)it.slot * ROWS + i) * 2 + 1] = NAN;
+          *reinterpret_cast<float2*>(p.part + (int64_t)2 * gridDim.x * ROWS * D + ((int64_t)it.slot * ROWS + i) * 2) = make_float2(0.f, NAN);
         } else if (row < p.tq * p.G && tok < it.n) {
-          for (int d = 0; d < D; ++d)
-            store16<F16>(p.o, (it.q0 + tok) * p.o_ts + (it.hk * p.G + row % p.G) * p.o_hs + d, NAN);
+          const int64_t gt = (int64_t)it.q0 + tok;
+          const int head = it.hk * p.G + row % p.G;
+          for (int d = 0; d < D; ++d) store16<F16>(p.o, gt * p.o_ts + head * p.o_hs + d, NAN);
+          if (p.lse) p.lse[gt * p.Hq + head] = NAN;
         }
       }
     }
@@ -999,11 +1025,13 @@ static bool shares(int64_t Tq, int64_t Tk, int64_t N, int64_t H, const Split& s,
 template <int D, bool F16>
 static int launch(const Maps& maps, const Params& p, int sms, cudaStream_t st) {
   const size_t smem = sizeof(Smem<D>) + 1024;
-  static std::atomic<uint64_t> done{0};
-  if (int e = allow_smem((const void*)attn_prompt_kernel<D, F16>, smem, done)) return e;
+  static std::atomic<uint64_t> done[2];
+  const bool bounded = p.wait_clocks > 0;
+  auto* kern = bounded ? attn_prompt_kernel<D, F16, true> : attn_prompt_kernel<D, F16, false>;
+  if (int e = allow_smem((const void*)kern, smem, done[bounded])) return e;
   const int64_t items = most_tiles(p.Tq, p.N, p.tq) * p.H;
   const int grid = p.split ? sms : (int)items;
-  attn_prompt_kernel<D, F16><<<grid, THREADS, smem, st>>>(maps, p);
+  kern<<<grid, THREADS, smem, st>>>(maps, p);
   if (int e = check_launch("attn_prompt_kernel")) return e;
   if (!p.split) return KB200_OK;
   cudaLaunchAttribute overlap{};
@@ -1053,6 +1081,8 @@ extern "C" int kb200_attn_prompt_fwd(const KB200PromptArgs* a, void* stream) {
   if (prompt::most_tiles(a->Tq, a->N, sp.tq) * a->Hkv * sp.parts > 0x7fffffffLL || a->N * a->Hkv * sp.parts > (1 << 24))
     return set_error(KB200_ERR_INVALID, "attn_prompt: too many rows, or sequences times kv heads");
   if (!(fabsf(a->softmax_scale) < INFINITY)) return set_error(KB200_ERR_INVALID, "attn_prompt: softmax_scale=%f", a->softmax_scale);
+  if (a->wait_clocks < 0 || a->wait_clocks > 4000000000LL)
+    return set_error(KB200_ERR_INVALID, "attn_prompt: wait_clocks=%lld", (long long)a->wait_clocks);
   // a scale of 0 becomes one too small to matter, so that a masked score stays -inf
   const float sl2 = fmaxf(fabsf(a->softmax_scale) * 1.4426950408889634f, 1e-30f);
   const int sms = sm_count();
@@ -1065,7 +1095,7 @@ extern "C" int kb200_attn_prompt_fwd(const KB200PromptArgs* a, void* stream) {
                    a->k_token_stride, a->k_head_stride, a->v_token_stride, a->v_head_stride, a->o_token_stride,
                    a->o_head_stride, a->Tq, a->Tk, (int)a->N, (int)a->Hq, (int)(a->Hkv * sp.parts), (int)sp.g,
                    (int)sp.parts, (int)sp.tq, sl2, a->softmax_scale < 0.f ? 0x80008000u : 0u, split, (float*)a->workspace,
-                   a->causal};
+                   a->causal, a->status, a->wait_clocks};
   prompt::Maps maps;
   memset(&maps, 0, sizeof(maps));
   const int D = (int)a->D;

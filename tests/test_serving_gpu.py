@@ -5,12 +5,13 @@ probabilities (attention_prompt rounds them to the input type, attention_cached 
 |o - ref| <= u_p A + u |ref| + c A, A = sum_j softmax_j |v_j|.  c covers the fp32 chain: a score's error
 is at most D 2^-24 sum_d |q_d k_d| scale <= 128 * 2^-24 * |q| |k| scale, and |q| |k| scale < 32 for the data
 here, so 2 * 128 * 32 * 2^-24 = 2^-11 relative in a probability at the very most; the sums add n 2^-24."""
+import ctypes
 import math
 
 import pytest
 import torch
 
-from kairos_sensenova_b200 import KVCache, attention_cached, attention_prompt, kv_cache_append, kv_cache_gather
+from kairos_sensenova_b200 import KVCache, _lib, attention_cached, attention_prompt, kv_cache_append, kv_cache_gather
 from oracle import serving as ref
 
 pytestmark = pytest.mark.gpu
@@ -181,6 +182,38 @@ def test_prompt_hidden_values_at_many_keys(nq, nk, heads, kv, dim, dtype):
     close_lse(lse, wlse)
     clean = milliseconds(lambda: attention_prompt(q, k, v, cq, ck))
     assert milliseconds(lambda: attention_prompt(q, k, bad, cq, ck)) <= 2 * clean + 0.2
+
+
+@pytest.mark.parametrize('clocks', [1, 2000, 10000, 50000])
+@pytest.mark.parametrize('nq,nk,heads,kv,dim', [([300] * 20 + [40, 0, 1], [300] * 20 + [90, 5, 1], 12, 4, 128),   # whole items
+                                                ([200, 30], [9000, 2100], 6, 2, 64)])                              # shares
+def test_prompt_wait_gives_up(nq, nk, heads, kv, dim, clocks):
+    """Waits of a few clocks run out: the status word says so, and a row is either finished or NaN, in o and in lse."""
+    L = _lib.lib()
+    g = gen(43)
+    q, k, v = randn(g, sum(nq), heads, dim), randn(g, sum(nk), kv, dim), randn(g, sum(nk), kv, dim)
+    cq, ck, status = i32(cu(nq)), i32(cu(nk)), i32([0])
+    o, lse = torch.full_like(q, 5.0), torch.full((sum(nq), heads), 5.0, device='cuda')
+    size = L.kb200_attn_prompt_workspace_size(sum(nq), sum(nk), len(nq), heads, kv, dim)
+    assert (size > 0) == (len(nq) == 2)
+    ws = torch.zeros(max(size, 16), device='cuda', dtype=torch.uint8)
+    a = _lib.PromptArgs(q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), o=o.data_ptr(), lse=lse.data_ptr(), cu_q=cq.data_ptr(),
+                        cu_k=ck.data_ptr(), Tq=sum(nq), Tk=sum(nk), N=len(nq), Hq=heads, Hkv=kv, D=dim, q_token_stride=heads * dim,
+                        q_head_stride=dim, k_token_stride=kv * dim, k_head_stride=dim, v_token_stride=kv * dim, v_head_stride=dim,
+                        o_token_stride=heads * dim, o_head_stride=dim, softmax_scale=dim ** -0.5, causal=1, dtype=0,
+                        workspace=ws.data_ptr() if size else None, workspace_bytes=size, status=status.data_ptr(), wait_clocks=clocks)
+    stream = torch.cuda.current_stream().cuda_stream
+    assert L.kb200_attn_prompt_fwd(ctypes.byref(a), stream) == 0
+    rc = L.kb200_read_error_word(status.data_ptr(), stream)
+    gone = torch.isnan(lse)
+    assert torch.equal(torch.isnan(o).any(-1), gone) and torch.equal(torch.isnan(o).all(-1), gone)
+    assert rc in (0, _lib.ERRORS_BY_NAME['timeout']) and (rc or (clocks > 1 and not gone.any()))
+    want, wlse, A = ref.prompt(q, k, v, cu(nq), cu(nk), dim ** -0.5)
+    close(o[~gone], want[~gone], A[~gone], torch.bfloat16)
+    close_lse(lse[~gone], wlse[~gone])
+    o2, lse2 = attention_prompt(q, k, v, cq, ck, return_lse=True, check=True)     # the device is as it was
+    close(o2, want, A, torch.bfloat16)
+    close_lse(lse2, wlse)
 
 
 @pytest.mark.parametrize('heads,kv,dim,dtype', [(32, 8, 128, torch.bfloat16), (10, 2, 64, torch.float16), (2, 1, 128, torch.float16)])

@@ -128,3 +128,12 @@ def test_oracle_attention_is_the_formula():
     v[4] = float('nan')
     o2 = ref.attend(q, k, v, torch.tensor([0, 2, 5]), 0.5)[0]
     assert torch.equal(o2[:2], o[:2]) and torch.isnan(o2[2]).all()
+
+
+def test_prompt_wait_bound():
+    """The bound of a device-side wait: 0 (the default) to 4e9 clocks."""
+    L = _lib.lib()
+    base = dict(q=16, k=16, v=16, o=16, cu_q=16, cu_k=16, Tq=4, Tk=4, N=1, Hq=4, Hkv=2, D=64, q_token_stride=64, softmax_scale=1.0)
+    for bad in (-1, 4_000_000_001):
+        assert L.kb200_attn_prompt_fwd(ctypes.byref(_lib.PromptArgs(**base, wait_clocks=bad)), None) == 1
+        assert b'wait_clocks' in L.kb200_last_error()
