@@ -38,7 +38,9 @@
 // (32x32b; the 16-lane shapes run at half the rate) and the two kinds of products have
 // an issuer each, so that no QK waits behind a PV's operands.
 // The row maximum is kept lazily: O and l are rescaled only when it grows by more than
-// TAU (log2 units), so P <= 2^(SHIFT + TAU) (inside f16) and most tiles rescale nothing.
+// TAU (log2 units), so P <= 2^(SHIFT + TAU) and most tiles rescale nothing.  In f16 P uses the type's range, up to
+// 2^14 (V is at most 2^16, so O is far from fp32's end); in bf16 it is at most 2^-8, so that O, which is summed
+// before it is divided by l, holds 256 keys with V up to the type's end, and 65536 of equal weight.
 // P is rounded to the input type (half a step, as the output is); l sums the unrounded P.
 //
 // Keys that a row does not see score -inf, so their P is 0.  V rows behind the last that a row of the
@@ -131,7 +133,9 @@ KB_DEVI uint32_t odd_halves(uint32_t x) {
 }
 
 constexpr int BM = 128, BN = 128, QT = 2, ROWS = QT * BM;
-constexpr float SHIFT = 6.f, TAU = 8.f;      // P = 2^(s - m + SHIFT) <= 2^14
+template <bool F16>
+constexpr float SHIFT = F16 ? 6.f : -16.f;   // P = 2^(s - m + SHIFT)
+constexpr float TAU = 8.f;
 constexpr int THREADS = 12 * 32;
 constexpr int SITE = 50;                     // of a wait that gives up, in the status word
 // Registers: the launch gives each thread 168 (its 384 threads share the SM's 65536); the softmax
@@ -793,7 +797,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
           l *= alpha;
         }
         // (no key of the row seen yet: every score here is -inf, and so is x)
-        const float b0 = mref == -INFINITY ? 0.f : SHIFT - mref;
+        const float b0 = mref == -INFINITY ? 0.f : SHIFT<F16> - mref;
         const float2 sc = make_float2(sl2, sl2), bias = make_float2(b0, b0);
         float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
@@ -881,7 +885,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
           }
         }
       }
-      if (p.lse && live) p.lse[gt * p.Hq + head] = l == 0.f ? -INFINITY : (mref - SHIFT + log2f(l)) * 0.6931471805599453f;
+      if (p.lse && live) p.lse[gt * p.Hq + head] = l == 0.f ? -INFINITY : (mref - SHIFT<F16> + log2f(l)) * 0.6931471805599453f;
       if (lane == 0) sm.done[warp] = c + 1;
     }
     if (!ok) sm.abort_flag = 1;
@@ -975,7 +979,7 @@ __global__ void __launch_bounds__(256) attn_prompt_join_kernel(Params p, int cta
       *reinterpret_cast<uint2*>(orow) = make_uint2(kv::pack16<F16>(acc[0] * inv, acc[1] * inv), kv::pack16<F16>(acc[2] * inv, acc[3] * inv));
     else
       *reinterpret_cast<uint32_t*>(orow) = kv::pack16<F16>(acc[0] * inv, acc[1] * inv);
-    if (lane == 0 && p.lse) p.lse[gt * p.Hq + head] = l == 0.f ? -INFINITY : (mx - SHIFT + log2f(l)) * 0.6931471805599453f;
+    if (lane == 0 && p.lse) p.lse[gt * p.Hq + head] = l == 0.f ? -INFINITY : (mx - SHIFT<F16> + log2f(l)) * 0.6931471805599453f;
   }
 }
 

@@ -324,6 +324,25 @@ def test_prompt_extremes():
     assert (o == 0).all()
 
 
+@pytest.mark.parametrize('nq,nk', [([1, 200, 30], [1, 200, 300]), ([60, 2], [9000, 2100])])      # whole items; shares
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
+def test_prompt_largest_values(nq, nk, dtype):
+    """V up to half of the type's largest value at 200 keys, in any channels and in one key that outweighs them, and values of 2^-90
+    (fp16: its smallest) beside them: an output is an average, so none leaves the type."""
+    g = gen(47)
+    q, k, v = (randn(g, n, 2, 128, dtype=dtype) for n in (sum(nq), sum(nk), sum(nk)))
+    top = torch.finfo(dtype).max / 2
+    for end, n in zip(cu(nk)[1:], nk):
+        rows = slice(max(end - 200, end - n), end)
+        v[rows, 0] = (v[rows, 0] / 8).clamp(-1, 1) * top
+        v[end - n:end, 1] *= 2.0 ** -90 if dtype == torch.bfloat16 else 2.0 ** -14
+    o, lse = attention_prompt(q, k, v, i32(cu(nq)), i32(cu(nk)), return_lse=True)
+    want, wlse, A = ref.prompt(q, k, v, cu(nq), cu(nk), 128 ** -0.5)
+    unit = torch.tensor([top, 2.0 ** -90 if dtype == torch.bfloat16 else 1.0], device='cuda', dtype=torch.float64)[:, None]
+    close(o.double() / unit, want / unit, A / unit, dtype)
+    close_lse(lse, wlse)
+
+
 @pytest.mark.parametrize('scale', [-0.3, 0.0, 1e-3, 2.0])
 def test_any_softmax_scale(scale):
     g = gen(13)
