@@ -41,6 +41,10 @@ namespace cached {
 
 constexpr float SHIFT = 8.f;       // P = 2^(s - m + SHIFT), s <= m + TAU: below 2^12, inside f16
 constexpr float TAU = 4.f;         // O and l are rescaled when the maximum grows by more than this (log2 units)
+// V scales are taken times DOWN and O is taken times UP when it is divided by l.  16 tokens' product is at most
+// 16 * 2^12 * 448 < 2^25, so without it O would leave fp32 at scales from 2^103 on, and scales reach 2^120; with it
+// 2^19 tokens at that scale fit.  The smallest scale, 2^-117, becomes fp32's smallest number: sums keep 2^-17.
+constexpr float DOWN = 0x1p-32f, UP = 0x1p32f;
 
 struct Params {
   const void* q;
@@ -355,7 +359,7 @@ struct Loader {
     if (pg2 >= 0 && pg2 < p.num_pages) {
       const int64_t i = (int64_t)pg2 * p.H + feed->h;
       sc2.x = __ldg(p.k_scale + i);
-      sc2.y = __ldg(p.v_scale + i);
+      sc2.y = __ldg(p.v_scale + i) * DOWN;
       const int tok = feed->tok0 + (lane / NT) * feed->step + (lane % NT) * 16;
       pg2 = (int)i * p.page + (tok & (p.page - 1));   // (below 2^31: the pool's limit)
     } else {
@@ -756,7 +760,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
           for (int w = 4; w < 32; w <<= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
           const int rr = rb * ROWS + n * 8 + 2 * t4 + c;
           if (rr >= p.R) continue;
-          const float inv = x > 0.f || x != x ? 1.f / x : 0.f;
+          const float inv = x > 0.f || x != x ? UP / x : 0.f;
           const int64_t orow = ((int64_t)b * p.Sq + rr / p.G) * p.Hq + h * p.G + rr % p.G;
           uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<char*>(p.o) + 2 * (orow * D + g * (D / 8)));
 #pragma unroll
@@ -804,7 +808,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::THREADS, Shape<D, NT>::OCC)
       } else {
         const int rr = rb * ROWS + r;
         if (rr < p.R) {
-          const float inv = ls > 0.f || ls != ls ? 1.f / ls : 0.f;
+          const float inv = ls > 0.f || ls != ls ? UP / ls : 0.f;
           const int64_t orow = ((int64_t)b * p.Sq + rr / p.G) * p.Hq + h * p.G + rr % p.G;
           uint2 w;
           w.x = kv::pack16<F16>(a.x * inv, a.y * inv);
@@ -918,7 +922,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::JOIN) attn_cached_join_kernel(Pa
     __syncthreads();
   }
   if (rr >= p.R) return;
-  const float l = run_l[r], inv = l > 0.f || l != l ? 1.f / l : 0.f;
+  const float l = run_l[r], inv = l > 0.f || l != l ? UP / l : 0.f;
   const int64_t orow = ((int64_t)b * p.Sq + rr / p.G) * p.Hq + h * p.G + rr % p.G;
   uint2 w;
   w.x = kv::pack16<F16>(acc.x * inv, acc.y * inv);

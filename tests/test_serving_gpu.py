@@ -551,6 +551,23 @@ def test_cached_scales_far_apart():
     close(o, want, A, torch.bfloat16, u_p=2.0 ** -11)
 
 
+@pytest.mark.parametrize('lens,sq,heads,H,D,page', [([1, 300, 0, 20], 1, 4, 2, 128, 16), ([5000, 700], 2, 8, 1, 64, 32),
+                                                    ([100] * 700, 1, 4, 2, 64, 64)])
+@pytest.mark.parametrize('exponent', [118, -117])
+def test_cached_largest_and_smallest_values(lens, sq, heads, H, D, page, exponent):
+    """V of the first head up to 448 * 2^118 (the largest bf16 is 1.99 * 448 * 2^118), or under the smallest scale there is: an output
+    is an average, so it is neither infinite nor lost.  (Whole units, joined ones, and short ones of a warp alone.)"""
+    cache, table, _ = make_cache(lens, H, D, page, seed=19)
+    cache.v_scale[:, 0] = 2.0 ** exponent
+    q = randn(gen(20), len(lens), sq, heads, D)
+    o, lse = attention_cached(q, cache, i32(table), i32(lens), return_lse=True)
+    want, wlse, A = ref.cached(q, values(cache.k_pages), values(cache.v_pages), cache.k_scale, cache.v_scale, table, lens, D ** -0.5)
+    unit = torch.ones(heads, 1, device='cuda', dtype=torch.float64)
+    unit[:heads // H] = 2.0 ** exponent
+    close(o.double() / unit, want / unit, A / unit, torch.bfloat16, u_p=2.0 ** -11)
+    close_lse(lse, wlse)
+
+
 def test_cached_hidden_nan_and_missing_pages():
     """A NaN code of the newest token reaches only the queries that see it; a missing page is skipped."""
     lens, H, D, page = [100], 2, 128, 32
