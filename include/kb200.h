@@ -277,7 +277,8 @@ typedef struct KB200KvCache {
  * cu_new[b] .. cu_new[b+1], and the LAST of its lengths[b] tokens (lengths count them
  * already).  A page's scale is the smallest power of two that holds the largest finite
  * magnitude of its tokens within 448; when it grows, the codes already in the page
- * are re-encoded.  NaN and infinities become NaN codes and set no scale.  Pages that
+ * are re-encoded.  NaN and infinities become NaN codes and set no scale; magnitudes over
+ * 1.875 * 2^15 (fp16) or 1.875 * 2^127 (bf16) are stored as that.  Pages that
  * the call writes must belong to one sequence only. */
 typedef struct KB200KvAppendArgs {
   KB200KvCache cache;

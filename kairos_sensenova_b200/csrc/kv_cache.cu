@@ -74,26 +74,33 @@ __global__ void __launch_bounds__(PAGE * D / 32 > 256 ? 512 : 256) kv_append_ker
     const int item = base + grp;
     fetch(item + stride, nx);
     // the largest magnitude, as 16-bit integers in pairs (the order of the magnitudes; NaN and
-    // infinities come out on top, and only if there are some is it done again without them)
-    constexpr uint32_t INF = F16 ? 0x7c00u : 0x7f80u;
+    // infinities come out on top, and only if there are some is it done again without them).  TOP is
+    // the type's largest magnitude of 4 significant bits, 1.875 * 2^15 or 2^127: what is larger would be
+    // rounded to a code whose value the type does not have, and becomes TOP (2^-4 of the value off at
+    // most, the half step of e4m3).
+    constexpr uint32_t INF = F16 ? 0x7c00u : 0x7f80u, TOP = F16 ? 0x7b80u : 0x7f70u;
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       top = __vmaxu2(__vmaxu2(__vmaxu2(top, x[i].x & 0x7fff7fffu), __vmaxu2(x[i].y & 0x7fff7fffu, x[i].z & 0x7fff7fffu)),
                      x[i].w & 0x7fff7fffu);
     uint32_t mag = max(top & 0xffffu, top >> 16);
-    const bool odd = mag >= INF;                         // this thread has a value that is not finite
+    const bool odd = mag > TOP;                          // this thread has a value that is not finite, or behind TOP
     if (odd) {
       mag = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+        uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const uint32_t lo = w[e] & 0x7fffu, hi = (w[e] >> 16) & 0x7fffu;
+          uint32_t lo = w[e] & 0x7fffu, hi = (w[e] >> 16) & 0x7fffu;
+          if (lo > TOP && lo < INF) lo = TOP;
+          if (hi > TOP && hi < INF) hi = TOP;
+          w[e] = (w[e] & 0x80008000u) | hi << 16 | lo;
           if (lo < INF) mag = max(mag, lo);
           if (hi < INF) mag = max(mag, hi);
         }
+        x[i] = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
     const float2 mag2 = unpack16<F16>(mag);

@@ -178,7 +178,8 @@ def kv_cache_append(cache: KVCache, k: torch.Tensor, v: torch.Tensor, page_table
     is left out.  The scale of a page and head is the smallest power of two that holds the
     largest finite magnitude within e4m3's 448; when a later token needs a larger one, the
     codes already there are re-encoded (exact but for subnormals).  NaN and infinities
-    are stored as NaN and set no scale.  The pages a call writes must each belong to one
+    are stored as NaN and set no scale; magnitudes over 1.875 * 2^15 (fp16) or 1.875 * 2^127 (bf16) are stored as that, so
+    that they stay inside the type.  The pages a call writes must each belong to one
     sequence (``check=True`` raises otherwise)."""
     what = 'kv_cache_append'
     index = _cuda_index(what, cache)
@@ -209,7 +210,8 @@ def kv_cache_append(cache: KVCache, k: torch.Tensor, v: torch.Tensor, page_table
 def kv_cache_gather(cache: KVCache, page_table: torch.Tensor, starts: torch.Tensor, cu_seqlens: torch.Tensor, total: int,
                     dtype: torch.dtype = torch.bfloat16, out=None, check: bool = False):
     """Tokens ``starts[b] ..`` of each sequence, ``cu_seqlens[b+1] - cu_seqlens[b]`` of them, as
-    packed ``(k, v)`` ``[total, heads, D]`` in ``dtype`` (bf16: exact).  ``total`` is known to
+    packed ``(k, v)`` ``[total, heads, D]`` in ``dtype`` (bf16: exact; fp16: rounded under 2^-14, infinities past 65504,
+    which tokens appended in fp16 do not reach).  ``total`` is known to
     the host (``cu_seqlens[-1]``, or more: rows behind it are left as they were).  ``out``:
     ``(k, v)`` to write into, contiguous."""
     what = 'kv_cache_gather'

@@ -8,6 +8,8 @@ import math
 import torch
 
 E4M3_MAX, SCALE_EXP_MIN = 448.0, -117
+# the largest value of 4 significant bits in a type: what is larger is stored as this, so that it can be read back
+LARGEST = {torch.float16: 1.875 * 2.0 ** 15, torch.bfloat16: 1.875 * 2.0 ** 127, torch.float32: math.inf, torch.float64: math.inf}
 
 
 def attend(q, k, v, seen, scale):
@@ -78,6 +80,7 @@ def append(codes, scale, x, table, lengths, cu):
             pg, off = table[b][pos // page], pos % page
             cnt = min(page - off, lengths[b] - pos)
             new = x[cu[b] + pos - first: cu[b] + pos - first + cnt].double().transpose(0, 1)   # [H, cnt, D]
+            new = torch.where(torch.isfinite(new), new.clamp(-LARGEST[x.dtype], LARGEST[x.dtype]), new)
             e = scale_exponent(torch.where(torch.isfinite(new), new.abs(), 0.0).amax((1, 2)))
             if off:
                 e_old = torch.frexp(scale[pg].double())[1] - 1

@@ -467,6 +467,27 @@ def test_append_extremes(dtype):
         assert torch.equal(torch.isnan(got), torch.isnan(w)) and torch.equal(got.nan_to_num(), w.nan_to_num()), i
 
 
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
+def test_append_largest(dtype):
+    """Tokens up to the type's end come back finite and within e4m3's half step (2^-4), alone and under a scale that they raise."""
+    H, D, page = 2, 64, 16
+    end = torch.finfo(dtype).max
+    x = torch.tensor([1.0, -0.25, 0.87, 0.9375, -0.953, 0.96875, 0.969, -0.999, 1.0], device='cuda', dtype=torch.float64)
+    x = (x * end).to(dtype)[:, None, None].expand(9, H, D).contiguous()
+    x[:, 1, ::3] /= 64
+    cache, table = KVCache.empty(2, H, D, page), i32([[1]])
+    w, s = values(cache.k_pages), cache.k_scale.clone()
+    for i in range(9):
+        ref.append(w, s, x[i:i + 1], [[1]], [i + 1], [0, 1])
+        kv_cache_append(cache, x[i:i + 1], x[i:i + 1], table, i32([i + 1]), i32([0, 1]))
+        assert torch.equal(cache.k_scale, s) and torch.equal(values(cache.k_pages), w), i
+    for got in kv_cache_gather(cache, table, i32([0]), i32([0, 9]), 9, dtype=dtype):
+        assert torch.isfinite(got).all() and ((got.double() - x.double()).abs() <= 2.0 ** -4 * x.double().abs()).all()
+    o = attention_cached(torch.zeros(1, 1, H, D, device='cuda', dtype=dtype), cache, table, i32([9]))      # the mean
+    mean = (w[1] * s[1].double()[:, None, None])[:, :9].mean(1)
+    assert torch.isfinite(o).all() and ((o[0, 0].double() - mean).abs() <= 2.0 ** -7 * mean.abs().amax()).all()
+
+
 def test_append_leaves_out_what_does_not_fit():
     """Pages outside the pool, lengths over the table row and new tokens over the length: nothing of them is written."""
     cache = KVCache.empty(4, 1, 64, 16)
