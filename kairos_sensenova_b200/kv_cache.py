@@ -37,9 +37,19 @@ class KVCache:
     (``torch.float8_e4m3fn`` or ``uint8`` codes), ``k_scale``, ``v_scale`` ``[num_pages, heads]``
     fp32 powers of two, all contiguous.  A value is ``code * scale``."""
 
-    __slots__ = ('_tensors', '_args', '_shape', '_row', '_device', '_index')
+    __slots__ = ('_tensors', '_at', '_args', '_shape', '_row', '_device', '_index')
 
     def __init__(self, k_pages, v_pages, k_scale, v_scale):
+        self._tensors, self._at = (k_pages, v_pages, k_scale, v_scale), None
+        self._look()
+
+    def _look(self):
+        """Takes the addresses, and all that is checked, from the tensors if they have moved since the last call
+        (``set_``, ``.data =``, a storage that was freed and allocated again)."""
+        k_pages, v_pages, k_scale, v_scale = self._tensors
+        at = (k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
+        if at == self._at:
+            return
         if k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
             raise ValueError(f'KVCache: k_pages and v_pages must share shape [pages, heads, page, D], got '
                              f'{tuple(k_pages.shape)}, {tuple(v_pages.shape)}')
@@ -61,11 +71,13 @@ class KVCache:
                 raise ValueError('KVCache: pages and scales must be on one device')
             if not t.is_contiguous():
                 raise ValueError('KVCache: pages and scales must be contiguous')
-        self._tensors = (k_pages, v_pages, k_scale, v_scale)
+            if k_pages.device.type != 'meta' and \
+                    t.untyped_storage().nbytes() < (t.storage_offset() + t.numel()) * t.element_size():
+                raise ValueError('KVCache: the storage of the pages or scales has been freed')
         self._shape, self._row, self._device = (P, H, page, D), (H, D), k_pages.device
         self._index = k_pages.get_device()              # -1 on the CPU
-        self._args = _lib.KV_CACHE_ARGS.pack(k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-                                             P, H, page, D)
+        self._args = _lib.KV_CACHE_ARGS.pack(*at, P, H, page, D)
+        self._at = at
 
     @classmethod
     def empty(cls, num_pages: int, num_heads: int, head_dim: int, page_size: int = 64, device='cuda'):
@@ -122,6 +134,7 @@ def _refuse_grad(what):
 
 
 def _cuda_index(what, cache):
+    cache._look()
     if cache._index < 0:
         raise RuntimeError(f'{what}: the cache must be on a CUDA device (no CPU path)')
     return cache._index

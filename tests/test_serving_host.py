@@ -137,3 +137,30 @@ def test_prompt_wait_bound():
     for bad in (-1, 4_000_000_001):
         assert L.kb200_attn_prompt_fwd(ctypes.byref(_lib.PromptArgs(**base, wait_clocks=bad)), None) == 1
         assert b'wait_clocks' in L.kb200_last_error()
+
+
+def test_cache_follows_its_tensors():
+    """Addresses are those of the tensors at the call: a storage that is freed is refused, a moved one is followed, one of another
+    layout is checked again."""
+    k, s = torch.zeros(4, 2, 16, 64, dtype=torch.uint8), torch.ones(4, 2)
+    tensors = [k, k.clone(), s, s.clone()]
+    c = KVCache(*tensors)
+    at = lambda: _lib.KV_CACHE_ARGS.unpack(c._args)  # noqa: E731
+    assert at() == (*(t.data_ptr() for t in tensors), 4, 2, 16, 64)
+    tensors[1].set_(torch.zeros(4, 2, 16, 64, dtype=torch.uint8))
+    tensors[2].data = torch.ones(4, 2)
+    c._look()
+    assert at() == (*(t.data_ptr() for t in tensors), 4, 2, 16, 64)
+    size = tensors[0].untyped_storage().nbytes()
+    tensors[0].untyped_storage().resize_(0)
+    x = torch.zeros(4, 2, 64, dtype=torch.bfloat16)
+    for call in (lambda: kv_cache_append(c, x, x, i32([[0]]), i32([4]), i32([0, 4])), lambda: attention_cached(x[None], c, i32([[0]]), i32([4])),
+                 lambda: kv_cache_gather(c, i32([[0]]), i32([0]), i32([0, 4]), 4)):
+        with pytest.raises(ValueError, match='freed'):
+            call()
+    tensors[0].untyped_storage().resize_(size)
+    c._look()
+    assert at()[0] == tensors[0].data_ptr() != 0
+    tensors[3].data = torch.ones(3, 2)
+    with pytest.raises(ValueError, match='scales must be'):
+        c._look()
