@@ -27,7 +27,9 @@ from . import _lib
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 _I32 = torch.int32
-_get_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+# (short ways to the current device and stream; a torch built without CUDA has neither, and needs none)
+_get_device = getattr(torch._C, '_cuda_getDevice', None)
+_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)
 PAGE_SIZES = (16, 32, 64, 128)
 HEAD_DIMS = (64, 128)
 

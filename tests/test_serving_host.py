@@ -164,3 +164,23 @@ def test_cache_follows_its_tensors():
     tensors[3].data = torch.ones(3, 2)
     with pytest.raises(ValueError, match='scales must be'):
         c._look()
+
+
+def test_imports_without_cuda():
+    """The package imports, and its host parts work, on a torch built without CUDA."""
+    import subprocess
+    import sys
+    code = """
+import torch
+for name in ('_cuda_getDevice', '_cuda_getCurrentRawStream'):
+    delattr(torch._C, name)
+from kairos_sensenova_b200 import KVCache, attention_cached
+c = KVCache.empty(3, 2, 64, 16, device='cpu')
+try:
+    attention_cached(torch.zeros(1, 1, 2, 64).bfloat16(), c, torch.zeros(1, 1).int(), torch.zeros(1).int())
+except RuntimeError as e:
+    assert 'CUDA' in str(e)
+    print('refused')
+"""
+    r = subprocess.run([sys.executable, '-c', code], capture_output=True, text=True, timeout=200)
+    assert r.returncode == 0 and 'refused' in r.stdout, r.stderr[-2000:]
