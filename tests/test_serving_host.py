@@ -172,6 +172,7 @@ def test_imports_without_cuda():
     import sys
     code = """
 import torch
+import torch._dynamo            # (torch's own modules of a build with CUDA take these names too)
 for name in ('_cuda_getDevice', '_cuda_getCurrentRawStream'):
     delattr(torch._C, name)
 from kairos_sensenova_b200 import KVCache, attention_cached
