@@ -39,19 +39,21 @@ class KVCache:
     (``torch.float8_e4m3fn`` or ``uint8`` codes), ``k_scale``, ``v_scale`` ``[num_pages, heads]``
     fp32 powers of two, all contiguous.  A value is ``code * scale``."""
 
-    __slots__ = ('_tensors', '_at', '_args', '_shape', '_row', '_device', '_index')
+    __slots__ = ('_tensors', '_pointers', '_at', '_args', '_shape', '_row', '_device', '_index')
 
     def __init__(self, k_pages, v_pages, k_scale, v_scale):
         self._tensors, self._at = (k_pages, v_pages, k_scale, v_scale), None
+        self._pointers = k_pages.data_ptr, v_pages.data_ptr, k_scale.data_ptr, v_scale.data_ptr
         self._look()
 
     def _look(self):
         """Takes the addresses, and all that is checked, from the tensors if they have moved since the last call
-        (``set_``, ``.data =``, a storage that was freed and allocated again)."""
-        k_pages, v_pages, k_scale, v_scale = self._tensors
-        at = (k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
+        (``set_``, ``.data =``, a storage that was freed and allocated again); returns the device's index."""
+        k, v, ks, vs = self._pointers
+        at = (k(), v(), ks(), vs())
         if at == self._at:
-            return
+            return self._index
+        k_pages, v_pages, k_scale, v_scale = self._tensors
         if k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
             raise ValueError(f'KVCache: k_pages and v_pages must share shape [pages, heads, page, D], got '
                              f'{tuple(k_pages.shape)}, {tuple(v_pages.shape)}')
@@ -73,13 +75,14 @@ class KVCache:
                 raise ValueError('KVCache: pages and scales must be on one device')
             if not t.is_contiguous():
                 raise ValueError('KVCache: pages and scales must be contiguous')
-            if k_pages.device.type != 'meta' and \
-                    t.untyped_storage().nbytes() < (t.storage_offset() + t.numel()) * t.element_size():
+            # (3 us for the four: when they have moved, not for a new cache)
+            if self._at and t.untyped_storage().nbytes() < (t.storage_offset() + t.numel()) * t.element_size():
                 raise ValueError('KVCache: the storage of the pages or scales has been freed')
         self._shape, self._row, self._device = (P, H, page, D), (H, D), k_pages.device
         self._index = k_pages.get_device()              # -1 on the CPU
         self._args = _lib.KV_CACHE_ARGS.pack(*at, P, H, page, D)
         self._at = at
+        return self._index
 
     @classmethod
     def empty(cls, num_pages: int, num_heads: int, head_dim: int, page_size: int = 64, device='cuda'):
@@ -135,11 +138,8 @@ def _refuse_grad(what):
     raise NotImplementedError(f'kairos_sensenova_b200.{what} is forward-only')
 
 
-def _cuda_index(what, cache):
-    cache._look()
-    if cache._index < 0:
-        raise RuntimeError(f'{what}: the cache must be on a CUDA device (no CPU path)')
-    return cache._index
+def _refuse_cpu(what):
+    raise RuntimeError(f'{what}: the cache must be on a CUDA device (no CPU path)')
 
 
 def _launch(index, what, fn, args):
@@ -197,7 +197,9 @@ def kv_cache_append(cache: KVCache, k: torch.Tensor, v: torch.Tensor, page_table
     that they stay inside the type.  The pages a call writes must each belong to one
     sequence (``check=True`` raises otherwise)."""
     what = 'kv_cache_append'
-    index = _cuda_index(what, cache)
+    index = cache._look()
+    if index < 0:
+        _refuse_cpu(what)
     shape, kd = k.shape, k.dtype
     if len(shape) != 3 or shape[1:] != cache._row or v.shape != shape:
         raise ValueError(f'{what}: k and v must be {["T", *cache._row]}, got {tuple(k.shape)}, {tuple(v.shape)}')
@@ -230,7 +232,9 @@ def kv_cache_gather(cache: KVCache, page_table: torch.Tensor, starts: torch.Tens
     the host (``cu_seqlens[-1]``, or more: rows behind it are left as they were).  ``out``:
     ``(k, v)`` to write into, contiguous."""
     what = 'kv_cache_gather'
-    index = _cuda_index(what, cache)
+    index = cache._look()
+    if index < 0:
+        _refuse_cpu(what)
     code = _DTYPES.get(dtype)
     if code is None:
         raise ValueError(f'{what}: dtype must be bfloat16 or float16, got {dtype}')
@@ -279,7 +283,9 @@ def attention_cached(q: torch.Tensor, cache: KVCache, page_table: torch.Tensor, 
     q's type (``out``: contiguous, to write into, apart from the inputs); with ``return_lse`` also the fp32 log of
     the softmax sum ``[B, Sq, Hq]`` (-inf where nothing is seen)."""
     what = 'attention_cached'
-    index = _cuda_index(what, cache)
+    index = cache._look()
+    if index < 0:
+        _refuse_cpu(what)
     _, H, page, D = cache._shape
     shape = q.shape
     if len(shape) != 4 or shape[3] != D or shape[2] < 1 or shape[2] % H:
