@@ -23,7 +23,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib
-from .kv_cache import _DTYPES, _int32, _launch, _refuse_grad, _rows
+from .kv_cache import _DTYPES, _forward_ad, _int32, _launch, _refuse_grad, _rows
 
 
 def attention_fp8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, num_heads: int,
@@ -139,8 +139,8 @@ def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         raise ValueError(f'{what}: q, k and v must all be bfloat16 or all float16, got {q.dtype}, {k.dtype}, {v.dtype}')
     if k.get_device() != index or v.get_device() != index:
         raise ValueError(f'{what}: q, k and v must be on one device')
-    if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
-        _refuse_grad(what)
+    if q.requires_grad or k.requires_grad or v.requires_grad or _forward_ad._current_level >= 0:   # (-1: not in a dual_level)
+        _refuse_grad(what, q, k, v)
     cu_q = _int32(cu_seqlens_q, (None,), what, 'cu_seqlens_q', index)
     N = cu_q.shape[0] - 1
     if N < 0:

@@ -22,6 +22,7 @@ from __future__ import annotations
 import functools
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 from . import _lib
 
@@ -134,8 +135,12 @@ def _rows(t):
     return t, t.data_ptr(), t.stride()
 
 
-def _refuse_grad(what):
-    raise NotImplementedError(f'kairos_sensenova_b200.{what} is forward-only')
+def _refuse_grad(what, *tensors):
+    """Raises if a derivative with respect to one of `tensors` would be lost: by autograd, or a forward-mode tangent."""
+    for t in tensors:
+        if t.requires_grad and torch.is_grad_enabled() or \
+                _forward_ad._current_level >= 0 and _forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f'kairos_sensenova_b200.{what} is forward-only')
 
 
 def _refuse_cpu(what):
@@ -208,8 +213,8 @@ def kv_cache_append(cache: KVCache, k: torch.Tensor, v: torch.Tensor, page_table
         raise ValueError(f'{what}: k and v must both be bfloat16 or float16, got {k.dtype}, {v.dtype}')
     if k.get_device() != index or v.get_device() != index:
         raise ValueError(f'{what}: k and v must be on {cache.device}')
-    if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
-        _refuse_grad(what)
+    if k.requires_grad or v.requires_grad or _forward_ad._current_level >= 0:   # (-1: not in a dual_level)
+        _refuse_grad(what, k, v)
     page_table, B, max_pages = _table(page_table, None, what, index)
     lengths = _int32(lengths, (B,), what, 'lengths', index)
     cu = _int32(cu_seqlens, (B + 1,), what, 'cu_seqlens', index)
@@ -295,8 +300,8 @@ def attention_cached(q: torch.Tensor, cache: KVCache, page_table: torch.Tensor, 
         raise ValueError(f'{what}: q must be bfloat16 or float16, got {q.dtype}')
     if q.get_device() != index:
         raise ValueError(f'{what}: q must be on {cache.device}, got {q.device}')
-    if q.requires_grad and torch.is_grad_enabled():
-        _refuse_grad(what)
+    if q.requires_grad or _forward_ad._current_level >= 0:
+        _refuse_grad(what, q)
     B, Sq, Hq, _ = shape
     page_table, _, max_pages = _table(page_table, B, what, index)
     lengths = _int32(lengths, (B,), what, 'lengths', index)

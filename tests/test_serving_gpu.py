@@ -306,6 +306,24 @@ print('same')
     assert r.returncode == 0 and 'same' in r.stdout, r.stderr[-2000:]
 
 
+def test_derivatives_are_refused():
+    """By autograd, in forward mode, and under torch.func: no operator drops a derivative without a word."""
+    from torch.autograd import forward_ad
+    x, cache = randn(gen(2), 8, 2, 64), KVCache.empty(2, 2, 64, 16)
+    calls = (lambda t: attention_prompt(x, x, t, i32([0, 8])), lambda t: attention_prompt(t, x, x, i32([0, 8])),
+             lambda t: kv_cache_append(cache, x, t, i32([[0]]), i32([8]), i32([0, 8])),
+             lambda t: attention_cached(t[None], cache, i32([[0]]), i32([8])))
+    for call in calls:
+        with pytest.raises(NotImplementedError):
+            call(x.clone().requires_grad_())
+        with forward_ad.dual_level(), pytest.raises(NotImplementedError):
+            call(forward_ad.make_dual(x, x))
+        with pytest.raises((NotImplementedError, RuntimeError)):
+            torch.func.jvp(call, (x,), (x,))
+        with torch.no_grad():
+            call(x.clone().requires_grad_())
+
+
 def test_prompt_extremes():
     """Scores up to the largest finite ones, equal scores, and a row maximum that keeps rising along the keys."""
     n, dt = 700, torch.bfloat16

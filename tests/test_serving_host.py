@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from kairos_sensenova_b200 import KVCache, _lib, attention_cached, attention_prompt, kv_cache_append, kv_cache_gather
-from kairos_sensenova_b200.kv_cache import _int32, _rows, check_tables
+from kairos_sensenova_b200.kv_cache import _int32, _refuse_grad, _rows, check_tables
 from oracle import serving as ref
 
 i32 = lambda x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
@@ -185,3 +185,21 @@ except RuntimeError as e:
 """
     r = subprocess.run([sys.executable, '-c', code], capture_output=True, text=True, timeout=200)
     assert r.returncode == 0 and 'refused' in r.stdout, r.stderr[-2000:]
+
+
+def test_derivatives_are_refused():
+    """Autograd's leaves and forward-mode duals; nothing is refused where no derivative is asked for."""
+    from torch.autograd import forward_ad
+    x = torch.zeros(3)
+    leaf = torch.zeros(3, requires_grad=True)
+    _refuse_grad('op', x, x)
+    with torch.no_grad():
+        _refuse_grad('op', x, leaf)
+    with pytest.raises(NotImplementedError, match='op is forward-only'):
+        _refuse_grad('op', x, leaf)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones(3))
+        _refuse_grad('op', x)
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError, match='op is forward-only'):
+                _refuse_grad('op', x, dual)
