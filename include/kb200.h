@@ -228,7 +228,8 @@ int kb200_residual_ln_mod(void* x, const void* r, int64_t rows, int64_t dim, int
  * the packed tokens; with n queries and m keys, query i sees keys j <= i + m - n (the
  * queries are the last n of the m tokens), or all m when `causal` is 0.  Query head h
  * reads kv head h / (Hq / Hkv).  A query that sees no key gets o = 0 and lse = -inf;
- * rows at and behind cu_q[N] are left as they were.  A masked key's values reach no
+ * rows at and behind cu_q[N] are left as they were.  Scores (scale q . k) may reach 2^22 in
+ * magnitude; past that results are not defined.  A masked key's values reach no
  * output, whatever they are.  D = 64 or 128; dtype 0 bf16, 1 fp16.  Strides in
  * elements, multiples of 8; channels contiguous.  cu_q, cu_k are device arrays, not
  * read by the host; offsets are clamped to the tokens there are.  o may not overlap the
@@ -306,7 +307,7 @@ int kb200_kv_gather(const KB200KvGatherArgs* a, void* stream);
 /* Attention of the last Sq tokens of each sequence over the cache: q [B, Sq, Hq, D]
  * (strides in elements, multiples of 8), o [B, Sq, Hq, D] contiguous, lse [B, Sq, Hq] or
  * NULL.  Query i sees the sequence's keys j < lengths[b] - Sq + 1 + i; none: o = 0,
- * lse = -inf.  Lengths are clamped to max_pages * page. */
+ * lse = -inf.  Lengths are clamped to max_pages * page.  Scores may reach 2^22 in magnitude. */
 size_t kb200_attn_cached_workspace_size(int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv, int64_t D, int64_t page,
                                         int64_t max_pages);
 typedef struct KB200AttnCachedArgs {

@@ -120,7 +120,8 @@ def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     keys the queries are the last n of the m tokens: query i sees the first ``i + 1 + m - n``
     keys (``causal=False``: all m).  A query that sees none gets 0; the values of keys that a
     query does not see never reach it, NaN and infinities included; V may be as large as the type allows (up to 256
-    such bf16 keys; O is summed in fp32).  Returns ``[Tq, Hq, D]``
+    such bf16 keys; O is summed in fp32), and scores (scale q . k) up to 2^22 in magnitude (past that fp32's steps exceed what a
+    probability bears, and results are not defined).  Returns ``[Tq, Hq, D]``
     (``out``: to write into, apart from the inputs; rows behind the last sequence are left as they
     were); with ``return_lse`` also the fp32 log of the softmax sum ``[Tq, Hq]``.  ``check=True``
     looks at the offsets on the host first (it synchronises) and raises ``ValueError``, and ``RuntimeError`` if a device-side

@@ -361,6 +361,48 @@ def test_prompt_largest_values(nq, nk, dtype):
     close_lse(lse, wlse)
 
 
+def signs(g, *shape):
+    return torch.randint(0, 2, shape, generator=g, device='cuda').double() * 2 - 1
+
+
+def close_large_lse(lse, want):
+    """Beside close_lse's terms, five fp32 roundings of the result."""
+    assert ((lse.double() - want).abs() <= 2.0 ** -11 + want.abs() * 5 * 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize('nq,nk,dim', [([300], [300], 64), ([100, 40], [6000, 2500], 128)])    # whole items; shares
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('largest', [2.0 ** 12, 2.0 ** 17, 2.0 ** 22])
+def test_prompt_large_scores(nq, nk, dim, dtype, largest):
+    """Scores of up to 2^22, where fp32's steps are up to 1/2: of equal ones every key has its share.  (q and k are
+    +-1 and the scale is large, so that every score's product is exact; those that differ, differ by two scales.)"""
+    g = gen(53)
+    q, k = (signs(g, n, 2, dim).to(dtype) for n in (sum(nq), sum(nk)))
+    k[: sum(nk) // 2] = k[sum(nk) - sum(nk) // 2:]            # every key twice: ties in every row that sees both
+    v = randn(g, sum(nk), 2, dim, dtype=dtype)
+    for scale in (largest / dim, -largest / dim):
+        o, lse = attention_prompt(q, k, v, i32(cu(nq)), i32(cu(nk)), softmax_scale=scale, return_lse=True)
+        want, wlse, A = ref.prompt(q, k, v, cu(nq), cu(nk), scale)
+        close(o, want, A, dtype)
+        close_large_lse(lse, wlse)
+
+
+@pytest.mark.parametrize('lens,sq,heads,H,D', [([300, 40], 1, 4, 2, 64), ([7000], 3, 12, 2, 128), ([90] * 600, 1, 8, 2, 128)])
+@pytest.mark.parametrize('largest', [2.0 ** 12, 2.0 ** 17, 2.0 ** 22])
+def test_cached_large_scores(lens, sq, heads, H, D, largest):
+    cache, table, _ = make_cache(lens, H, D, 16, seed=22)
+    g = gen(22)
+    half = signs(g, cache.num_pages, H, 8, D).float()
+    cache.k_pages.copy_(torch.cat([half, half], 2).to(torch.float8_e4m3fn))     # every key of a page twice
+    cache.k_scale.fill_(2.0 ** 10)
+    q = signs(g, len(lens), sq, heads, D).to(torch.bfloat16)
+    for scale in (largest / D / 2 ** 10, -largest / D / 2 ** 10):
+        o, lse = attention_cached(q, cache, i32(table), i32(lens), softmax_scale=scale, return_lse=True)
+        want, wlse, A = ref.cached(q, values(cache.k_pages), values(cache.v_pages), cache.k_scale, cache.v_scale, table, lens, scale)
+        close(o, want, A, torch.bfloat16, u_p=2.0 ** -11)
+        close_large_lse(lse, wlse)
+
+
 @pytest.mark.parametrize('scale', [-0.3, 0.0, 1e-3, 2.0])
 def test_any_softmax_scale(scale):
     g = gen(13)
