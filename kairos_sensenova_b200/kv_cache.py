@@ -287,7 +287,8 @@ def attention_cached(q: torch.Tensor, cache: KVCache, page_table: torch.Tensor, 
     query that sees none (an idle slot of length 0) gets 0.  Returns ``[B, Sq, Hq, D]`` in
     q's type (``out``: contiguous, to write into, apart from the inputs); with ``return_lse`` also the fp32 log of
     the softmax sum ``[B, Sq, Hq]`` (-inf where nothing is seen).  Scores (scale q . k) may reach 2^22 in magnitude; past that
-    fp32's steps exceed what a probability bears, and results are not defined."""
+    fp32's steps exceed what a probability bears, and results are not defined.  Probabilities are rounded to fp16: 2^-11 of
+    themselves, or 2^-33 of the row's largest where they are under 2^-22 of it."""
     what = 'attention_cached'
     index = cache._look()
     if index < 0:

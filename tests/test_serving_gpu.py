@@ -649,6 +649,35 @@ def test_cached_largest_and_smallest_values(lens, sq, heads, H, D, page, exponen
     close_lse(lse, wlse)
 
 
+@pytest.mark.parametrize('sq,heads,D,page,spread', [(1, 4, 128, 16, 30), (3, 4, 64, 32, 30), (6, 4, 128, 32, 40), (1, 4, 64, 16, 12)])
+def test_cached_small_weights_of_large_values(sq, heads, D, page, spread):
+    """Keys with weights of about 2^-28 (and 2^-10, in the second sequence) of the largest, on pages whose V scale is 2^30 (2^40, 2^12) larger than
+    the others'.  Beside close's terms: a probability under 2^-22 of the row's largest P, which is 2^8 at least, is rounded in f16's
+    subnormals, 2^-25 off at most, 2^-33 of the largest; that is 2^-33 of each |v| in the output."""
+    lens = [1000, 700, 260]
+    cache, table, _ = make_cache(lens, 1, D, page, seed=23)
+    g = gen(23)
+    cache.k_pages.copy_(torch.full(cache.k_pages.shape, 0.5, device='cuda').to(torch.float8_e4m3fn))
+    cache.k_scale.fill_(2.0 ** -3)
+    cache.v_scale.fill_(2.0 ** -6)
+    q = (1 + 0.02 * torch.randn(3, sq, heads, D, generator=g, device='cuda')).to(torch.bfloat16)
+    # a score is 1/16 a channel, times the scale: so far above those of keys of code -0.5
+    bits = [28, 10, 28]
+    for b, where in enumerate(([3, 17, 18], [0, 9], [2])):
+        for i in where:
+            pg = table[b][i]
+            cache.k_pages[pg] = torch.tensor(-0.5 if bits[b] == 28 else 0.15625, device='cuda').to(torch.float8_e4m3fn)
+            cache.v_scale[pg] = 2.0 ** (spread - 6)
+    scale = 28 * math.log(2) / (D / 8)                       # between codes 0.5 and -0.5: 28 bits
+    o, lse = attention_cached(q, cache, i32(table), i32(lens), softmax_scale=scale, return_lse=True)
+    want, wlse, A = ref.cached(q, values(cache.k_pages), values(cache.v_pages), cache.k_scale, cache.v_scale, table, lens, scale)
+    for b, n in enumerate(lens):
+        total = sum((values(cache.v_pages[pg]) * cache.v_scale[pg].double()[:, None, None])[0, :n - i * page].abs().sum(0)
+                    for i, pg in enumerate(table[b][:-(-n // page)]))
+        close(o[b], want[b], A[b] + total * 2.0 ** -33 * 2.0 ** 11, torch.bfloat16, u_p=2.0 ** -11)
+    close_lse(lse, wlse)
+
+
 def test_cached_hidden_nan_and_missing_pages():
     """A NaN code of the newest token reaches only the queries that see it; a missing page is skipped."""
     lens, H, D, page = [100], 2, 128, 32
