@@ -279,7 +279,7 @@ static int launch_append(const AppendParams& p, cudaStream_t st) {
   // (32760 tokens of 8 heads: 46.8 us with four, 49 with two, 47.5 with eight; a unit's blocks next to
   // each other in a one-dimensional grid: 53.8)
   const int64_t units = p.T / PAGE + 2 * (int64_t)p.B, groups = (2 * p.H + PER - 1) / PER;
-  const int64_t items = units * groups <= 148 * 8 ? 1 : 4;
+  const int64_t items = units * groups <= sm_count() * 8 ? 1 : 4;
   kv_append_kernel<D, PAGE, F16><<<dim3((unsigned)units, (unsigned)((groups + items - 1) / items)), THREADS, 0, st>>>(p);
   return check_launch("kv_append_kernel");
 }

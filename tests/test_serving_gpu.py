@@ -579,6 +579,40 @@ def test_append_and_gather_many_sequences():
     assert torch.equal(kg, ref.gather(w, s, table, old, n).bfloat16())
 
 
+@pytest.mark.parametrize('H,D,page,dtype,new,old', [
+    (8, 128, 64, torch.bfloat16, [6000, 1, 300], [37, 63, 128]),
+    (7, 64, 16, torch.float16, [9000, 5, 1, 2000], [9, 16, 15, 100]),
+    (5, 128, 128, torch.bfloat16, [15000], [100]),
+    (24, 128, 32, torch.float16, [2500, 0, 40], [31, 7, 0]),
+    (32, 128, 16, torch.bfloat16, [600] * 3, [1, 2, 3]),
+    (9, 64, 128, torch.float16, [20000, 17], [1, 127]),
+])
+def test_append_and_gather_at_size(H, D, page, dtype, new, old):
+    """Enough pages that a block takes several (head, k or v) items one after the other, numbers of items that the blocks do not
+    divide, scales that grow over the tokens of a page's first ones, and tokens of more than a block's threads."""
+    lens = [a + b for a, b in zip(new, old)]
+    cache, table, _ = make_cache(lens, H, D, page, seed=H + D)
+    g = gen(H * page)
+    grow = torch.exp2(torch.randint(-3, 7, (sum(new), H, 1), generator=g, device='cuda').float()).to(dtype)
+    k, v = randn(g, sum(new), H, D, dtype=dtype) * grow, randn(g, sum(new), H, D, dtype=dtype) * grow.flip(1)
+    want = []
+    for codes, scale, x in ((cache.k_pages, cache.k_scale, k), (cache.v_pages, cache.v_scale, v)):
+        w, s = values(codes), scale.clone()
+        ref.append(w, s, x, table, lens, cu(new))
+        want.append((w, s))
+    kv_cache_append(cache, k, v, i32(table), i32(lens), i32(cu(new)), check=True)
+    for codes, scale, (w, s) in ((cache.k_pages, cache.k_scale, want[0]), (cache.v_pages, cache.v_scale, want[1])):
+        got = values(codes)
+        assert torch.equal(scale, s) and torch.equal(torch.isnan(got), torch.isnan(w)) and torch.equal(got.nan_to_num(), w.nan_to_num())
+    counts = [n - n // 3 for n in lens]
+    kg, vg = kv_cache_gather(cache, i32(table), i32([n // 3 for n in lens]), i32(cu(counts)), sum(counts), dtype=dtype, check=True)
+    for got, (w, s) in ((kg, want[0]), (vg, want[1])):
+        flat = w * s.double()[:, :, None, None]              # [pages, H, page, D]
+        for b, n in enumerate(lens):
+            rows = flat[table[b][:-(-n // page)]].transpose(1, 2).reshape(-1, H, D)[n // 3:n] if n else flat.new_zeros(0, H, D)
+            assert torch.equal(got[cu(counts)[b]:cu(counts)[b + 1]], rows.to(dtype))
+
+
 def test_gather_leaves_other_rows():
     cache, table, _ = make_cache([30], 2, 128, 16, 1)
     out = [torch.full((50, 2, 128), 5.0, device='cuda', dtype=torch.bfloat16) for _ in range(2)]
