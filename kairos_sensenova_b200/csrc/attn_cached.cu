@@ -172,9 +172,9 @@ KB_DEVI int o_chunk(int r, int c) {
 }
 
 // The launch shapes.  NT: 8-row tiles of a CTA (rows up to 8: 1, else 2); a group is NT * 16
-// tokens.  WK warps, OCC CTAs per SM: as many as the registers allow without spilling the loop (16 rows
-// at D = 128 take all 255; with 12 warps of 168, 32 queries of 32 sequences of 4000 tokens took 176 us
-// and not 133).
+// tokens.  WK warps, OCC CTAs per SM: as many as the registers allow with little spilling (8 to 188 bytes a thread;
+// 16 rows at D = 128 take all 255 registers: with 12 warps of 168, 32 queries of 32 sequences of 4000 tokens
+// took 176-180 us and not 130-133).
 template <int D, int NT>
 struct Shape {
   static constexpr int GT = NT * 16, ROWS = NT * 8;

@@ -6,8 +6,8 @@
 // Bound: the tensor pipe and the exponentials together.  A tile of 256 rows x 128 keys is
 // 4 * 256 * 128 * D flops (2048 cycles at D = 128) and 32768 exponentials (2048 cycles of MUFU).
 //
-// Measured: 16380 tokens, 24/24 heads of 128: 1.3-1.5 ms, 1.1-1.27 PFLOP/s as the clock goes; 8192 tokens of
-// 24/8 heads 341 us with the tensor pipe active 70 % of the time.
+// Measured: 16380 tokens, 24/24 heads of 128: 1.3-1.5 ms, 1.1-1.27 PFLOP/s as the clock goes, of 64 1.01 ms; 8192
+// tokens of 24/8 heads of 128 345 us with the tensor pipe active 68 % of the time.
 //
 // Rows.  The G = Hq / Hkv heads that share a kv head are rows of one matrix: a query tile of 128
 // rows holds T = 128 / G tokens (rounded down) with G heads each, row = token * G + head, so a
@@ -302,7 +302,9 @@ KB_DEVI void find_tile(const Params& p, int64_t r, int lane, int& seq, int& tile
   }
   // Many sequences: sequence s owns the numbers from cu_q[s] / tokens of a tile + s on (it has at most
   // n / tokens + 1 tiles, so these do not overlap), found without going through all of them; a number
-  // that no tile has gives tile = -1.  A sequence's last tiles come first.
+  // that no tile has gives tile = -1.  A sequence's last tiles come first, but the sequences are taken in order: 70 prompts
+  // of 100 tokens and one of 6000, 24/8 heads of 128, take 254-270 us if that is the first and 295-304 if it is the
+  // last (61 prompts, sorted: 241).
   const int per = QT * p.tq;
   auto first = [&](int s) { return min(max((int64_t)p.cu_q[s], (int64_t)0), p.Tq) / per + s; };
   seq = kv::warp_last(p.N, lane, [&](int s) { return first(s) <= r; });
@@ -451,7 +453,8 @@ KB_DEVI void warp_arrive(uint64_t* bar, int lane) {
 }
 
 // Which of every 8 pairs of exponentials go to the FMA pipe (measured with none, 1, 2, 3 and 4 of 8;
-// 2 of 8 was fastest for D = 128: 170, 161, 156, 165 and 166 us for two pieces of prompts).
+// 2 of 8 was fastest at both head dims: D = 128, two pieces of prompts, 170, 161, 156, 165 and 166 us; D = 64, 16380
+// tokens of 24/24 heads, 1044, 1033, 1013, 1030 and 1120 us).
 constexpr int POLY = 0x88;
 
 // (BOUNDED: with the caller's bound of a wait, instead of 4e9 clocks)
