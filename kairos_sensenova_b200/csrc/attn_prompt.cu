@@ -187,19 +187,17 @@ struct Smem {
   int took[4], taken;                        // whole items: the CTAs whose items this one took last, and how many
   int done[8];                               // items that each softmax warp has finished
   int abort_flag, keep_tmem;
-  // Keys with a V that is not finite, from the first that some row of the item does not see on (a row sees fewer than
-  // ROWS of these); the items with keys take the two in turn.
-  uint32_t odd[2][ROWS / 32];
-  int any_odd[2];
+  // For each query tile, keys with a V that is not finite, counted from the first that some row of the item does not see
+  // (a row sees fewer than ROWS from there on), and whether there are some; the items with keys take the two in turn.
+  uint32_t odd[2][QT][ROWS / 32];
+  int any_odd[2][QT];
 };
 
 // What is not finite in the rows [r0, r1) of a V tile in shared memory becomes 0, by one warp; row r is key r + key0
-// of those that `odd` marks (`clear`: it has none yet).  (The two functions are not inlined: they are hardly ever
+// of those that `odd` marks, for query tile `t` and those behind it.  (The two functions are not inlined: they are hardly ever
 // called, and in line their code alone cost 5 % of a packed batch's time.)
 template <int D, bool F16>
-__device__ __noinline__ void take_out(uint4* v, int r0, int r1, int key0, uint32_t* odd, bool clear, int lane) {
-  if (clear && lane < ROWS / 32) odd[lane] = 0;
-  __syncwarp();
+__device__ __noinline__ void take_out(uint4* v, int r0, int r1, int key0, uint32_t (*odd)[ROWS / 32], int t, int lane) {
   for (int r = r0; r < r1; ++r) {            // (a row is 8 chunks of each atom: its channels, in some order)
     bool mine = false;
     if (lane < D / 8) {
@@ -209,7 +207,7 @@ __device__ __noinline__ void take_out(uint4* v, int r0, int r1, int key0, uint32
       if (mine) x = make_uint4(x.x & ~z.x, x.y & ~z.y, x.z & ~z.z, x.w & ~z.w);
     }
     const int k = r + key0;
-    if (__any_sync(0xffffffffu, mine) && lane == 0 && k < ROWS) odd[k >> 5] |= 1u << (k & 31);
+    if (__any_sync(0xffffffffu, mine) && lane >= t && lane < QT && k < ROWS) odd[lane][k >> 5] |= 1u << (k & 31);
   }
   tc::fence_proxy_async_smem();
   __syncwarp();
@@ -509,7 +507,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
   const uint32_t tmem = sm.tmem_base;
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");   // the join, if any: it waits for this grid's end
 
-  auto wait_for = [&](uint64_t* bar, uint32_t parity) { 
+  auto wait_for = [&](uint64_t* bar, uint32_t parity) {
     // (a thread suspended in try_wait looks at no clock: short bounds need the polling loop)
     if constexpr (BOUNDED) return tc::mbar_test_wait_loop(bar, parity, p.wait_clocks);
     else return tc::mbar_wait(bar, parity);
@@ -681,7 +679,6 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
           const int hidden = seen_by(p, it.tile * QT * p.tq, it.n, it.m);
           const int beyond0 = seen_by(p, min(it.n, it.tile * QT * p.tq + p.tq) - 1, it.n, it.m);
           const int beyond = seen_by(p, min((int64_t)it.n, (int64_t)(it.tile + 1) * QT * p.tq) - 1, it.n, it.m);
-          bool odd = false;                                  // V is not finite somewhere from there on
           for (int j = it.j0; ok && j < it.j1; ++j, ++g) {
             const int slot = g % VS;
             ok = wait(&sm.v_full[slot], (g / VS) & 1);
@@ -696,8 +693,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
               tc::fence_proxy_async_smem();
               __syncwarp();
             }
-            if (j == it.j0 && lane == 0) sm.any_odd[uses & 1] = 0;   // (two items on, this warp has had the P of the item
-                                                             // between, and so every softmax warp has read it)
+            if (j == it.j0) {                                // (two items on, this warp has had the P of the item
+              if (lane < QT * ROWS / 32) (&sm.odd[uses & 1][0][0])[lane] = 0;   // between, and so every softmax warp
+              if (lane < QT) sm.any_odd[uses & 1][lane] = 0;                    // has read these)
+              __syncwarp();
+            }
             const uint64_t dv = dv0 + (uint64_t)(slot * ATOMS) * ATOM;
             for (int t = 0; ok && t < QT; ++t) {             // O_t += P_t V_j, 16 keys per instruction
               const int from = t == 0 ? r0 : mid, to = t == 0 ? mid : r1, steps = t == 0 ? steps0 : steps1;
@@ -711,9 +711,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
                     x2 = not_finite<F16>(x.z, x2); x3 = not_finite<F16>(x.w, x3);
                   }
                 if (__any_sync(0xffffffffu, ((x0 | x1 | x2 | x3) & 0x7fff7fffu) != 0)) {
-                  take_out<D, F16>(v, from, to, j * BN - hidden, sm.odd[uses & 1], !odd, lane);
-                  odd = true;
-                  if (lane == 0) sm.any_odd[uses & 1] = 1;
+                  take_out<D, F16>(v, from, to, j * BN - hidden, sm.odd[uses & 1], t, lane);
+                  if (lane >= t && lane < QT) sm.any_odd[uses & 1][lane] = 1;
+                  __syncwarp();
                 }
               }
               // (the softmax publishes an item's first P_t when it has read the O_t before)
@@ -842,9 +842,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prompt_kernel(const __grid_co
       if (ok && any) ok = __all_sync(0xffffffffu, wait_for(&sm.pv_done[qt], (g - 1) & 1));
       if (!ok) break;
       tc::tc_fence_after();
-      if (any && sm.any_odd[uses & 1]) {                     // V that was taken out of the product: added where the row sees it
+      if (any && sm.any_odd[uses & 1][qt]) {                     // V that was taken out of the product: added where the row sees it
         const char* v = reinterpret_cast<const char*>(p.v) + 2 * (((int64_t)it.k0 + hidden) * p.v_ts + (it.hk / p.parts) * p.v_hs);
-        put_back<D, F16>(tO, v, 2 * p.v_ts, live ? lim - hidden : 0, sm.odd[uses & 1]);
+        put_back<D, F16>(tO, v, 2 * p.v_ts, live ? lim - hidden : 0, sm.odd[uses & 1][qt]);
       }
       uses += any;
       if (it.slot >= 0) {                                    // a partial: O and l under this row's m
