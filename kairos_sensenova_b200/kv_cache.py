@@ -85,6 +85,9 @@ class KVCache:
         self._at = at
         return self._index
 
+    def __reduce__(self):                               # (a copy, or an unpickled one, is of its own tensors)
+        return KVCache, self._tensors
+
     @classmethod
     def empty(cls, num_pages: int, num_heads: int, head_dim: int, page_size: int = 64, device='cuda'):
         """A pool without tokens (codes 0, scales 1)."""

@@ -203,3 +203,18 @@ def test_derivatives_are_refused():
         for grad in (True, False):
             with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError, match='op is forward-only'):
                 _refuse_grad('op', x, dual)
+
+
+def test_copies_of_a_cache():
+    """A deep copy and an unpickled cache have tensors and addresses of their own; a shallow copy has the same ones."""
+    import copy
+    import pickle
+    c = KVCache.empty(3, 2, 64, 16, device='cpu')
+    c.k_scale.fill_(4.0)
+    for d, same in ((copy.deepcopy(c), False), (pickle.loads(pickle.dumps(c)), False), (copy.copy(c), True)):
+        assert d.k_pages.shape == c.k_pages.shape and (d.k_scale == 4.0).all()
+        at = _lib.KV_CACHE_ARGS.unpack(d._args)[:4]
+        assert at == tuple(t.data_ptr() for t in (d.k_pages, d.v_pages, d.k_scale, d.v_scale))
+        assert all((t.data_ptr() == u.data_ptr()) == same for t, u in zip(d._tensors, c._tensors))
+        d._look()
+        assert _lib.KV_CACHE_ARGS.unpack(d._args)[:4] == at
